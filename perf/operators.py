@@ -1,0 +1,497 @@
+"""What the sequence operators of crnn_amd.seq cost: the cases that are timed, their plain forms and their definition in 64 bits.
+
+Three operators: the short causal convolution, the selective state space scan (a diagonal linear ODE with learned rates, stepped
+exactly) and activation checkpoints in 8 bits.  Rows are packed: sequence s holds rows seq_start[s] .. seq_start[s + 1] - 1 of every
+array, a dense batch is the case of equal lengths.
+"""
+import math
+
+import numpy as np
+import torch
+
+own = False
+
+DTYPES = {"f32": torch.float32, "bf16": torch.bfloat16, "f16": torch.float16}
+BLOCK = 32  # channels that share a scale of a checkpoint
+
+
+def listed():
+    return [
+        # one short series, no batch to fill the card: latency
+        dict(name="conv_short", op="conv", dtype="f32", rows=130, seqs=1, ragged=False, D=768, W=4, silu=True, bias=True),
+        # a batch of series of unequal length, some empty, in one packed array, continued from and into carried states
+        dict(name="conv_packed", op="conv", dtype="bf16", rows=12001, seqs=17, ragged=True, D=4096, W=4, silu=True, bias=True),
+        # training: the gradient, its input kept as an 8-bit checkpoint
+        dict(name="conv_grad_8bit", op="conv_grad", dtype="bf16", rows=8192, seqs=4, ragged=False, D=2048, W=4, silu=True, bias=True, packed=True),
+        # serving: one new row for each of many running series
+        dict(name="conv_step", op="conv_step", dtype="bf16", rows=192, slots=256, D=4096, W=4, silu=True, bias=True),
+        # one short series
+        dict(name="scan_short", op="scan", dtype="bf16", rows=64, seqs=1, ragged=False, D=1536, N=16, G=1, gate=True, softplus=True),
+        # a batch of unequal series in one packed array, continued from and into carried states
+        dict(name="scan_packed", op="scan", dtype="bf16", rows=8190, seqs=9, ragged=True, D=4096, N=16, G=1, gate=True, softplus=True),
+        # the gradient in the parameters' own precision, several groups of input and output maps, odd sizes, no gate
+        dict(name="scan_grad_groups", op="scan_grad", dtype="f32", rows=2 * 203, seqs=2, ragged=False, D=640, N=8, G=4, gate=False, softplus=True, packed=False),
+        # training: the gradient from 8-bit checkpoints of the input and of the gate
+        dict(name="scan_grad_8bit", op="scan_grad", dtype="bf16", rows=4 * 1536, seqs=4, ragged=False, D=2048, N=16, G=1, gate=True, softplus=True, packed=True),
+        # serving: one series, then many
+        dict(name="scan_step_one", op="scan_step", dtype="bf16", rows=1, slots=4, D=2048, N=16, G=1, gate=True, softplus=True),
+        dict(name="scan_step_many", op="scan_step", dtype="bf16", rows=250, slots=256, D=4096, N=16, G=1, gate=True, softplus=True),
+        # a small activation of odd sizes kept in 8 bits and restored; the activations of a layer
+        dict(name="checkpoint_small", op="checkpoint", dtype="f16", rows=37, D=1000),
+        dict(name="checkpoint_large", op="checkpoint", dtype="bf16", rows=16384, D=4096),
+    ]
+
+
+def _log(rng, lo, hi):
+    return int(round(math.exp(rng.uniform(math.log(lo), math.log(hi)))))
+
+
+def draw(rng):
+    op = rng.choice(["conv", "conv_grad", "conv_step", "scan", "scan", "scan_grad", "scan_grad", "scan_step", "checkpoint"])
+    c = dict(op=op, dtype=rng.choice(["f32", "bf16", "f16"]), D=8 * _log(rng, 24, 510) + rng.choice([0, 0, 4, 1]))
+    if op in ("conv_step", "scan_step"):
+        c["rows"] = _log(rng, 1, 250)
+        c["slots"] = c["rows"] + rng.randrange(20)
+    elif op == "checkpoint":
+        c["rows"] = _log(rng, 1, 16384)
+        return c
+    else:
+        c["rows"] = _log(rng, 24, 8000 if op == "scan" else 12000 if op.startswith("conv") else 3000)
+        c["ragged"] = rng.random() < 0.6
+        c["seqs"] = _log(rng, 1, 24)
+        if not c["ragged"]:
+            c["seqs"] = min(c["seqs"], 6)
+            c["rows"] = c["seqs"] * max(1, c["rows"] // c["seqs"])
+    if op.startswith("conv"):
+        c.update(W=rng.choice([2, 3, 4, 4]), silu=rng.random() < 0.7, bias=rng.random() < 0.8)
+    else:
+        G = rng.choice([1, 1, 2, 4])
+        c["D"] = -(-c["D"] // G) * G
+        c.update(N=rng.choice([4, 8, 16, 16, 11]), G=G, gate=rng.random() < 0.7, softplus=rng.random() < 0.8)
+    if op.endswith("_grad"):
+        c["packed"] = rng.random() < 0.5
+    return c
+
+
+def _lengths(case, seed):
+    n, rows = case["seqs"], case["rows"]
+    if not case["ragged"]:
+        return [rows // n] * n
+    rng = np.random.default_rng(1000 + seed)
+    cut = np.sort(rng.integers(0, rows + 1, n - 1))
+    at = np.concatenate([[0], cut, [rows]])
+    lens = list(np.diff(at))
+    if n > 3:  # a series without rows and one of a single row are part of a ragged batch
+        lens[0], lens[1] = 0, lens[0] + lens[1]
+    return [int(v) for v in lens]
+
+
+def prepare(case, seed):
+    gen = torch.Generator(device="cuda").manual_seed(seed * 7919 + 13)
+    dev, dt_ = "cuda", DTYPES[case["dtype"]]
+    op, D, T = case["op"], case["D"], case["rows"]
+
+    def randn(*shape, dtype=dt_, scale=1.0):
+        return (torch.randn(*shape, generator=gen, device=dev) * scale).to(dtype)
+
+    s = dict(case=case)
+    if op == "checkpoint":
+        # activations: channels of unequal size, a few large outliers
+        s["x"] = (torch.randn(T, D, generator=gen, device=dev) * torch.exp(torch.randn(D, generator=gen, device=dev))).to(dt_)
+        return s
+    if "seqs" in case:
+        lens = _lengths(case, seed)
+        starts = torch.tensor([0] + list(np.cumsum(lens)), dtype=torch.int32, device=dev)
+        s["seq_start"], s["n_state"] = starts, case["seqs"]
+    else:
+        s["n_state"] = case["slots"]
+        s["slots"] = torch.randperm(case["slots"], generator=gen, device=dev)[:T].to(torch.int32)
+    if op.startswith("conv"):
+        W = case["W"]
+        s["x"] = randn(T, D)
+        s["weight"] = randn(D, W, dtype=torch.float32, scale=W ** -0.5)
+        s["bias"] = randn(D, dtype=torch.float32, scale=0.1) if case["bias"] else None
+        s["state"] = randn(s["n_state"], W - 1, D)
+    else:
+        N, G = case["N"], case["G"]
+        s["u"] = torch.nn.functional.silu(torch.randn(T, D, generator=gen, device=dev)).to(dt_)
+        # steps between 1e-3 and 1e-1 of the unit of time, as after the usual initialisation
+        step0 = torch.exp(torch.rand(D, generator=gen, device=dev) * math.log(100.0) + math.log(1e-3))
+        if case["softplus"]:
+            s["dt"] = randn(T, D, scale=0.5)
+            s["dt_bias"] = step0 + torch.log(-torch.expm1(-step0))
+        else:
+            s["dt"] = (step0 * torch.exp(0.3 * torch.randn(T, D, generator=gen, device=dev))).to(dt_)
+            s["dt_bias"] = None
+        s["A"] = -torch.arange(1, N + 1, device=dev, dtype=torch.float32) * torch.exp(0.1 * torch.randn(D, N, generator=gen, device=dev))
+        s["B"], s["C"] = randn(T, G, N), randn(T, G, N)
+        s["D"] = 1 + randn(D, dtype=torch.float32, scale=0.1)
+        s["z"] = randn(T, D) if case["gate"] else None
+        s["state"] = randn(s["n_state"], D, N, dtype=torch.float32, scale=0.3)
+    if op.endswith("_grad"):
+        s["dy"] = randn(T, D)
+        s["dstate"] = randn(*s["state"].shape, dtype=s["state"].dtype, scale=0.1)
+        if case["packed"]:  # what the training step kept of its forward pass
+            for k in ("x", "u", "z"):
+                if s.get(k) is not None:
+                    s[k + "_codes"], s[k + "_scales"] = _codes(s[k])
+                    s[k] = None
+    return s
+
+
+# ---------------------------------------------------------------- plain forms
+def _codes(x):
+    """(int8 codes, scale bytes) of a checkpoint: blocks of 32 channels, scales powers of two, byte = exponent + 127."""
+    T, D = x.shape
+    nb = -(-D // BLOCK)
+    v = torch.nn.functional.pad(x.float(), (0, nb * BLOCK - D)).view(T, nb, BLOCK)
+    m = v.abs().amax(-1)
+    e = torch.frexp(m)[1] - 7
+    e = e + (torch.round(torch.ldexp(m, -e)) > 127)
+    e = torch.where(m > 0, e.clamp(min=-127), torch.full_like(e, -127))
+    q = torch.round(torch.ldexp(v, -e[..., None])).clamp(-127, 127)
+    return q.view(T, nb * BLOCK)[:, :D].to(torch.int8).contiguous(), (e + 127).to(torch.uint8)
+
+
+def _values(codes, scales):
+    e = scales.to(torch.int32).repeat_interleave(BLOCK, -1)[:, :codes.shape[1]] - 127
+    return torch.ldexp(codes.float(), e)
+
+
+def _input(s, k):
+    if s.get(k + "_codes") is not None:
+        return _values(s[k + "_codes"], s[k + "_scales"])
+    return None if s.get(k) is None else s[k].float()
+
+
+def _silu_grad(p):
+    g = torch.sigmoid(p)
+    return g * (1 + p * (1 - g))
+
+
+def _rows(s, T):
+    """(sequence of each row, whether it is the first of its sequence, first rows, row counts)."""
+    st = s["seq_start"].long()
+    t = torch.arange(T, device=st.device)
+    seg = torch.bucketize(t, st[1:], right=True)
+    return seg, t == st[seg], st[:-1], st[1:] - st[:-1]
+
+
+def _windows(x, s, W):
+    """[T, W, D]: the W inputs of each row, the oldest first, from the sequence's state where they lie before it; and the states out."""
+    T = x.shape[0]
+    seg, _, first, lens = _rows(s, T)
+    src = torch.cat([x, s["state"].float().flatten(0, 1)])
+    back = torch.arange(-(W - 1), 1, device=x.device)
+
+    def at(row, seq):  # row counted within its sequence, may be negative
+        return torch.where(row >= 0, first[seq] + row, T + seq * (W - 1) + (W - 1) + row)
+
+    t = torch.arange(T, device=x.device)
+    win = src[at((t - first[seg])[:, None] + back, seg[:, None])]
+    n = torch.arange(len(lens), device=x.device)
+    out = src[at(lens[:, None] + back[:-1], n[:, None])]
+    return win, out, at, seg, first, lens
+
+
+def _conv(s):
+    c, o = s["case"], DTYPES[s["case"]["dtype"]]
+    win, out, *_ = _windows(s["x"].float(), s, c["W"])
+    p = (win * s["weight"].T).sum(1)
+    if c["bias"]:
+        p = p + s["bias"]
+    y = p * torch.sigmoid(p) if c["silu"] else p
+    return y.to(o), out.to(o)
+
+
+def _conv_grad(s):
+    c, o = s["case"], DTYPES[s["case"]["dtype"]]
+    x, W = _input(s, "x"), c["W"]
+    T, D = x.shape
+    win, _, at, seg, first, lens = _windows(x, s, W)
+    w = s["weight"].T
+    p = (win * w).sum(1)
+    if c["bias"]:
+        p = p + s["bias"]
+    dp = s["dy"].float() * (_silu_grad(p) if c["silu"] else torch.ones_like(p))
+    dw = (win * dp[:, None]).sum(0).T
+    db = dp.sum(0) if c["bias"] else None
+    # every row, and behind them every row of the states, counted within its sequence, collects what its uses pass back
+    n = torch.arange(len(lens), device=x.device)
+    back = torch.arange(-(W - 1), 0, device=x.device)
+    of = torch.cat([seg, n.repeat_interleave(W - 1)])
+    row = torch.cat([torch.arange(T, device=x.device) - first[seg], back.repeat(len(lens))])
+    use = row[:, None] + torch.arange(W, device=x.device)
+    there = (use >= 0) & (use < lens[of][:, None])
+    total = (torch.where(there[..., None], dp[(first[of][:, None] + use) * there], 0.0) * w.flip(0)).sum(1)
+    kept = row - lens[of] + W - 1
+    total = total + torch.where((kept >= 0)[:, None], s["dstate"].float()[of, kept.clamp(min=0)], 0.0)
+    return total[:T].to(o), dw.contiguous(), db, total[T:].view(len(lens), W - 1, D).to(o)
+
+
+def _conv_step(s):
+    c, o = s["case"], DTYPES[s["case"]["dtype"]]
+    sl = s["slots"].long()
+    win = torch.cat([s["state"][sl].float(), s["x"].float()[:, None]], 1)
+    p = (win * s["weight"].T).sum(1)
+    if c["bias"]:
+        p = p + s["bias"]
+    s["state"][sl] = win[:, 1:].to(o)
+    return (p * torch.sigmoid(p) if c["silu"] else p).to(o), s["state"]
+
+
+def _delta(s):
+    v = s["dt"].float()
+    if s["dt_bias"] is not None:
+        v = v + s["dt_bias"]
+    return (torch.nn.functional.softplus(v, threshold=40.0) if s["case"]["softplus"] else v), v
+
+
+def _wide(m, D):
+    """[T, G, N] -> [T, D, N]"""
+    return m.float().repeat_interleave(D // m.shape[1], 1)
+
+
+def _prefix(a, b):
+    """h[t] = a[t] h[t-1] + b[t], h before the first row 0, by doubling."""
+    k, T = 1, a.shape[0]
+    while k < T:
+        b = torch.cat([b[:k], b[k:] + a[k:] * b[:-k]])
+        a = torch.cat([a[:k], a[k:] * a[:-k]])
+        k *= 2
+    return b
+
+
+def _states(s, u, delta):
+    T, D = u.shape
+    seg, start, first, lens = _rows(s, T)
+    a = torch.exp(delta[..., None] * s["A"])
+    b = (delta * u)[..., None] * _wide(s["B"], D)
+    h0 = s["state"]
+    b = b + torch.where(start[:, None, None], a * h0[seg], 0.0)
+    h = _prefix(torch.where(start[:, None, None], 0.0, a), b)
+    return a, h, seg, start, first, lens
+
+
+def _scan(s):
+    c, o = s["case"], DTYPES[s["case"]["dtype"]]
+    u = s["u"].float()
+    delta, _ = _delta(s)
+    _, h, seg, start, first, lens = _states(s, u, delta)
+    y = (h * _wide(s["C"], c["D"])).sum(-1) + s["D"] * u
+    if s["z"] is not None:
+        z = s["z"].float()
+        y = y * z * torch.sigmoid(z)
+    last = (first + lens - 1).clamp(min=0)
+    return y.to(o), torch.where((lens > 0)[:, None, None], h[last], s["state"])
+
+
+def _scan_grad(s):
+    c, o = s["case"], DTYPES[s["case"]["dtype"]]
+    u, z, dy, D, N, G = _input(s, "u"), _input(s, "z"), s["dy"].float(), c["D"], c["N"], c["G"]
+    T = c["rows"]
+    delta, pre = _delta(s)
+    a, h, seg, start, first, lens = _states(s, u, delta)
+    B, C = _wide(s["B"], D), _wide(s["C"], D)
+    dz, r = None, dy
+    if z is not None:
+        v = (h * C).sum(-1) + s["D"] * u
+        dz = (dy * v * _silu_grad(z)).to(o)
+        r = dy * z * torch.sigmoid(z)
+    q = r[..., None] * C
+    filled = lens > 0
+    last = first + lens - 1
+    q.index_add_(0, last[filled], s["dstate"][filled])
+    nxt = torch.cat([torch.where(start[1:, None, None], 0.0, a[1:]), torch.zeros_like(a[:1])])
+    q = _prefix(nxt.flip(0), q.flip(0)).flip(0)
+    hp = torch.where(start[:, None, None], s["state"][seg], torch.cat([h[:1], h[:-1]]))
+    qah = q * a * hp
+    dA = (qah * delta[..., None]).sum(0)
+    qb = (q * B).sum(-1)
+    ddelta = (qah * s["A"]).sum(-1) + qb * u
+    du = delta * qb + r * s["D"]
+    dB = (q * (delta * u)[..., None]).view(T, G, D // G, N).sum(2)
+    dC = (r[..., None] * h).view(T, G, D // G, N).sum(2)
+    ddt = ddelta * torch.sigmoid(pre) if c["softplus"] else ddelta
+    dD = (r * u).sum(0)
+    at = first.clamp(max=T - 1)
+    dstate = torch.where(filled[:, None, None], a[at] * q[at], s["dstate"])
+    return dict(u=du.to(o), dt=ddt.to(o), A=dA, B=dB.to(o), C=dC.to(o), D=dD, z=dz, dt_bias=None if s["dt_bias"] is None else ddt.sum(0), state=dstate)
+
+
+def _scan_step(s):
+    c, o = s["case"], DTYPES[s["case"]["dtype"]]
+    u, sl = s["u"].float(), s["slots"].long()
+    delta, _ = _delta(s)
+    h = torch.exp(delta[..., None] * s["A"]) * s["state"][sl] + (delta * u)[..., None] * _wide(s["B"], c["D"])
+    s["state"][sl] = h
+    y = (h * _wide(s["C"], c["D"])).sum(-1) + s["D"] * u
+    if s["z"] is not None:
+        z = s["z"].float()
+        y = y * z * torch.sigmoid(z)
+    return y.to(o), s["state"]
+
+
+def _checkpoint(s):
+    codes, scales = _codes(s["x"])
+    return _values(codes, scales).to(s["x"].dtype), scales
+
+
+# ---------------------------------------------------------------- one pass
+def run(state):
+    op = state["case"]["op"]
+    if not own:
+        return {"conv": _conv, "conv_grad": _conv_grad, "conv_step": _conv_step, "scan": _scan, "scan_grad": _scan_grad, "scan_step": _scan_step,
+                "checkpoint": _checkpoint}[op](state)
+    from crnn_amd import seq
+    s, c = state, state["case"]
+    dt_ = DTYPES[c["dtype"]]
+
+    def held(k):
+        return seq.Packed8(s[k + "_codes"], s[k + "_scales"], dt_) if s.get(k + "_codes") is not None else s.get(k)
+
+    if op == "checkpoint":
+        p = seq.pack8(s["x"])
+        return seq.unpack8(p), p.scales
+    if op == "conv":
+        return seq.causal_conv(s["x"], s["weight"], s["bias"], silu=c["silu"], seq_start=s["seq_start"], state=s["state"], return_state=True)
+    if op == "conv_grad":
+        g = seq.causal_conv_grad(s["dy"], held("x"), s["weight"], s["bias"], silu=c["silu"], seq_start=s["seq_start"], state=s["state"], dstate=s["dstate"])
+        return g.x, g.weight, g.bias, g.state
+    if op == "conv_step":
+        return seq.causal_conv_step(s["x"], s["weight"], s["bias"], s["state"], s["slots"], silu=c["silu"]), s["state"]
+    more = dict(D=s["D"], dt_bias=s["dt_bias"], softplus=c["softplus"])
+    if op == "scan":
+        return seq.selective_scan(s["u"], s["dt"], s["A"], s["B"], s["C"], z=s["z"], seq_start=s["seq_start"], state=s["state"], return_state=True, **more)
+    if op == "scan_step":
+        return seq.selective_scan_step(s["u"], s["dt"], s["A"], s["B"], s["C"], s["state"], s["slots"], z=s["z"], **more), s["state"]
+    g = seq.selective_scan_grad(s["dy"], held("u"), s["dt"], s["A"], s["B"], s["C"], z=held("z"), seq_start=s["seq_start"], state=s["state"],
+                                dstate=s["dstate"], **more)
+    return dict(u=g.u, dt=g.dt, A=g.A, B=g.B, C=g.C, D=g.D, z=g.z, dt_bias=g.dt_bias, state=g.state)
+
+
+def work(case):
+    op, T, D, io = case["op"], case["rows"], case["D"], 4 if case["dtype"] == "f32" else 2
+    kept = (1 + 1 / BLOCK) if case.get("packed") else io
+    if op == "checkpoint":
+        return {"bytes": T * D * (2 * io + 2 * (1 + 1 / BLOCK)), "flops": T * D * 4}
+    if op.startswith("conv"):
+        W, n = case["W"], case.get("seqs", T)
+        st, par = n * (W - 1) * D * io, D * (W + 1) * 4
+        if op == "conv_grad":
+            return {"bytes": T * D * (kept + 2 * io) + 3 * st + 2 * par, "flops": T * D * (6 * W + 12)}
+        return {"bytes": T * D * 2 * io + 2 * st + par, "flops": T * D * (2 * W + 5)}
+    N, G, n = case["N"], case["G"], case.get("seqs", T)
+    st, par, maps, gate = n * D * N * 4, D * (N + 2) * 4, 2 * T * G * N * io, int(case["gate"])
+    if op == "scan_grad":
+        return {"bytes": T * D * ((1 + gate) * (kept + io) + 3 * io) + 3 * st + 2 * par + 2 * maps, "flops": T * D * (20 * N + 20)}
+    return {"bytes": T * D * (3 + gate) * io + 2 * st + par + maps, "flops": T * D * (7 * N + 10)}
+
+
+# ---------------------------------------------------------------- the definition in 64 bits, row by row
+def _restored(s, k):
+    if s.get(k + "_codes") is not None:
+        q, e = s[k + "_codes"].double(), s[k + "_scales"].double() - 127
+        return q * torch.exp2(e)[:, torch.arange(q.shape[1], device=q.device) // BLOCK]
+    return None if s.get(k) is None else s[k].double()
+
+
+def exact(case, seed):
+    s = prepare(case, seed)
+    op, T, D = case["op"], case["rows"], case["D"]
+    sig = lambda v: 1 / (1 + torch.exp(-v))  # noqa: E731
+    if op == "checkpoint":
+        x = s["x"].double()
+        e, out = torch.zeros(T, -(-D // BLOCK), dtype=torch.float64, device=x.device), torch.empty_like(x)
+        for k in range(e.shape[1]):
+            b = x[:, k * BLOCK:(k + 1) * BLOCK]
+            m = b.abs().max(1).values
+            p = torch.floor(torch.log2(m.clamp(min=1e-300))) - 6
+            p = torch.where(torch.round(m / torch.exp2(p)) > 127, p + 1, p).clamp(min=-127)
+            p = torch.where(m > 0, p, torch.full_like(p, -127.0))
+            e[:, k] = p + 127
+            out[:, k * BLOCK:(k + 1) * BLOCK] = torch.round(b / torch.exp2(p)[:, None]) * torch.exp2(p)[:, None]
+        return out, e.to(torch.uint8)
+    if op in ("conv", "conv_grad", "conv_step"):
+        W, w, st = case["W"], s["weight"].double(), s["state"].double()
+        bias = s["bias"].double() if case["bias"] else 0.0
+        if op == "conv_step":
+            sl = s["slots"].tolist()
+            y = torch.empty(T, D, dtype=torch.float64, device=w.device)
+            for r, k in enumerate(sl):
+                win = torch.cat([st[k], s["x"][r:r + 1].double()])
+                p = (w * win.T).sum(1) + bias
+                y[r] = p * sig(p) if case["silu"] else p
+                st[k] = win[1:]
+            return y, st
+        x, at = _restored(s, "x"), s["seq_start"].tolist()
+        y, out = torch.empty_like(x), st.clone()
+        dx, dst, dw, db = torch.zeros_like(x), torch.zeros_like(st), torch.zeros_like(w), torch.zeros(D, dtype=torch.float64, device=w.device)
+        for k in range(len(at) - 1):
+            lo, hi = at[k], at[k + 1]
+            line = torch.cat([st[k], x[lo:hi]])
+            L = hi - lo
+            out[k] = line[L:]
+            p = sum(w[:, j] * line[j:j + L] for j in range(W)) + bias
+            y[lo:hi] = p * sig(p) if case["silu"] else p
+            if op == "conv_grad":
+                dp = s["dy"][lo:hi].double() * ((sig(p) + p * sig(p) * (1 - sig(p))) if case["silu"] else 1.0)
+                dline = torch.zeros_like(line)
+                dline[L:] += s["dstate"][k].double()
+                for j in range(W):
+                    dline[j:j + L] += dp * w[:, j]
+                    dw[:, j] += (dp * line[j:j + L]).sum(0)
+                db += dp.sum(0)
+                dst[k], dx[lo:hi] = dline[:W - 1], dline[W - 1:]
+        return (y, out) if op == "conv" else (dx, dw, db if case["bias"] else None, dst)
+    if T * D * case["N"] > 700_000_000:
+        return None
+    N, G, A = case["N"], case["G"], s["A"].double()
+    u, z, Dk = _restored(s, "u"), _restored(s, "z"), s["D"].double()
+    pre = s["dt"].double() + (s["dt_bias"].double() if s["dt_bias"] is not None else 0.0)
+    delta = torch.log1p(torch.exp(-pre.abs())) + pre.clamp(min=0) if case["softplus"] else pre
+    of = torch.arange(D, device=u.device) // (D // G)
+    B, C = s["B"].double(), s["C"].double()
+    gate = z * sig(z) if z is not None else None
+    st = s["state"].double()
+    if op == "scan_step":
+        y = torch.empty(T, D, dtype=torch.float64, device=u.device)
+        for r, k in enumerate(s["slots"].tolist()):
+            st[k] = torch.exp(delta[r, :, None] * A) * st[k] + (delta[r] * u[r])[:, None] * B[r][of]
+            y[r] = (st[k] * C[r][of]).sum(1) + Dk * u[r]
+        return (y * gate if gate is not None else y), st
+    at = s["seq_start"].tolist()
+    v, out = torch.empty(T, D, dtype=torch.float64, device=u.device), st.clone()
+    hs = torch.empty(T, D, N, dtype=torch.float64, device=u.device) if op == "scan_grad" else None
+    for k in range(len(at) - 1):
+        h = st[k]
+        for t in range(at[k], at[k + 1]):
+            h = torch.exp(delta[t, :, None] * A) * h + (delta[t] * u[t])[:, None] * B[t][of]
+            v[t] = (h * C[t][of]).sum(1)
+            if hs is not None:
+                hs[t] = h
+        out[k] = h
+    v += Dk * u
+    if op == "scan":
+        return (v * gate if gate is not None else v), out
+    dy = s["dy"].double()
+    r = dy * gate if gate is not None else dy
+    du, ddelta, dB, dC, dA = torch.empty_like(u), torch.empty_like(u), torch.zeros_like(B), torch.zeros_like(C), torch.zeros_like(A)
+    dst = s["dstate"].double()
+    for k in range(len(at) - 1):
+        q = dst[k]
+        for t in range(at[k + 1] - 1, at[k] - 1, -1):
+            before = hs[t - 1] if t > at[k] else st[k]
+            a = torch.exp(delta[t, :, None] * A)
+            q = q + r[t][:, None] * C[t][of]
+            dC[t] = (r[t][:, None] * hs[t]).view(G, D // G, N).sum(1)
+            dB[t] = (q * (delta[t] * u[t])[:, None]).view(G, D // G, N).sum(1)
+            qb = (q * B[t][of]).sum(1)
+            du[t] = qb * delta[t]
+            dA += q * a * before * delta[t][:, None]
+            ddelta[t] = (q * a * before * A).sum(1) + qb * u[t]
+            q = q * a
+        dst[k] = q
+    ddt = ddelta * sig(pre) if case["softplus"] else ddelta
+    dz = dy * v * (sig(z) + z * sig(z) * (1 - sig(z))) if z is not None else None
+    return dict(u=du + r * Dk, dt=ddt, A=dA, B=dB, C=dC, D=(r * u).sum(0), z=dz, dt_bias=ddt.sum(0) if s["dt_bias"] is not None else None, state=dst)
