@@ -201,8 +201,26 @@ def ensure_built(force: bool = False) -> str:
     return want
 
 
+def _share_hip_runtime():
+    """PyTorch-ROCm wheels carry a HIP runtime of their own beside the system's.  A process that maps both gives the device to the
+    one that is initialised first; the other then reports "no ROCm-capable device".  So the runtime PyTorch will use is mapped before
+    libcrnn_hip.so asks for one (same SONAME: the loader takes the copy that is there), without importing torch.  Streams and device
+    pointers then mean the same thing on both sides.  Without torch, or with one that uses the system's runtime, nothing happens."""
+    import importlib.util
+    try:
+        spec = importlib.util.find_spec("torch")
+    except (ImportError, ValueError):
+        spec = None
+    for root in (spec.submodule_search_locations or []) if spec else []:
+        path = os.path.join(root, "lib", "libamdhip64.so")
+        if os.path.exists(path):
+            C.CDLL(path, mode=C.RTLD_GLOBAL)
+            return
+
+
 def _load():
     want = None if _OVERRIDE else ensure_built()      # an explicit CRNN_HIP_LIB is the caller's responsibility
+    _share_hip_runtime()
     lib = C.CDLL(LIB_PATH)
     for name, (res, args) in SYMBOLS.items():
         fn = getattr(lib, name)  # AttributeError if the library does not export a declared symbol
