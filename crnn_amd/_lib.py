@@ -68,6 +68,38 @@ class OptConfig(C.Structure):
                 ("beta2", C.c_double), ("wd", C.c_double), ("grad_clip_norm", C.c_double)]
 
 
+DT_F32, DT_BF16, DT_F16, DT_F64, DT_PACKED8 = 0, 1, 2, 3, 4
+SEQ_MAX_STATES, SEQ_MAX_TAPS = 256, 8
+
+
+class View(C.Structure):
+    _fields_ = [("ptr", C.c_void_p), ("scales", C.c_void_p), ("seq_stride", C.c_int64), ("row_stride", C.c_int64),
+                ("scale_seq_stride", C.c_int64), ("scale_row_stride", C.c_int64), ("dtype", C.c_int32), ("reserved", C.c_int32)]
+
+
+class ConvArgs(C.Structure):
+    _fields_ = [("struct_size", C.c_int32), ("device", C.c_int32), ("stream", C.c_void_p),
+                ("n_seq", C.c_int32), ("D", C.c_int32), ("W", C.c_int32), ("silu", C.c_int32), ("rows", C.c_int64),
+                ("seq_start", C.c_void_p), ("seq_len", C.c_void_p), ("dtype", C.c_int32), ("zero_outside", C.c_int32),
+                ("weight", C.c_void_p), ("bias", C.c_void_p), ("x", View), ("y", View), ("state_in", View), ("state_out", View),
+                ("dy", View), ("dx", View), ("dstate_out", View), ("dstate_in", View), ("dweight", C.c_void_p), ("dbias", C.c_void_p),
+                ("slot", C.c_void_p), ("n_slots", C.c_int64), ("workspace", C.c_void_p), ("workspace_bytes", C.c_int64)]
+
+
+class ScanArgs(C.Structure):
+    _fields_ = [("struct_size", C.c_int32), ("device", C.c_int32), ("stream", C.c_void_p),
+                ("n_seq", C.c_int32), ("D", C.c_int32), ("N", C.c_int32), ("G", C.c_int32), ("rows", C.c_int64),
+                ("seq_start", C.c_void_p), ("seq_len", C.c_void_p),
+                ("dtype", C.c_int32), ("zero_outside", C.c_int32), ("softplus", C.c_int32), ("reserved", C.c_int32),
+                ("A", C.c_void_p), ("skip", C.c_void_p), ("dt_bias", C.c_void_p),
+                ("u", View), ("dt", View), ("z", View), ("y", View), ("B", View), ("C", View),
+                ("B_group", C.c_int64), ("B_state", C.c_int64), ("C_group", C.c_int64), ("C_state", C.c_int64),
+                ("state_in", C.c_void_p), ("state_out", C.c_void_p),
+                ("dy", View), ("du", View), ("ddt", View), ("dz", View), ("dB", View), ("dC", View),
+                ("dA", C.c_void_p), ("dskip", C.c_void_p), ("ddt_bias", C.c_void_p), ("dstate_out", C.c_void_p), ("dstate_in", C.c_void_p),
+                ("slot", C.c_void_p), ("n_slots", C.c_int64), ("workspace", C.c_void_p), ("workspace_bytes", C.c_int64)]
+
+
 # every symbol include/crnn_hip.h declares: name -> (restype, argtypes)
 _DP = C.POINTER(C.c_double)
 _IP = C.POINTER(C.c_int32)
@@ -142,6 +174,16 @@ SYMBOLS = {
     "crnn_cathode_get_particles": (C.c_int32, [_CTX, _DP]),
     "crnn_svgd_update": (C.c_int32, [C.c_int32, _DP, _DP, C.c_int64, C.c_int32, C.c_double, C.c_double, _DP,
                                      C.POINTER(C.c_double), _DP, _DP]),
+    "crnn_conv_workspace": (C.c_int64, [C.POINTER(ConvArgs)]),
+    "crnn_conv_forward": (C.c_int32, [C.POINTER(ConvArgs)]),
+    "crnn_conv_backward": (C.c_int32, [C.POINTER(ConvArgs)]),
+    "crnn_conv_step": (C.c_int32, [C.POINTER(ConvArgs)]),
+    "crnn_scan_workspace": (C.c_int64, [C.POINTER(ScanArgs), C.c_int32]),
+    "crnn_scan_forward": (C.c_int32, [C.POINTER(ScanArgs)]),
+    "crnn_scan_backward": (C.c_int32, [C.POINTER(ScanArgs)]),
+    "crnn_scan_step": (C.c_int32, [C.POINTER(ScanArgs)]),
+    "crnn_pack8": (C.c_int32, [C.c_int32, C.c_void_p, C.POINTER(View), C.c_int64, C.c_int32, C.c_void_p, C.c_void_p]),
+    "crnn_unpack8": (C.c_int32, [C.c_int32, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int64, C.c_int32, C.POINTER(View)]),
 }
 
 

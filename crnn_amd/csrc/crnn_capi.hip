@@ -2762,3 +2762,5 @@ int32_t crnn_svgd_update(int32_t device, const double *p, const double *lnpgrad,
 }
 
 }
+
+#include "seq_capi.hpp"

@@ -1,0 +1,533 @@
+// crnn_amd/csrc/seq_capi.hpp -- the sequence operators' entry points of include/crnn_hip.h (part of crnn_capi.hip's translation unit).
+// Device pointers in and out, everything enqueued on the caller's stream, workspace from the caller: a call may be captured.
+#pragma once
+#include "seq_common.hpp"
+#include "seq_scan_kernel.hpp"
+#include "seq_conv_kernel.hpp"
+#include "seq_pack_kernel.hpp"
+
+namespace {
+
+int32_t sfail(const std::string &msg) {
+    g_last_error = msg;
+    return -1;
+}
+
+// the caller's device for the length of a call
+struct SeqDevice {
+    int prev = -1;
+    bool moved = false;
+    hipError_t enter(int device) {
+        int n = 0;
+        hipError_t e = hipGetDeviceCount(&n);
+        if (e != hipSuccess) return e;
+        if (device < 0 || device >= n) return hipErrorInvalidValue;
+        e = hipGetDevice(&prev);
+        if (e == hipSuccess && prev != device) {
+            e = hipSetDevice(device);
+            moved = e == hipSuccess;
+        }
+        return e;
+    }
+    ~SeqDevice() {
+        if (moved) (void)hipSetDevice(prev);
+    }
+};
+
+int seq_size(int dt) { return dt == CRNN_DT_F64 ? 8 : dt == CRNN_DT_F32 ? 4 : dt == CRNN_DT_PACKED8 ? 1 : 2; }
+
+crnn::SeqV seq_view(const crnn_view &v, int nvec) {
+    crnn::SeqV o{};
+    o.p = v.ptr;
+    o.sc = (const uint8_t *)v.scales;
+    o.bs = v.seq_stride; o.rs = v.row_stride; o.sbs = v.scale_seq_stride; o.srs = v.scale_row_stride;
+    o.dt = v.dtype;
+    const int64_t bytes = (int64_t)nvec * seq_size(v.dtype);
+    o.vec = (uintptr_t)v.ptr % (uintptr_t)bytes == 0 && v.row_stride % nvec == 0 && v.seq_stride % nvec == 0;
+    return o;
+}
+
+struct SeqCheck {
+    const char *who;
+    std::string err;
+    bool bad(const std::string &what) {
+        if (err.empty()) err = std::string(who) + ": " + what;
+        return false;
+    }
+    // a view of the call's type (or, where allowed, a checkpoint); out: rows may not overlap
+    bool view(const crnn_view &v, const char *name, int dtype, bool needed, bool packed_ok, bool out, int64_t width) {
+        if (!v.ptr) return needed ? bad(std::string(name) + " is missing") : true;
+        if (v.dtype == CRNN_DT_PACKED8) {
+            if (!packed_ok || dtype == CRNN_DT_F64) return bad(std::string(name) + " cannot be an 8-bit checkpoint here");
+            if (!v.scales) return bad(std::string(name) + ": a checkpoint needs its scales");
+            if (v.scale_seq_stride < 0 || v.scale_row_stride < 0) return bad(std::string(name) + ": negative stride");
+        } else if (v.dtype != dtype) return bad(std::string(name) + " has another element type than the call");
+        if (v.seq_stride < 0 || v.row_stride < 0) return bad(std::string(name) + ": negative stride");
+        if (out && v.row_stride < width) return bad(std::string(name) + ": rows of an output overlap");
+        return true;
+    }
+};
+
+bool seq_rows_ok(SeqCheck &c, int32_t n_seq, int64_t rows, const int32_t *start, const int32_t *len, int32_t D, int32_t dtype) {
+    if (n_seq < 0 || rows < 0) return c.bad("negative number of sequences or rows");
+    if (rows > 0x7fffffc0LL) return c.bad("more than 2^31 - 64 rows");
+    if (start && len) return c.bad("seq_start and seq_len exclude each other");
+    if (D < 1 || D > (1 << 24)) return c.bad("D must be in 1 .. 2^24");
+    if (dtype < CRNN_DT_F32 || dtype > CRNN_DT_F64) return c.bad("unknown element type");
+    return true;
+}
+
+// chunks of Q rows; Q <= 0: one chunk a sequence
+crnn::SeqMap seq_map(int32_t n_seq, int64_t rows, const int32_t *start, const int32_t *len, int64_t Q) {
+    crnn::SeqMap m{};
+    m.start = start; m.len = len; m.rows = rows; m.n_seq = n_seq;
+    m.Q = Q > 0 ? Q : rows + 1;
+    m.nch = rows > 0 ? (rows + m.Q - 1) / m.Q : 1;
+    m.nblk = start ? rows / m.Q + n_seq : m.nch * n_seq;
+    return m;
+}
+int64_t seq_flat(int32_t n_seq, int64_t rows, bool packed) { return packed ? rows : rows * n_seq; }
+constexpr int64_t kSeqMaxGrid = 0x7fffffff;
+
+#define SEQ_ENTER(a, who)                                                                                                   \
+    if (!(a)) return sfail(who ": null arguments");                                                                          \
+    if ((a)->struct_size != (int32_t)sizeof(*(a))) return sfail(who ": struct_size does not match this library's struct");
+#define SEQ_DEVICE(device, who)                                                                                             \
+    SeqDevice guard;                                                                                                         \
+    {                                                                                                                        \
+        const hipError_t e_ = guard.enter(device);                                                                           \
+        if (e_ != hipSuccess) return sfail(std::string(who ": device: ") + hipGetErrorString(e_));                           \
+    }
+#define SEQ_DONE(who)                                                                                                       \
+    do {                                                                                                                     \
+        const hipError_t e_ = hipGetLastError();                                                                             \
+        if (e_ != hipSuccess) return sfail(std::string(who ": ") + hipGetErrorString(e_));                                   \
+        return 0;                                                                                                            \
+    } while (0)
+
+// ------------------------------------------------------------------ scan
+struct ScanPlan {
+    bool f64, p8, split;
+    int NS, nb;                 // states of a launch, launches over the states
+    int64_t flat;
+    crnn::ScanP p;
+    // workspace, in elements of the compute type
+    int64_t maps, S, G, sdel, part, dA, dD, db, acc, total;
+};
+
+// Rows of a chunk of the forward scan.  Cutting costs a second look at every row (the chunk's end without its past), so it is done only where
+// the sequences and channel tiles alone leave most of the card idle.
+int64_t scan_forward_rows(int64_t flat, int32_t n_seq, int64_t ntile) {
+    const int64_t waves = 4096;                                   // four wavefronts a SIMD
+    if ((int64_t)n_seq * ntile * 4 >= waves) return 0;
+    int64_t q = (flat * ntile + waves - 1) / waves;
+    q = (q + crnn::kScanTB - 1) / crnn::kScanTB * crnn::kScanTB;
+    return q < 4 * crnn::kScanTB ? 4 * crnn::kScanTB : q;
+}
+
+bool scan_plan(SeqCheck &c, const crnn_scan_args *a, bool backward, ScanPlan &s) {
+    if (!seq_rows_ok(c, a->n_seq, a->rows, a->seq_start, a->seq_len, a->D, a->dtype)) return false;
+    if (a->N < 1 || a->N > CRNN_SEQ_MAX_STATES) return c.bad("N must be in 1 .. 256");
+    if (a->G < 1 || a->D % a->G) return c.bad("G must divide D");
+    s.f64 = a->dtype == CRNN_DT_F64;
+    s.p8 = a->u.dtype == CRNN_DT_PACKED8 || (a->z.ptr && a->z.dtype == CRNN_DT_PACKED8);
+    s.NS = s.f64 || a->N <= 8 ? 8 : 16;
+    s.nb = (a->N + s.NS - 1) / s.NS;
+    s.flat = seq_flat(a->n_seq, a->rows, a->seq_start != nullptr);
+    crnn::ScanP &p = s.p;
+    p = crnn::ScanP{};
+    p.D = a->D; p.N = a->N; p.G = a->G; p.Dg = a->D / a->G;
+    p.tpg = (p.Dg + 63) / 64;
+    p.ntile = p.tpg * a->G;
+    const int64_t Q = backward ? crnn::kScanBwdQ : scan_forward_rows(s.flat, a->n_seq, p.ntile);
+    p.m = seq_map(a->n_seq, a->rows, a->seq_start, a->seq_len, Q);
+    s.split = backward || Q > 0;
+    const int64_t blk = p.m.nblk * a->D;
+    if (p.m.nblk * ((p.ntile + crnn::kScanWaves - 1) / crnn::kScanWaves) > kSeqMaxGrid || (int64_t)a->n_seq * s.NS * a->D / 256 >= kSeqMaxGrid)
+        return c.bad("too many sequences, rows and channels for one launch");
+    int64_t at = 0;
+    auto take = [&](int64_t n) { const int64_t o = at; at += (n + 31) / 32 * 32; return o; };
+    s.maps = take(s.flat * a->G * 2 * s.NS);
+    s.S = take(s.split ? blk * s.NS : 0);
+    s.sdel = take(s.split ? blk : 0);
+    s.G = take(backward ? blk * s.NS : 0);
+    s.part = take(backward ? (int64_t)p.ntile * s.flat * 2 * s.NS : 0);
+    s.dA = take(backward ? blk * s.NS : 0);
+    s.dD = take(backward ? blk : 0);
+    s.db = take(backward ? blk : 0);
+    s.acc = take(s.nb > 1 ? s.flat * a->D * (backward ? 3 : 1) : 0);
+    s.total = at * (s.f64 ? 8 : 4);
+    return true;
+}
+
+void scan_fill(const crnn_scan_args *a, ScanPlan &s) {
+    crnn::ScanP &p = s.p;
+    p.u = seq_view(a->u, 4); p.dt = seq_view(a->dt, 4); p.z = seq_view(a->z, 4); p.y = seq_view(a->y, 4);
+    p.dy = seq_view(a->dy, 4); p.du = seq_view(a->du, 4); p.ddt = seq_view(a->ddt, 4); p.dz = seq_view(a->dz, 4);
+    p.A = a->A; p.Dskip = a->skip; p.dt_bias = a->dt_bias;
+    p.state_in = a->state_in; p.state_out = a->state_out; p.dstate_out = a->dstate_out; p.dstate_in = a->dstate_in;
+    p.softplus = a->softplus; p.zero_outside = a->zero_outside;
+    p.acc_n = s.flat;
+}
+crnn::ScanMapsP scan_maps(const crnn_scan_args *a, const ScanPlan &s, const crnn_view &B, const crnn_view &C, int64_t Bg, int64_t Bn, int64_t Cg, int64_t Cn) {
+    crnn::ScanMapsP m{};
+    m.B = seq_view(B, 1); m.C = seq_view(C, 1);
+    m.Bg = Bg; m.Cg = Cg; m.Bn = Bn; m.Cn = Cn;
+    m.rows = s.flat;
+    m.srows = a->seq_start ? 0 : a->rows;
+    m.G = a->G; m.N = a->N;
+    return m;
+}
+
+unsigned seq_grid(int64_t n) { return (unsigned)std::min<int64_t>((n + 255) / 256, 65536); }
+
+template <class CT, int NS, bool P8>
+void scan_forward_run(const crnn_scan_args *a, ScanPlan &s, hipStream_t st) {
+    crnn::ScanP p = s.p;
+    CT *ws = (CT *)a->workspace, *maps = ws + s.maps, *S = ws + s.S, *sdel = ws + s.sdel;
+    p.acc = s.nb > 1 ? ws + s.acc : nullptr;
+    const dim3 grid((unsigned)(p.m.nblk * ((p.ntile + crnn::kScanWaves - 1) / crnn::kScanWaves))), block(64 * crnn::kScanWaves);
+    crnn::ScanMapsP mp = scan_maps(a, s, a->B, a->C, a->B_group, a->B_state, a->C_group, a->C_state);
+    for (int b = 0; b < s.nb; ++b) {
+        p.n0 = mp.n0 = b * NS;
+        p.first = b == 0;
+        p.fin = b == s.nb - 1;
+        if (s.flat > 0) hipLaunchKernelGGL((crnn::seq_scan_maps_kernel<CT, NS>), dim3(seq_grid(s.flat * p.G * 2 * NS)), dim3(256), 0, st, mp, maps);
+        if (s.split) {
+            hipLaunchKernelGGL((crnn::seq_scan_ends_kernel<CT, NS, P8, false>), grid, block, 0, st, p, (const CT *)maps, S, (CT *)nullptr, sdel);
+            hipLaunchKernelGGL((crnn::seq_scan_carry_kernel<CT, NS>), dim3((unsigned)(((int64_t)p.m.n_seq * NS * p.D + 255) / 256)), dim3(256), 0, st, p, S,
+                               (CT *)nullptr, (const CT *)sdel);
+        }
+        hipLaunchKernelGGL((crnn::seq_scan_out_kernel<CT, NS, P8>), grid, block, 0, st, p, (const CT *)maps, (const CT *)(s.split ? S : nullptr));
+    }
+}
+
+template <class CT, int NS, bool P8>
+void scan_backward_run(const crnn_scan_args *a, ScanPlan &s, hipStream_t st) {
+    crnn::ScanP p = s.p;
+    CT *ws = (CT *)a->workspace, *maps = ws + s.maps, *S = ws + s.S, *Gb = ws + s.G, *sdel = ws + s.sdel, *part = ws + s.part, *dA = ws + s.dA, *dD = ws + s.dD,
+       *db = ws + s.db;
+    p.acc = s.nb > 1 ? ws + s.acc : nullptr;
+    const dim3 grid((unsigned)(p.m.nblk * ((p.ntile + crnn::kScanWaves - 1) / crnn::kScanWaves))), block(64 * crnn::kScanWaves);
+    crnn::ScanMapsP mp = scan_maps(a, s, a->B, a->C, a->B_group, a->B_state, a->C_group, a->C_state);
+    crnn::ScanMapsP mo = scan_maps(a, s, a->dB, a->dC, a->N, 1, a->N, 1);
+    const int64_t cA = (int64_t)NS * p.D;
+    for (int b = 0; b < s.nb; ++b) {
+        p.n0 = mp.n0 = mo.n0 = b * NS;
+        p.first = b == 0;
+        p.fin = b == s.nb - 1;
+        if (s.flat > 0) hipLaunchKernelGGL((crnn::seq_scan_maps_kernel<CT, NS>), dim3(seq_grid(s.flat * p.G * 2 * NS)), dim3(256), 0, st, mp, maps);
+        hipLaunchKernelGGL((crnn::seq_scan_ends_kernel<CT, NS, P8, true>), grid, block, 0, st, p, (const CT *)maps, S, Gb, sdel);
+        hipLaunchKernelGGL((crnn::seq_scan_carry_kernel<CT, NS>), dim3((unsigned)(((int64_t)p.m.n_seq * NS * p.D + 255) / 256)), dim3(256), 0, st, p, S, Gb,
+                           (const CT *)sdel);
+        hipLaunchKernelGGL((crnn::seq_scan_bwd_kernel<CT, NS, P8>), grid, block, 0, st, p, (const CT *)maps, (const CT *)S, (const CT *)Gb, part, dA, dD, db);
+        if (s.flat > 0)
+            hipLaunchKernelGGL((crnn::seq_scan_sum_maps_kernel<CT, NS>), dim3(seq_grid(s.flat * p.G * 2 * NS)), dim3(256), 0, st, p.m, mo, (const CT *)part, p.tpg);
+        hipLaunchKernelGGL((crnn::seq_sum_blocks_kernel<CT>), dim3((unsigned)((cA + 255) / 256)), dim3(256), 0, st, (const CT *)dA, p.m.nblk, cA, (CT *)a->dA, p.D, p.N,
+                           p.n0);
+    }
+    const dim3 gd((unsigned)((p.D + 255) / 256));
+    if (a->dskip) hipLaunchKernelGGL((crnn::seq_sum_blocks_kernel<CT>), gd, dim3(256), 0, st, (const CT *)dD, p.m.nblk, (int64_t)p.D, (CT *)a->dskip, p.D, 0, 0);
+    if (a->ddt_bias) hipLaunchKernelGGL((crnn::seq_sum_blocks_kernel<CT>), gd, dim3(256), 0, st, (const CT *)db, p.m.nblk, (int64_t)p.D, (CT *)a->ddt_bias, p.D, 0, 0);
+}
+
+bool scan_views(SeqCheck &c, const crnn_scan_args *a, bool backward) {
+    const int dt = a->dtype;
+    const int64_t D = a->D, GN = (int64_t)a->G * a->N;
+    if (!a->A) return c.bad("A is missing");
+    if (!c.view(a->u, "u", dt, true, true, false, D) || !c.view(a->dt, "dt", dt, true, false, false, D) || !c.view(a->z, "z", dt, false, true, false, D) ||
+        !c.view(a->B, "B", dt, true, false, false, 0) || !c.view(a->C, "C", dt, true, false, false, 0))
+        return false;
+    if (a->B_group < 0 || a->B_state < 0 || a->C_group < 0 || a->C_state < 0) return c.bad("negative stride of B or C");
+    if (!backward) return c.view(a->y, "y", dt, true, false, true, D);
+    if (!a->dA) return c.bad("dA is missing");
+    if ((a->z.ptr != nullptr) != (a->dz.ptr != nullptr)) return c.bad("dz goes with z");
+    return c.view(a->dy, "dy", dt, true, false, false, D) && c.view(a->du, "du", dt, true, false, true, D) && c.view(a->ddt, "ddt", dt, true, false, true, D) &&
+           c.view(a->dz, "dz", dt, false, false, true, D) && c.view(a->dB, "dB", dt, true, false, true, GN) && c.view(a->dC, "dC", dt, true, false, true, GN);
+}
+
+#define SCAN_RUN(run)                                                                                                         \
+    do {                                                                                                                      \
+        const hipStream_t st_ = (hipStream_t)a->stream;                                                                       \
+        if (s.f64) run<double, 8, false>(a, s, st_);                                                                          \
+        else if (s.NS == 8) { if (s.p8) run<float, 8, true>(a, s, st_); else run<float, 8, false>(a, s, st_); }                \
+        else { if (s.p8) run<float, 16, true>(a, s, st_); else run<float, 16, false>(a, s, st_); }                             \
+    } while (0)
+
+// ------------------------------------------------------------------ convolution
+// Rows of a strip: short enough that strips and channels give each SIMD some wavefronts, long enough that the rows read twice (W - 1 a strip;
+// the gradient 2 (W - 1)) stay few.
+int64_t conv_strip(int64_t flat, int32_t D, bool backward) {
+    const int64_t waves = (D + 64 * crnn::kConvV - 1) / (64 * crnn::kConvV);
+    int64_t q = flat * waves / 8192;
+    const int64_t lo = backward ? 16 : 8, hi = backward ? 64 : 32;
+    return q < lo ? lo : q > hi ? hi : q;
+}
+bool conv_check(SeqCheck &c, const crnn_conv_args *a, bool backward, crnn::ConvP &p) {
+    if (!seq_rows_ok(c, a->n_seq, a->rows, a->seq_start, a->seq_len, a->D, a->dtype)) return false;
+    if (a->W < 1 || a->W > CRNN_SEQ_MAX_TAPS) return c.bad("W must be in 1 .. 8");
+    p = crnn::ConvP{};
+    p.D = a->D; p.W = a->W; p.silu = a->silu; p.zero_outside = a->zero_outside;
+    p.m = seq_map(a->n_seq, a->rows, a->seq_start, a->seq_len, conv_strip(seq_flat(a->n_seq, a->rows, a->seq_start != nullptr), a->D, backward));
+    const int64_t gx = (a->D + 64 * crnn::kConvV - 1) / (64 * crnn::kConvV);
+    if ((p.m.nblk + 3) / 4 * gx > kSeqMaxGrid) return c.bad("too many sequences, rows and channels for one launch");
+    return true;
+}
+bool conv_views(SeqCheck &c, const crnn_conv_args *a, bool backward, crnn::ConvP &p) {
+    const int dt = a->dtype;
+    if (!a->weight) return c.bad("weight is missing");
+    if (!c.view(a->x, "x", dt, true, true, false, a->D) || !c.view(a->state_in, "state_in", dt, false, false, false, a->D)) return false;
+    if (backward) {
+        if (!a->dweight) return c.bad("dweight is missing");
+        if (!c.view(a->dy, "dy", dt, true, false, false, a->D) || !c.view(a->dx, "dx", dt, true, false, true, a->D) ||
+            !c.view(a->dstate_out, "dstate_out", dt, false, false, false, a->D) || !c.view(a->dstate_in, "dstate_in", dt, false, false, true, a->D))
+            return false;
+    } else {
+        if (!c.view(a->y, "y", dt, true, false, true, a->D) || !c.view(a->state_out, "state_out", dt, false, false, true, a->D)) return false;
+        if (a->state_out.ptr && a->state_out.ptr == a->state_in.ptr) return c.bad("state_out may not be state_in");
+    }
+    const int V = crnn::kConvV;
+    p.x = seq_view(a->x, V); p.y = seq_view(a->y, V); p.dy = seq_view(a->dy, V); p.dx = seq_view(a->dx, V);
+    p.st_in = seq_view(a->state_in, V); p.st_out = seq_view(a->state_out, V); p.dst_out = seq_view(a->dstate_out, V); p.dst_in = seq_view(a->dstate_in, V);
+    p.w = a->weight; p.bias = a->bias;
+    return true;
+}
+template <int XT, int YT, int WM>
+void conv_launch(const crnn::ConvP &p, bool backward, hipStream_t st) {
+    const int64_t gx = (p.D + 64 * crnn::kConvV - 1) / (64 * crnn::kConvV);
+    const dim3 grid((unsigned)((p.m.nblk + 3) / 4 * gx));
+    if (backward) hipLaunchKernelGGL((crnn::seq_conv_bwd_kernel<XT, YT, WM>), grid, dim3(256), 0, st, p);
+    else hipLaunchKernelGGL((crnn::seq_conv_fwd_kernel<XT, YT, WM>), grid, dim3(256), 0, st, p);
+}
+template <int XT, int YT>
+void conv_launch_w(const crnn::ConvP &p, bool backward, hipStream_t st) {
+    if (p.W <= 4) conv_launch<XT, YT, 4>(p, backward, st);
+    else conv_launch<XT, YT, 8>(p, backward, st);
+}
+void conv_launch_t(const crnn::ConvP &p, int dtype, bool backward, hipStream_t st) {
+    const bool q = p.x.dt == CRNN_DT_PACKED8;
+    if (dtype == CRNN_DT_F64) conv_launch_w<CRNN_DT_F64, CRNN_DT_F64>(p, backward, st);
+    else if (dtype == CRNN_DT_F32) { if (q) conv_launch_w<CRNN_DT_PACKED8, CRNN_DT_F32>(p, backward, st); else conv_launch_w<CRNN_DT_F32, CRNN_DT_F32>(p, backward, st); }
+    else if (dtype == CRNN_DT_BF16) { if (q) conv_launch_w<CRNN_DT_PACKED8, CRNN_DT_BF16>(p, backward, st); else conv_launch_w<CRNN_DT_BF16, CRNN_DT_BF16>(p, backward, st); }
+    else { if (q) conv_launch_w<CRNN_DT_PACKED8, CRNN_DT_F16>(p, backward, st); else conv_launch_w<CRNN_DT_F16, CRNN_DT_F16>(p, backward, st); }
+}
+template <int YT>
+void conv_step_launch(const crnn::ConvStepP &p, hipStream_t st) {
+    const int64_t gx = (p.D + 256 * crnn::kConvV - 1) / (256 * crnn::kConvV);
+    const dim3 grid((unsigned)(p.rows * gx));
+    if (p.W <= 4) hipLaunchKernelGGL((crnn::seq_conv_step_kernel<YT, 4>), grid, dim3(256), 0, st, p);
+    else hipLaunchKernelGGL((crnn::seq_conv_step_kernel<YT, 8>), grid, dim3(256), 0, st, p);
+}
+// weight gradients: the strips' parts [block][W + 1][D], in order and in double -> dweight [D][W], dbias [D]
+template <class CT>
+__global__ __launch_bounds__(256) void seq_conv_sum_kernel(const CT *__restrict__ part, int64_t nblk, int32_t W, int32_t D, CT *__restrict__ dw, CT *__restrict__ db) {
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, count = (int64_t)(W + 1) * D;
+    if (i >= count) return;
+    double s = 0.0;
+    for (int64_t b = 0; b < nblk; ++b) s += (double)part[b * count + i];
+    const int64_t j = i / D, d = i % D;
+    if (j < W) dw[d * W + j] = (CT)s;
+    else if (db) db[d] = (CT)s;
+}
+
+}  // namespace
+
+extern "C" {
+
+int64_t crnn_conv_workspace(const crnn_conv_args *a) {
+    try {
+        SEQ_ENTER(a, "crnn_conv_workspace");
+        SeqCheck c{"crnn_conv_workspace", {}};
+        crnn::ConvP p;
+        if (!conv_check(c, a, true, p)) return sfail(c.err);
+        return p.m.nblk * (a->W + 1) * a->D * (a->dtype == CRNN_DT_F64 ? 8 : 4);
+    } catch (...) { return -1; }
+}
+
+int32_t crnn_conv_forward(const crnn_conv_args *a) {
+    try {
+        SEQ_ENTER(a, "crnn_conv_forward");
+        SeqCheck c{"crnn_conv_forward", {}};
+        crnn::ConvP p;
+        if (!conv_check(c, a, false, p)) return sfail(c.err);
+        if (a->n_seq == 0) return 0;
+        if (!conv_views(c, a, false, p)) return sfail(c.err);
+        SEQ_DEVICE(a->device, "crnn_conv_forward");
+        conv_launch_t(p, a->dtype, false, (hipStream_t)a->stream);
+        SEQ_DONE("crnn_conv_forward");
+    } catch (...) { return -1; }
+}
+
+int32_t crnn_conv_backward(const crnn_conv_args *a) {
+    try {
+        SEQ_ENTER(a, "crnn_conv_backward");
+        SeqCheck c{"crnn_conv_backward", {}};
+        crnn::ConvP p;
+        if (!conv_check(c, a, true, p) || !conv_views(c, a, true, p)) return sfail(c.err);
+        const bool f64 = a->dtype == CRNN_DT_F64;
+        const int64_t need = p.m.nblk * (a->W + 1) * a->D * (f64 ? 8 : 4);
+        if (need > 0 && (!a->workspace || a->workspace_bytes < need)) return sfail("crnn_conv_backward: workspace is missing or too small");
+        SEQ_DEVICE(a->device, "crnn_conv_backward");
+        p.part = a->workspace;
+        const hipStream_t st = (hipStream_t)a->stream;
+        if (a->n_seq > 0) conv_launch_t(p, a->dtype, true, st);
+        const dim3 grid((unsigned)(((int64_t)(a->W + 1) * a->D + 255) / 256));
+        if (f64) hipLaunchKernelGGL((seq_conv_sum_kernel<double>), grid, dim3(256), 0, st, (const double *)p.part, p.m.nblk, a->W, a->D, (double *)a->dweight, (double *)a->dbias);
+        else hipLaunchKernelGGL((seq_conv_sum_kernel<float>), grid, dim3(256), 0, st, (const float *)p.part, p.m.nblk, a->W, a->D, (float *)a->dweight, (float *)a->dbias);
+        SEQ_DONE("crnn_conv_backward");
+    } catch (...) { return -1; }
+}
+
+int32_t crnn_conv_step(const crnn_conv_args *a) {
+    try {
+        SEQ_ENTER(a, "crnn_conv_step");
+        SeqCheck c{"crnn_conv_step", {}};
+        crnn::ConvP q;
+        if (!conv_check(c, a, false, q)) return sfail(c.err);
+        if (a->seq_start || a->seq_len) return sfail("crnn_conv_step: rows are one per sequence (no seq_start, seq_len)");
+        if (a->n_slots < 0 || a->n_slots > 0x7fffffff || (!a->slot && a->n_seq > a->n_slots)) return sfail("crnn_conv_step: n_slots does not fit the rows");
+        if (a->n_seq == 0) return 0;
+        if (!c.view(a->x, "x", a->dtype, true, false, false, a->D) || !c.view(a->y, "y", a->dtype, true, false, true, a->D) ||
+            !c.view(a->state_in, "state_in", a->dtype, a->W > 1 && a->n_slots > 0, false, true, a->D))
+            return sfail(c.err);
+        if (!a->weight) return sfail("crnn_conv_step: weight is missing");
+        if (a->W > 1 && a->n_slots > 1 && a->state_in.seq_stride < (a->W - 1) * a->state_in.row_stride) return sfail("crnn_conv_step: the states of two slots overlap");
+        const int64_t gx = (a->D + 256 * crnn::kConvV - 1) / (256 * crnn::kConvV);
+        if (a->n_seq * gx > kSeqMaxGrid) return sfail("crnn_conv_step: too many rows and channels for one launch");
+        SEQ_DEVICE(a->device, "crnn_conv_step");
+        crnn::ConvStepP p{};
+        p.x = seq_view(a->x, crnn::kConvV); p.y = seq_view(a->y, crnn::kConvV); p.st = seq_view(a->state_in, crnn::kConvV);
+        p.w = a->weight; p.bias = a->bias; p.slot = a->slot; p.rows = a->n_seq; p.n_slots = a->n_slots;
+        p.D = a->D; p.W = a->W; p.silu = a->silu;
+        const hipStream_t st = (hipStream_t)a->stream;
+        if (a->dtype == CRNN_DT_F64) conv_step_launch<CRNN_DT_F64>(p, st);
+        else if (a->dtype == CRNN_DT_F32) conv_step_launch<CRNN_DT_F32>(p, st);
+        else if (a->dtype == CRNN_DT_BF16) conv_step_launch<CRNN_DT_BF16>(p, st);
+        else conv_step_launch<CRNN_DT_F16>(p, st);
+        SEQ_DONE("crnn_conv_step");
+    } catch (...) { return -1; }
+}
+
+int64_t crnn_scan_workspace(const crnn_scan_args *a, int32_t which) {
+    try {
+        SEQ_ENTER(a, "crnn_scan_workspace");
+        if (which < 0 || which > 1) return sfail("crnn_scan_workspace: which must be 0 or 1");
+        SeqCheck c{"crnn_scan_workspace", {}};
+        ScanPlan s;
+        if (!scan_plan(c, a, which == 1, s)) return sfail(c.err);
+        return s.total;
+    } catch (...) { return -1; }
+}
+
+int32_t crnn_scan_forward(const crnn_scan_args *a) {
+    try {
+        SEQ_ENTER(a, "crnn_scan_forward");
+        SeqCheck c{"crnn_scan_forward", {}};
+        ScanPlan s;
+        if (!scan_plan(c, a, false, s)) return sfail(c.err);
+        if (a->n_seq == 0) return 0;
+        if (!scan_views(c, a, false)) return sfail(c.err);
+        if (s.total > 0 && (!a->workspace || a->workspace_bytes < s.total)) return sfail("crnn_scan_forward: workspace is missing or too small");
+        SEQ_DEVICE(a->device, "crnn_scan_forward");
+        scan_fill(a, s);
+        SCAN_RUN(scan_forward_run);
+        SEQ_DONE("crnn_scan_forward");
+    } catch (...) { return -1; }
+}
+
+int32_t crnn_scan_backward(const crnn_scan_args *a) {
+    try {
+        SEQ_ENTER(a, "crnn_scan_backward");
+        SeqCheck c{"crnn_scan_backward", {}};
+        ScanPlan s;
+        if (!scan_plan(c, a, true, s) || !scan_views(c, a, true)) return sfail(c.err);
+        if (s.total > 0 && (!a->workspace || a->workspace_bytes < s.total)) return sfail("crnn_scan_backward: workspace is missing or too small");
+        if (a->n_seq == 0) return sfail("crnn_scan_backward: no sequences");
+        SEQ_DEVICE(a->device, "crnn_scan_backward");
+        scan_fill(a, s);
+        SCAN_RUN(scan_backward_run);
+        SEQ_DONE("crnn_scan_backward");
+    } catch (...) { return -1; }
+}
+
+int32_t crnn_scan_step(const crnn_scan_args *a) {
+    try {
+        SEQ_ENTER(a, "crnn_scan_step");
+        SeqCheck c{"crnn_scan_step", {}};
+        ScanPlan s;
+        if (!scan_plan(c, a, false, s)) return sfail(c.err);
+        if (a->seq_start || a->seq_len) return sfail("crnn_scan_step: rows are one per sequence (no seq_start, seq_len)");
+        if (a->n_slots < 0 || a->n_slots > 0x7fffffff || (!a->slot && a->n_seq > a->n_slots)) return sfail("crnn_scan_step: n_slots does not fit the rows");
+        if (a->n_seq == 0) return 0;
+        if (!scan_views(c, a, false)) return sfail(c.err);
+        if (s.p8) return sfail("crnn_scan_step: u and z cannot be 8-bit checkpoints here");
+        if (!a->state_out && a->n_slots > 0) return sfail("crnn_scan_step: the states are missing");
+        crnn::ScanStepP p{};
+        p.u = seq_view(a->u, 4); p.dt = seq_view(a->dt, 4); p.z = seq_view(a->z, 4); p.y = seq_view(a->y, 4); p.B = seq_view(a->B, 1); p.C = seq_view(a->C, 1);
+        p.Bg = a->B_group; p.Cg = a->C_group; p.Bn = a->B_state; p.Cn = a->C_state;
+        p.A = a->A; p.Dskip = a->skip; p.dt_bias = a->dt_bias; p.state = a->state_out; p.slot = a->slot;
+        p.rows = a->n_seq; p.n_slots = a->n_slots;
+        p.D = a->D; p.N = a->N; p.G = a->G; p.Dg = a->D / a->G; p.softplus = a->softplus;
+        for (p.lpc = 1; p.lpc * 4 < a->N;) p.lpc *= 2;
+        const uintptr_t align = s.f64 ? 32 : 16;
+        p.vec = a->N == 4 * p.lpc && (uintptr_t)a->A % align == 0 && (uintptr_t)a->state_out % align == 0;
+        const int cpb = 256 / p.lpc;
+        const int64_t grid = (int64_t)a->n_seq * ((a->D + cpb - 1) / cpb);
+        if (grid > kSeqMaxGrid) return sfail("crnn_scan_step: too many rows and channels for one launch");
+        SEQ_DEVICE(a->device, "crnn_scan_step");
+        const hipStream_t st = (hipStream_t)a->stream;
+        if (s.f64) hipLaunchKernelGGL((crnn::seq_scan_step_kernel<double>), dim3((unsigned)grid), dim3(256), 0, st, p);
+        else hipLaunchKernelGGL((crnn::seq_scan_step_kernel<float>), dim3((unsigned)grid), dim3(256), 0, st, p);
+        SEQ_DONE("crnn_scan_step");
+    } catch (...) { return -1; }
+}
+
+static bool pack_plan(SeqCheck &c, const crnn_view *x, int64_t rows, int32_t D, const void *codes, const void *scales, bool out, crnn::PackP &p) {
+    if (!x) return c.bad("null view");
+    if (rows < 0 || D < 1 || D > (1 << 24)) return c.bad("bad sizes");
+    if (x->dtype < CRNN_DT_F32 || x->dtype > CRNN_DT_F16) return c.bad("float, bfloat16 or half only");
+    p = crnn::PackP{};
+    p.rows = rows; p.D = D; p.nb = (D + 31) / 32;
+    if (rows == 0) return true;
+    if (!codes || !scales) return c.bad("codes or scales are missing");
+    if (!c.view(*x, "x", x->dtype, true, false, out, D)) return false;
+    p.x = seq_view(*x, 16 / seq_size(x->dtype));
+    p.q = (int8_t *)codes; p.sc = (uint8_t *)scales;
+    p.vecq = (uintptr_t)codes % 16 == 0 && D % 16 == 0;
+    if ((rows * 2 * p.nb + 255) / 256 > kSeqMaxGrid) return c.bad("too many rows and channels for one launch");
+    return true;
+}
+
+int32_t crnn_pack8(int32_t device, void *stream, const crnn_view *x, int64_t rows, int32_t D, void *codes, void *scales) {
+    try {
+        SeqCheck c{"crnn_pack8", {}};
+        crnn::PackP p;
+        if (!pack_plan(c, x, rows, D, codes, scales, false, p)) return sfail(c.err);
+        if (rows == 0) return 0;
+        SEQ_DEVICE(device, "crnn_pack8");
+        const dim3 grid((unsigned)((rows * 2 * p.nb + 255) / 256));
+        const hipStream_t st = (hipStream_t)stream;
+        if (x->dtype == CRNN_DT_F32) hipLaunchKernelGGL((crnn::seq_pack_kernel<CRNN_DT_F32>), grid, dim3(256), 0, st, p);
+        else if (x->dtype == CRNN_DT_BF16) hipLaunchKernelGGL((crnn::seq_pack_kernel<CRNN_DT_BF16>), grid, dim3(256), 0, st, p);
+        else hipLaunchKernelGGL((crnn::seq_pack_kernel<CRNN_DT_F16>), grid, dim3(256), 0, st, p);
+        SEQ_DONE("crnn_pack8");
+    } catch (...) { return -1; }
+}
+
+int32_t crnn_unpack8(int32_t device, void *stream, const void *codes, const void *scales, int64_t rows, int32_t D, const crnn_view *x) {
+    try {
+        SeqCheck c{"crnn_unpack8", {}};
+        crnn::PackP p;
+        if (!pack_plan(c, x, rows, D, codes, scales, true, p)) return sfail(c.err);
+        if (rows == 0) return 0;
+        SEQ_DEVICE(device, "crnn_unpack8");
+        const dim3 grid((unsigned)((rows * 2 * p.nb + 255) / 256));
+        const hipStream_t st = (hipStream_t)stream;
+        if (x->dtype == CRNN_DT_F32) hipLaunchKernelGGL((crnn::seq_unpack_kernel<CRNN_DT_F32>), grid, dim3(256), 0, st, p);
+        else if (x->dtype == CRNN_DT_BF16) hipLaunchKernelGGL((crnn::seq_unpack_kernel<CRNN_DT_BF16>), grid, dim3(256), 0, st, p);
+        else hipLaunchKernelGGL((crnn::seq_unpack_kernel<CRNN_DT_F16>), grid, dim3(256), 0, st, p);
+        SEQ_DONE("crnn_unpack8");
+    } catch (...) { return -1; }
+}
+
+}  // extern "C"

@@ -1,0 +1,288 @@
+// crnn_amd/csrc/seq_common.hpp -- gfx950: what the sequence operators share (causal convolution, selective scan, 8-bit checkpoints):
+// element types, views of caller-owned arrays, the map from a launch's blocks to pieces of sequences.
+//
+// Rows are time, channels run fastest in memory.  A view is addressed by sequence and row: a dense batch has a stride between sequences, a
+// packed one holds all rows in one array and seq_start[s] .. seq_start[s + 1] - 1 are sequence s.  The offsets live on the device and are
+// clamped to the array before use, so that no content of theirs can move an access outside the arrays of the call.
+#pragma once
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "../../include/crnn_hip.h"
+
+namespace crnn {
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr double kLog2eD = 1.4426950408889634;
+
+__device__ __forceinline__ float seq_as_float(uint32_t b) { return __builtin_bit_cast(float, b); }
+__device__ __forceinline__ uint32_t seq_as_bits(float f) { return __builtin_bit_cast(uint32_t, f); }
+// round to nearest even; a NaN stays one
+__device__ __forceinline__ uint16_t seq_to_bf16(float f) {
+#if defined(__HIP_DEVICE_COMPILE__)
+    return __builtin_bit_cast(uint16_t, (__bf16)f);
+#else
+    const uint32_t b = seq_as_bits(f);
+    if ((b & 0x7fffffffu) > 0x7f800000u) return (uint16_t)((b >> 16) | 0x40u);
+    return (uint16_t)((b + 0x7fffu + ((b >> 16) & 1u)) >> 16);
+#endif
+}
+__device__ __forceinline__ uint16_t seq_to_f16(float f) { return __builtin_bit_cast(uint16_t, (_Float16)f); }
+__device__ __forceinline__ float seq_from_f16(uint32_t b) { return (float)__builtin_bit_cast(_Float16, (uint16_t)b); }
+// 2^(byte - 127), byte 255: NaN (E8M0).  byte 0 is the denormal 2^-127.
+__device__ __forceinline__ float seq_scale(uint32_t byte) {
+    return seq_as_float(byte == 255u ? 0x7fc00000u : byte == 0u ? 0x00400000u : byte << 23);
+}
+
+// ---- functions in the compute type.  The float forms use the hardware's exp2 and reciprocal (about one unit in the last place).
+__device__ __forceinline__ float seq_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
+__device__ __forceinline__ double seq_exp2(double x) { return exp2(x); }
+__device__ __forceinline__ float seq_rcp(float x) { return __builtin_amdgcn_rcpf(x); }
+__device__ __forceinline__ double seq_rcp(double x) { return 1.0 / x; }
+__device__ __forceinline__ float seq_fma(float a, float b, float c) { return __builtin_fmaf(a, b, c); }
+__device__ __forceinline__ double seq_fma(double a, double b, double c) { return __builtin_fma(a, b, c); }
+__device__ __forceinline__ float seq_sigmoid(float x) { return seq_rcp(1.0f + seq_exp2(x * -kLog2e)); }
+__device__ __forceinline__ double seq_sigmoid(double x) { return 1.0 / (1.0 + exp(-x)); }
+// log(1 + e^x) = max(x, 0) + log1p(e^-|x|).  log1p(e) = 2 artanh(e / (2 + e)): the small values that step lengths usually have keep their
+// relative accuracy, which log2(1 + e) would lose.  Polynomial in s^2 on [0, 1/9], off by 1e-10 at most.
+__device__ __forceinline__ float seq_softplus(float x) {
+    const float e = seq_exp2(-__builtin_fabsf(x) * kLog2e);
+    const float s = e * seq_rcp(2.0f + e), z = s * s;
+    float p = 0.12204702f;
+    p = seq_fma(p, z, 0.10697134f);
+    p = seq_fma(p, z, 0.14310312f);
+    p = seq_fma(p, z, 0.19999347f);
+    p = seq_fma(p, z, 0.33333340f);
+    p = seq_fma(p, z, 1.0f);
+    return seq_fma(2.0f * s, p, x > 0.0f ? x : (x == x ? 0.0f : x));
+}
+__device__ __forceinline__ double seq_softplus(double x) {
+    return (x > 0.0 ? x : (x == x ? 0.0 : x)) + log1p(exp(-fabs(x)));
+}
+
+// ---- a caller-owned array [sequence][row][channel], channels contiguous
+struct SeqV {
+    void *p;
+    const uint8_t *sc;      // CRNN_DT_PACKED8: one scale byte per 32 channels of a row
+    int64_t bs, rs;         // elements between sequences (dense), between rows
+    int64_t sbs, srs;       // the same of the scales
+    int32_t dt;
+    int32_t vec;            // base and strides allow whole vectors to be loaded and stored (set by the host for the kernel's vector)
+};
+
+struct SeqMap {
+    const int32_t *start;   // packed: [n_seq + 1] first rows; null: dense
+    const int32_t *len;     // dense: rows of each sequence, or null (all of them)
+    int64_t rows;           // packed: rows of the array; dense: rows of a sequence
+    int64_t Q;              // rows of a chunk
+    int64_t nch;            // dense: chunks of a sequence (at least 1)
+    int64_t nblk;           // chunk blocks in all (an upper bound where packed)
+    int32_t n_seq;
+};
+
+// A chunk block b: sequence s, its chunk c.  Packed sequences get their blocks from floor(first row / Q) + s on: sequence s then has at
+// least max(1, ceil(rows / Q)) blocks and none is shared, whatever the lengths are, without a table.
+struct SeqChunk {
+    int64_t begin;          // packed: first row of the sequence in the array; dense: 0
+    int64_t len;            // rows of the sequence
+    int64_t t0;             // first row of the chunk, counted in its sequence
+    int32_t n;              // rows of the chunk (0: an empty sequence's only chunk)
+    int32_t s;
+    bool live, last;
+    int64_t flat;           // begin (packed) or s * rows (dense): row of the sequence's first row in arrays of the operators' own
+};
+
+__device__ __forceinline__ int64_t seq_clamp(int64_t x, int64_t lo, int64_t hi) { return x < lo ? lo : x > hi ? hi : x; }
+
+__device__ __forceinline__ void seq_bounds(const SeqMap &m, int64_t s, int64_t &begin, int64_t &len) {
+    if (m.start) {
+        begin = seq_clamp(m.start[s], 0, m.rows);
+        len = seq_clamp(m.start[s + 1], begin, m.rows) - begin;
+    } else {
+        begin = 0;
+        len = m.len ? seq_clamp(m.len[s], 0, m.rows) : m.rows;
+    }
+}
+
+__device__ __forceinline__ int64_t seq_first_block(const SeqMap &m, int64_t s) {
+    if (!m.start) return s * m.nch;
+    return (int64_t)((uint32_t)seq_clamp(m.start[s], 0, m.rows) / (uint32_t)m.Q) + s;
+}
+
+// all lanes of the wavefront call it with the same b
+__device__ __forceinline__ SeqChunk seq_locate(const SeqMap &m, int64_t b) {
+    SeqChunk k;
+    int64_t s, c;
+    if (!m.start) {
+        s = (int64_t)((uint64_t)b / (uint64_t)m.nch);
+        c = b - s * m.nch;
+        if (s >= m.n_seq) s = -1;
+    } else {
+        const int lane = threadIdx.x & 63;
+        int cnt = 0;
+        for (int i0 = 0; i0 < m.n_seq; i0 += 64) {
+            const int i = i0 + lane;
+            const bool at = i < m.n_seq && seq_first_block(m, i) <= b;
+            cnt += __popcll(__builtin_amdgcn_ballot_w64(at));
+        }
+        s = cnt - 1;
+        c = s >= 0 ? b - seq_first_block(m, s) : 0;
+    }
+    k.live = s >= 0 && c >= 0;
+    k.s = (int32_t)(s >= 0 ? s : 0);
+    k.begin = k.len = 0;
+    if (k.live) seq_bounds(m, s, k.begin, k.len);
+    k.t0 = c * m.Q;
+    k.live = k.live && (k.t0 < k.len || (c == 0 && k.len == 0));
+    const int64_t left = k.len - k.t0;
+    k.n = (int32_t)(k.live ? (left < m.Q ? left : m.Q) : 0);
+    k.last = k.live && k.t0 + m.Q >= k.len;
+    k.flat = m.start ? k.begin : (int64_t)k.s * m.rows;
+    return k;
+}
+
+// element offset of a view's row t of the chunk's sequence
+__device__ __forceinline__ int64_t seq_off(const SeqMap &m, const SeqV &v, const SeqChunk &k, int64_t t) {
+    return (m.start ? k.begin * v.rs : (int64_t)k.s * v.bs) + t * v.rs;
+}
+__device__ __forceinline__ int64_t seq_soff(const SeqMap &m, const SeqV &v, const SeqChunk &k, int64_t t) {
+    return (m.start ? k.begin * v.srs : (int64_t)k.s * v.sbs) + t * v.srs;
+}
+// whether row r of the array (packed: row; dense: s * rows + t) belongs to a sequence
+__device__ __forceinline__ bool seq_inside(const SeqMap &m, int64_t r) {
+    if (m.start) return m.n_seq > 0 && r >= seq_clamp(m.start[0], 0, m.rows) && r < seq_clamp(m.start[m.n_seq], 0, m.rows);
+    if (!m.len) return true;
+    const int64_t s = r / m.rows;
+    return r - s * m.rows < seq_clamp(m.len[s], 0, m.rows);
+}
+
+__device__ __forceinline__ void seq_store(const SeqV &v, int64_t off, float x) {
+    if (v.dt == CRNN_DT_F32) ((float *)v.p)[off] = x;
+    else ((uint16_t *)v.p)[off] = v.dt == CRNN_DT_BF16 ? seq_to_bf16(x) : seq_to_f16(x);
+}
+__device__ __forceinline__ void seq_store(const SeqV &v, int64_t off, double x) { ((double *)v.p)[off] = x; }
+
+__device__ __forceinline__ float seq_load1(const SeqV &v, int64_t off, float) {
+    if (v.dt == CRNN_DT_F32) return ((const float *)v.p)[off];
+    const uint32_t b = ((const uint16_t *)v.p)[off];
+    return v.dt == CRNN_DT_BF16 ? seq_as_float(b << 16) : seq_from_f16(b);
+}
+__device__ __forceinline__ double seq_load1(const SeqV &v, int64_t off, double) { return ((const double *)v.p)[off]; }
+
+// Rows of an output that belong to no sequence become 0 (the caller asked for it by SeqMap-wide flag): block b of the launch takes its
+// share of the array's rows, a lane its channel.
+__device__ __forceinline__ void seq_zero_outside(const SeqMap &m, const SeqV &v, int64_t b, int64_t d, bool valid) {
+    if (!v.p) return;
+    if (m.start) {
+        const int64_t per = (m.rows + m.nblk - 1) / m.nblk;
+        const int64_t lo = b * per, hi = lo + per < m.rows ? lo + per : m.rows;
+        const int64_t first = m.n_seq > 0 ? seq_clamp(m.start[0], 0, m.rows) : m.rows, end = m.n_seq > 0 ? seq_clamp(m.start[m.n_seq], 0, m.rows) : m.rows;
+        if (lo >= first && hi <= end) return;
+        for (int64_t r = lo; r < hi; ++r)
+            if ((r < first || r >= end) && valid) {
+                if (v.dt == CRNN_DT_F64) seq_store(v, r * v.rs + d, 0.0);
+                else seq_store(v, r * v.rs + d, 0.0f);
+            }
+    } else if (m.len) {
+        const int64_t s = b / m.nch, c = b - s * m.nch, n = seq_clamp(m.len[s], 0, m.rows);
+        const int64_t hi = (c + 1) * m.Q < m.rows ? (c + 1) * m.Q : m.rows;
+        for (int64_t r = c * m.Q > n ? c * m.Q : n; r < hi; ++r)
+            if (valid) {
+                if (v.dt == CRNN_DT_F64) seq_store(v, s * v.bs + r * v.rs + d, 0.0);
+                else seq_store(v, s * v.bs + r * v.rs + d, 0.0f);
+            }
+    }
+}
+
+// TB consecutive rows of one channel on their way into registers: the loads of several arrays are issued before the first one is needed,
+// conversion comes afterwards.  The type is the launch's, so each branch is uniform.
+template <class CT, bool P8, int TB>
+struct SeqRows {
+    uint32_t r[TB];
+    uint32_t s[P8 ? TB : 1];
+    __device__ __forceinline__ void load(const SeqMap &m, const SeqV &v, const SeqChunk &k, int64_t t, int64_t d, int n) {
+        const int64_t off = seq_off(m, v, k, t) + d;
+        if (P8 && v.dt == CRNN_DT_PACKED8) {
+            const int64_t so = seq_soff(m, v, k, t) + (d >> 5);
+#pragma unroll
+            for (int i = 0; i < TB; ++i) {
+                const int64_t ii = i < n ? i : n - 1;
+                r[i] = (uint32_t)(int32_t)((const int8_t *)v.p)[off + ii * v.rs];
+                s[P8 ? i : 0] = v.sc[so + ii * v.srs];
+            }
+        } else if (v.dt == CRNN_DT_F32) {
+#pragma unroll
+            for (int i = 0; i < TB; ++i) r[i] = ((const uint32_t *)v.p)[off + (int64_t)(i < n ? i : n - 1) * v.rs];
+        } else {
+#pragma unroll
+            for (int i = 0; i < TB; ++i) r[i] = ((const uint16_t *)v.p)[off + (int64_t)(i < n ? i : n - 1) * v.rs];
+        }
+    }
+    __device__ __forceinline__ void get(const SeqV &v, float (&o)[TB]) const {
+        if (P8 && v.dt == CRNN_DT_PACKED8) {
+#pragma unroll
+            for (int i = 0; i < TB; ++i) o[i] = (float)(int32_t)r[i] * seq_scale(s[P8 ? i : 0]);
+        } else if (v.dt == CRNN_DT_F32) {
+#pragma unroll
+            for (int i = 0; i < TB; ++i) o[i] = seq_as_float(r[i]);
+        } else if (v.dt == CRNN_DT_BF16) {
+#pragma unroll
+            for (int i = 0; i < TB; ++i) o[i] = seq_as_float(r[i] << 16);
+        } else {
+#pragma unroll
+            for (int i = 0; i < TB; ++i) o[i] = seq_from_f16(r[i]);
+        }
+    }
+};
+template <bool P8, int TB>
+struct SeqRows<double, P8, TB> {
+    double r[TB];
+    __device__ __forceinline__ void load(const SeqMap &m, const SeqV &v, const SeqChunk &k, int64_t t, int64_t d, int n) {
+        const int64_t off = seq_off(m, v, k, t) + d;
+#pragma unroll
+        for (int i = 0; i < TB; ++i) r[i] = ((const double *)v.p)[off + (int64_t)(i < n ? i : n - 1) * v.rs];
+    }
+    __device__ __forceinline__ void get(const SeqV &, double (&o)[TB]) const {
+#pragma unroll
+        for (int i = 0; i < TB; ++i) o[i] = r[i];
+    }
+};
+
+// sum over the wavefront's lanes of V values at once: every exchange halves how many values a lane still carries, 2 V lane exchanges
+// in all where separate sums would take 6 V.  Afterwards the lane holds the sum of value seq_spread_index<V>(lane).
+template <int V>
+__device__ __forceinline__ int seq_spread_index(int lane) {
+    int idx = 0, w = V / 2;
+    for (int bit = 32; w >= 1; bit >>= 1, w >>= 1) idx += (lane & bit) ? w : 0;
+    return idx;
+}
+template <int V, class CT>
+__device__ __forceinline__ CT seq_spread_sum(CT (&v)[V]) {
+    const int lane = threadIdx.x & 63;
+    int bit = 32;
+#pragma unroll
+    for (int w = V / 2; w >= 1; w >>= 1) {
+        const bool hi = (lane & bit) != 0;
+#pragma unroll
+        for (int j = 0; j < w; ++j) {
+            const CT send = hi ? v[j] : v[j + w], keep = hi ? v[j + w] : v[j];
+            v[j] = keep + __shfl_xor(send, bit);
+        }
+        bit >>= 1;
+    }
+    for (; bit >= 1; bit >>= 1) v[0] += __shfl_xor(v[0], bit);
+    return v[0];
+}
+
+// Rows of one launch that name the same slot are consecutive rows of that sequence: the first of them in row order does them all.
+// A thread finds for row r whether an earlier row has its slot, and which row is the next.
+__device__ __forceinline__ void seq_same_slot(const int32_t *slot, int64_t rows, int64_t r, int *before, int *next) {
+    const int32_t k = slot[r];
+    for (int64_t j = threadIdx.x; j < rows; j += blockDim.x)
+        if (j != r && slot[j] == k) {
+            if (j < r) atomicMax(before, 1);
+            else atomicMin(next, (int)j);
+        }
+}
+
+}  // namespace crnn

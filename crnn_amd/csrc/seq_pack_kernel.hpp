@@ -1,0 +1,149 @@
+// crnn_amd/csrc/seq_pack_kernel.hpp -- gfx950: activation checkpoints in 8 bits.
+//
+// A row's channels in blocks of 32, one scale 2^e a block (stored e + 127): e = floor(log2 max|x|) - 6, one more where the largest value would
+// round to 128; code = x / 2^e rounded half to even, within +-127.  Scales are powers of two, so that the rounding to a code is the only one:
+// a value comes back within 2^(e - 1), at most max|x| / 128 (the type's largest values, from 127.5 of 128 of its last binade on, within 2^e).  A block that holds an infinity or a NaN, comes back
+// as NaN (scale byte 255).  Reads once, writes 33/32 bytes a value: bound by memory.
+#pragma once
+#include "seq_common.hpp"
+
+namespace crnn {
+
+constexpr int kPackV = 16;      // values of a thread: half a block
+
+struct PackP {
+    SeqV x;                     // source / destination rows
+    int8_t *q;                  // [rows][D]
+    uint8_t *sc;                // [rows][ceil(D / 32)]
+    int64_t rows;
+    int32_t D, nb, vecq;        // vecq: the codes can be stored 16 bytes at a time
+};
+
+template <int DT>
+__device__ __forceinline__ void pack_load(const SeqV &v, int64_t off, int d, int D, float (&o)[kPackV]) {
+    typedef uint32_t U4 __attribute__((ext_vector_type(4)));
+    if (v.vec && d + kPackV <= D) {
+        if (DT == CRNN_DT_F32) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const U4 b = *(const U4 *)((const float *)v.p + off + 4 * k);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) o[4 * k + i] = seq_as_float(b[i]);
+            }
+        } else {
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                const U4 b = *(const U4 *)((const uint16_t *)v.p + off + 8 * k);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    o[8 * k + 2 * i] = DT == CRNN_DT_BF16 ? seq_as_float(b[i] << 16) : seq_from_f16(b[i] & 0xffffu);
+                    o[8 * k + 2 * i + 1] = DT == CRNN_DT_BF16 ? seq_as_float(b[i] & 0xffff0000u) : seq_from_f16(b[i] >> 16);
+                }
+            }
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < kPackV; ++i) o[i] = d + i < D ? seq_load1(v, off + i, 0.0f) : 0.0f;
+    }
+}
+
+// threads along (row, half blocks of the row, an even number of them): a block's two halves are neighbouring lanes
+template <int DT>
+__global__ __launch_bounds__(256) void seq_pack_kernel(const PackP p) {
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    const int64_t r0 = i / (2 * p.nb);
+    const int d = (int)(i - r0 * (2 * p.nb)) * kPackV;
+    const bool in = r0 < p.rows;
+    const int64_t r = in ? r0 : p.rows - 1;
+    float x[kPackV];
+    uint32_t m = 0;                                       // |x| as bits: ordered like the values, NaN above all
+#pragma unroll
+    for (int k = 0; k < kPackV; ++k) x[k] = 0.0f;
+    if (d < p.D) pack_load<DT>(p.x, r * p.x.rs + d, d, p.D, x);
+#pragma unroll
+    for (int k = 0; k < kPackV; ++k) {
+        const uint32_t b = seq_as_bits(x[k]) & 0x7fffffffu;
+        m = b > m ? b : m;
+    }
+    const uint32_t o = (uint32_t)__shfl_xor((int)m, 1);
+    m = o > m ? o : m;
+    uint32_t byte;
+    if (m >= 0x7f800000u) byte = 255u;
+    else {
+        // exponent of the largest value; a mantissa from 1.9921875 = 255/128 on rounds to 128 with 7 bits.  Not in the type's last binade,
+        // where 128 would come back as infinity
+        const int top = DT == CRNN_DT_F16 ? 142 : 254, eb = (int)(m >> 23);
+        int e = eb - 6 + (eb < top && (m & 0x7fffffu) >= 0x7f0000u ? 1 : 0);
+        byte = (uint32_t)(e < 0 ? 0 : e);
+    }
+    const float inv = byte == 255u ? 0.0f : seq_as_float((254u - byte) << 23);    // 2^(127 - byte)
+    uint32_t w[kPackV / 4];
+#pragma unroll
+    for (int k = 0; k < kPackV / 4; ++k) {
+        w[k] = 0;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            int c = byte == 255u ? 0 : (int)__builtin_rintf(x[4 * k + j] * inv);
+            c = c > 127 ? 127 : c < -127 ? -127 : c;
+            w[k] |= ((uint32_t)c & 0xffu) << (8 * j);
+        }
+    }
+    if (!in || d >= p.D) return;
+    int8_t *q = p.q + r * p.D + d;
+    if (p.vecq && d + kPackV <= p.D) {
+        typedef uint32_t U4 __attribute__((ext_vector_type(4)));
+        U4 b;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) b[k] = w[k];
+        *(U4 *)q = b;
+    } else {
+#pragma unroll
+        for (int k = 0; k < kPackV; ++k)
+            if (d + k < p.D) q[k] = (int8_t)(w[k / 4] >> (8 * (k % 4)));
+    }
+    if (!((d / kPackV) & 1)) p.sc[r * p.nb + d / 32] = (uint8_t)byte;
+}
+
+template <int DT>
+__global__ __launch_bounds__(256) void seq_unpack_kernel(const PackP p) {
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    const int64_t r = i / (2 * p.nb);
+    const int d = (int)(i - r * (2 * p.nb)) * kPackV;
+    if (r >= p.rows || d >= p.D) return;
+    const float e = seq_scale(p.sc[r * p.nb + d / 32]);
+    const int8_t *q = p.q + r * p.D + d;
+    const int64_t off = r * p.x.rs + d;
+    typedef uint32_t U4 __attribute__((ext_vector_type(4)));
+    if (p.vecq && p.x.vec && d + kPackV <= p.D) {
+        const U4 b = *(const U4 *)q;
+        float x[kPackV];
+#pragma unroll
+        for (int k = 0; k < kPackV; ++k) x[k] = (float)(int32_t)(int8_t)(b[k / 4] >> (8 * (k % 4))) * e;
+        if (DT == CRNN_DT_F32) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                U4 o;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) o[j] = seq_as_bits(x[4 * k + j]);
+                *(U4 *)((float *)p.x.p + off + 4 * k) = o;
+            }
+        } else {
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                U4 o;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const float lo = x[8 * k + 2 * j], hi = x[8 * k + 2 * j + 1];
+                    o[j] = DT == CRNN_DT_BF16 ? (uint32_t)seq_to_bf16(lo) | (uint32_t)seq_to_bf16(hi) << 16 : (uint32_t)seq_to_f16(lo) | (uint32_t)seq_to_f16(hi) << 16;
+                }
+                *(U4 *)((uint16_t *)p.x.p + off + 8 * k) = o;
+            }
+        }
+    } else {
+#pragma unroll
+        for (int k = 0; k < kPackV; ++k)
+            if (d + k < p.D) seq_store(p.x, off + k, (float)(int32_t)q[k] * e);
+    }
+}
+
+}  // namespace crnn

@@ -1,0 +1,531 @@
+// crnn_amd/csrc/seq_scan_kernel.hpp -- gfx950: the selective state space scan, its discrete adjoint and its single step.
+//
+//     delta = softplus(dt + dt_bias) (or dt + dt_bias)
+//     h[t, d, n] = exp(delta A[d, n]) h[t - 1, d, n] + delta u B[t, g, n],   v[t, d] = sum_n C[t, g, n] h[t, d, n] + D[d] u
+//     y = v, or v z sigmoid(z);   g = d / (channels of a group)
+//
+// the diagonal linear ODE h' = A h + B u stepped exactly over steps of their own length, input held.
+//
+// Split: a lane owns a channel and NS of its states in registers, a wavefront 64 channels of one group, so that B and C of a row are the
+// same for all its lanes and reach the arithmetic as scalar operands (scalar loads from a float copy, seq_scan_maps_kernel).  Per row,
+// channel and state the sweep is one multiplication and one exponential for the decay and three multiply-adds: bound by the vector
+// units, not by memory.  Where sequences and channels do not fill the card, time is cut into chunks: their ends without what came
+// before (mode of seq_scan_ends_kernel), the carry over the chunks of a sequence (seq_scan_carry_kernel: its decay over a chunk is
+// exp(A sum delta)), then the chunks proper.
+#pragma once
+#include "seq_common.hpp"
+
+namespace crnn {
+
+constexpr int kScanTB = 8;      // rows whose loads are in flight together
+constexpr int kScanWaves = 4;   // wavefronts of a block, each on its own channel tile
+
+struct ScanP {
+    SeqMap m;
+    SeqV u, dt, z, y, dy, du, ddt, dz;
+    const void *A, *Dskip, *dt_bias;              // in the compute type
+    const void *state_in, *dstate_out;            // [n_seq][D][N]
+    void *state_out, *dstate_in;
+    void *acc;                                    // N > NS: sums over the states so far, 3 x [rows of all sequences][D]
+    int64_t acc_n;                                // elements of one of them
+    int32_t D, N, G, Dg, tpg, ntile;              // Dg channels and tpg tiles of 64 a group
+    int32_t n0;                                   // first state of this launch
+    int32_t first, fin;                           // first / last launch over the states
+    int32_t softplus, zero_outside;
+};
+
+// ---- B and C of this launch's states in the compute type, [row][group][B: NS | C: NS], 0 behind the last state
+struct ScanMapsP {
+    SeqV B, C;              // rs: elements between rows, group stride below
+    int64_t Bg, Cg;         // elements between groups
+    int64_t Bn, Cn;         // elements between states
+    int64_t rows;           // rows of all sequences
+    int64_t srows;          // dense: rows of a sequence (0: packed)
+    int32_t G, N, n0;
+};
+template <class CT, int NS>
+__global__ __launch_bounds__(256) void seq_scan_maps_kernel(const ScanMapsP p, CT *__restrict__ out) {
+    const int64_t total = p.rows * p.G * 2 * NS;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
+        const int j = (int)(i % (2 * NS));
+        const int64_t rg = i / (2 * NS), g = rg % p.G, r = rg / p.G;
+        const int n = p.n0 + (j % NS);
+        CT x = CT(0);
+        if (n < p.N) {
+            const SeqV &v = j < NS ? p.B : p.C;
+            const int64_t at = p.srows ? (r / p.srows) * v.bs + (r % p.srows) * v.rs : r * v.rs;
+            x = seq_load1(v, at + g * (j < NS ? p.Bg : p.Cg) + n * (j < NS ? p.Bn : p.Cn), CT(0));
+        }
+        out[i] = x;
+    }
+}
+
+// the place of a wavefront: chunk block, channel tile, channel of the lane
+struct ScanAt {
+    SeqChunk k;
+    int64_t b;
+    int32_t tile, g, d;
+    bool on, valid;         // on: the wavefront has a tile; valid: the lane has a channel
+};
+__device__ __forceinline__ ScanAt scan_at(const ScanP &p) {
+    ScanAt a;
+    const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)), lane = threadIdx.x & 63;
+    const int64_t tb = (p.ntile + kScanWaves - 1) / kScanWaves;
+    a.b = (int64_t)blockIdx.x / tb;
+    a.tile = (int32_t)((int64_t)blockIdx.x - a.b * tb) * kScanWaves + wave;
+    a.on = a.tile < p.ntile;
+    const int t = a.on ? a.tile : p.ntile - 1;
+    a.g = t / p.tpg;
+    const int dl = (t - a.g * p.tpg) * 64 + lane;
+    a.valid = a.on && dl < p.Dg;
+    a.d = a.g * p.Dg + (dl < p.Dg ? dl : p.Dg - 1);
+    a.k = seq_locate(p.m, a.b);
+    return a;
+}
+
+template <class CT, int NS>
+__device__ __forceinline__ void scan_rates(const ScanP &p, int d, CT (&A2)[NS]) {
+#pragma unroll
+    for (int n = 0; n < NS; ++n) A2[n] = p.n0 + n < p.N ? ((const CT *)p.A)[(int64_t)d * p.N + p.n0 + n] * CT(kLog2eD) : CT(0);
+}
+template <class CT, int NS>
+__device__ __forceinline__ void scan_state(const ScanP &p, const void *st, int64_t s, int d, CT (&h)[NS]) {
+#pragma unroll
+    for (int n = 0; n < NS; ++n) h[n] = st && p.n0 + n < p.N ? ((const CT *)st)[(s * p.D + d) * p.N + p.n0 + n] : CT(0);
+}
+template <class CT, int NS>
+__device__ __forceinline__ void scan_state_put(const ScanP &p, void *st, int64_t s, int d, const CT (&h)[NS]) {
+#pragma unroll
+    for (int n = 0; n < NS; ++n)
+        if (p.n0 + n < p.N) ((CT *)st)[(s * p.D + d) * p.N + p.n0 + n] = h[n];
+}
+template <class CT>
+__device__ __forceinline__ CT scan_delta(const ScanP &p, CT x, CT bias, CT &pre) {
+    pre = x + bias;
+    return p.softplus ? seq_softplus(pre) : pre;
+}
+
+// ---- forward: outputs of a chunk from its first state (start[block][n][d]; null: one chunk a sequence, from state_in)
+template <class CT, int NS, bool P8>
+__global__ __launch_bounds__(64 * kScanWaves) void seq_scan_out_kernel(const ScanP p, const CT *__restrict__ maps, const CT *__restrict__ start) {
+    const ScanAt a = scan_at(p);
+    if (!a.on) return;
+    if (p.zero_outside && p.fin) seq_zero_outside(p.m, p.y, a.b, a.d, a.valid);
+    if (!a.k.live) return;
+    CT A2[NS], h[NS];
+    scan_rates<CT, NS>(p, a.d, A2);
+    if (start) {
+#pragma unroll
+        for (int n = 0; n < NS; ++n) h[n] = start[(a.b * NS + n) * p.D + a.d];
+    } else {
+        scan_state<CT, NS>(p, p.state_in, a.k.s, a.d, h);
+    }
+    const CT bias = p.dt_bias ? ((const CT *)p.dt_bias)[a.d] : CT(0), skip = p.Dskip ? ((const CT *)p.Dskip)[a.d] : CT(0);
+    SeqRows<CT, P8, kScanTB> ru, rz;
+    SeqRows<CT, false, kScanTB> rd;
+    int t = 0;
+    if (a.k.n > 0) {
+        const int nv = a.k.n < kScanTB ? a.k.n : kScanTB;
+        ru.load(p.m, p.u, a.k, a.k.t0, a.d, nv);
+        rd.load(p.m, p.dt, a.k, a.k.t0, a.d, nv);
+        if (p.z.p && p.fin) rz.load(p.m, p.z, a.k, a.k.t0, a.d, nv);
+    }
+    for (; t < a.k.n; t += kScanTB) {
+        const int nv = a.k.n - t < kScanTB ? a.k.n - t : kScanTB;
+        CT u[kScanTB], x[kScanTB], z[kScanTB];
+        ru.get(p.u, u);
+        rd.get(p.dt, x);
+        if (p.z.p && p.fin) rz.get(p.z, z);
+        const int left = a.k.n - t - kScanTB;
+        if (left > 0) {
+            const int nn = left < kScanTB ? left : kScanTB;
+            ru.load(p.m, p.u, a.k, a.k.t0 + t + kScanTB, a.d, nn);
+            rd.load(p.m, p.dt, a.k, a.k.t0 + t + kScanTB, a.d, nn);
+            if (p.z.p && p.fin) rz.load(p.m, p.z, a.k, a.k.t0 + t + kScanTB, a.d, nn);
+        }
+        const CT *row = maps + ((a.k.flat + a.k.t0 + t) * p.G + a.g) * (2 * NS);
+        const int64_t yo = seq_off(p.m, p.y, a.k, a.k.t0 + t) + a.d, ao = (a.k.flat + a.k.t0 + t) * p.D + a.d;
+#pragma unroll
+        for (int i = 0; i < kScanTB; ++i) {
+            if (i >= nv) break;
+            CT pre;
+            const CT dl = scan_delta(p, x[i], bias, pre), du = dl * u[i];
+            const CT *bc = row + (int64_t)i * p.G * (2 * NS);
+            CT v = CT(0);
+#pragma unroll
+            for (int n = 0; n < NS; ++n) {
+                h[n] = seq_fma(seq_exp2(dl * A2[n]), h[n], du * bc[n]);
+                v = seq_fma(h[n], bc[NS + n], v);
+            }
+            if (p.acc) {
+                CT *acc = (CT *)p.acc + ao + (int64_t)i * p.D;
+                if (!p.first) v += *acc;
+                if (!p.fin && a.valid) *acc = v;
+            }
+            if (p.fin) {
+                v = seq_fma(skip, u[i], v);
+                if (p.z.p) v = v * (z[i] * seq_sigmoid(z[i]));
+                if (a.valid) seq_store(p.y, yo + (int64_t)i * p.y.rs, v);
+            }
+        }
+    }
+    if (a.k.last && p.state_out && a.valid) scan_state_put<CT, NS>(p, p.state_out, a.k.s, a.d, h);
+}
+
+// ---- a chunk by itself: S = its last state from zero, sum of delta; BOTH: also G = what its outputs' gradients r pass back to the state
+// before it, sum_t (prod of the decays up to t) r C -- taken in the forward direction, so that one exponential serves both.
+template <class CT, int NS, bool P8, bool BOTH>
+__global__ __launch_bounds__(64 * kScanWaves) void seq_scan_ends_kernel(const ScanP p, const CT *__restrict__ maps, CT *__restrict__ S, CT *__restrict__ Gb,
+                                                                        CT *__restrict__ sdel) {
+    const ScanAt a = scan_at(p);
+    if (!a.on || !a.k.live) return;
+    CT A2[NS], h[NS], P[BOTH ? NS : 1], g[BOTH ? NS : 1];
+    scan_rates<CT, NS>(p, a.d, A2);
+#pragma unroll
+    for (int n = 0; n < NS; ++n) {
+        h[n] = CT(0);
+        if (BOTH) { P[BOTH ? n : 0] = CT(1); g[BOTH ? n : 0] = CT(0); }
+    }
+    const CT bias = p.dt_bias ? ((const CT *)p.dt_bias)[a.d] : CT(0);
+    CT sd = CT(0);
+    for (int t = 0; t < a.k.n; t += kScanTB) {
+        const int nv = a.k.n - t < kScanTB ? a.k.n - t : kScanTB;
+        SeqRows<CT, P8, kScanTB> ru, rz;
+        SeqRows<CT, false, kScanTB> rd, ry;
+        CT u[kScanTB], x[kScanTB], z[kScanTB], y[kScanTB];
+        ru.load(p.m, p.u, a.k, a.k.t0 + t, a.d, nv);
+        rd.load(p.m, p.dt, a.k, a.k.t0 + t, a.d, nv);
+        if (BOTH) {
+            ry.load(p.m, p.dy, a.k, a.k.t0 + t, a.d, nv);
+            if (p.z.p) rz.load(p.m, p.z, a.k, a.k.t0 + t, a.d, nv);
+        }
+        ru.get(p.u, u);
+        rd.get(p.dt, x);
+        if (BOTH) {
+            ry.get(p.dy, y);
+            if (p.z.p) rz.get(p.z, z);
+        }
+        const CT *row = maps + ((a.k.flat + a.k.t0 + t) * p.G + a.g) * (2 * NS);
+#pragma unroll
+        for (int i = 0; i < kScanTB; ++i) {
+            if (i >= nv) break;
+            CT pre;
+            const CT dl = scan_delta(p, x[i], bias, pre), du = dl * u[i];
+            sd += dl;
+            const CT *bc = row + (int64_t)i * p.G * (2 * NS);
+            CT r = CT(0);
+            if (BOTH) r = p.z.p ? y[i] * (z[i] * seq_sigmoid(z[i])) : y[i];
+#pragma unroll
+            for (int n = 0; n < NS; ++n) {
+                const CT e = seq_exp2(dl * A2[n]);
+                h[n] = seq_fma(e, h[n], du * bc[n]);
+                if (BOTH) {
+                    P[BOTH ? n : 0] *= e;
+                    g[BOTH ? n : 0] = seq_fma(P[BOTH ? n : 0], r * bc[NS + n], g[BOTH ? n : 0]);
+                }
+            }
+        }
+    }
+    if (!a.valid) return;
+#pragma unroll
+    for (int n = 0; n < NS; ++n) {
+        S[(a.b * NS + n) * p.D + a.d] = h[n];
+        if (BOTH) Gb[(a.b * NS + n) * p.D + a.d] = g[BOTH ? n : 0];
+    }
+    sdel[a.b * p.D + a.d] = sd;
+}
+
+// ---- carry over the chunks of a sequence: S becomes each chunk's first state, G (may be null) what reaches each chunk's last state from
+// the rows behind it.  A thread per (sequence, state, channel).
+template <class CT, int NS>
+__global__ __launch_bounds__(256) void seq_scan_carry_kernel(const ScanP p, CT *__restrict__ S, CT *__restrict__ Gb, const CT *__restrict__ sdel) {
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, per = (int64_t)NS * p.D;
+    if (i >= per * p.m.n_seq) return;
+    const int64_t s = i / per;
+    const int n = (int)((i - s * per) / p.D), d = (int)(i % p.D);
+    if (p.n0 + n >= p.N) return;      // behind the last state S and G are 0 and stay so
+    int64_t begin, len;
+    seq_bounds(p.m, s, begin, len);
+    const int64_t b0 = seq_first_block(p.m, s), nc = len > 0 ? (len + p.m.Q - 1) / p.m.Q : 1;
+    const int64_t at = (s * p.D + d) * p.N + p.n0 + n;
+    const CT A2 = ((const CT *)p.A)[(int64_t)d * p.N + p.n0 + n] * CT(kLog2eD);
+    CT h = p.state_in ? ((const CT *)p.state_in)[at] : CT(0);
+    for (int64_t c = 0; c < nc; ++c) {
+        const int64_t o = ((b0 + c) * NS + n) * p.D + d;
+        const CT own = S[o];
+        S[o] = h;
+        h = seq_fma(seq_exp2(A2 * sdel[(b0 + c) * p.D + d]), h, own);
+    }
+    if (!Gb) return;
+    CT q = p.dstate_out ? ((const CT *)p.dstate_out)[at] : CT(0);
+    for (int64_t c = nc - 1; c >= 0; --c) {
+        const int64_t o = ((b0 + c) * NS + n) * p.D + d;
+        const CT own = Gb[o];
+        Gb[o] = q;
+        if (len > 0) q = seq_fma(seq_exp2(A2 * sdel[(b0 + c) * p.D + d]), q, own);
+    }
+    if (p.dstate_in) ((CT *)p.dstate_in)[at] = q;
+}
+
+// ---- adjoint of a chunk of at most kScanBwdQ rows.  Forward over the chunk once, keeping every kScanTB-th state in LDS; then, from the
+// last kScanTB rows to the first: the states of those rows once more, a h[t - 1] of each row kept in registers (NS x kScanTB of them;
+// h[t] is one multiply-add away, and dA needs the product itself), and the reverse sweep over them.  dB and dC are sums over channels: a
+// wavefront's part goes to part[tile][row][B: NS | C: NS], summed over the tiles in a fixed order by seq_scan_sum_maps_kernel.
+constexpr int kScanBwdQ = 4 * kScanTB;
+template <class CT, int NS, bool P8>
+__global__ __launch_bounds__(64 * kScanWaves) void seq_scan_bwd_kernel(const ScanP p, const CT *__restrict__ maps, const CT *__restrict__ start,
+                                                                       const CT *__restrict__ back, CT *__restrict__ part, CT *__restrict__ dApart,
+                                                                       CT *__restrict__ dDpart, CT *__restrict__ dbpart) {
+    constexpr int TB = kScanTB, NSUB = kScanBwdQ / kScanTB;
+    __shared__ CT keep[kScanWaves][NSUB - 1][NS][64];
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    const ScanAt a = scan_at(p);
+    if (!a.on) return;
+    if (p.zero_outside && p.fin) {
+        seq_zero_outside(p.m, p.du, a.b, a.d, a.valid);
+        seq_zero_outside(p.m, p.ddt, a.b, a.d, a.valid);
+        seq_zero_outside(p.m, p.dz, a.b, a.d, a.valid);
+    }
+    CT dA[NS], dD = CT(0), db = CT(0);
+#pragma unroll
+    for (int n = 0; n < NS; ++n) dA[n] = CT(0);
+    if (a.k.live && a.k.n > 0) {
+        CT A2[NS], h[NS], q[NS];
+        scan_rates<CT, NS>(p, a.d, A2);
+#pragma unroll
+        for (int n = 0; n < NS; ++n) {
+            h[n] = start[(a.b * NS + n) * p.D + a.d];
+            q[n] = back[(a.b * NS + n) * p.D + a.d];
+        }
+        const CT bias = p.dt_bias ? ((const CT *)p.dt_bias)[a.d] : CT(0), skip = p.Dskip ? ((const CT *)p.Dskip)[a.d] : CT(0);
+        const int nsub = (a.k.n + TB - 1) / TB;
+        for (int k = 0; k < nsub - 1; ++k) {
+            SeqRows<CT, P8, TB> ru;
+            SeqRows<CT, false, TB> rd;
+            CT u[TB], x[TB];
+            ru.load(p.m, p.u, a.k, a.k.t0 + k * TB, a.d, TB);
+            rd.load(p.m, p.dt, a.k, a.k.t0 + k * TB, a.d, TB);
+            ru.get(p.u, u);
+            rd.get(p.dt, x);
+            const CT *row = maps + ((a.k.flat + a.k.t0 + k * TB) * p.G + a.g) * (2 * NS);
+#pragma unroll
+            for (int i = 0; i < TB; ++i) {
+                CT pre;
+                const CT dl = scan_delta(p, x[i], bias, pre), du = dl * u[i];
+                const CT *bc = row + (int64_t)i * p.G * (2 * NS);
+#pragma unroll
+                for (int n = 0; n < NS; ++n) h[n] = seq_fma(seq_exp2(dl * A2[n]), h[n], du * bc[n]);
+            }
+#pragma unroll
+            for (int n = 0; n < NS; ++n) keep[wave][k][n][lane] = h[n];
+        }
+        for (int k = nsub - 1; k >= 0; --k) {
+            const int nv = a.k.n - k * TB < TB ? a.k.n - k * TB : TB;
+            const int64_t t = a.k.t0 + k * TB;
+            SeqRows<CT, P8, TB> ru, rz;
+            SeqRows<CT, false, TB> rd, ry;
+            CT u[TB], x[TB], z[TB], y[TB], ah[TB][NS];
+            ru.load(p.m, p.u, a.k, t, a.d, nv);
+            rd.load(p.m, p.dt, a.k, t, a.d, nv);
+            ry.load(p.m, p.dy, a.k, t, a.d, nv);
+            if (p.z.p) rz.load(p.m, p.z, a.k, t, a.d, nv);
+#pragma unroll
+            for (int n = 0; n < NS; ++n) h[n] = k ? keep[wave][k - 1][n][lane] : start[(a.b * NS + n) * p.D + a.d];
+            ru.get(p.u, u);
+            rd.get(p.dt, x);
+            ry.get(p.dy, y);
+            if (p.z.p) rz.get(p.z, z);
+            const int64_t frow = a.k.flat + t;
+            const CT *row = maps + (frow * p.G + a.g) * (2 * NS);
+#pragma unroll
+            for (int i = 0; i < TB; ++i) {
+                if (i >= nv) break;
+                CT pre;
+                const CT dl = scan_delta(p, x[i], bias, pre), du = dl * u[i];
+                const CT *bc = row + (int64_t)i * p.G * (2 * NS);
+#pragma unroll
+                for (int n = 0; n < NS; ++n) {
+                    ah[i][n] = seq_exp2(dl * A2[n]) * h[n];
+                    h[n] = seq_fma(du, bc[n], ah[i][n]);
+                }
+            }
+            const int64_t uo = seq_off(p.m, p.du, a.k, t) + a.d, to = seq_off(p.m, p.ddt, a.k, t) + a.d, zo = p.dz.p ? seq_off(p.m, p.dz, a.k, t) + a.d : 0;
+#pragma unroll
+            for (int i = TB - 1; i >= 0; --i) {
+                if (i >= nv) continue;
+                CT pre;
+                const CT dl = scan_delta(p, x[i], bias, pre), du = dl * u[i];
+                const CT sg = p.z.p ? seq_sigmoid(z[i]) : CT(1);
+                const CT r = p.z.p ? y[i] * (z[i] * sg) : y[i];
+                const CT *bc = row + (int64_t)i * p.G * (2 * NS);
+                CT v = CT(0), qb = CT(0), qa = CT(0), w[2 * NS];
+#pragma unroll
+                for (int n = 0; n < NS; ++n) {
+                    const CT hn = seq_fma(du, bc[n], ah[i][n]);
+                    q[n] = seq_fma(r, bc[NS + n], q[n]);
+                    v = seq_fma(hn, bc[NS + n], v);
+                    qb = seq_fma(q[n], bc[n], qb);
+                    const CT m = q[n] * ah[i][n];
+                    qa = seq_fma(m, A2[n], qa);
+                    dA[n] = seq_fma(m, dl, dA[n]);
+                    w[n] = a.valid ? q[n] * du : CT(0);
+                    w[NS + n] = a.valid ? r * hn : CT(0);
+                    q[n] *= seq_exp2(dl * A2[n]);
+                }
+                const CT sum = seq_spread_sum<2 * NS>(w);
+                if ((lane & (64 / (2 * NS) - 1)) == 0)
+                    part[((int64_t)a.tile * p.acc_n + frow + i) * (2 * NS) + seq_spread_index<2 * NS>(lane)] = sum;
+                if (p.acc) {
+                    CT *acc = (CT *)p.acc + (frow + i) * p.D + a.d;
+                    const int64_t stride = p.acc_n * p.D;
+                    if (!p.first) { v += acc[0]; qb += acc[stride]; qa += acc[2 * stride]; }
+                    if (!p.fin && a.valid) { acc[0] = v; acc[stride] = qb; acc[2 * stride] = qa; }
+                }
+                if (p.fin) {
+                    CT ddt = seq_fma(qa, CT(0.6931471805599453), qb * u[i]);
+                    if (p.softplus) ddt *= seq_sigmoid(pre);
+                    dD = seq_fma(r, u[i], dD);
+                    db += ddt;
+                    if (a.valid) {
+                        seq_store(p.du, uo + (int64_t)i * p.du.rs, seq_fma(dl, qb, r * skip));
+                        seq_store(p.ddt, to + (int64_t)i * p.ddt.rs, ddt);
+                        if (p.dz.p) seq_store(p.dz, zo + (int64_t)i * p.dz.rs, y[i] * seq_fma(skip, u[i], v) * (sg * seq_fma(z[i], CT(1) - sg, CT(1))));
+                    }
+                }
+            }
+        }
+    }
+    if (!a.valid) return;
+#pragma unroll
+    for (int n = 0; n < NS; ++n) dApart[(a.b * NS + n) * p.D + a.d] = dA[n];
+    if (p.fin) {
+        dDpart[a.b * p.D + a.d] = dD;
+        dbpart[a.b * p.D + a.d] = db;
+    }
+}
+
+// ---- dB, dC: the tiles of a group in order.  dst: views like B and C.
+template <class CT, int NS>
+__global__ __launch_bounds__(256) void seq_scan_sum_maps_kernel(const SeqMap m, const ScanMapsP p, const CT *__restrict__ part, int32_t tpg) {
+    const int64_t total = p.rows * p.G * 2 * NS;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
+        const int j = (int)(i % (2 * NS));
+        const int64_t rg = i / (2 * NS), g = rg % p.G, r = rg / p.G;
+        const int n = p.n0 + (j % NS);
+        if (n >= p.N) continue;
+        CT sum = CT(0);
+        if (seq_inside(m, r))
+            for (int k = 0; k < tpg; ++k) sum += part[((g * tpg + k) * p.rows + r) * (2 * NS) + j];
+        const SeqV &v = j < NS ? p.B : p.C;
+        const int64_t at = p.srows ? (r / p.srows) * v.bs + (r % p.srows) * v.rs : r * v.rs;
+        seq_store(v, at + g * (j < NS ? p.Bg : p.Cg) + n * (j < NS ? p.Bn : p.Cn), sum);
+    }
+}
+
+// ---- sums over the chunk blocks, in order and in double: in[block][count] -> out.  transposed: count = NS x D, out[d][N] at n0
+template <class CT>
+__global__ __launch_bounds__(256) void seq_sum_blocks_kernel(const CT *__restrict__ in, int64_t nblk, int64_t count, CT *__restrict__ out, int32_t D, int32_t N, int32_t n0) {
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (i >= count) return;
+    double s = 0.0;
+    for (int64_t b = 0; b < nblk; ++b) s += (double)in[b * count + i];
+    if (N <= 0) { out[i] = (CT)s; return; }
+    const int64_t n = n0 + i / D, d = i % D;
+    if (n < N) out[d * N + n] = (CT)s;
+}
+
+// ---- one row for each of many running sequences, states updated in place.  LPC lanes share a channel, four states each (16-byte loads of
+// the state where its rows are so aligned), so that a wavefront's state accesses are contiguous: the step is bound by them.
+struct ScanStepP {
+    SeqV u, dt, z, y, B, C;             // rs: between rows
+    int64_t Bg, Cg, Bn, Cn;
+    const void *A, *Dskip, *dt_bias;
+    void *state;                        // [n_slots][D][N]
+    const int32_t *slot;                // null: row r has slot r
+    int64_t rows, n_slots;
+    int32_t D, N, G, Dg, softplus, lpc, vec;
+};
+template <class CT>
+__global__ __launch_bounds__(256) void seq_scan_step_kernel(const ScanStepP p) {
+    __shared__ int before, next;
+    const int cpb = 256 / p.lpc, sub = threadIdx.x % p.lpc, dl = threadIdx.x / p.lpc;
+    const int64_t cb = (p.D + cpb - 1) / cpb;
+    int64_t r = (int64_t)blockIdx.x / cb;
+    const int d0 = (int)((int64_t)blockIdx.x - r * cb) * cpb + dl;
+    const bool valid = d0 < p.D;
+    const int d = valid ? d0 : p.D - 1;
+    const int64_t slot = p.slot ? p.slot[r] : r;
+    const bool there = slot >= 0 && slot < p.n_slots;
+    int64_t nx = -1;
+    if (p.slot && there && p.rows > 1) {
+        if (threadIdx.x == 0) { before = 0; next = 0x7fffffff; }
+        __syncthreads();
+        seq_same_slot(p.slot, p.rows, r, &before, &next);
+        __syncthreads();
+        if (before) return;
+        nx = next == 0x7fffffff ? -1 : next;
+    }
+    if (!there) {
+        if (valid && sub == 0) seq_store(p.y, r * p.y.rs + d, CT(0));
+        return;
+    }
+    const int n0 = sub * 4, g = d / p.Dg;
+    CT A2[4], h[4];
+    CT *st = (CT *)p.state + (slot * p.D + d) * p.N + n0;
+    typedef CT V4 __attribute__((ext_vector_type(4)));
+    if (p.vec) {
+        const V4 a = *(const V4 *)((const CT *)p.A + (int64_t)d * p.N + n0), s = *(const V4 *)st;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) { A2[i] = a[i] * CT(kLog2eD); h[i] = s[i]; }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const bool in = n0 + i < p.N;
+            A2[i] = in ? ((const CT *)p.A)[(int64_t)d * p.N + n0 + i] * CT(kLog2eD) : CT(0);
+            h[i] = in ? st[i] : CT(0);
+        }
+    }
+    const CT bias = p.dt_bias ? ((const CT *)p.dt_bias)[d] : CT(0), skip = p.Dskip ? ((const CT *)p.Dskip)[d] : CT(0);
+    for (;;) {
+        const CT u = seq_load1(p.u, r * p.u.rs + d, CT(0)), pre = seq_load1(p.dt, r * p.dt.rs + d, CT(0)) + bias;
+        const CT dl = p.softplus ? seq_softplus(pre) : pre, du = dl * u;
+        CT v = CT(0);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int n = n0 + i;
+            if (n < p.N) {
+                const CT b = seq_load1(p.B, r * p.B.rs + g * p.Bg + n * p.Bn, CT(0)), c = seq_load1(p.C, r * p.C.rs + g * p.Cg + n * p.Cn, CT(0));
+                h[i] = seq_fma(seq_exp2(dl * A2[i]), h[i], du * b);
+                v = seq_fma(h[i], c, v);
+            }
+        }
+        for (int x = 1; x < p.lpc; x <<= 1) v += __shfl_xor(v, x);
+        v = seq_fma(skip, u, v);
+        if (p.z.p) {
+            const CT z = seq_load1(p.z, r * p.z.rs + d, CT(0));
+            v = v * (z * seq_sigmoid(z));
+        }
+        if (valid && sub == 0) seq_store(p.y, r * p.y.rs + d, v);
+        if (nx < 0) break;
+        r = nx;
+        __syncthreads();
+        if (threadIdx.x == 0) next = 0x7fffffff;
+        __syncthreads();
+        seq_same_slot(p.slot, p.rows, r, &before, &next);
+        __syncthreads();
+        nx = next == 0x7fffffff ? -1 : next;
+    }
+    if (!valid) return;
+    if (p.vec) {
+        V4 s;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s[i] = h[i];
+        *(V4 *)st = s;
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (n0 + i < p.N) st[i] = h[i];
+    }
+}
+
+}  // namespace crnn

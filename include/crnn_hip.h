@@ -458,6 +458,100 @@ int32_t crnn_cathode_svgd_step(crnn_cathode_ctx *ctx, int32_t i_set, const doubl
                                double *loss_mean, double *h_out, double *ms);
 int32_t crnn_cathode_get_particles(crnn_cathode_ctx *ctx, double *p);
 
+/* ======================================================================== *
+ * Sequence operators: the linear member of the family of ODE models above, at the sizes of sequence models.  A diagonal linear ODE
+ * h' = A h + B(t) u(t) with learned rates, thousands of channels and steps of their own length (an irregular time grid), integrated
+ * exactly (input held over a step), with its discrete adjoint: the selective state space scan.  In front of it a short causal
+ * convolution over time; for training, activation checkpoints in 8 bits, which both gradients read as they are.
+ *
+ * Unlike the entry points above, these take DEVICE pointers and enqueue on the caller's stream: nothing is copied to the host, nothing
+ * is allocated, nothing outlives the call, so that a call may be captured into a graph.  Every struct starts with its own size
+ * (struct_size = sizeof): a binding whose mirror differs is refused.  `device` is the HIP ordinal the pointers belong to (the calling
+ * thread's current device is put back).  Errors: crnn_last_error(NULL).
+ *
+ * Rows.  Time runs over rows, channels are contiguous in memory.  Dense: n_seq sequences of `rows` rows (seq_len, if given, says how
+ * many of them each has; the others are padding).  Packed: seq_start[n_seq + 1] on the device, sequence s is rows seq_start[s] ..
+ * seq_start[s + 1] - 1 of arrays of `rows` rows.  Sequences may be empty.  Offsets and lengths are clamped to the arrays (offsets that
+ * decrease make the sequence empty; what sequences that overlap give is not defined).  Rows of an output that belong to no sequence are
+ * left as they were, or set to 0 where zero_outside is set.
+ * Element types: input, output and state activations of one call share one type (CRNN_DT_F32, _BF16, _F16, _F64); x of the convolution
+ * and u, z of the scan may be checkpoints (_PACKED8) unless the call's type is _F64.  Weights, A, D, biases, scan states and the gradients of
+ * all of these are float (double where the type is _F64); arithmetic is in that type, activations are rounded once, when stored.
+ * ======================================================================== */
+enum { CRNN_DT_F32 = 0, CRNN_DT_BF16 = 1, CRNN_DT_F16 = 2, CRNN_DT_F64 = 3, CRNN_DT_PACKED8 = 4 };
+#define CRNN_SEQ_MAX_STATES 256  /* states per channel of a scan */
+#define CRNN_SEQ_MAX_TAPS 8      /* taps of a convolution */
+/* seq_stride: elements between sequences (dense only), row_stride: between rows.  PACKED8: ptr = int8 codes, scales = a byte per 32 channels,
+ * with their own strides.  ptr NULL: absent. */
+typedef struct crnn_view {
+    void *ptr;
+    const void *scales;
+    int64_t seq_stride, row_stride, scale_seq_stride, scale_row_stride;
+    int32_t dtype, reserved;
+} crnn_view;
+
+typedef struct crnn_conv_args {
+    int32_t struct_size, device;
+    void *stream;
+    int32_t n_seq, D, W, silu;     /* silu: y = p sigmoid(p) instead of p */
+    int64_t rows;
+    const int32_t *seq_start, *seq_len;
+    int32_t dtype, zero_outside;
+    const void *weight, *bias;     /* [D][W] (the last tap is the row itself), [D] or NULL */
+    crnn_view x, y;
+    crnn_view state_in, state_out; /* [n_seq][W - 1][D] the rows before the first / the last rows; either may be absent */
+    crnn_view dy, dx, dstate_out, dstate_in;   /* backward; both dstates may be absent */
+    void *dweight, *dbias;         /* backward: [D][W], [D] (may be NULL) */
+    const int32_t *slot;           /* step: row r continues the state in slot[r]; NULL: in r */
+    int64_t n_slots;
+    void *workspace;
+    int64_t workspace_bytes;
+} crnn_conv_args;
+/* Bytes of workspace crnn_conv_backward needs (the others need none); -1: bad arguments. */
+int64_t crnn_conv_workspace(const crnn_conv_args *a);
+int32_t crnn_conv_forward(const crnn_conv_args *a);
+/* dx, dweight, dbias, dstate_in from dy and dstate_out (gradient of state_out).  Sums in a fixed order: same inputs, same bits. */
+int32_t crnn_conv_backward(const crnn_conv_args *a);
+/* One row for each of many running sequences: n_seq rows (x, y: row r at r row_stride), state_in = the states [n_slots][W - 1][D], moved up
+ * in place.  slot out of [0, n_slots): the row is padding, its output 0.  Rows that name one slot are consecutive rows of its sequence. */
+int32_t crnn_conv_step(const crnn_conv_args *a);
+
+typedef struct crnn_scan_args {
+    int32_t struct_size, device;
+    void *stream;
+    int32_t n_seq, D, N, G;        /* D channels in G groups of D / G, N states a channel */
+    int64_t rows;
+    const int32_t *seq_start, *seq_len;
+    int32_t dtype, zero_outside, softplus, reserved;
+    const void *A, *skip, *dt_bias;    /* [D][N]; [D] or NULL (0); [D] or NULL (0) */
+    crnn_view u, dt, z, y;             /* z may be absent: no gate */
+    crnn_view B, C;                    /* row [G][N] */
+    int64_t B_group, B_state, C_group, C_state;   /* elements between groups, between states */
+    const void *state_in;              /* [n_seq][D][N] or NULL (0) */
+    void *state_out;                   /* or NULL */
+    crnn_view dy, du, ddt, dz, dB, dC; /* backward; dB, dC [row][G][N] contiguous in states and groups */
+    void *dA, *dskip, *ddt_bias;       /* dskip, ddt_bias may be NULL */
+    const void *dstate_out;            /* gradient of state_out or NULL */
+    void *dstate_in;                   /* or NULL */
+    const int32_t *slot;               /* step */
+    int64_t n_slots;
+    void *workspace;
+    int64_t workspace_bytes;
+} crnn_scan_args;
+/* Bytes of workspace the forward (which = 0) or the backward (1) call needs for these sizes; -1: bad arguments. */
+int64_t crnn_scan_workspace(const crnn_scan_args *a, int32_t which);
+/* delta = softplus(dt + dt_bias) or dt + dt_bias;  h = exp(delta A) h + delta u B;  v = sum_n C h + skip u;  y = v or v z sigmoid(z). */
+int32_t crnn_scan_forward(const crnn_scan_args *a);
+/* Gradients of everything, states re-formed from the inputs.  Sums in a fixed order: same inputs, same bits. */
+int32_t crnn_scan_backward(const crnn_scan_args *a);
+/* One row for each of n_seq running sequences; states state_out [n_slots][D][N] updated in place; slots as in crnn_conv_step. */
+int32_t crnn_scan_step(const crnn_scan_args *a);
+
+/* Checkpoint of x [rows][D] (float, bfloat16 or half; row_stride): codes [rows][D] int8, scales [rows][ceil(D / 32)] bytes e + 127, value = code
+ * 2^e.  Within half a code: at most max|x| / 128 of the 32 channels (within one where max|x| is within 0.4 % of the type's largest).  A block with an infinity or a NaN comes back as NaN. */
+int32_t crnn_pack8(int32_t device, void *stream, const crnn_view *x, int64_t rows, int32_t D, void *codes, void *scales);
+int32_t crnn_unpack8(int32_t device, void *stream, const void *codes, const void *scales, int64_t rows, int32_t D, const crnn_view *x);
+
 #ifdef __cplusplus
 }
 #endif

@@ -501,4 +501,112 @@ function last_chunk_stats(c::Cathode)
     return Tuple(out)
 end
 
+# ---------------------------------------------------------------------------------------------------------------------------
+# Sequence operators (include/crnn_hip.h, last section): device pointers (AMDGPU.jl: `pointer(x)`) on the caller's stream.  Time runs over rows,
+# channels are the fastest index, so a Julia array is [D, rows, n_seq].  Same status as everything above: not executed.
+
+"""`crnn_view`: an array of the caller's on the device; element types 0 Float32, 1 BFloat16, 2 Float16, 3 Float64, 4 an 8-bit checkpoint."""
+Base.@kwdef struct View
+    ptr::Ptr{Cvoid} = C_NULL
+    scales::Ptr{Cvoid} = C_NULL
+    seq_stride::Int64 = 0
+    row_stride::Int64 = 0
+    scale_seq_stride::Int64 = 0
+    scale_row_stride::Int64 = 0
+    dtype::Int32 = 0
+    reserved::Int32 = 0
+end
+
+Base.@kwdef struct ConvArgs
+    struct_size::Int32 = 0
+    device::Int32 = 0
+    stream::Ptr{Cvoid} = C_NULL
+    n_seq::Int32 = 0
+    D::Int32 = 0
+    W::Int32 = 0
+    silu::Int32 = 0
+    rows::Int64 = 0
+    seq_start::Ptr{Cvoid} = C_NULL
+    seq_len::Ptr{Cvoid} = C_NULL
+    dtype::Int32 = 0
+    zero_outside::Int32 = 0
+    weight::Ptr{Cvoid} = C_NULL
+    bias::Ptr{Cvoid} = C_NULL
+    x::View = View()
+    y::View = View()
+    state_in::View = View()
+    state_out::View = View()
+    dy::View = View()
+    dx::View = View()
+    dstate_out::View = View()
+    dstate_in::View = View()
+    dweight::Ptr{Cvoid} = C_NULL
+    dbias::Ptr{Cvoid} = C_NULL
+    slot::Ptr{Cvoid} = C_NULL
+    n_slots::Int64 = 0
+    workspace::Ptr{Cvoid} = C_NULL
+    workspace_bytes::Int64 = 0
+end
+
+Base.@kwdef struct ScanArgs
+    struct_size::Int32 = 0
+    device::Int32 = 0
+    stream::Ptr{Cvoid} = C_NULL
+    n_seq::Int32 = 0
+    D::Int32 = 0
+    N::Int32 = 0
+    G::Int32 = 0
+    rows::Int64 = 0
+    seq_start::Ptr{Cvoid} = C_NULL
+    seq_len::Ptr{Cvoid} = C_NULL
+    dtype::Int32 = 0
+    zero_outside::Int32 = 0
+    softplus::Int32 = 0
+    reserved::Int32 = 0
+    A::Ptr{Cvoid} = C_NULL
+    skip::Ptr{Cvoid} = C_NULL
+    dt_bias::Ptr{Cvoid} = C_NULL
+    u::View = View()
+    dt::View = View()
+    z::View = View()
+    y::View = View()
+    B::View = View()
+    C::View = View()
+    B_group::Int64 = 0
+    B_state::Int64 = 0
+    C_group::Int64 = 0
+    C_state::Int64 = 0
+    state_in::Ptr{Cvoid} = C_NULL
+    state_out::Ptr{Cvoid} = C_NULL
+    dy::View = View()
+    du::View = View()
+    ddt::View = View()
+    dz::View = View()
+    dB::View = View()
+    dC::View = View()
+    dA::Ptr{Cvoid} = C_NULL
+    dskip::Ptr{Cvoid} = C_NULL
+    ddt_bias::Ptr{Cvoid} = C_NULL
+    dstate_out::Ptr{Cvoid} = C_NULL
+    dstate_in::Ptr{Cvoid} = C_NULL
+    slot::Ptr{Cvoid} = C_NULL
+    n_slots::Int64 = 0
+    workspace::Ptr{Cvoid} = C_NULL
+    workspace_bytes::Int64 = 0
+end
+
+"""Set `struct_size = sizeof(ConvArgs)` / `sizeof(ScanArgs)`: the library refuses a mirror of another size."""
+conv_workspace(a::ConvArgs) = ccall((:crnn_conv_workspace, LIB), Int64, (Ref{ConvArgs},), a)
+conv_forward!(a::ConvArgs) = check(ccall((:crnn_conv_forward, LIB), Int32, (Ref{ConvArgs},), a))
+conv_backward!(a::ConvArgs) = check(ccall((:crnn_conv_backward, LIB), Int32, (Ref{ConvArgs},), a))
+conv_step!(a::ConvArgs) = check(ccall((:crnn_conv_step, LIB), Int32, (Ref{ConvArgs},), a))
+scan_workspace(a::ScanArgs, backward::Bool) = ccall((:crnn_scan_workspace, LIB), Int64, (Ref{ScanArgs}, Int32), a, Int32(backward))
+scan_forward!(a::ScanArgs) = check(ccall((:crnn_scan_forward, LIB), Int32, (Ref{ScanArgs},), a))
+scan_backward!(a::ScanArgs) = check(ccall((:crnn_scan_backward, LIB), Int32, (Ref{ScanArgs},), a))
+scan_step!(a::ScanArgs) = check(ccall((:crnn_scan_step, LIB), Int32, (Ref{ScanArgs},), a))
+pack8!(x::View, rows::Integer, D::Integer, codes::Ptr{Cvoid}, scales::Ptr{Cvoid}; device::Integer=0, stream::Ptr{Cvoid}=C_NULL) =
+    check(ccall((:crnn_pack8, LIB), Int32, (Int32, Ptr{Cvoid}, Ref{View}, Int64, Int32, Ptr{Cvoid}, Ptr{Cvoid}), device, stream, x, rows, D, codes, scales))
+unpack8!(codes::Ptr{Cvoid}, scales::Ptr{Cvoid}, rows::Integer, D::Integer, x::View; device::Integer=0, stream::Ptr{Cvoid}=C_NULL) =
+    check(ccall((:crnn_unpack8, LIB), Int32, (Int32, Ptr{Cvoid}, Ptr{Cvoid}, Ptr{Cvoid}, Int64, Int32, Ref{View}), device, stream, codes, scales, rows, D, x))
+
 end # module

@@ -483,6 +483,7 @@ inline double __builtin_amdgcn_rcp(double x) { return 1.0 / x; }
 inline float __builtin_amdgcn_rcpf(float x) { return 1.0f / x; }
 inline double __builtin_amdgcn_rsq(double x) { return 1.0 / std::sqrt(x); }
 #endif
+inline float __builtin_amdgcn_exp2f(float x) { return ::exp2f(x); }
 inline double __ocml_exp_f64(double x) { return std::exp(x); }
 inline double __ocml_log_f64(double x) { return std::log(x); }
 inline long long __double_as_longlong(double x) { long long r; memcpy(&r, &x, 8); return r; }

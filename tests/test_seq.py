@@ -1,0 +1,767 @@
+"""The sequence operators (crnn_amd.seq) against plain implementations in 64 bits: convolution, scan, their gradients and single steps,
+8-bit checkpoints, refusals, and a run of them together.
+
+Tolerances.  A result of type T is rounded once: half a unit, finfo(T).eps / 2 relative to it.  The arithmetic before is in float32 (float64): a
+sum of n products is off by at most about (n + 2) eps / 2 of the sum of their magnitudes, the exponentials and reciprocals by a few eps of
+theirs; a recurrence adds each row's share, weighted by decays below one.  So every result is allowed half a unit of its own type of itself
+plus `k` eps of the compute type of the *scale* it was summed at (the same formula with every term's magnitude, computed beside it), with k
+the number of roundings a term meets: see `check`.  The device tests also run on the emulated device (tests/test_seq_emulated.py).
+"""
+import math
+import os
+import sys
+
+import numpy as np
+import pytest
+
+torch = pytest.importorskip("torch")
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+if ROOT not in sys.path:
+    sys.path.insert(0, ROOT)
+
+from crnn_amd import seq  # noqa: E402
+from crnn_amd import _lib as L  # noqa: E402
+
+DEV = "cpu" if seq._EMULATED else "cuda"
+DT = {"f32": torch.float32, "bf16": torch.bfloat16, "f16": torch.float16, "f64": torch.float64}
+gpu = pytest.mark.gpu
+
+
+def rnd(g, *shape, dtype=torch.float32, scale=1.0):
+    return (torch.randn(*shape, generator=g, dtype=torch.float64) * scale).to(dtype).to(DEV)
+
+
+def param_of(dtype):
+    return torch.float64 if dtype == torch.float64 else torch.float32
+
+
+def check(got, want, scale, k, what):
+    assert got is not None and tuple(got.shape) == tuple(want.shape), (what, None if got is None else got.shape, want.shape)
+    own = torch.finfo(got.dtype)
+    eps = torch.finfo(param_of(got.dtype)).eps
+    g, w, s = got.detach().cpu().double(), want.detach().cpu().double(), scale.detach().cpu().double()
+    # float16 / bfloat16 below the normal range: half the spacing there
+    limit = own.eps / 2 * (w.abs() + k * eps * s) + k * eps * s + own.smallest_normal * own.eps
+    bad = ~((g - w).abs() <= limit)
+    assert not bool(bad.any()), f"{what}: {int(bad.sum())} of {bad.numel()} off, worst {float(((g - w).abs() / limit)[bad].max()):.3g} of the limit"
+
+
+# ---------------------------------------------------------------- plain implementations, float64 on the CPU, sequence by sequence
+def spans(B, Lr, starts=None, lens=None):
+    """[(rows of the flat array)] of the sequences."""
+    if starts is not None:
+        return [(int(a), int(b)) for a, b in zip(starts[:-1], starts[1:])]
+    return [(s * Lr, s * Lr + (Lr if lens is None else int(lens[s]))) for s in range(B)]
+
+
+def sig(x):
+    return 1 / (1 + torch.exp(-x))
+
+
+def plain_conv(x, w, b, silu, spans_, state, dy=None, dstate=None):
+    """x [rows, D]; everything float64.  Returns values, and beside each the scale its terms add up to."""
+    D, W = w.shape
+    bias = torch.zeros(D, dtype=torch.float64) if b is None else b
+    y, ys = torch.zeros_like(x), torch.zeros_like(x)
+    n = len(spans_)
+    st = torch.zeros(n, W - 1, D, dtype=torch.float64) if state is None else state
+    out = torch.zeros(n, W - 1, D, dtype=torch.float64)
+    dx, dxs = torch.zeros_like(x), torch.zeros_like(x)
+    dw, dws, db, dbs = (torch.zeros(D, W, dtype=torch.float64), torch.zeros(D, W, dtype=torch.float64), torch.zeros(D, dtype=torch.float64), torch.zeros(D, dtype=torch.float64))
+    dst, dsts = torch.zeros_like(out), torch.zeros_like(out)
+    for s, (lo, hi) in enumerate(spans_):
+        line = torch.cat([st[s], x[lo:hi]])
+        n_ = hi - lo
+        p = sum((w[:, j] * line[j:j + n_] for j in range(W)), torch.zeros(n_, D, dtype=torch.float64)) + bias
+        ps = sum(((w[:, j] * line[j:j + n_]).abs() for j in range(W)), torch.zeros(n_, D, dtype=torch.float64)) + bias.abs()
+        y[lo:hi] = p * sig(p) if silu else p
+        ys[lo:hi] = ps * (1 + ps) if silu else ps
+        out[s] = line[n_:]
+        if dy is None:
+            continue
+        act = sig(p) * (1 + p * (1 - sig(p))) if silu else torch.ones_like(p)
+        dp, dps = dy[lo:hi] * act, dy[lo:hi].abs() * (1 + ps) ** 2 if silu else dy[lo:hi].abs()
+        dl, dls = torch.zeros_like(line), torch.zeros_like(line)
+        if dstate is not None:
+            dl[n_:] += dstate[s]
+            dls[n_:] += dstate[s].abs()
+        for j in range(W):
+            dl[j:j + n_] += dp * w[:, j]
+            dls[j:j + n_] += dps * w[:, j].abs()
+            dw[:, j] += (dp * line[j:j + n_]).sum(0)
+            dws[:, j] += (dps * line[j:j + n_].abs()).sum(0)
+        db += dp.sum(0)
+        dbs += dps.sum(0)
+        dst[s], dsts[s], dx[lo:hi], dxs[lo:hi] = dl[:W - 1], dls[:W - 1], dl[W - 1:], dls[W - 1:]
+    return dict(y=(y, ys), state=(out, out.abs()), dx=(dx, dxs), dw=(dw, dws), db=(db, dbs), dstate=(dst, dsts))
+
+
+def plain_scan(u, dt, A, B, C, D, z, bias, softplus, spans_, state, dy=None, dstate=None, mag=None):
+    """u, dt, z [rows, D], B, C [rows, G, N]; everything float64.  mag: the scale `state` was summed at, where that is more than its size."""
+    T, Dn = u.shape
+    G, N = B.shape[1:]
+    of = torch.arange(Dn) // (Dn // G)
+    n = len(spans_)
+    pre = dt + (0 if bias is None else bias)
+    dl = torch.clamp(pre, min=0) + torch.log1p(torch.exp(-pre.abs())) if softplus else pre
+    h0 = torch.zeros(n, Dn, N, dtype=torch.float64) if state is None else state
+    gate = z * sig(z) if z is not None else None
+    skip = torch.zeros(Dn, dtype=torch.float64) if D is None else D
+    v, vs = torch.zeros(T, Dn, dtype=torch.float64), torch.zeros(T, Dn, dtype=torch.float64)
+    hs, hm = torch.zeros(T, Dn, N, dtype=torch.float64), torch.zeros(T, Dn, N, dtype=torch.float64)
+    m0 = h0.abs() if mag is None else mag
+    end, ends = h0.clone(), m0.clone()
+    for s, (lo, hi) in enumerate(spans_):
+        h, m = h0[s], m0[s]
+        for t in range(lo, hi):
+            e = dl[t][:, None] * A
+            a = torch.exp(e)
+            x = (dl[t] * u[t])[:, None] * B[t][of]
+            # the exponent's rounding weighs |e|
+            h, m = a * h + x, a * m * (1 + e.abs()) + x.abs()
+            hs[t], hm[t] = h, m
+            v[t] = (h * C[t][of]).sum(1) + skip * u[t]
+            vs[t] = (m * C[t][of].abs()).sum(1) + (skip * u[t]).abs()
+        end[s], ends[s] = h, m
+    y, ys = (v * gate, vs * gate.abs() * (1 + z.abs())) if gate is not None else (v, vs)
+    r = dict(y=(y, ys), state=(end, ends))
+    if dy is None:
+        return r
+    z64 = lambda *s_: torch.zeros(*s_, dtype=torch.float64)  # noqa: E731
+    g = {k: [z64(*sh), z64(*sh)] for k, sh in dict(u=(T, Dn), dt=(T, Dn), A=(Dn, N), B=(T, G, N), C=(T, G, N), D=(Dn,), dt_bias=(Dn,), state=(n, Dn, N)).items()}
+    rr = dy * gate if gate is not None else dy
+    rs = rr.abs() * (1 + z.abs()) if gate is not None else rr.abs()
+    for s, (lo, hi) in enumerate(spans_):
+        q = z64(Dn, N) if dstate is None else dstate[s].clone()
+        qs = q.abs()
+        for t in range(hi - 1, lo - 1, -1):
+            e = dl[t][:, None] * A
+            a = torch.exp(e)
+            hp, hpm = (hs[t - 1], hm[t - 1]) if t > lo else (h0[s], h0[s].abs())
+            Bt, Ct = B[t][of], C[t][of]
+            q, qs = q + rr[t][:, None] * Ct, qs + rs[t][:, None] * Ct.abs()
+            ah, ahm = a * hp, a * hpm * (1 + e.abs())
+            x = (dl[t] * u[t])[:, None]
+            for key, val, mag in (("C", rr[t][:, None] * hs[t], rs[t][:, None] * hm[t]), ("B", q * x, qs * x.abs())):
+                g[key][0][t] = val.view(G, Dn // G, N).sum(1)
+                g[key][1][t] = mag.view(G, Dn // G, N).sum(1)
+            qb, qbs = (q * Bt).sum(1), (qs * Bt.abs()).sum(1)
+            g["u"][0][t], g["u"][1][t] = qb * dl[t] + rr[t] * skip, qbs * dl[t].abs() + rs[t] * skip.abs()
+            g["A"][0] += q * ah * dl[t][:, None]
+            g["A"][1] += qs * ahm * dl[t].abs()[:, None]
+            dd, dds = (q * ah * A).sum(1) + qb * u[t], (qs * ahm * A.abs()).sum(1) + qbs * u[t].abs()
+            if softplus:
+                dd, dds = dd * sig(pre[t]), dds * sig(pre[t]) * (1 + pre[t].abs())
+            g["dt"][0][t], g["dt"][1][t] = dd, dds
+            g["D"][0] += rr[t] * u[t]
+            g["D"][1] += rs[t] * u[t].abs()
+            q, qs = q * a, qs * a * (1 + e.abs())
+        g["state"][0][s], g["state"][1][s] = q, qs
+    g["dt_bias"] = [g["dt"][0].sum(0), g["dt"][1].sum(0)]
+    if z is not None:
+        g["z"] = [dy * v * sig(z) * (1 + z * (1 - sig(z))), dy.abs() * vs * (1 + z.abs())]
+    r["grad"] = g
+    return r
+
+
+def plain_codes(x, top=2.0 ** 127):
+    """One block at a time; (codes, scale bytes).  From `top`, the last binade of the type, on 128 would come back as infinity."""
+    T, D = x.shape
+    nb = -(-D // 32)
+    q, e = np.zeros((T, D), np.int64), np.zeros((T, nb), np.int64)
+    for t in range(T):
+        for k in range(nb):
+            b = x[t, 32 * k:32 * k + 32].double().numpy()
+            if not np.isfinite(b).all():
+                e[t, k] = 255
+                continue
+            m = np.abs(b).max()
+            p = -127 if m == 0 else max(math.frexp(m)[1] - 7, -127)
+            if np.rint(m / 2.0 ** p) > 127 and m < top:
+                p += 1
+            q[t, 32 * k:32 * k + len(b)], e[t, k] = np.clip(np.rint(b / 2.0 ** p), -127, 127), p + 127
+    return torch.from_numpy(q).to(torch.int8), torch.from_numpy(e).to(torch.uint8)
+
+
+def cpu64(x):
+    return None if x is None else x.detach().cpu().double()
+
+
+# ---------------------------------------------------------------- layouts
+#: name -> (sequences, rows, lengths or None, packed lengths or None)
+LAYOUTS = {
+    "one_row": (1, 1, None, None),
+    "dense": (2, 37, None, None),
+    "padded": (3, 40, [40, 0, 33], None),
+    "packed": (None, None, None, [0, 1, 65, 3, 0, 32]),
+    "gap": (None, None, None, [5, 31]),     # rows in front of and behind the sequences
+}
+
+
+def layout(name):
+    """(shape of the leading dimensions, seq keyword arguments, spans in the flat rows, rows outside)"""
+    B, Lr, lens, packed = LAYOUTS[name]
+    if packed is None:
+        kw = {} if lens is None else dict(lengths=torch.tensor(lens, dtype=torch.int32, device=DEV))
+        sp = spans(B, Lr, None, lens)
+        lead = (B, Lr)
+    else:
+        front, behind = (4, 7) if name == "gap" else (0, 0)
+        starts = np.concatenate([[0], np.cumsum(packed)]) + front
+        lead = (int(starts[-1]) + behind,)
+        kw = dict(seq_start=torch.tensor(starts, dtype=torch.int32, device=DEV))
+        sp = spans(None, None, starts)
+    inside = torch.zeros(math.prod(lead), dtype=torch.bool)
+    for lo, hi in sp:
+        inside[lo:hi] = True
+    return lead, kw, sp, ~inside
+
+
+def poison(x, outside, rows_dim):
+    """NaN in the rows that belong to no sequence: they may not be looked at."""
+    x.view(-1, *x.shape[rows_dim:])[outside.to(x.device)] = float("nan")
+    return x
+
+
+def strided(x, pad):
+    """The same values with rows `pad` elements further apart (pad odd: rows whose alignment changes)."""
+    wide = torch.full((*x.shape[:-1], x.shape[-1] + pad), 7.0, dtype=x.dtype, device=x.device)
+    wide[..., :x.shape[-1]] = x
+    return wide[..., :x.shape[-1]]
+
+
+# ---------------------------------------------------------------- convolution
+CONV = [("one_row", "f32", 5, 4, True, True, 0), ("dense", "bf16", 64, 4, True, True, 0), ("dense", "f32", 260, 3, False, False, 3), ("padded", "f16", 72, 4, True, False, 0),
+        ("packed", "bf16", 130, 4, True, True, 1), ("packed", "f64", 20, 2, True, True, 0), ("gap", "f32", 12, 8, True, True, 0), ("packed", "f16", 33, 1, True, True, 5),
+        ("padded", "f64", 8, 5, False, True, 0), ("packed", "f32", 516, 6, True, True, 4)]
+
+
+def conv_case(lay, dtype, D, W, silu, bias, pad, seed=0):
+    g = torch.Generator().manual_seed(seed + D + W)
+    lead, kw, sp, outside = layout(lay)
+    dt = DT[dtype]
+    x = strided(poison(rnd(g, *lead, D, dtype=dt), outside, len(lead)), pad) if pad else poison(rnd(g, *lead, D, dtype=dt), outside, len(lead))
+    c = dict(x=x, w=rnd(g, D, W, dtype=param_of(dt), scale=0.5), b=rnd(g, D, dtype=param_of(dt)) if bias else None, dy=poison(rnd(g, *lead, D, dtype=dt), outside, len(lead)),
+             state=rnd(g, len(sp), W - 1, D, dtype=dt), dstate=rnd(g, len(sp), W - 1, D, dtype=dt), silu=silu, kw=kw, spans=sp, outside=outside, D=D)
+    return c
+
+
+def rows_of(x):
+    return cpu64(x).reshape(-1, x.shape[-1])
+
+
+@gpu
+@pytest.mark.parametrize("lay,dtype,D,W,silu,bias,pad", CONV)
+@pytest.mark.parametrize("with_state", [True, False])
+def test_conv_forward(lay, dtype, D, W, silu, bias, pad, with_state):
+    c = conv_case(lay, dtype, D, W, silu, bias, pad)
+    st = c["state"] if with_state else None
+    y, end = seq.causal_conv(c["x"], c["w"], c["b"], silu=silu, state=st, return_state=True, **c["kw"])
+    p = plain_conv(torch.nan_to_num(rows_of(c["x"])), cpu64(c["w"]), cpu64(c["b"]), silu, c["spans"], cpu64(st))
+    # a product and a sum per tap, the bias, exponential + reciprocal + products of the gate
+    check(y.reshape(-1, D), *p["y"], 3 * W + 10, "y")
+    assert torch.equal(end.cpu().double(), p["state"][0])
+    assert bool((y.reshape(-1, D).cpu()[c["outside"]] == 0).all())
+    # an array of the caller's keeps what stands outside the sequences
+    own = torch.full_like(y, 3.0)
+    assert seq.causal_conv(c["x"], c["w"], c["b"], silu=silu, state=st, out=own, **c["kw"]) is own
+    assert bool((own.reshape(-1, D).cpu()[c["outside"]] == 3).all())
+    assert torch.equal(own.reshape(-1, D).cpu()[~c["outside"]], y.reshape(-1, D).cpu()[~c["outside"]])
+
+
+def held(x, packed):
+    """(what the call gets, the values that holds)"""
+    if not packed:
+        return x, x
+    p = seq.pack8(torch.nan_to_num(x))
+    return p, seq.unpack8(p, dtype=torch.float32)
+
+
+@gpu
+@pytest.mark.parametrize("lay,dtype,D,W,silu,bias,pad", CONV)
+@pytest.mark.parametrize("packed,with_state", [(False, True), (True, True), (False, False)])
+def test_conv_gradient(lay, dtype, D, W, silu, bias, pad, packed, with_state):
+    if packed and dtype == "f64":
+        pytest.skip("checkpoints hold float32, bfloat16 and float16")
+    c = conv_case(lay, dtype, D, W, silu, bias, pad, seed=1)
+    x, values = held(c["x"], packed)
+    st, ds = (c["state"], c["dstate"]) if with_state else (None, None)
+    g = seq.causal_conv_grad(c["dy"], x, c["w"], c["b"], silu=silu, state=st, dstate=ds, **c["kw"])
+    p = plain_conv(torch.nan_to_num(rows_of(values)), cpu64(c["w"]), cpu64(c["b"]), silu, c["spans"], cpu64(st), torch.nan_to_num(rows_of(c["dy"])), cpu64(ds))
+    check(g.x.reshape(-1, D), *p["dx"], 4 * W + 20, "dx")
+    n = sum(hi - lo for lo, hi in c["spans"])
+    k = 3 * W + 20 + min(n, 64)         # a strip's rows are summed in the compute type, the strips in double
+    check(g.weight, *p["dw"], k, "dweight")
+    if bias:
+        check(g.bias, *p["db"], k, "dbias")
+    else:
+        assert g.bias is None
+    if with_state:
+        check(g.state, *p["dstate"], 4 * W + 20, "dstate")
+    else:
+        assert g.state is None
+    again = seq.causal_conv_grad(c["dy"], x, c["w"], c["b"], silu=silu, state=st, dstate=ds, **c["kw"])
+    assert all(a is None or torch.equal(a.nan_to_num(), b.nan_to_num()) for a, b in zip(g, again))
+
+
+@gpu
+def test_conv_gradient_against_differences():
+    c = conv_case("packed", "f64", 6, 4, True, True, 0, seed=2)
+    f = lambda k: sum(float((a * b).sum()) for a, b in zip(seq.causal_conv(k["x"], k["w"], k["b"], silu=True, state=k["state"], return_state=True, **c["kw"]),  # noqa: E731
+                                                           (c["dy"], c["dstate"])))
+    g = seq.causal_conv_grad(c["dy"], c["x"], c["w"], c["b"], silu=True, state=c["state"], dstate=c["dstate"], **c["kw"])
+    difference_test(f, {k: c[k] for k in ("x", "w", "b", "state")}, dict(x=g.x, w=g.weight, b=g.bias, state=g.state))
+
+
+def difference_test(f, at, grads, n=4):
+    """Central differences in random directions: error h^2 f'''/6 + eps |f| / h, with h = 1e-4 about 1e-8 of the terms' size."""
+    g = torch.Generator().manual_seed(5)
+    for name in at:
+        for _ in range(n):
+            d = torch.randn(at[name].shape, generator=g, dtype=torch.float64).to(at[name].device)
+            h = 1e-4
+            up, down = f({**at, name: at[name] + h * d}), f({**at, name: at[name] - h * d})
+            want = float((grads[name].double() * d).sum())
+            size = float((grads[name].double() * d).abs().sum()) + 1
+            assert abs((up - down) / (2 * h) - want) <= 2e-6 * size, (name, (up - down) / (2 * h), want)
+
+
+STEP = [("f32", 5, 9, 7, 4), ("bf16", 1, 1, 256, 4), ("bf16", 6, 8, 130, 4), ("f16", 4, 6, 33, 2), ("f64", 3, 3, 12, 5), ("f32", 7, 20, 1030, 1)]
+
+
+@gpu
+@pytest.mark.parametrize("dtype,n,slots,D,W", STEP)
+def test_conv_step(dtype, n, slots, D, W):
+    g = torch.Generator().manual_seed(n * D)
+    dt = DT[dtype]
+    w, b, cache = rnd(g, D, W, dtype=param_of(dt), scale=0.5), rnd(g, D, dtype=param_of(dt)), rnd(g, slots, W - 1, D, dtype=dt)
+    at = torch.randperm(slots, generator=g)[:n].to(torch.int32)
+    if n > 3:
+        at[1], at[3] = at[0], -1                # two rows of one sequence, a row that is padding
+    x = rnd(g, n, D, dtype=dt)
+    mine = cache.clone()
+    y = seq.causal_conv_step(x, w, b, mine, at.to(DEV), silu=True)
+    ref, st = torch.zeros(n, D, dtype=torch.float64), cpu64(cache).clone()
+    scale = torch.zeros(n, D, dtype=torch.float64)
+    for r, k in enumerate(at.tolist()):
+        if k < 0:
+            continue
+        p = plain_conv(cpu64(x)[r:r + 1], cpu64(w), cpu64(b), True, [(0, 1)], st[k:k + 1])
+        ref[r], scale[r], st[k] = p["y"][0][0], p["y"][1][0], p["state"][0][0]
+    check(y, ref, scale, 3 * W + 10, "y")
+    assert torch.equal(mine.cpu().double(), st)
+    if n <= slots:          # without slots: row r continues state r
+        mine = cache.clone()
+        y = seq.causal_conv_step(x, w, b, mine, silu=True)
+        z = [seq.causal_conv(x[r:r + 1, None], w, b, silu=True, state=cache[r:r + 1], return_state=True) for r in range(n)]
+        assert torch.equal(y, torch.cat([a[0][:, 0] for a in z])) and torch.equal(mine[:n], torch.cat([a[1] for a in z])) and torch.equal(mine[n:], cache[n:])
+
+
+# ---------------------------------------------------------------- scan
+#: layout, type, D, N, G, gate, softplus, skip, bias, extra elements between rows
+SCAN = [("one_row", "f32", 3, 1, 1, False, True, True, True, 0), ("dense", "bf16", 96, 16, 1, True, True, True, True, 0), ("dense", "f32", 70, 16, 2, False, False, False, False, 0),
+        ("padded", "f16", 65, 8, 1, True, True, True, True, 0), ("packed", "f32", 130, 16, 1, True, True, True, True, 0), ("packed", "bf16", 48, 11, 4, True, True, False, True, 3),
+        ("gap", "f32", 40, 5, 2, True, False, True, True, 2), ("packed", "f64", 10, 9, 1, True, True, True, True, 0), ("packed", "f32", 24, 37, 3, True, True, True, False, 0),
+        ("padded", "f64", 6, 3, 2, False, True, True, True, 1), ("dense", "f16", 12, 64, 1, True, True, True, True, 0)]
+
+
+def scan_case(lay, dtype, D, N, G, gate, softplus, skip, bias, pad, seed=0):
+    g = torch.Generator().manual_seed(seed + 31 * D + N)
+    lead, kw, sp, outside = layout(lay)
+    dt, pt = DT[dtype], param_of(DT[dtype])
+
+    def act(scale=1.0, *tail):
+        x = poison(rnd(g, *lead, *(tail or (D,)), dtype=dt, scale=scale), outside, len(lead))
+        return strided(x, pad) if pad else x
+
+    c = dict(u=act(), z=act() if gate else None, dy=act(), A=-torch.exp(rnd(g, D, N, dtype=pt, scale=0.7)),
+             B=act(1.0, G, N) if G > 1 else act(1.0, N), C=act(1.0, G, N) if G > 1 else act(1.0, N), D=rnd(g, D, dtype=pt) if skip else None,
+             state=rnd(g, len(sp), D, N, dtype=pt), dstate=rnd(g, len(sp), D, N, dtype=pt), kw=kw, spans=sp, outside=outside)
+    c["dt"] = act(0.8) if softplus else act(0.2).abs()
+    c["bias"] = rnd(g, D, dtype=pt, scale=0.5) - 1.0 if bias and softplus else (rnd(g, D, dtype=pt).abs() * 0.1 if bias else None)
+    return c
+
+
+def scan_ref(c, D, G, N, softplus, state, u=None, z=None, **kw):
+    f = lambda x: torch.nan_to_num(rows_of(x))  # noqa: E731
+    m = lambda x: torch.nan_to_num(cpu64(x)).reshape(-1, G, N)  # noqa: E731
+    zz = c["z"] if z is None else z
+    return plain_scan(f(c["u"] if u is None else u), f(c["dt"]), cpu64(c["A"]), m(c["B"]), m(c["C"]), cpu64(c["D"]), None if zz is None else f(zz), cpu64(c["bias"]), softplus,
+                      c["spans"], cpu64(state), **{k: f(v) if k == "dy" else cpu64(v) for k, v in kw.items()})
+
+
+def longest(c):
+    return max(hi - lo for lo, hi in c["spans"])
+
+
+@gpu
+@pytest.mark.parametrize("lay,dtype,D,N,G,gate,softplus,skip,bias,pad", SCAN)
+@pytest.mark.parametrize("with_state", [True, False])
+def test_scan_forward(lay, dtype, D, N, G, gate, softplus, skip, bias, pad, with_state):
+    c = scan_case(lay, dtype, D, N, G, gate, softplus, skip, bias, pad)
+    st = c["state"] if with_state else None
+    kw = dict(D=c["D"], z=c["z"], dt_bias=c["bias"], softplus=softplus, state=st, **c["kw"])
+    y, end = seq.selective_scan(c["u"], c["dt"], c["A"], c["B"], c["C"], return_state=True, **kw)
+    p = scan_ref(c, D, G, N, softplus, st)
+    # a row's input meets: step length (about 12 roundings), decay and product of each later row (the scale carries the decays, so the rows
+    # that still weigh are few; 6 a row for the rows of a chunk), the sum over N states, the gate
+    k = 30 + N + 4 * min(longest(c), 16)
+    check(y.reshape(-1, D), *p["y"], k, "y")
+    check(end, *p["state"], k, "state")
+    assert bool((y.reshape(-1, D).cpu()[c["outside"]] == 0).all())
+    own = torch.full_like(y, 3.0)
+    assert seq.selective_scan(c["u"], c["dt"], c["A"], c["B"], c["C"], out=own, **kw) is own
+    assert bool((own.reshape(-1, D).cpu()[c["outside"]] == 3).all())
+    assert torch.equal(own.reshape(-1, D).cpu()[~c["outside"]], y.reshape(-1, D).cpu()[~c["outside"]])
+
+
+@gpu
+@pytest.mark.parametrize("lay,dtype,D,N,G,gate,softplus,skip,bias,pad", SCAN)
+@pytest.mark.parametrize("packed,with_state", [(False, True), (True, True), (False, False)])
+def test_scan_gradient(lay, dtype, D, N, G, gate, softplus, skip, bias, pad, packed, with_state):
+    if packed and dtype == "f64":
+        pytest.skip("checkpoints hold float32, bfloat16 and float16")
+    c = scan_case(lay, dtype, D, N, G, gate, softplus, skip, bias, pad, seed=1)
+    st, ds = (c["state"], c["dstate"]) if with_state else (None, None)
+    u, uv = held(c["u"], packed)
+    z, zv = held(c["z"], packed) if gate else (None, None)
+    call = lambda: seq.selective_scan_grad(c["dy"], u, c["dt"], c["A"], c["B"], c["C"], D=c["D"], z=z, dt_bias=c["bias"], softplus=softplus, state=st, dstate=ds, **c["kw"])  # noqa: E731
+    g = call()
+    p = scan_ref(c, D, G, N, softplus, st, u=uv, z=zv, dy=c["dy"], dstate=ds)["grad"]
+    n = longest(c)
+    k = 60 + N + 8 * min(n, 16)
+    for name in ("u", "dt"):
+        check(getattr(g, name).reshape(-1, D), *p[name], k, name)
+        assert bool((getattr(g, name).reshape(-1, D).cpu()[c["outside"]] == 0).all())
+    if gate:
+        check(g.z.reshape(-1, D), *p["z"], k, "z")
+    else:
+        assert g.z is None
+    for name in ("B", "C"):
+        check(getattr(g, name).reshape(-1, G, N), *p[name], k + D // G, name)
+        assert getattr(g, name).shape == c[name].shape
+        assert bool((getattr(g, name).reshape(-1, G * N).cpu()[c["outside"]] == 0).all())
+    check(g.A, *p["A"], k + 32, "A")
+    for name, there in (("D", skip), ("dt_bias", bias)):
+        if there:
+            check(getattr(g, name), *p[name], k + 32, name)
+        else:
+            assert getattr(g, name) is None
+    if with_state:
+        check(g.state, *p["state"], k, "state")
+    else:
+        assert g.state is None
+    assert all(a is None or torch.equal(a, b) for a, b in zip(g, call()))
+
+
+@gpu
+def test_scan_gradient_against_differences():
+    D, N, G = 4, 3, 2
+    c = scan_case("packed", "f64", D, N, G, True, True, True, True, 0, seed=3)
+    names = ("u", "dt", "A", "B", "C", "D", "z", "bias", "state")
+
+    def f(k):
+        y, end = seq.selective_scan(k["u"], k["dt"], k["A"], k["B"], k["C"], D=k["D"], z=k["z"], dt_bias=k["bias"], state=k["state"], return_state=True, **c["kw"])
+        return float((y * c["dy"]).sum()) + float((end * c["dstate"]).sum())
+
+    g = seq.selective_scan_grad(c["dy"], c["u"], c["dt"], c["A"], c["B"], c["C"], D=c["D"], z=c["z"], dt_bias=c["bias"], state=c["state"], dstate=c["dstate"], **c["kw"])
+    difference_test(f, {k: c[k] for k in names}, {**{k: getattr(g, k) for k in names if k != "bias"}, "bias": g.dt_bias})
+
+
+@gpu
+@pytest.mark.parametrize("rows,D,N", [(1000, 64, 16), (517, 200, 8)])
+def test_long_scan_is_cut_into_chunks_like_one(rows, D, N):
+    """A sequence much longer than a chunk, alone, against the same sequence in pieces that carry their state on."""
+    g = torch.Generator().manual_seed(rows)
+    u, dt, z = rnd(g, 1, rows, D), rnd(g, 1, rows, D, scale=0.5) - 3, rnd(g, 1, rows, D)
+    A, B, C, skip = -torch.exp(rnd(g, D, N)), rnd(g, 1, rows, N), rnd(g, 1, rows, N), rnd(g, D)
+    y, end = seq.selective_scan(u, dt, A, B, C, D=skip, z=z, return_state=True)
+    st, parts = None, []
+    for lo in range(0, rows, 100):
+        s = slice(lo, lo + 100)
+        yy, st = seq.selective_scan(u[:, s], dt[:, s], A, B[:, s], C[:, s], D=skip, z=z[:, s], state=st, return_state=True)
+        parts.append(yy)
+    p = plain_scan(*(rows_of(x) for x in (u, dt)), cpu64(A), cpu64(B).view(rows, 1, N), cpu64(C).view(rows, 1, N), cpu64(skip), rows_of(z), None, True, [(0, rows)], None)
+    for got, e in ((y, end), (torch.cat(parts, 1), st)):
+        check(got.reshape(-1, D), *p["y"], 30 + N + 64, "y")
+        check(e, *p["state"], 30 + N + 64, "state")
+
+
+@gpu
+@pytest.mark.parametrize("dtype,n,slots,D,N,G,gate", [("f32", 5, 9, 7, 16, 1, True), ("bf16", 1, 1, 256, 16, 1, True), ("bf16", 6, 8, 130, 16, 2, True), ("f16", 4, 6, 33, 5, 3, False),
+                                                       ("f64", 5, 5, 12, 9, 1, True), ("f32", 7, 20, 70, 64, 1, True), ("f32", 2, 2, 3, 1, 1, False), ("f32", 4, 4, 20, 200, 2, True)])
+def test_scan_step(dtype, n, slots, D, N, G, gate):
+    g = torch.Generator().manual_seed(n * D + N)
+    dt, pt = DT[dtype], param_of(DT[dtype])
+    u, d, z = rnd(g, n, D, dtype=dt), rnd(g, n, D, dtype=dt, scale=0.5), rnd(g, n, D, dtype=dt) if gate else None
+    A, B, C = -torch.exp(rnd(g, D, N, dtype=pt)), rnd(g, n, G, N, dtype=dt), rnd(g, n, G, N, dtype=dt)
+    skip, bias, cache = rnd(g, D, dtype=pt), rnd(g, D, dtype=pt), rnd(g, slots, D, N, dtype=pt)
+    at = torch.randperm(slots, generator=g)[:n].to(torch.int32)
+    if n > 3:
+        at[1], at[3] = at[0], slots
+    mine = cache.clone()
+    y = seq.selective_scan_step(u, d, A, B, C, mine, at.to(DEV), D=skip, z=z, dt_bias=bias)
+    st, ref, scale = cpu64(cache).clone(), torch.zeros(n, D, dtype=torch.float64), torch.zeros(n, D, dtype=torch.float64)
+    hs = st.abs()
+    for r, k in enumerate(at.tolist()):
+        if k >= slots:
+            continue
+        one = lambda x: None if x is None else cpu64(x)[r:r + 1]  # noqa: E731
+        # (a second row of one sequence: its state's error is eps of what the first row's terms added up to, whatever of them cancelled)
+        p = plain_scan(one(u), one(d), cpu64(A), one(B), one(C), cpu64(skip), one(z), cpu64(bias), True, [(0, 1)], st[k:k + 1], mag=hs[k:k + 1])
+        ref[r], scale[r], st[k], hs[k] = p["y"][0][0], p["y"][1][0], p["state"][0][0], p["state"][1][0]
+    check(y, ref, scale, 40 + N, "y")
+    check(mine, st, hs, 40, "state")
+    left = torch.ones(slots, dtype=torch.bool)
+    left[at[at < slots].long()] = False
+    assert torch.equal(mine.cpu()[left], cache.cpu()[left])
+
+
+# ---------------------------------------------------------------- what happens at the edges of numbers
+@gpu
+def test_step_length_keeps_its_relative_accuracy():
+    """softplus from -80 (1e-35) to 80: the state after one row from 0 with B = u = 1 is the step length itself."""
+    x = torch.cat([torch.linspace(-80, 80, 4001), torch.tensor([0.0, -1e-7, 1e-7, -19.99, 20.01])]).to(DEV)
+    D = x.numel()
+    one = torch.ones(1, 1, 1, device=DEV)
+    _, end = seq.selective_scan(torch.ones(1, 1, D, device=DEV), x.view(1, 1, D), -torch.ones(D, 1, device=DEV), one, one, return_state=True)
+    want = torch.nn.functional.softplus(x.double().cpu(), threshold=1e9)
+    want = torch.where(x.cpu() < -30, torch.exp(x.double().cpu()), want)
+    # the exponent x log2(e) is rounded to 24 bits: |x| eps / 2 of the value each for the product and the constant; then about 8 roundings
+    limit = (8 + x.double().cpu().abs()) * 2.0 ** -23
+    assert bool(((end.view(-1).cpu().double() / want - 1).abs() <= limit).all())
+
+
+@gpu
+def test_infinities_and_nan_stay_in_their_channel_and_after_their_row():
+    g = torch.Generator().manual_seed(0)
+    u, dt, z = rnd(g, 2, 50, 80), rnd(g, 2, 50, 80), rnd(g, 2, 50, 80)
+    A, B, C = -torch.exp(rnd(g, 80, 16)), rnd(g, 2, 50, 16), rnd(g, 2, 50, 16)
+    y = seq.selective_scan(u, dt, A, B, C, z=z)
+    u[0, 20, 3], dt[1, 10, 70], z[0, 5, 9] = float("inf"), float("nan"), float("nan")
+    w = seq.selective_scan(u, dt, A, B, C, z=z)
+    touched = torch.zeros(2, 50, 80, dtype=torch.bool, device=DEV)
+    touched[0, 20:, 3], touched[1, 10:, 70], touched[0, 5, 9] = True, True, True
+    assert torch.equal(y[~touched], w[~touched]) and not bool(torch.isfinite(w[touched]).any())
+    c = seq.causal_conv(u, rnd(g, 80, 4))
+    assert int((~torch.isfinite(c)).sum()) == 4 and not bool(torch.isfinite(c[0, 20:24, 3]).any())
+
+
+@gpu
+@pytest.mark.parametrize("starts", [[0, 90, 40, 60], [-5, 20, 300], [50, 10], [0]])
+def test_offsets_that_make_no_sense_stay_inside_the_arrays(starts):
+    g = torch.Generator().manual_seed(1)
+    at = torch.tensor(starts, dtype=torch.int32, device=DEV)
+    u, dt, dy, B, C = (rnd(g, 60, n) for n in (20, 20, 20, 16, 16))
+    A = -torch.exp(rnd(g, 20, 16))
+    assert seq.causal_conv(u, rnd(g, 20, 4), seq_start=at, return_state=True)[1].shape == (len(starts) - 1, 3, 20)
+    seq.causal_conv_grad(dy, u, rnd(g, 20, 4), seq_start=at)
+    assert seq.selective_scan(u, dt, A, B, C, seq_start=at, return_state=True)[1].shape == (len(starts) - 1, 20, 16)
+    seq.selective_scan_grad(dy, u, dt, A, B, C, seq_start=at)
+
+
+# ---------------------------------------------------------------- checkpoints
+@gpu
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("shape,pad", [((3, 64), 0), ((2, 5, 33), 0), ((7, 1), 0), ((4, 100), 3), ((1, 31), 0), ((0, 40), 0), ((9, 48), 16), ((5, 160), 8)])
+def test_checkpoint_codes_and_values(dtype, shape, pad):
+    g = torch.Generator().manual_seed(shape[-1])
+    x = rnd(g, *shape, dtype=torch.float32) * torch.exp(3 * rnd(g, *shape[:-1], 1))
+    x = x.to(DT[dtype])
+    if x.numel() > 50:
+        x.view(-1)[:5] = torch.tensor([0.0, 127.5, -127.5, 1.0, 255.0], dtype=torch.float32).to(DT[dtype]).to(DEV)
+    p = seq.pack8(strided(x, pad) if pad else x)
+    codes, scales = plain_codes(x.reshape(math.prod(shape[:-1]), shape[-1]).cpu().float())
+    assert torch.equal(p.codes.cpu().view(codes.shape), codes) and torch.equal(p.scales.cpu().view(scales.shape), scales)
+    back = seq.unpack8(p)
+    want = (codes.double() * torch.exp2(scales.double() - 127).repeat_interleave(32, 1)[:, :shape[-1]])
+    assert back.dtype == x.dtype and torch.equal(back.cpu().double().view(want.shape), want.to(DT[dtype]).double())
+    wide = seq.unpack8(p, dtype=torch.float32)
+    assert torch.equal(wide.cpu().double().view(want.shape), want)
+    # within half a code, and a code is at most max|x| / 64 of its block
+    if x.numel():
+        big = torch.nn.functional.pad(x.cpu().double().view(-1, shape[-1]).abs(), (0, -shape[-1] % 32)).view(len(codes), -1, 32).amax(-1)
+        assert bool(((wide.cpu().double().view(-1, shape[-1]) - x.cpu().double().view(-1, shape[-1])).abs() <= big.repeat_interleave(32, 1)[:, :shape[-1]] / 128 + 2.0 ** -128).all())
+
+
+@gpu
+def test_checkpoint_of_extreme_values():
+    x = torch.zeros(8, 64, device=DEV)
+    x[0, 3], x[1, 40], x[2, 0] = float("nan"), float("inf"), float("-inf")
+    x[3, 5], x[4, 7], x[5, 33] = torch.finfo(torch.float32).max, 2.0 ** -149, -(2.0 ** -126)
+    x[6, :32] = 2.0 ** -121 * 1.9999
+    v = seq.unpack8(seq.pack8(x))
+    codes, scales = plain_codes(x.cpu())
+    want = codes.double() * torch.exp2(scales.double() - 127).repeat_interleave(32, 1)
+    for r, block in ((0, 0), (1, 1), (2, 0)):
+        assert bool(torch.isnan(v[r, 32 * block:32 * block + 32]).all()) and bool((v[r, 32 - 32 * block:64 - 32 * block] == 0).all())
+    assert torch.equal(v[3:].cpu().double(), want[3:]) and bool((v[7] == 0).all()) and bool(torch.isfinite(v[3:]).all())
+    for dt, top in ((torch.float16, 2.0 ** 15), (torch.bfloat16, 2.0 ** 127)):
+        x = torch.tensor([[torch.finfo(dt).max, 1.0] + [0.0] * 30, [-torch.finfo(dt).max] * 32], dtype=dt, device=DEV)
+        codes, scales = plain_codes(x.cpu().float(), top)
+        v = seq.unpack8(seq.pack8(x))
+        assert torch.equal(v.cpu().double(), codes.double() * torch.exp2(scales.double() - 127)) and bool(torch.isfinite(v).all())
+
+
+# ---------------------------------------------------------------- together
+@gpu
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_prompts_then_single_rows_give_what_one_pass_gives(dtype):
+    """Convolution and scan over packed prompts of unequal length, their states put into a cache, then row by row through the cache, against
+    one pass over the whole series."""
+    g = torch.Generator().manual_seed(11)
+    D, N, W, dt = 72, 16, 4, DT[dtype]
+    lens, more, slots = [3, 0, 41, 1], 4, 6
+    total = [n + more for n in lens]
+    w, b, A, skip, bias = rnd(g, D, W, scale=0.5), rnd(g, D), -torch.exp(rnd(g, D, N)), rnd(g, D), rnd(g, D) - 2
+    x, z = [rnd(g, n, D, dtype=dt) for n in total], [rnd(g, n, D, dtype=dt) for n in total]
+    d, Bm, Cm = [rnd(g, n, D, dtype=dt) for n in total], [rnd(g, n, N, dtype=dt) for n in total], [rnd(g, n, N, dtype=dt) for n in total]
+    at = torch.tensor(np.concatenate([[0], np.cumsum(lens)]), dtype=torch.int32, device=DEV)
+    head = lambda v: torch.cat([a[:n] for a, n in zip(v, lens)])  # noqa: E731
+    c, cst = seq.causal_conv(head(x), w, b, silu=True, seq_start=at, return_state=True)
+    y, hst = seq.selective_scan(c, head(d), A, head(Bm), head(Cm), D=skip, z=head(z), dt_bias=bias, seq_start=at, return_state=True)
+    where = torch.tensor([4, 0, 5, 2], device=DEV)
+    ccache, hcache = torch.zeros(slots, W - 1, D, dtype=dt, device=DEV), torch.zeros(slots, D, N, device=DEV)
+    ccache[where], hcache[where] = cst, hst
+    got = [[y[lo:hi]] for lo, hi in zip(at[:-1].tolist(), at[1:].tolist())]
+    for k in range(more):
+        row = lambda v: torch.stack([a[n + k] for a, n in zip(v, lens)])  # noqa: E731
+        c1 = seq.causal_conv_step(row(x), w, b, ccache, where.to(torch.int32), silu=True)
+        y1 = seq.selective_scan_step(c1, row(d), A, row(Bm), row(Cm), hcache, where.to(torch.int32), D=skip, z=row(z), dt_bias=bias)
+        for s in range(4):
+            got[s].append(y1[s:s + 1])
+    for s in range(4):
+        c1, cend = seq.causal_conv(x[s][None], w, b, silu=True, return_state=True)
+        y1, hend = seq.selective_scan(c1, d[s][None], A, Bm[s][None], Cm[s][None], D=skip, z=z[s][None], dt_bias=bias, return_state=True)
+        a, e = torch.cat(got[s]).double(), y1[0].double()
+        # both are roundings of the same sums, formed in another order: a unit of the type, and 1e-5 for the order
+        assert bool(((a - e).abs() <= torch.finfo(dt).eps * e.abs() + 1e-5 * (1 + e.abs())).all())
+        assert torch.equal(ccache[where[s]], cend[0]) and bool(((hcache[where[s]] - hend[0]).abs() <= 1e-5 * (1 + hend[0].abs())).all())
+
+
+@gpu
+@pytest.mark.parametrize("packed", [False, True])
+def test_training_step_through_both_operators(packed):
+    """conv -> scan and back, the inputs kept as they are or in 8 bits: the gradients against differences of the whole (kept as they are), and
+    against the same chain at the restored values (8 bits)."""
+    g = torch.Generator().manual_seed(4)
+    D, N, W, B, T = 40, 4, 4, 2, 45
+    dt = torch.float32 if packed else torch.float64
+    pt = param_of(dt)
+    x, z, d = (rnd(g, B, T, D, dtype=dt) for _ in range(3))
+    w, b, A, skip, bias = rnd(g, D, W, dtype=pt, scale=0.5), rnd(g, D, dtype=pt), -torch.exp(rnd(g, D, N, dtype=pt)), rnd(g, D, dtype=pt), rnd(g, D, dtype=pt) - 1
+    Bm, Cm, dy = rnd(g, B, T, N, dtype=dt), rnd(g, B, T, N, dtype=dt), rnd(g, B, T, D, dtype=dt)
+
+    def forward(k):
+        return seq.selective_scan(seq.causal_conv(k["x"], k["w"], k["b"], silu=True), d, k["A"], Bm, Cm, D=skip, z=k["z"], dt_bias=bias)
+
+    def backward(x_, z_):
+        u = seq.causal_conv(x_, w, b, silu=True)
+        s = seq.selective_scan_grad(dy, u, d, A, Bm, Cm, D=skip, z=z_, dt_bias=bias)
+        c = seq.causal_conv_grad(s.u, x_, w, b, silu=True)
+        return dict(x=c.x, w=c.weight, b=c.bias, A=s.A, z=s.z)
+
+    if not packed:
+        difference_test(lambda k: float((forward(k) * dy).sum()), dict(x=x, w=w, b=b, A=A, z=z), backward(x, z))
+        return
+    px, pz = seq.pack8(x), seq.pack8(z)
+    got, want = backward(px, pz), backward(seq.unpack8(px), seq.unpack8(pz))
+    for k in got:
+        assert torch.equal(got[k], want[k]), k
+
+
+# ---------------------------------------------------------------- refusals: before any launch
+def args(**over):
+    g = torch.Generator().manual_seed(0)
+    a = dict(u=rnd(g, 2, 6, 8), dt=rnd(g, 2, 6, 8), A=-torch.ones(8, 4, device=DEV), B=rnd(g, 2, 6, 4), C_=rnd(g, 2, 6, 4))
+    a.update(over)
+    return a
+
+
+def bad_scans():
+    z = lambda *s, **k: torch.zeros(*s, device=DEV, **k)  # noqa: E731
+    return {"u shape": (ValueError, args(u=z(2, 6, 9))), "u type": (ValueError, args(u=z(2, 6, 8, dtype=torch.float16))), "integer": (TypeError, args(dt=z(2, 6, 8, dtype=torch.int32))),
+            "A rows": (ValueError, args(A=z(9, 4))), "no states": (ValueError, args(A=z(8, 0))), "states": (ValueError, args(A=z(8, 257), B=z(2, 6, 257), C_=z(2, 6, 257))),
+            "B rows": (ValueError, args(B=z(2, 5, 4))), "B states": (ValueError, args(B=z(2, 6, 5))), "groups": (ValueError, args(B=z(2, 6, 3, 4), C_=z(2, 6, 3, 4))),
+            "B and C": (ValueError, args(B=z(2, 6, 2, 4))), "D": (ValueError, args(D=z(7))), "bias": (ValueError, args(dt_bias=z(8, 1))), "state": (ValueError, args(state=z(2, 8, 5))),
+            "state type": (ValueError, args(state=z(2, 8, 4, dtype=torch.float16))), "starts type": (ValueError, args(seq_start=z(3, dtype=torch.int64))),
+            "dense rows with offsets": (ValueError, args(seq_start=z(3, dtype=torch.int32))), "both": (ValueError, args(seq_start=z(3, dtype=torch.int32), lengths=z(2, dtype=torch.int32))),
+            "lengths": (ValueError, args(lengths=z(3, dtype=torch.int32))), "out": (ValueError, args(out=z(2, 6, 8, dtype=torch.float16)))}
+
+
+@gpu
+@pytest.mark.parametrize("what", ["u shape", "u type", "integer", "A rows", "no states", "states", "B rows", "B states", "groups", "B and C", "D", "bias", "state", "state type", "starts type",
+                                  "dense rows with offsets", "both", "lengths", "out"])
+def test_scan_refuses(what):
+    err, a = bad_scans()[what]
+    with pytest.raises(err):
+        seq.selective_scan(**a)
+
+
+@gpu
+def test_other_refusals():
+    z = lambda *s, **k: torch.zeros(*s, device=DEV, **k)  # noqa: E731
+    p = seq.pack8(z(2, 6, 8))
+    for err, call in [
+            (ValueError, lambda: seq.causal_conv(z(2, 6, 8), z(8, 9))), (ValueError, lambda: seq.causal_conv(z(2, 6, 8), z(7, 4))), (ValueError, lambda: seq.causal_conv(z(6, 8), z(8, 4))),
+            (ValueError, lambda: seq.causal_conv(z(2, 6, 8), z(8, 4), state=z(2, 4, 8))), (ValueError, lambda: seq.causal_conv_grad(z(2, 6, 7), z(2, 6, 8), z(8, 4))),
+            (TypeError, lambda: seq.causal_conv_grad(p, z(2, 6, 8), z(8, 4))), (TypeError, lambda: seq.selective_scan(**args(dt=p))),
+            (ValueError, lambda: seq.causal_conv_step(z(3, 8), z(8, 4), None, z(2, 3, 8))), (ValueError, lambda: seq.causal_conv_step(z(3, 8), z(8, 4), None, z(4, 3, 8), z(2, dtype=torch.int32))),
+            (ValueError, lambda: seq.selective_scan_step(z(3, 8), z(3, 8), z(8, 4), z(3, 4), z(3, 4), z(2, 8, 4))),
+            (TypeError, lambda: seq.selective_scan_step(p, z(3, 8), z(8, 4), z(3, 4), z(3, 4), z(4, 8, 4))), (TypeError, lambda: seq.pack8(z(4, 8, dtype=torch.float64))),
+            (ValueError, lambda: seq.Packed8(z(4, 33, dtype=torch.int8), z(4, 1, dtype=torch.uint8), torch.float32)),
+            (TypeError, lambda: seq.Packed8(z(4, 32), z(4, 1, dtype=torch.uint8), torch.float32)), (TypeError, lambda: seq.unpack8(p, dtype=torch.float64))]:
+        with pytest.raises(err):
+            call()
+
+
+def test_there_is_no_cpu_path():
+    if seq._EMULATED:
+        pytest.skip("the emulated device's memory is the host's")
+    with pytest.raises(ValueError):
+        seq.causal_conv(torch.zeros(1, 2, 3), torch.zeros(3, 4))
+    with pytest.raises(ValueError):
+        seq.pack8(torch.zeros(2, 32))
+
+
+def test_c_entry_points_refuse_before_any_launch():
+    """The C ABI by itself: sizes, missing arrays, types, workspace -- refused with a message, on a host without a device too."""
+    import ctypes as C
+    lib = L.lib
+    said = lambda: lib.crnn_last_error(None).decode()  # noqa: E731
+
+    def view(dt=L.DT_F32, rs=8, ptr=4096):
+        return L.View(ptr=ptr, row_stride=rs, seq_stride=48, dtype=dt)
+
+    def scan(**over):
+        a = L.ScanArgs(struct_size=C.sizeof(L.ScanArgs), n_seq=2, D=8, N=4, G=1, rows=6, A=4096, u=view(), dt=view(), y=view(), B=view(rs=4), C=view(rs=4))
+        for k, v in over.items():
+            setattr(a, k, v)
+        return a
+
+    for over, word in [(dict(struct_size=8), "struct_size"), (dict(N=0), "N must"), (dict(N=257), "N must"), (dict(G=3), "divide"), (dict(rows=-1), "negative"), (dict(rows=1 << 31), "rows"),
+                       (dict(D=0), "D must"), (dict(A=None), "A is missing"), (dict(u=view(ptr=None)), "u is missing"), (dict(u=view(L.DT_BF16)), "element type"),
+                       (dict(u=view(L.DT_PACKED8)), "scales"), (dict(dt=view(L.DT_PACKED8)), "checkpoint"), (dict(y=view(rs=7)), "overlap"), (dict(dtype=9), "element type"),
+                       (dict(seq_start=64, seq_len=64), "exclude"), ({}, "workspace")]:
+        assert lib.crnn_scan_forward(C.byref(scan(**over))) == -1 and word in said(), (over, said())
+    assert lib.crnn_scan_forward(None) == -1 and "null" in said()
+    assert lib.crnn_scan_workspace(C.byref(scan()), 2) == -1 and lib.crnn_scan_workspace(C.byref(scan()), 0) > 0
+    assert lib.crnn_scan_backward(C.byref(scan())) == -1 and "dA" in said()
+    assert lib.crnn_scan_step(C.byref(scan(n_slots=1))) == -1 and "n_slots" in said()
+
+    def conv(**over):
+        a = L.ConvArgs(struct_size=C.sizeof(L.ConvArgs), n_seq=2, D=8, W=4, rows=6, weight=4096, x=view(), y=view())
+        for k, v in over.items():
+            setattr(a, k, v)
+        return a
+
+    for over, word in [(dict(struct_size=0), "struct_size"), (dict(W=0), "W must"), (dict(W=9), "W must"), (dict(weight=None), "weight"), (dict(x=view(ptr=None)), "x is missing"),
+                       (dict(y=view(rs=4)), "overlap"), (dict(state_in=view(), state_out=view()), "state_out")]:
+        assert lib.crnn_conv_forward(C.byref(conv(**over))) == -1 and word in said(), (over, said())
+    assert lib.crnn_conv_backward(C.byref(conv(dx=view(), dy=view(), dweight=64))) == -1 and "workspace" in said()
+    assert lib.crnn_conv_step(C.byref(conv(n_slots=1))) == -1 and "n_slots" in said()
+    v = view(L.DT_F64)
+    assert lib.crnn_pack8(0, None, C.byref(v), 2, 8, 4096, 4096) == -1 and "half" in said()
+    v = view()
+    assert lib.crnn_unpack8(0, None, 4096, None, 2, 8, C.byref(v)) == -1 and "missing" in said()

@@ -35,7 +35,7 @@ ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 CSRC = os.path.join(ROOT, "crnn_amd", "csrc")
 DBG = os.path.join(CSRC, "dbg")
 VARIANTS = {"O3": "-O3", "O2": "-O2", "O1": "-O1", "O3prof": "-O3 -DCRNN_ADJ_PROF", "O3chk": "-O3 -DCRNN_BOUNDS_CHECK"}
-BASE = "-std=c++17 -fPIC --offload-arch=gfx950 -ffp-contract=on -Wno-unused-result"
+BASE = "-std=c++17 -fPIC --offload-arch=gfx950 -ffp-contract=on -Wno-unused-result -Xclang -target-feature -Xclang -packed-fp32-ops"
 LINK = "-shared -L/opt/rocm/lib -lrccl -Wl,-rpath,/opt/rocm/lib"
 
 
