@@ -40,7 +40,7 @@ crnn::SeqV seq_view(const crnn_view &v, int nvec) {
     crnn::SeqV o{};
     o.p = v.ptr;
     o.sc = (const uint8_t *)v.scales;
-    o.bs = v.seq_stride; o.rs = v.row_stride; o.sbs = v.scale_seq_stride; o.srs = v.scale_row_stride;
+    o.bs = v.seq_stride; o.rs = (int32_t)v.row_stride; o.sbs = v.scale_seq_stride; o.srs = (int32_t)v.scale_row_stride;
     o.dt = v.dtype;
     const int64_t bytes = (int64_t)nvec * seq_size(v.dtype);
     o.vec = (uintptr_t)v.ptr % (uintptr_t)bytes == 0 && v.row_stride % nvec == 0 && v.seq_stride % nvec == 0;
@@ -63,6 +63,7 @@ struct SeqCheck {
             if (v.scale_seq_stride < 0 || v.scale_row_stride < 0) return bad(std::string(name) + ": negative stride");
         } else if (v.dtype != dtype) return bad(std::string(name) + " has another element type than the call");
         if (v.seq_stride < 0 || v.row_stride < 0) return bad(std::string(name) + ": negative stride");
+        if (v.row_stride > 0x7fffffff || v.scale_row_stride > 0x7fffffff) return bad(std::string(name) + ": rows are too far apart");
         if (out && v.row_stride < width) return bad(std::string(name) + ": rows of an output overlap");
         return true;
     }
@@ -181,8 +182,9 @@ crnn::ScanMapsP scan_maps(const crnn_scan_args *a, const ScanPlan &s, const crnn
 
 unsigned seq_grid(int64_t n) { return (unsigned)std::min<int64_t>((n + 255) / 256, 65536); }
 
-template <class CT, int NS, bool P8>
+template <int IO, int NS, bool P8>
 void scan_forward_run(const crnn_scan_args *a, ScanPlan &s, hipStream_t st) {
+    using CT = typename crnn::SeqIO<IO>::C;
     crnn::ScanP p = s.p;
     CT *ws = (CT *)a->workspace, *maps = ws + s.maps, *S = ws + s.S, *sdel = ws + s.sdel;
     p.acc = s.nb > 1 ? ws + s.acc : nullptr;
@@ -194,16 +196,17 @@ void scan_forward_run(const crnn_scan_args *a, ScanPlan &s, hipStream_t st) {
         p.fin = b == s.nb - 1;
         if (s.flat > 0) hipLaunchKernelGGL((crnn::seq_scan_maps_kernel<CT, NS>), dim3(seq_grid(s.flat * p.G * 2 * NS)), dim3(256), 0, st, mp, maps);
         if (s.split) {
-            hipLaunchKernelGGL((crnn::seq_scan_ends_kernel<CT, NS, P8, false>), grid, block, 0, st, p, (const CT *)maps, S, (CT *)nullptr, sdel);
+            hipLaunchKernelGGL((crnn::seq_scan_ends_kernel<IO, NS, P8, false>), grid, block, 0, st, p, (const CT *)maps, S, (CT *)nullptr, sdel);
             hipLaunchKernelGGL((crnn::seq_scan_carry_kernel<CT, NS>), dim3((unsigned)(((int64_t)p.m.n_seq * NS * p.D + 255) / 256)), dim3(256), 0, st, p, S,
                                (CT *)nullptr, (const CT *)sdel);
         }
-        hipLaunchKernelGGL((crnn::seq_scan_out_kernel<CT, NS, P8>), grid, block, 0, st, p, (const CT *)maps, (const CT *)(s.split ? S : nullptr));
+        hipLaunchKernelGGL((crnn::seq_scan_out_kernel<IO, NS, P8>), grid, block, 0, st, p, (const CT *)maps, (const CT *)(s.split ? S : nullptr));
     }
 }
 
-template <class CT, int NS, bool P8>
+template <int IO, int NS, bool P8>
 void scan_backward_run(const crnn_scan_args *a, ScanPlan &s, hipStream_t st) {
+    using CT = typename crnn::SeqIO<IO>::C;
     crnn::ScanP p = s.p;
     CT *ws = (CT *)a->workspace, *maps = ws + s.maps, *S = ws + s.S, *Gb = ws + s.G, *sdel = ws + s.sdel, *part = ws + s.part, *dA = ws + s.dA, *dD = ws + s.dD,
        *db = ws + s.db;
@@ -217,18 +220,20 @@ void scan_backward_run(const crnn_scan_args *a, ScanPlan &s, hipStream_t st) {
         p.first = b == 0;
         p.fin = b == s.nb - 1;
         if (s.flat > 0) hipLaunchKernelGGL((crnn::seq_scan_maps_kernel<CT, NS>), dim3(seq_grid(s.flat * p.G * 2 * NS)), dim3(256), 0, st, mp, maps);
-        hipLaunchKernelGGL((crnn::seq_scan_ends_kernel<CT, NS, P8, true>), grid, block, 0, st, p, (const CT *)maps, S, Gb, sdel);
+        hipLaunchKernelGGL((crnn::seq_scan_ends_kernel<IO, NS, P8, true>), grid, block, 0, st, p, (const CT *)maps, S, Gb, sdel);
         hipLaunchKernelGGL((crnn::seq_scan_carry_kernel<CT, NS>), dim3((unsigned)(((int64_t)p.m.n_seq * NS * p.D + 255) / 256)), dim3(256), 0, st, p, S, Gb,
                            (const CT *)sdel);
-        hipLaunchKernelGGL((crnn::seq_scan_bwd_kernel<CT, NS, P8>), grid, block, 0, st, p, (const CT *)maps, (const CT *)S, (const CT *)Gb, part, dA, dD, db);
+        hipLaunchKernelGGL((crnn::seq_scan_bwd_kernel<IO, NS, P8>), grid, block, 0, st, p, (const CT *)maps, (const CT *)S, (const CT *)Gb, part, dA, dD, db);
         if (s.flat > 0)
             hipLaunchKernelGGL((crnn::seq_scan_sum_maps_kernel<CT, NS>), dim3(seq_grid(s.flat * p.G * 2 * NS)), dim3(256), 0, st, p.m, mo, (const CT *)part, p.tpg);
-        hipLaunchKernelGGL((crnn::seq_sum_blocks_kernel<CT>), dim3((unsigned)((cA + 255) / 256)), dim3(256), 0, st, (const CT *)dA, p.m.nblk, cA, (CT *)a->dA, p.D, p.N,
-                           p.n0);
+        hipLaunchKernelGGL((crnn::seq_sum_blocks_kernel<CT>), dim3((unsigned)((cA + 31) / 32)), dim3(256), 0, st, (const CT *)dA, p.m.nblk, cA, (CT *)a->dA, (CT *)nullptr, p.D,
+                           p.N, p.n0, std::min(NS, p.N - p.n0));
     }
-    const dim3 gd((unsigned)((p.D + 255) / 256));
-    if (a->dskip) hipLaunchKernelGGL((crnn::seq_sum_blocks_kernel<CT>), gd, dim3(256), 0, st, (const CT *)dD, p.m.nblk, (int64_t)p.D, (CT *)a->dskip, p.D, 0, 0);
-    if (a->ddt_bias) hipLaunchKernelGGL((crnn::seq_sum_blocks_kernel<CT>), gd, dim3(256), 0, st, (const CT *)db, p.m.nblk, (int64_t)p.D, (CT *)a->ddt_bias, p.D, 0, 0);
+    const dim3 gd((unsigned)((p.D + 31) / 32));
+    if (a->dskip)
+        hipLaunchKernelGGL((crnn::seq_sum_blocks_kernel<CT>), gd, dim3(256), 0, st, (const CT *)dD, p.m.nblk, (int64_t)p.D, (CT *)a->dskip, (CT *)nullptr, p.D, 1, 0, 1);
+    if (a->ddt_bias)
+        hipLaunchKernelGGL((crnn::seq_sum_blocks_kernel<CT>), gd, dim3(256), 0, st, (const CT *)db, p.m.nblk, (int64_t)p.D, (CT *)a->ddt_bias, (CT *)nullptr, p.D, 1, 0, 1);
 }
 
 bool scan_views(SeqCheck &c, const crnn_scan_args *a, bool backward) {
@@ -249,9 +254,14 @@ bool scan_views(SeqCheck &c, const crnn_scan_args *a, bool backward) {
 #define SCAN_RUN(run)                                                                                                         \
     do {                                                                                                                      \
         const hipStream_t st_ = (hipStream_t)a->stream;                                                                       \
-        if (s.f64) run<double, 8, false>(a, s, st_);                                                                          \
-        else if (s.NS == 8) { if (s.p8) run<float, 8, true>(a, s, st_); else run<float, 8, false>(a, s, st_); }                \
-        else { if (s.p8) run<float, 16, true>(a, s, st_); else run<float, 16, false>(a, s, st_); }                             \
+        if (s.f64) run<8, 8, false>(a, s, st_);                                                                               \
+        else if (a->dtype == CRNN_DT_F32) SCAN_RUN_IO(run, 4);                                                                \
+        else SCAN_RUN_IO(run, 2);                                                                                             \
+    } while (0)
+#define SCAN_RUN_IO(run, IO)                                                                                                  \
+    do {                                                                                                                      \
+        if (s.NS == 8) { if (s.p8) run<IO, 8, true>(a, s, st_); else run<IO, 8, false>(a, s, st_); }                           \
+        else { if (s.p8) run<IO, 16, true>(a, s, st_); else run<IO, 16, false>(a, s, st_); }                                   \
     } while (0)
 
 // ------------------------------------------------------------------ convolution
@@ -318,18 +328,6 @@ void conv_step_launch(const crnn::ConvStepP &p, hipStream_t st) {
     if (p.W <= 4) hipLaunchKernelGGL((crnn::seq_conv_step_kernel<YT, 4>), grid, dim3(256), 0, st, p);
     else hipLaunchKernelGGL((crnn::seq_conv_step_kernel<YT, 8>), grid, dim3(256), 0, st, p);
 }
-// weight gradients: the strips' parts [block][W + 1][D], in order and in double -> dweight [D][W], dbias [D]
-template <class CT>
-__global__ __launch_bounds__(256) void seq_conv_sum_kernel(const CT *__restrict__ part, int64_t nblk, int32_t W, int32_t D, CT *__restrict__ dw, CT *__restrict__ db) {
-    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, count = (int64_t)(W + 1) * D;
-    if (i >= count) return;
-    double s = 0.0;
-    for (int64_t b = 0; b < nblk; ++b) s += (double)part[b * count + i];
-    const int64_t j = i / D, d = i % D;
-    if (j < W) dw[d * W + j] = (CT)s;
-    else if (db) db[d] = (CT)s;
-}
-
 }  // namespace
 
 extern "C" {
@@ -371,9 +369,14 @@ int32_t crnn_conv_backward(const crnn_conv_args *a) {
         p.part = a->workspace;
         const hipStream_t st = (hipStream_t)a->stream;
         if (a->n_seq > 0) conv_launch_t(p, a->dtype, true, st);
-        const dim3 grid((unsigned)(((int64_t)(a->W + 1) * a->D + 255) / 256));
-        if (f64) hipLaunchKernelGGL((seq_conv_sum_kernel<double>), grid, dim3(256), 0, st, (const double *)p.part, p.m.nblk, a->W, a->D, (double *)a->dweight, (double *)a->dbias);
-        else hipLaunchKernelGGL((seq_conv_sum_kernel<float>), grid, dim3(256), 0, st, (const float *)p.part, p.m.nblk, a->W, a->D, (float *)a->dweight, (float *)a->dbias);
+        const int64_t count = (int64_t)(a->W + 1) * a->D;       // [tap][D], then the bias
+        const dim3 grid((unsigned)((count + 31) / 32));
+        if (f64)
+            hipLaunchKernelGGL((crnn::seq_sum_blocks_kernel<double>), grid, dim3(256), 0, st, (const double *)p.part, p.m.nblk, count, (double *)a->dweight, (double *)a->dbias,
+                               a->D, a->W, 0, a->W);
+        else
+            hipLaunchKernelGGL((crnn::seq_sum_blocks_kernel<float>), grid, dim3(256), 0, st, (const float *)p.part, p.m.nblk, count, (float *)a->dweight, (float *)a->dbias, a->D,
+                               a->W, 0, a->W);
         SEQ_DONE("crnn_conv_backward");
     } catch (...) { return -1; }
 }

@@ -64,8 +64,8 @@ __device__ __forceinline__ double seq_softplus(double x) {
 struct SeqV {
     void *p;
     const uint8_t *sc;      // CRNN_DT_PACKED8: one scale byte per 32 channels of a row
-    int64_t bs, rs;         // elements between sequences (dense), between rows
-    int64_t sbs, srs;       // the same of the scales
+    int64_t bs, sbs;        // elements between sequences (dense), and of the scales
+    int32_t rs, srs;        // elements between rows
     int32_t dt;
     int32_t vec;            // base and strides allow whole vectors to be loaded and stored (set by the host for the kernel's vector)
 };
@@ -143,7 +143,7 @@ __device__ __forceinline__ SeqChunk seq_locate(const SeqMap &m, int64_t b) {
 
 // element offset of a view's row t of the chunk's sequence
 __device__ __forceinline__ int64_t seq_off(const SeqMap &m, const SeqV &v, const SeqChunk &k, int64_t t) {
-    return (m.start ? k.begin * v.rs : (int64_t)k.s * v.bs) + t * v.rs;
+    return (m.start ? k.begin * v.rs : (int64_t)k.s * v.bs) + t * (int64_t)v.rs;
 }
 __device__ __forceinline__ int64_t seq_soff(const SeqMap &m, const SeqV &v, const SeqChunk &k, int64_t t) {
     return (m.start ? k.begin * v.srs : (int64_t)k.s * v.sbs) + t * v.srs;
@@ -195,85 +195,141 @@ __device__ __forceinline__ void seq_zero_outside(const SeqMap &m, const SeqV &v,
 }
 
 // TB consecutive rows of one channel on their way into registers: the loads of several arrays are issued before the first one is needed,
-// conversion comes afterwards.  The type is the launch's, so each branch is uniform.
-template <class CT, bool P8, int TB>
+// conversion comes afterwards.  IO: bytes of an element (8: double).  Row addresses are uniform, the lane adds a 32-bit offset; rows
+// behind the n-th are read as the n-th (n >= 1).  P8: the array may be a checkpoint instead.
+template <int IO> struct SeqIO { using C = float; using E = uint32_t; };
+template <> struct SeqIO<2> { using C = float; using E = uint16_t; };
+template <> struct SeqIO<8> { using C = double; using E = double; };
+
+template <int IO, bool P8, int TB>
 struct SeqRows {
-    uint32_t r[TB];
-    uint32_t s[P8 ? TB : 1];
-    __device__ __forceinline__ void load(const SeqMap &m, const SeqV &v, const SeqChunk &k, int64_t t, int64_t d, int n) {
-        const int64_t off = seq_off(m, v, k, t) + d;
+    using CT = typename SeqIO<IO>::C;
+    using E = typename SeqIO<IO>::E;
+    E r[TB];                     // checkpoint: the code, its scale byte above it
+    __device__ __forceinline__ void load(const SeqMap &m, const SeqV &v, const SeqChunk &k, int64_t t, uint32_t d, int n) {
         if (P8 && v.dt == CRNN_DT_PACKED8) {
-            const int64_t so = seq_soff(m, v, k, t) + (d >> 5);
+            const int8_t *c = (const int8_t *)v.p + seq_off(m, v, k, t);
+            const uint8_t *e = v.sc + seq_soff(m, v, k, t);
 #pragma unroll
             for (int i = 0; i < TB; ++i) {
                 const int64_t ii = i < n ? i : n - 1;
-                r[i] = (uint32_t)(int32_t)((const int8_t *)v.p)[off + ii * v.rs];
-                s[P8 ? i : 0] = v.sc[so + ii * v.srs];
+                r[i] = (E)((uint32_t)(uint8_t)(c + ii * v.rs)[d] | (uint32_t)(e + ii * v.srs)[d >> 5] << 8);
             }
-        } else if (v.dt == CRNN_DT_F32) {
-#pragma unroll
-            for (int i = 0; i < TB; ++i) r[i] = ((const uint32_t *)v.p)[off + (int64_t)(i < n ? i : n - 1) * v.rs];
         } else {
+            const E *c = (const E *)v.p + seq_off(m, v, k, t);
 #pragma unroll
-            for (int i = 0; i < TB; ++i) r[i] = ((const uint16_t *)v.p)[off + (int64_t)(i < n ? i : n - 1) * v.rs];
+            for (int i = 0; i < TB; ++i) {
+                const int64_t ii = i < n ? i : n - 1;
+                r[i] = (c + ii * v.rs)[d];
+            }
         }
     }
-    __device__ __forceinline__ void get(const SeqV &v, float (&o)[TB]) const {
+    __device__ __forceinline__ void get(const SeqV &v, CT (&o)[TB]) const {
         if (P8 && v.dt == CRNN_DT_PACKED8) {
 #pragma unroll
-            for (int i = 0; i < TB; ++i) o[i] = (float)(int32_t)r[i] * seq_scale(s[P8 ? i : 0]);
-        } else if (v.dt == CRNN_DT_F32) {
+            for (int i = 0; i < TB; ++i) o[i] = (CT)(int32_t)(int8_t)((uint32_t)r[i] & 0xffu) * (CT)seq_scale((uint32_t)r[i] >> 8);
+        } else if (IO == 8) {
 #pragma unroll
-            for (int i = 0; i < TB; ++i) o[i] = seq_as_float(r[i]);
+            for (int i = 0; i < TB; ++i) o[i] = (CT)r[i];
+        } else if (IO == 4) {
+#pragma unroll
+            for (int i = 0; i < TB; ++i) o[i] = (CT)seq_as_float((uint32_t)r[i]);
         } else if (v.dt == CRNN_DT_BF16) {
 #pragma unroll
-            for (int i = 0; i < TB; ++i) o[i] = seq_as_float(r[i] << 16);
+            for (int i = 0; i < TB; ++i) o[i] = (CT)seq_as_float((uint32_t)r[i] << 16);
         } else {
 #pragma unroll
-            for (int i = 0; i < TB; ++i) o[i] = seq_from_f16(r[i]);
+            for (int i = 0; i < TB; ++i) o[i] = (CT)seq_from_f16((uint32_t)r[i]);
         }
-    }
-};
-template <bool P8, int TB>
-struct SeqRows<double, P8, TB> {
-    double r[TB];
-    __device__ __forceinline__ void load(const SeqMap &m, const SeqV &v, const SeqChunk &k, int64_t t, int64_t d, int n) {
-        const int64_t off = seq_off(m, v, k, t) + d;
-#pragma unroll
-        for (int i = 0; i < TB; ++i) r[i] = ((const double *)v.p)[off + (int64_t)(i < n ? i : n - 1) * v.rs];
-    }
-    __device__ __forceinline__ void get(const SeqV &, double (&o)[TB]) const {
-#pragma unroll
-        for (int i = 0; i < TB; ++i) o[i] = r[i];
     }
 };
 
-// sum over the wavefront's lanes of V values at once: every exchange halves how many values a lane still carries, 2 V lane exchanges
-// in all where separate sums would take 6 V.  Afterwards the lane holds the sum of value seq_spread_index<V>(lane).
+// TB rows of an output from a lane's registers; only the first n are stored
+template <int IO, int TB>
+__device__ __forceinline__ void seq_put_rows(const SeqMap &m, const SeqV &v, const SeqChunk &k, int64_t t, uint32_t d, int n, bool valid, const typename SeqIO<IO>::C (&x)[TB]) {
+    using E = typename SeqIO<IO>::E;
+    E *c = (E *)v.p + seq_off(m, v, k, t);
+    E b[TB];
+#pragma unroll
+    for (int i = 0; i < TB; ++i) {
+        if (IO == 8) b[i] = (E)x[i];
+        else if (IO == 4) b[i] = (E)seq_as_bits((float)x[i]);
+    }
+    if (IO == 2) {
+        if (v.dt == CRNN_DT_BF16) {
+#pragma unroll
+            for (int i = 0; i < TB; ++i) b[i] = (E)seq_to_bf16((float)x[i]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < TB; ++i) b[i] = (E)seq_to_f16((float)x[i]);
+        }
+    }
+    if (!valid) return;
+#pragma unroll
+    for (int i = 0; i < TB; ++i)
+        if (i < n) (c + (int64_t)i * v.rs)[d] = b[i];
+}
+
+// sum over the wavefront's lanes of V values at once: every exchange halves how many values a lane still carries, about 2 V operations in
+// all where separate sums would take 6 V.  Afterwards the lane holds the sum of value seq_spread_index<V>(lane).
 template <int V>
 __device__ __forceinline__ int seq_spread_index(int lane) {
     int idx = 0, w = V / 2;
     for (int bit = 32; w >= 1; bit >>= 1, w >>= 1) idx += (lane & bit) ? w : 0;
     return idx;
 }
-template <int V, class CT>
-__device__ __forceinline__ CT seq_spread_sum(CT (&v)[V]) {
-    const int lane = threadIdx.x & 63;
-    int bit = 32;
-#pragma unroll
-    for (int w = V / 2; w >= 1; w >>= 1) {
-        const bool hi = (lane & bit) != 0;
-#pragma unroll
-        for (int j = 0; j < w; ++j) {
-            const CT send = hi ? v[j] : v[j + w], keep = hi ? v[j + w] : v[j];
-            v[j] = keep + __shfl_xor(send, bit);
-        }
-        bit >>= 1;
-    }
-    for (; bit >= 1; bit >>= 1) v[0] += __shfl_xor(v[0], bit);
-    return v[0];
+// float: the exchanges across 32 and 16 lanes are the swaps of half registers, the closer ones lane moves inside a row of 16 (DPP: by 8
+// within the row, mirrored halves, pairs, neighbours; a mirrored partner differs in the bit in question and that is all it takes)
+template <int CTRL>
+__device__ __forceinline__ float seq_dpp(float x) {
+    return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), CTRL, 0xf, 0xf, true));
 }
-
+template <int CTRL>
+__device__ __forceinline__ float seq_fold(float a, float b, bool hi) {
+    const float send = hi ? a : b, keep = hi ? b : a;
+    return keep + seq_dpp<CTRL>(send);
+}
+// one exchange of the two largest: lanes below / from bit 32 on (16) carry a / b on
+__device__ __forceinline__ float seq_fold32(float a, float b) {
+    const auto s = __builtin_amdgcn_permlane32_swap(seq_as_bits(a), seq_as_bits(b), false, false);
+    return seq_as_float(s[0]) + seq_as_float(s[1]);
+}
+__device__ __forceinline__ float seq_fold16(float a, float b) {
+    const auto s = __builtin_amdgcn_permlane16_swap(seq_as_bits(a), seq_as_bits(b), false, false);
+    return seq_as_float(s[0]) + seq_as_float(s[1]);
+}
+__device__ __forceinline__ double seq_fold32(double a, double b) {
+    const bool hi = (threadIdx.x & 32) != 0;
+    return (hi ? b : a) + __shfl_xor(hi ? a : b, 32);
+}
+__device__ __forceinline__ double seq_fold16(double a, double b) {
+    const bool hi = (threadIdx.x & 16) != 0;
+    return (hi ? b : a) + __shfl_xor(hi ? a : b, 16);
+}
+template <int CTRL>
+__device__ __forceinline__ double seq_fold(double a, double b, bool hi) {
+    constexpr int BIT = CTRL == 0x128 ? 8 : CTRL == 0x141 ? 4 : CTRL == 0x4e ? 2 : 1;
+    return (hi ? b : a) + __shfl_xor(hi ? a : b, BIT);
+}
+template <int CTRL>
+__device__ __forceinline__ double seq_dpp(double x) {
+    constexpr int BIT = CTRL == 0x128 ? 8 : CTRL == 0x141 ? 4 : CTRL == 0x4e ? 2 : 1;
+    return __shfl_xor(x, BIT);
+}
+// the exchanges within 16 lanes of the F values that are left after those across 32 and 16
+template <int F, class CT>
+__device__ __forceinline__ CT seq_spread_rest(CT (&v)[F]) {
+    static_assert(F == 4 || F == 8, "values of a row");
+    const int lane = threadIdx.x & 63;
+    const bool b8 = (lane & 8) != 0, b4 = (lane & 4) != 0, b2 = (lane & 2) != 0;
+#pragma unroll
+    for (int j = 0; j < F / 2; ++j) v[j] = seq_fold<0x128>(v[j], v[j + F / 2], b8);
+#pragma unroll
+    for (int j = 0; j < F / 4; ++j) v[j] = seq_fold<0x141>(v[j], v[j + F / 4], b4);
+    if (F == 8) v[0] = seq_fold<0x4e>(v[0], v[F == 8 ? 1 : 0], b2);
+    else v[0] += seq_dpp<0x4e>(v[0]);
+    return v[0] + seq_dpp<0xb1>(v[0]);
+}
 // Rows of one launch that name the same slot are consecutive rows of that sequence: the first of them in row order does them all.
 // A thread finds for row r whether an earlier row has its slot, and which row is the next.
 __device__ __forceinline__ void seq_same_slot(const int32_t *slot, int64_t rows, int64_t r, int *before, int *next) {

@@ -322,7 +322,7 @@ __global__ __launch_bounds__(256) void seq_conv_step_kernel(const ConvStepP p) {
     if (!there) {
 #pragma unroll
         for (int i = 0; i < kConvV; ++i) bias[i] = CT(0);
-        if (on) conv_store<YT>(p.y, r * p.y.rs + d, d, p.D, bias);
+        if (on) conv_store<YT>(p.y, r * (int64_t)p.y.rs + d, d, p.D, bias);
         return;
     }
     ConvP q;
@@ -339,7 +339,7 @@ __global__ __launch_bounds__(256) void seq_conv_step_kernel(const ConvStepP p) {
     }
     for (;;) {
         CT y[kConvV];
-        conv_load<YT>(p.x, r * p.x.rs + at, 0, at, p.D, x[WM - 1]);
+        conv_load<YT>(p.x, r * (int64_t)p.x.rs + at, 0, at, p.D, x[WM - 1]);
 #pragma unroll
         for (int i = 0; i < kConvV; ++i) {
             CT s = bias[i];
@@ -349,7 +349,7 @@ __global__ __launch_bounds__(256) void seq_conv_step_kernel(const ConvStepP p) {
 #pragma unroll
             for (int j = 0; j < WM - 1; ++j) x[j][i] = x[j + 1][i];
         }
-        if (on) conv_store<YT>(p.y, r * p.y.rs + d, d, p.D, y);
+        if (on) conv_store<YT>(p.y, r * (int64_t)p.y.rs + d, d, p.D, y);
         if (nx < 0) break;
         r = nx;
         __syncthreads();

@@ -59,7 +59,7 @@ __global__ __launch_bounds__(256) void seq_pack_kernel(const PackP p) {
     uint32_t m = 0;                                       // |x| as bits: ordered like the values, NaN above all
 #pragma unroll
     for (int k = 0; k < kPackV; ++k) x[k] = 0.0f;
-    if (d < p.D) pack_load<DT>(p.x, r * p.x.rs + d, d, p.D, x);
+    if (d < p.D) pack_load<DT>(p.x, r * (int64_t)p.x.rs + d, d, p.D, x);
 #pragma unroll
     for (int k = 0; k < kPackV; ++k) {
         const uint32_t b = seq_as_bits(x[k]) & 0x7fffffffu;
@@ -112,7 +112,7 @@ __global__ __launch_bounds__(256) void seq_unpack_kernel(const PackP p) {
     if (r >= p.rows || d >= p.D) return;
     const float e = seq_scale(p.sc[r * p.nb + d / 32]);
     const int8_t *q = p.q + r * p.D + d;
-    const int64_t off = r * p.x.rs + d;
+    const int64_t off = r * (int64_t)p.x.rs + d;
     typedef uint32_t U4 __attribute__((ext_vector_type(4)));
     if (p.vecq && p.x.vec && d + kPackV <= p.D) {
         const U4 b = *(const U4 *)q;

@@ -99,15 +99,35 @@ __device__ __forceinline__ void scan_state_put(const ScanP &p, void *st, int64_t
     for (int n = 0; n < NS; ++n)
         if (p.n0 + n < p.N) ((CT *)st)[(s * p.D + d) * p.N + p.n0 + n] = h[n];
 }
-template <class CT>
-__device__ __forceinline__ CT scan_delta(const ScanP &p, CT x, CT bias, CT &pre) {
-    pre = x + bias;
-    return p.softplus ? seq_softplus(pre) : pre;
+// step lengths and inputs of TB rows; rows behind the n-th become steps of length 0 with nothing to add, so that the rows need no branches
+template <int IO, int TB>
+__device__ __forceinline__ void scan_steps(const ScanP &p, int n, typename SeqIO<IO>::C bias, typename SeqIO<IO>::C (&x)[TB], typename SeqIO<IO>::C (&u)[TB],
+                                           typename SeqIO<IO>::C (&dl)[TB]) {
+    using CT = typename SeqIO<IO>::C;
+#pragma unroll
+    for (int i = 0; i < TB; ++i) x[i] += bias;
+    if (p.softplus) {
+#pragma unroll
+        for (int i = 0; i < TB; ++i) dl[i] = seq_softplus(x[i]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < TB; ++i) dl[i] = x[i];
+    }
+    if (n < TB) {
+#pragma unroll
+        for (int i = 0; i < TB; ++i) {
+            dl[i] = i < n ? dl[i] : CT(0);
+            u[i] = i < n ? u[i] : CT(0);
+        }
+    }
 }
 
 // ---- forward: outputs of a chunk from its first state (start[block][n][d]; null: one chunk a sequence, from state_in)
-template <class CT, int NS, bool P8>
-__global__ __launch_bounds__(64 * kScanWaves) void seq_scan_out_kernel(const ScanP p, const CT *__restrict__ maps, const CT *__restrict__ start) {
+template <int IO, int NS, bool P8>
+__global__ __launch_bounds__(64 * kScanWaves) void seq_scan_out_kernel(const ScanP p, const typename SeqIO<IO>::C *__restrict__ maps,
+                                                                       const typename SeqIO<IO>::C *__restrict__ start) {
+    using CT = typename SeqIO<IO>::C;
+    constexpr int TB = kScanTB;
     const ScanAt a = scan_at(p);
     if (!a.on) return;
     if (p.zero_outside && p.fin) seq_zero_outside(p.m, p.y, a.b, a.d, a.valid);
@@ -121,52 +141,65 @@ __global__ __launch_bounds__(64 * kScanWaves) void seq_scan_out_kernel(const Sca
         scan_state<CT, NS>(p, p.state_in, a.k.s, a.d, h);
     }
     const CT bias = p.dt_bias ? ((const CT *)p.dt_bias)[a.d] : CT(0), skip = p.Dskip ? ((const CT *)p.Dskip)[a.d] : CT(0);
-    SeqRows<CT, P8, kScanTB> ru, rz;
-    SeqRows<CT, false, kScanTB> rd;
-    int t = 0;
+    const bool gate = p.z.p && p.fin;
+    SeqRows<IO, P8, TB> ru, rz;
+    SeqRows<IO, false, TB> rd;
     if (a.k.n > 0) {
-        const int nv = a.k.n < kScanTB ? a.k.n : kScanTB;
+        const int nv = a.k.n < TB ? a.k.n : TB;
         ru.load(p.m, p.u, a.k, a.k.t0, a.d, nv);
         rd.load(p.m, p.dt, a.k, a.k.t0, a.d, nv);
-        if (p.z.p && p.fin) rz.load(p.m, p.z, a.k, a.k.t0, a.d, nv);
+        if (gate) rz.load(p.m, p.z, a.k, a.k.t0, a.d, nv);
     }
-    for (; t < a.k.n; t += kScanTB) {
-        const int nv = a.k.n - t < kScanTB ? a.k.n - t : kScanTB;
-        CT u[kScanTB], x[kScanTB], z[kScanTB];
+#pragma unroll 1
+    for (int t = 0; t < a.k.n; t += TB) {
+        const int left = a.k.n - t, nv = left < TB ? left : TB;
+        CT u[TB], x[TB], z[TB], dl[TB], v[TB];
         ru.get(p.u, u);
         rd.get(p.dt, x);
-        if (p.z.p && p.fin) rz.get(p.z, z);
-        const int left = a.k.n - t - kScanTB;
-        if (left > 0) {
-            const int nn = left < kScanTB ? left : kScanTB;
-            ru.load(p.m, p.u, a.k, a.k.t0 + t + kScanTB, a.d, nn);
-            rd.load(p.m, p.dt, a.k, a.k.t0 + t + kScanTB, a.d, nn);
-            if (p.z.p && p.fin) rz.load(p.m, p.z, a.k, a.k.t0 + t + kScanTB, a.d, nn);
+        if (gate) rz.get(p.z, z);
+        if (left > TB) {
+            const int nn = left - TB < TB ? left - TB : TB;
+            ru.load(p.m, p.u, a.k, a.k.t0 + t + TB, a.d, nn);
+            rd.load(p.m, p.dt, a.k, a.k.t0 + t + TB, a.d, nn);
+            if (gate) rz.load(p.m, p.z, a.k, a.k.t0 + t + TB, a.d, nn);
         }
-        const CT *row = maps + ((a.k.flat + a.k.t0 + t) * p.G + a.g) * (2 * NS);
-        const int64_t yo = seq_off(p.m, p.y, a.k, a.k.t0 + t) + a.d, ao = (a.k.flat + a.k.t0 + t) * p.D + a.d;
+        scan_steps<IO, TB>(p, nv, bias, x, u, dl);
+        const int64_t frow = a.k.flat + a.k.t0 + t;
+        const CT *row = maps + (frow * p.G + a.g) * (2 * NS);
+        const int64_t step = (int64_t)p.G * (2 * NS);
 #pragma unroll
-        for (int i = 0; i < kScanTB; ++i) {
-            if (i >= nv) break;
-            CT pre;
-            const CT dl = scan_delta(p, x[i], bias, pre), du = dl * u[i];
-            const CT *bc = row + (int64_t)i * p.G * (2 * NS);
-            CT v = CT(0);
+        for (int i = 0; i < TB; ++i) {
+            const CT *bc = row + (i < nv ? i : nv - 1) * step;
+            const CT du = dl[i] * u[i];
+            CT s0 = CT(0), s1 = CT(0);
 #pragma unroll
-            for (int n = 0; n < NS; ++n) {
-                h[n] = seq_fma(seq_exp2(dl * A2[n]), h[n], du * bc[n]);
-                v = seq_fma(h[n], bc[NS + n], v);
+            for (int n = 0; n < NS; n += 2) {
+                h[n] = seq_fma(seq_exp2(dl[i] * A2[n]), h[n], du * bc[n]);
+                h[n + 1] = seq_fma(seq_exp2(dl[i] * A2[n + 1]), h[n + 1], du * bc[n + 1]);
+                s0 = seq_fma(h[n], bc[NS + n], s0);
+                s1 = seq_fma(h[n + 1], bc[NS + n + 1], s1);
             }
-            if (p.acc) {
-                CT *acc = (CT *)p.acc + ao + (int64_t)i * p.D;
-                if (!p.first) v += *acc;
-                if (!p.fin && a.valid) *acc = v;
+            v[i] = s0 + s1;
+        }
+        if (p.acc) {
+            for (int i = 0; i < nv; ++i) {
+                CT *acc = (CT *)p.acc + (frow + i) * p.D + a.d;
+#pragma unroll
+                for (int j = 0; j < TB; ++j)
+                    if (j == i) {
+                        if (!p.first) v[j] += *acc;
+                        if (!p.fin && a.valid) *acc = v[j];
+                    }
             }
-            if (p.fin) {
-                v = seq_fma(skip, u[i], v);
-                if (p.z.p) v = v * (z[i] * seq_sigmoid(z[i]));
-                if (a.valid) seq_store(p.y, yo + (int64_t)i * p.y.rs, v);
+        }
+        if (p.fin) {
+#pragma unroll
+            for (int i = 0; i < TB; ++i) v[i] = seq_fma(skip, u[i], v[i]);
+            if (gate) {
+#pragma unroll
+                for (int i = 0; i < TB; ++i) v[i] *= z[i] * seq_sigmoid(z[i]);
             }
+            seq_put_rows<IO, TB>(p.m, p.y, a.k, a.k.t0 + t, a.d, nv, a.valid, v);
         }
     }
     if (a.k.last && p.state_out && a.valid) scan_state_put<CT, NS>(p, p.state_out, a.k.s, a.d, h);
@@ -174,9 +207,12 @@ __global__ __launch_bounds__(64 * kScanWaves) void seq_scan_out_kernel(const Sca
 
 // ---- a chunk by itself: S = its last state from zero, sum of delta; BOTH: also G = what its outputs' gradients r pass back to the state
 // before it, sum_t (prod of the decays up to t) r C -- taken in the forward direction, so that one exponential serves both.
-template <class CT, int NS, bool P8, bool BOTH>
-__global__ __launch_bounds__(64 * kScanWaves) void seq_scan_ends_kernel(const ScanP p, const CT *__restrict__ maps, CT *__restrict__ S, CT *__restrict__ Gb,
-                                                                        CT *__restrict__ sdel) {
+template <int IO, int NS, bool P8, bool BOTH>
+__global__ __launch_bounds__(64 * kScanWaves) void seq_scan_ends_kernel(const ScanP p, const typename SeqIO<IO>::C *__restrict__ maps,
+                                                                        typename SeqIO<IO>::C *__restrict__ S, typename SeqIO<IO>::C *__restrict__ Gb,
+                                                                        typename SeqIO<IO>::C *__restrict__ sdel) {
+    using CT = typename SeqIO<IO>::C;
+    constexpr int TB = BOTH ? kScanTB / 2 : kScanTB;
     const ScanAt a = scan_at(p);
     if (!a.on || !a.k.live) return;
     CT A2[NS], h[NS], P[BOTH ? NS : 1], g[BOTH ? NS : 1];
@@ -187,41 +223,55 @@ __global__ __launch_bounds__(64 * kScanWaves) void seq_scan_ends_kernel(const Sc
         if (BOTH) { P[BOTH ? n : 0] = CT(1); g[BOTH ? n : 0] = CT(0); }
     }
     const CT bias = p.dt_bias ? ((const CT *)p.dt_bias)[a.d] : CT(0);
+    const bool gate = BOTH && p.z.p;
     CT sd = CT(0);
-    for (int t = 0; t < a.k.n; t += kScanTB) {
-        const int nv = a.k.n - t < kScanTB ? a.k.n - t : kScanTB;
-        SeqRows<CT, P8, kScanTB> ru, rz;
-        SeqRows<CT, false, kScanTB> rd, ry;
-        CT u[kScanTB], x[kScanTB], z[kScanTB], y[kScanTB];
-        ru.load(p.m, p.u, a.k, a.k.t0 + t, a.d, nv);
-        rd.load(p.m, p.dt, a.k, a.k.t0 + t, a.d, nv);
-        if (BOTH) {
-            ry.load(p.m, p.dy, a.k, a.k.t0 + t, a.d, nv);
-            if (p.z.p) rz.load(p.m, p.z, a.k, a.k.t0 + t, a.d, nv);
-        }
+    SeqRows<IO, P8, TB> ru, rz;
+    SeqRows<IO, false, TB> rd, ry;
+    if (a.k.n > 0) {
+        const int nv = a.k.n < TB ? a.k.n : TB;
+        ru.load(p.m, p.u, a.k, a.k.t0, a.d, nv);
+        rd.load(p.m, p.dt, a.k, a.k.t0, a.d, nv);
+        if (BOTH) ry.load(p.m, p.dy, a.k, a.k.t0, a.d, nv);
+        if (gate) rz.load(p.m, p.z, a.k, a.k.t0, a.d, nv);
+    }
+#pragma unroll 1
+    for (int t = 0; t < a.k.n; t += TB) {
+        const int left = a.k.n - t, nv = left < TB ? left : TB;
+        CT u[TB], x[TB], z[TB], y[TB], dl[TB];
         ru.get(p.u, u);
         rd.get(p.dt, x);
-        if (BOTH) {
-            ry.get(p.dy, y);
-            if (p.z.p) rz.get(p.z, z);
+        if (BOTH) ry.get(p.dy, y);
+        if (gate) rz.get(p.z, z);
+        if (left > TB) {
+            const int nn = left - TB < TB ? left - TB : TB;
+            ru.load(p.m, p.u, a.k, a.k.t0 + t + TB, a.d, nn);
+            rd.load(p.m, p.dt, a.k, a.k.t0 + t + TB, a.d, nn);
+            if (BOTH) ry.load(p.m, p.dy, a.k, a.k.t0 + t + TB, a.d, nn);
+            if (gate) rz.load(p.m, p.z, a.k, a.k.t0 + t + TB, a.d, nn);
+        }
+        scan_steps<IO, TB>(p, nv, bias, x, u, dl);
+        if (gate) {
+#pragma unroll
+            for (int i = 0; i < TB; ++i) y[i] *= z[i] * seq_sigmoid(z[i]);
+        }
+        if (BOTH && nv < TB) {
+#pragma unroll
+            for (int i = 0; i < TB; ++i) y[i] = i < nv ? y[i] : CT(0);
         }
         const CT *row = maps + ((a.k.flat + a.k.t0 + t) * p.G + a.g) * (2 * NS);
+        const int64_t step = (int64_t)p.G * (2 * NS);
 #pragma unroll
-        for (int i = 0; i < kScanTB; ++i) {
-            if (i >= nv) break;
-            CT pre;
-            const CT dl = scan_delta(p, x[i], bias, pre), du = dl * u[i];
-            sd += dl;
-            const CT *bc = row + (int64_t)i * p.G * (2 * NS);
-            CT r = CT(0);
-            if (BOTH) r = p.z.p ? y[i] * (z[i] * seq_sigmoid(z[i])) : y[i];
+        for (int i = 0; i < TB; ++i) {
+            const CT *bc = row + (i < nv ? i : nv - 1) * step;
+            const CT du = dl[i] * u[i];
+            sd += dl[i];
 #pragma unroll
             for (int n = 0; n < NS; ++n) {
-                const CT e = seq_exp2(dl * A2[n]);
+                const CT e = seq_exp2(dl[i] * A2[n]);
                 h[n] = seq_fma(e, h[n], du * bc[n]);
                 if (BOTH) {
                     P[BOTH ? n : 0] *= e;
-                    g[BOTH ? n : 0] = seq_fma(P[BOTH ? n : 0], r * bc[NS + n], g[BOTH ? n : 0]);
+                    g[BOTH ? n : 0] = seq_fma(P[BOTH ? n : 0], y[i] * bc[NS + n], g[BOTH ? n : 0]);
                 }
             }
         }
@@ -267,17 +317,20 @@ __global__ __launch_bounds__(256) void seq_scan_carry_kernel(const ScanP p, CT *
     if (p.dstate_in) ((CT *)p.dstate_in)[at] = q;
 }
 
-// ---- adjoint of a chunk of at most kScanBwdQ rows.  Forward over the chunk once, keeping every kScanTB-th state in LDS; then, from the
-// last kScanTB rows to the first: the states of those rows once more, a h[t - 1] of each row kept in registers (NS x kScanTB of them;
+// ---- adjoint of a chunk of at most kScanBwdQ rows.  Forward over the chunk once, keeping the state in front of every kScanBwdTB rows in LDS; then,
+// from the last kScanBwdTB rows to the first: those rows once more, each row's decay a and a h[t - 1] kept in registers (2 NS x kScanBwdTB;
 // h[t] is one multiply-add away, and dA needs the product itself), and the reverse sweep over them.  dB and dC are sums over channels: a
 // wavefront's part goes to part[tile][row][B: NS | C: NS], summed over the tiles in a fixed order by seq_scan_sum_maps_kernel.
-constexpr int kScanBwdQ = 4 * kScanTB;
-template <class CT, int NS, bool P8>
-__global__ __launch_bounds__(64 * kScanWaves) void seq_scan_bwd_kernel(const ScanP p, const CT *__restrict__ maps, const CT *__restrict__ start,
-                                                                       const CT *__restrict__ back, CT *__restrict__ part, CT *__restrict__ dApart,
-                                                                       CT *__restrict__ dDpart, CT *__restrict__ dbpart) {
-    constexpr int TB = kScanTB, NSUB = kScanBwdQ / kScanTB;
-    __shared__ CT keep[kScanWaves][NSUB - 1][NS][64];
+// Four rows and six times four a chunk: two wavefronts a SIMD fill the registers (256 a lane) and the LDS (20 KB each) together.
+constexpr int kScanBwdTB = 4, kScanBwdSub = 6, kScanBwdQ = kScanBwdTB * kScanBwdSub;
+template <int IO, int NS, bool P8>
+__global__ __launch_bounds__(64 * kScanWaves, 2) void seq_scan_bwd_kernel(const ScanP p, const typename SeqIO<IO>::C *__restrict__ maps,
+                                                                          const typename SeqIO<IO>::C *__restrict__ start, const typename SeqIO<IO>::C *__restrict__ back,
+                                                                          typename SeqIO<IO>::C *__restrict__ part, typename SeqIO<IO>::C *__restrict__ dApart,
+                                                                          typename SeqIO<IO>::C *__restrict__ dDpart, typename SeqIO<IO>::C *__restrict__ dbpart) {
+    using CT = typename SeqIO<IO>::C;
+    constexpr int TB = kScanBwdTB, H = NS / 2;
+    __shared__ CT keep[kScanWaves][kScanBwdSub - 1][NS][64];
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
     const ScanAt a = scan_at(p);
     if (!a.on) return;
@@ -298,100 +351,121 @@ __global__ __launch_bounds__(64 * kScanWaves) void seq_scan_bwd_kernel(const Sca
             q[n] = back[(a.b * NS + n) * p.D + a.d];
         }
         const CT bias = p.dt_bias ? ((const CT *)p.dt_bias)[a.d] : CT(0), skip = p.Dskip ? ((const CT *)p.Dskip)[a.d] : CT(0);
+        const int64_t step = (int64_t)p.G * (2 * NS);
         const int nsub = (a.k.n + TB - 1) / TB;
+#pragma unroll 1
         for (int k = 0; k < nsub - 1; ++k) {
-            SeqRows<CT, P8, TB> ru;
-            SeqRows<CT, false, TB> rd;
-            CT u[TB], x[TB];
+            SeqRows<IO, P8, TB> ru;
+            SeqRows<IO, false, TB> rd;
+            CT u[TB], x[TB], dl[TB];
             ru.load(p.m, p.u, a.k, a.k.t0 + k * TB, a.d, TB);
             rd.load(p.m, p.dt, a.k, a.k.t0 + k * TB, a.d, TB);
             ru.get(p.u, u);
             rd.get(p.dt, x);
+            scan_steps<IO, TB>(p, TB, bias, x, u, dl);
             const CT *row = maps + ((a.k.flat + a.k.t0 + k * TB) * p.G + a.g) * (2 * NS);
 #pragma unroll
             for (int i = 0; i < TB; ++i) {
-                CT pre;
-                const CT dl = scan_delta(p, x[i], bias, pre), du = dl * u[i];
-                const CT *bc = row + (int64_t)i * p.G * (2 * NS);
+                const CT *bc = row + i * step;
+                const CT du = dl[i] * u[i];
 #pragma unroll
-                for (int n = 0; n < NS; ++n) h[n] = seq_fma(seq_exp2(dl * A2[n]), h[n], du * bc[n]);
+                for (int n = 0; n < NS; ++n) h[n] = seq_fma(seq_exp2(dl[i] * A2[n]), h[n], du * bc[n]);
             }
 #pragma unroll
             for (int n = 0; n < NS; ++n) keep[wave][k][n][lane] = h[n];
         }
+#pragma unroll 1
         for (int k = nsub - 1; k >= 0; --k) {
             const int nv = a.k.n - k * TB < TB ? a.k.n - k * TB : TB;
-            const int64_t t = a.k.t0 + k * TB;
-            SeqRows<CT, P8, TB> ru, rz;
-            SeqRows<CT, false, TB> rd, ry;
-            CT u[TB], x[TB], z[TB], y[TB], ah[TB][NS];
-            ru.load(p.m, p.u, a.k, t, a.d, nv);
-            rd.load(p.m, p.dt, a.k, t, a.d, nv);
-            ry.load(p.m, p.dy, a.k, t, a.d, nv);
-            if (p.z.p) rz.load(p.m, p.z, a.k, t, a.d, nv);
+            const int64_t t = a.k.t0 + k * TB, frow = a.k.flat + t;
+            CT u[TB], x[TB], z[TB], y[TB], dl[TB], ah[TB][NS], e[TB][NS];
+            {
+                SeqRows<IO, P8, TB> ru, rz;
+                SeqRows<IO, false, TB> rd, ry;
+                ru.load(p.m, p.u, a.k, t, a.d, nv);
+                rd.load(p.m, p.dt, a.k, t, a.d, nv);
+                ry.load(p.m, p.dy, a.k, t, a.d, nv);
+                if (p.z.p) rz.load(p.m, p.z, a.k, t, a.d, nv);
+                ru.get(p.u, u);
+                rd.get(p.dt, x);
+                ry.get(p.dy, y);
+                if (p.z.p) rz.get(p.z, z);
+            }
+            if (nv < TB) {
 #pragma unroll
-            for (int n = 0; n < NS; ++n) h[n] = k ? keep[wave][k - 1][n][lane] : start[(a.b * NS + n) * p.D + a.d];
-            ru.get(p.u, u);
-            rd.get(p.dt, x);
-            ry.get(p.dy, y);
-            if (p.z.p) rz.get(p.z, z);
-            const int64_t frow = a.k.flat + t;
+                for (int i = 0; i < TB; ++i) {
+                    y[i] = i < nv ? y[i] : CT(0);
+                    z[i] = i < nv ? z[i] : CT(0);
+                }
+            }
+#pragma unroll
+            for (int n = 0; n < NS; ++n) h[n] = keep[wave][k > 0 ? k - 1 : 0][n][lane];
+            if (k == 0) {
+#pragma unroll
+                for (int n = 0; n < NS; ++n) h[n] = start[(a.b * NS + n) * p.D + a.d];
+            }
+            scan_steps<IO, TB>(p, nv, bias, x, u, dl);
             const CT *row = maps + (frow * p.G + a.g) * (2 * NS);
 #pragma unroll
             for (int i = 0; i < TB; ++i) {
-                if (i >= nv) break;
-                CT pre;
-                const CT dl = scan_delta(p, x[i], bias, pre), du = dl * u[i];
-                const CT *bc = row + (int64_t)i * p.G * (2 * NS);
+                const CT *bc = row + (i < nv ? i : nv - 1) * step;
+                const CT du = dl[i] * u[i];
 #pragma unroll
                 for (int n = 0; n < NS; ++n) {
-                    ah[i][n] = seq_exp2(dl * A2[n]) * h[n];
+                    e[i][n] = seq_exp2(dl[i] * A2[n]);
+                    ah[i][n] = e[i][n] * h[n];
                     h[n] = seq_fma(du, bc[n], ah[i][n]);
                 }
             }
-            const int64_t uo = seq_off(p.m, p.du, a.k, t) + a.d, to = seq_off(p.m, p.ddt, a.k, t) + a.d, zo = p.dz.p ? seq_off(p.m, p.dz, a.k, t) + a.d : 0;
+            CT odu[TB], odt[TB], odz[TB];
 #pragma unroll
             for (int i = TB - 1; i >= 0; --i) {
-                if (i >= nv) continue;
-                CT pre;
-                const CT dl = scan_delta(p, x[i], bias, pre), du = dl * u[i];
+                const CT du = dl[i] * u[i];
                 const CT sg = p.z.p ? seq_sigmoid(z[i]) : CT(1);
                 const CT r = p.z.p ? y[i] * (z[i] * sg) : y[i];
-                const CT *bc = row + (int64_t)i * p.G * (2 * NS);
-                CT v = CT(0), qb = CT(0), qa = CT(0), w[2 * NS];
+                const CT *bc = row + (i < nv ? i : nv - 1) * step;
+                CT v = CT(0), qb = CT(0), qa = CT(0), f[H];
+                const CT duv = a.valid ? du : CT(0), rv = a.valid ? r : CT(0);
 #pragma unroll
-                for (int n = 0; n < NS; ++n) {
-                    const CT hn = seq_fma(du, bc[n], ah[i][n]);
-                    q[n] = seq_fma(r, bc[NS + n], q[n]);
-                    v = seq_fma(hn, bc[NS + n], v);
-                    qb = seq_fma(q[n], bc[n], qb);
-                    const CT m = q[n] * ah[i][n];
-                    qa = seq_fma(m, A2[n], qa);
-                    dA[n] = seq_fma(m, dl, dA[n]);
-                    w[n] = a.valid ? q[n] * du : CT(0);
-                    w[NS + n] = a.valid ? r * hn : CT(0);
-                    q[n] *= seq_exp2(dl * A2[n]);
+                for (int j = 0; j < H; ++j) {       // states j and j + NS / 2 together: their parts of dB, dC fold at once
+                    CT w[2];
+#pragma unroll
+                    for (int s = 0; s < 2; ++s) {
+                        const int n = j + s * H;
+                        const CT hn = seq_fma(du, bc[n], ah[i][n]);
+                        q[n] = seq_fma(r, bc[NS + n], q[n]);
+                        v = seq_fma(hn, bc[NS + n], v);
+                        qb = seq_fma(q[n], bc[n], qb);
+                        const CT m = q[n] * ah[i][n];
+                        qa = seq_fma(m, A2[n], qa);
+                        dA[n] = seq_fma(m, dl[i], dA[n]);
+                        w[s] = seq_fold32(q[n] * duv, rv * hn);
+                        q[n] *= e[i][n];
+                    }
+                    f[j] = seq_fold16(w[0], w[1]);
                 }
-                const CT sum = seq_spread_sum<2 * NS>(w);
-                if ((lane & (64 / (2 * NS) - 1)) == 0)
+                const CT sum = seq_spread_rest(f);
+                if (i < nv && (lane & (64 / (2 * NS) - 1)) == 0)
                     part[((int64_t)a.tile * p.acc_n + frow + i) * (2 * NS) + seq_spread_index<2 * NS>(lane)] = sum;
-                if (p.acc) {
+                if (p.acc && i < nv) {
                     CT *acc = (CT *)p.acc + (frow + i) * p.D + a.d;
                     const int64_t stride = p.acc_n * p.D;
                     if (!p.first) { v += acc[0]; qb += acc[stride]; qa += acc[2 * stride]; }
                     if (!p.fin && a.valid) { acc[0] = v; acc[stride] = qb; acc[2 * stride] = qa; }
                 }
-                if (p.fin) {
-                    CT ddt = seq_fma(qa, CT(0.6931471805599453), qb * u[i]);
-                    if (p.softplus) ddt *= seq_sigmoid(pre);
-                    dD = seq_fma(r, u[i], dD);
-                    db += ddt;
-                    if (a.valid) {
-                        seq_store(p.du, uo + (int64_t)i * p.du.rs, seq_fma(dl, qb, r * skip));
-                        seq_store(p.ddt, to + (int64_t)i * p.ddt.rs, ddt);
-                        if (p.dz.p) seq_store(p.dz, zo + (int64_t)i * p.dz.rs, y[i] * seq_fma(skip, u[i], v) * (sg * seq_fma(z[i], CT(1) - sg, CT(1))));
-                    }
-                }
+                CT ddt = seq_fma(qa, CT(0.6931471805599453), qb * u[i]);
+                if (p.softplus) ddt *= seq_sigmoid(x[i]);
+                ddt = i < nv ? ddt : CT(0);
+                dD = seq_fma(r, u[i], dD);
+                db += ddt;
+                odu[i] = seq_fma(dl[i], qb, r * skip);
+                odt[i] = ddt;
+                odz[i] = y[i] * seq_fma(skip, u[i], v) * (sg * seq_fma(z[i], CT(1) - sg, CT(1)));
+            }
+            if (p.fin) {
+                seq_put_rows<IO, TB>(p.m, p.du, a.k, t, a.d, nv, a.valid, odu);
+                seq_put_rows<IO, TB>(p.m, p.ddt, a.k, t, a.d, nv, a.valid, odt);
+                if (p.dz.p) seq_put_rows<IO, TB>(p.m, p.dz, a.k, t, a.d, nv, a.valid, odz);
             }
         }
     }
@@ -422,16 +496,34 @@ __global__ __launch_bounds__(256) void seq_scan_sum_maps_kernel(const SeqMap m, 
     }
 }
 
-// ---- sums over the chunk blocks, in order and in double: in[block][count] -> out.  transposed: count = NS x D, out[d][N] at n0
+// ---- sums over the blocks of a launch, in double and in a fixed order: in[block][count] -> out.  A thread block takes 32 neighbouring columns, eight
+// threads each every eighth block of its own, then one of them adds the eight.  Column i goes to out[(i % D) width + off + i / D] while i / D <
+// lim (a [width][D] array transposed: width 1 leaves it as it is), the others to rest[i % D] (may be null).
 template <class CT>
-__global__ __launch_bounds__(256) void seq_sum_blocks_kernel(const CT *__restrict__ in, int64_t nblk, int64_t count, CT *__restrict__ out, int32_t D, int32_t N, int32_t n0) {
-    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (i >= count) return;
+__global__ __launch_bounds__(256) void seq_sum_blocks_kernel(const CT *__restrict__ in, int64_t nblk, int64_t count, CT *__restrict__ out, CT *__restrict__ rest, int32_t D,
+                                                             int32_t width, int32_t off, int32_t lim) {
+    __shared__ double sh[8][32];
+    const int col = threadIdx.x & 31, k = threadIdx.x >> 5;
+    const int64_t i = (int64_t)blockIdx.x * 32 + col;
     double s = 0.0;
-    for (int64_t b = 0; b < nblk; ++b) s += (double)in[b * count + i];
-    if (N <= 0) { out[i] = (CT)s; return; }
-    const int64_t n = n0 + i / D, d = i % D;
-    if (n < N) out[d * N + n] = (CT)s;
+    if (i < count) {
+        int64_t b = k;
+        for (; b + 24 < nblk; b += 32) {
+            const CT x0 = in[b * count + i], x1 = in[(b + 8) * count + i], x2 = in[(b + 16) * count + i], x3 = in[(b + 24) * count + i];
+            s += (double)x0;
+            s += (double)x1;
+            s += (double)x2;
+            s += (double)x3;
+        }
+        for (; b < nblk; b += 8) s += (double)in[b * count + i];
+    }
+    sh[k][col] = s;
+    __syncthreads();
+    if (k || i >= count) return;
+    for (int j = 1; j < 8; ++j) s += sh[j][col];
+    const int64_t j = i / D, d = i % D;
+    if (j < lim) out[d * width + off + j] = (CT)s;
+    else if (rest) rest[d] = (CT)s;
 }
 
 // ---- one row for each of many running sequences, states updated in place.  LPC lanes share a channel, four states each (16-byte loads of
@@ -466,7 +558,7 @@ __global__ __launch_bounds__(256) void seq_scan_step_kernel(const ScanStepP p) {
         nx = next == 0x7fffffff ? -1 : next;
     }
     if (!there) {
-        if (valid && sub == 0) seq_store(p.y, r * p.y.rs + d, CT(0));
+        if (valid && sub == 0) seq_store(p.y, r * (int64_t)p.y.rs + d, CT(0));
         return;
     }
     const int n0 = sub * 4, g = d / p.Dg;
@@ -487,14 +579,14 @@ __global__ __launch_bounds__(256) void seq_scan_step_kernel(const ScanStepP p) {
     }
     const CT bias = p.dt_bias ? ((const CT *)p.dt_bias)[d] : CT(0), skip = p.Dskip ? ((const CT *)p.Dskip)[d] : CT(0);
     for (;;) {
-        const CT u = seq_load1(p.u, r * p.u.rs + d, CT(0)), pre = seq_load1(p.dt, r * p.dt.rs + d, CT(0)) + bias;
+        const CT u = seq_load1(p.u, r * (int64_t)p.u.rs + d, CT(0)), pre = seq_load1(p.dt, r * (int64_t)p.dt.rs + d, CT(0)) + bias;
         const CT dl = p.softplus ? seq_softplus(pre) : pre, du = dl * u;
         CT v = CT(0);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const int n = n0 + i;
             if (n < p.N) {
-                const CT b = seq_load1(p.B, r * p.B.rs + g * p.Bg + n * p.Bn, CT(0)), c = seq_load1(p.C, r * p.C.rs + g * p.Cg + n * p.Cn, CT(0));
+                const CT b = seq_load1(p.B, r * (int64_t)p.B.rs + g * p.Bg + n * p.Bn, CT(0)), c = seq_load1(p.C, r * (int64_t)p.C.rs + g * p.Cg + n * p.Cn, CT(0));
                 h[i] = seq_fma(seq_exp2(dl * A2[i]), h[i], du * b);
                 v = seq_fma(h[i], c, v);
             }
@@ -502,10 +594,10 @@ __global__ __launch_bounds__(256) void seq_scan_step_kernel(const ScanStepP p) {
         for (int x = 1; x < p.lpc; x <<= 1) v += __shfl_xor(v, x);
         v = seq_fma(skip, u, v);
         if (p.z.p) {
-            const CT z = seq_load1(p.z, r * p.z.rs + d, CT(0));
+            const CT z = seq_load1(p.z, r * (int64_t)p.z.rs + d, CT(0));
             v = v * (z * seq_sigmoid(z));
         }
-        if (valid && sub == 0) seq_store(p.y, r * p.y.rs + d, v);
+        if (valid && sub == 0) seq_store(p.y, r * (int64_t)p.y.rs + d, v);
         if (nx < 0) break;
         r = nx;
         __syncthreads();

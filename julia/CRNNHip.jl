@@ -505,7 +505,7 @@ end
 # Sequence operators (include/crnn_hip.h, last section): device pointers (AMDGPU.jl: `pointer(x)`) on the caller's stream.  Time runs over rows,
 # channels are the fastest index, so a Julia array is [D, rows, n_seq].  Same status as everything above: not executed.
 
-"""`crnn_view`: an array of the caller's on the device; element types 0 Float32, 1 BFloat16, 2 Float16, 3 Float64, 4 an 8-bit checkpoint."""
+# `crnn_view`: an array on the device; element types 0 Float32, 1 BFloat16, 2 Float16, 3 Float64, 4 an 8-bit checkpoint
 Base.@kwdef struct View
     ptr::Ptr{Cvoid} = C_NULL
     scales::Ptr{Cvoid} = C_NULL
@@ -595,7 +595,7 @@ Base.@kwdef struct ScanArgs
     workspace_bytes::Int64 = 0
 end
 
-"""Set `struct_size = sizeof(ConvArgs)` / `sizeof(ScanArgs)`: the library refuses a mirror of another size."""
+# struct_size = sizeof(ConvArgs) or sizeof(ScanArgs): the library refuses a mirror of another size
 conv_workspace(a::ConvArgs) = ccall((:crnn_conv_workspace, LIB), Int64, (Ref{ConvArgs},), a)
 conv_forward!(a::ConvArgs) = check(ccall((:crnn_conv_forward, LIB), Int32, (Ref{ConvArgs},), a))
 conv_backward!(a::ConvArgs) = check(ccall((:crnn_conv_backward, LIB), Int32, (Ref{ConvArgs},), a))

@@ -387,9 +387,10 @@ template <class T> inline T shfl_down(int site, T v, unsigned delta, int width =
     return shfl_to(site, v, idx);
 }
 inline int update_dpp(int site, int old, int src, int ctrl, int row_mask, int bank_mask, bool bound_ctrl) {
-    if (ctrl < 0 || ctrl > 0xFF) die("update_dpp: only quad_perm controls are emulated");
+    const bool ror8 = ctrl == 0x128, half_mirror = ctrl == 0x141;
+    if ((ctrl < 0 || ctrl > 0xFF) && !ror8 && !half_mirror) die("update_dpp: only quad_perm, row_ror:8 and row_half_mirror controls are emulated");
     if ((row_mask & 0xF) != 0xF || (bank_mask & 0xF) != 0xF) die("update_dpp: row/bank masks are not emulated");
-    const int self = lane_id(), from = (self & ~3) | ((ctrl >> (2 * (self & 3))) & 3);
+    const int self = lane_id(), from = ror8 ? self ^ 8 : half_mirror ? self ^ 7 : (self & ~3) | ((ctrl >> (2 * (self & 3))) & 3);
     uint64_t u = (uint32_t)src; int act;
     const uint64_t r = pull(site, u, from, &act);
     return act ? (int)(uint32_t)r : (bound_ctrl ? 0 : old);
@@ -410,6 +411,15 @@ template <class T> inline T readfirstlane(int site, T v) {
     const uint64_t r = readfirstlane64(site, u);
     T out; memcpy(&out, &r, sizeof(T));
     return out;
+}
+// v_permlane32_swap / v_permlane16_swap: odd halves (rows of 16) of the first register against even ones of the second
+struct u32x2 { unsigned v[2]; unsigned operator[](int i) const { return v[i]; } };
+inline u32x2 permlane_swap(int site, unsigned a, unsigned b, int width) {
+    const int self = lane_id(); int act;
+    const bool odd = (self & width) != 0;
+    const uint64_t other = pull(site, (uint64_t)a | (uint64_t)b << 32, self ^ width, &act);
+    const unsigned oa = (unsigned)other, ob = (unsigned)(other >> 32);
+    return odd ? u32x2{{ob, b}} : u32x2{{a, oa}};
 }
 inline void soft_barrier(int site) { block_on(OP_SOFT, site); }
 inline void syncthreads(int site) { block_on(OP_SYNC, site); }
@@ -442,6 +452,8 @@ static constexpr int warpSize = 64;
 #define __shfl_xor(...) simt::shfl_xor(SIMT_SITE, __VA_ARGS__)
 #define __shfl_down(...) simt::shfl_down(SIMT_SITE, __VA_ARGS__)
 #define __builtin_amdgcn_update_dpp(...) simt::update_dpp(SIMT_SITE, __VA_ARGS__)
+#define __builtin_amdgcn_permlane32_swap(a, b, fi, bc) simt::permlane_swap(SIMT_SITE, (a), (b), 32)
+#define __builtin_amdgcn_permlane16_swap(a, b, fi, bc) simt::permlane_swap(SIMT_SITE, (a), (b), 16)
 #define __builtin_amdgcn_ballot_w64(p) simt::ballot(SIMT_SITE, (p))
 #define __builtin_amdgcn_readfirstlane(v) simt::readfirstlane(SIMT_SITE, (v))
 #define __builtin_amdgcn_wave_barrier() simt::soft_barrier(SIMT_SITE)
