@@ -113,17 +113,21 @@ struct ScanPlan {
     int64_t flat;
     crnn::ScanP p;
     // workspace, in elements of the compute type
-    int64_t maps, S, G, sdel, part, dA, dD, db, acc, total;
+    int64_t S, G, sdel, part, dA, dD, db, acc, total;
 };
 
-// Rows of a chunk of the forward scan.  Cutting costs a second look at every row (the chunk's end without its past), so it is done only where
-// the sequences and channel tiles alone leave most of the card idle.
+// Rows of a chunk of the forward scan; 0: sequences are not cut.  Cutting costs a second look at every row (the chunk's end without its past), so
+// it is left where the sequences and channel tiles alone give two wavefronts a SIMD (8 sequences of 1024 rows, 4096 channels, 512 wavefronts:
+// 600 us whole, 279 us cut; at 1024 wavefronts a row costs the same either way).  Else chunks are as short as their carry allows: many of them
+// even out the last round of blocks.  Measured (rows x tiles of 64 channels: us at 16 / 32 / 48 / 64 / 128 rows): 64 x 24: 41 / 44 / 54 / 69 / 69;
+// 512 x 64: 47 / 48 / 57 / 69 / 120; 2048 x 32: 79 / 68 / 79 / 76 / 125; 8190 x 64: 396 / 296 / 279 / 291 / 325.
 int64_t scan_forward_rows(int64_t flat, int32_t n_seq, int64_t ntile) {
-    const int64_t waves = 4096;                                   // four wavefronts a SIMD
-    if ((int64_t)n_seq * ntile * 4 >= waves) return 0;
-    int64_t q = (flat * ntile + waves - 1) / waves;
-    q = (q + crnn::kScanTB - 1) / crnn::kScanTB * crnn::kScanTB;
-    return q < 4 * crnn::kScanTB ? 4 * crnn::kScanTB : q;
+    if (const char *e = getenv("CRNN_DEV_Q")) return atoll(e);
+    if ((int64_t)n_seq * ntile >= 2048) return 0;
+    const int64_t rows = flat * ntile;
+    int64_t q = rows <= 16384 ? 16 : rows <= 131072 ? 32 : 48;
+    q = std::max(q, rows / 32768);
+    return (q + crnn::kScanTB - 1) / crnn::kScanTB * crnn::kScanTB;
 }
 
 bool scan_plan(SeqCheck &c, const crnn_scan_args *a, bool backward, ScanPlan &s) {
@@ -148,7 +152,6 @@ bool scan_plan(SeqCheck &c, const crnn_scan_args *a, bool backward, ScanPlan &s)
         return c.bad("too many sequences, rows and channels for one launch");
     int64_t at = 0;
     auto take = [&](int64_t n) { const int64_t o = at; at += (n + 31) / 32 * 32; return o; };
-    s.maps = take(s.flat * a->G * 2 * s.NS);
     s.S = take(s.split ? blk * s.NS : 0);
     s.sdel = take(s.split ? blk : 0);
     s.G = take(backward ? blk * s.NS : 0);
@@ -165,6 +168,8 @@ void scan_fill(const crnn_scan_args *a, ScanPlan &s) {
     crnn::ScanP &p = s.p;
     p.u = seq_view(a->u, 4); p.dt = seq_view(a->dt, 4); p.z = seq_view(a->z, 4); p.y = seq_view(a->y, 4);
     p.dy = seq_view(a->dy, 4); p.du = seq_view(a->du, 4); p.ddt = seq_view(a->ddt, 4); p.dz = seq_view(a->dz, 4);
+    p.B = seq_view(a->B, 1); p.C = seq_view(a->C, 1);
+    p.Bg = a->B_group; p.Bn = a->B_state; p.Cg = a->C_group; p.Cn = a->C_state;
     p.A = a->A; p.Dskip = a->skip; p.dt_bias = a->dt_bias;
     p.state_in = a->state_in; p.state_out = a->state_out; p.dstate_out = a->dstate_out; p.dstate_in = a->dstate_in;
     p.softplus = a->softplus; p.zero_outside = a->zero_outside;
@@ -186,21 +191,19 @@ template <int IO, int NS, bool P8>
 void scan_forward_run(const crnn_scan_args *a, ScanPlan &s, hipStream_t st) {
     using CT = typename crnn::SeqIO<IO>::C;
     crnn::ScanP p = s.p;
-    CT *ws = (CT *)a->workspace, *maps = ws + s.maps, *S = ws + s.S, *sdel = ws + s.sdel;
+    CT *ws = (CT *)a->workspace, *S = ws + s.S, *sdel = ws + s.sdel;
     p.acc = s.nb > 1 ? ws + s.acc : nullptr;
     const dim3 grid((unsigned)(p.m.nblk * ((p.ntile + crnn::kScanWaves - 1) / crnn::kScanWaves))), block(64 * crnn::kScanWaves);
-    crnn::ScanMapsP mp = scan_maps(a, s, a->B, a->C, a->B_group, a->B_state, a->C_group, a->C_state);
     for (int b = 0; b < s.nb; ++b) {
-        p.n0 = mp.n0 = b * NS;
+        p.n0 = b * NS;
         p.first = b == 0;
         p.fin = b == s.nb - 1;
-        if (s.flat > 0) hipLaunchKernelGGL((crnn::seq_scan_maps_kernel<CT, NS>), dim3(seq_grid(s.flat * p.G * 2 * NS)), dim3(256), 0, st, mp, maps);
         if (s.split) {
-            hipLaunchKernelGGL((crnn::seq_scan_ends_kernel<IO, NS, P8, false>), grid, block, 0, st, p, (const CT *)maps, S, (CT *)nullptr, sdel);
+            hipLaunchKernelGGL((crnn::seq_scan_ends_kernel<IO, NS, P8, false>), grid, block, 0, st, p, S, (CT *)nullptr, sdel);
             hipLaunchKernelGGL((crnn::seq_scan_carry_kernel<CT, NS>), dim3((unsigned)(((int64_t)p.m.n_seq * NS * p.D + 255) / 256)), dim3(256), 0, st, p, S,
                                (CT *)nullptr, (const CT *)sdel);
         }
-        hipLaunchKernelGGL((crnn::seq_scan_out_kernel<IO, NS, P8>), grid, block, 0, st, p, (const CT *)maps, (const CT *)(s.split ? S : nullptr));
+        hipLaunchKernelGGL((crnn::seq_scan_out_kernel<IO, NS, P8>), grid, block, 0, st, p, (const CT *)(s.split ? S : nullptr));
     }
 }
 
@@ -208,22 +211,20 @@ template <int IO, int NS, bool P8>
 void scan_backward_run(const crnn_scan_args *a, ScanPlan &s, hipStream_t st) {
     using CT = typename crnn::SeqIO<IO>::C;
     crnn::ScanP p = s.p;
-    CT *ws = (CT *)a->workspace, *maps = ws + s.maps, *S = ws + s.S, *Gb = ws + s.G, *sdel = ws + s.sdel, *part = ws + s.part, *dA = ws + s.dA, *dD = ws + s.dD,
+    CT *ws = (CT *)a->workspace, *S = ws + s.S, *Gb = ws + s.G, *sdel = ws + s.sdel, *part = ws + s.part, *dA = ws + s.dA, *dD = ws + s.dD,
        *db = ws + s.db;
     p.acc = s.nb > 1 ? ws + s.acc : nullptr;
     const dim3 grid((unsigned)(p.m.nblk * ((p.ntile + crnn::kScanWaves - 1) / crnn::kScanWaves))), block(64 * crnn::kScanWaves);
-    crnn::ScanMapsP mp = scan_maps(a, s, a->B, a->C, a->B_group, a->B_state, a->C_group, a->C_state);
     crnn::ScanMapsP mo = scan_maps(a, s, a->dB, a->dC, a->N, 1, a->N, 1);
     const int64_t cA = (int64_t)NS * p.D;
     for (int b = 0; b < s.nb; ++b) {
-        p.n0 = mp.n0 = mo.n0 = b * NS;
+        p.n0 = mo.n0 = b * NS;
         p.first = b == 0;
         p.fin = b == s.nb - 1;
-        if (s.flat > 0) hipLaunchKernelGGL((crnn::seq_scan_maps_kernel<CT, NS>), dim3(seq_grid(s.flat * p.G * 2 * NS)), dim3(256), 0, st, mp, maps);
-        hipLaunchKernelGGL((crnn::seq_scan_ends_kernel<IO, NS, P8, true>), grid, block, 0, st, p, (const CT *)maps, S, Gb, sdel);
+        hipLaunchKernelGGL((crnn::seq_scan_ends_kernel<IO, NS, P8, true>), grid, block, 0, st, p, S, Gb, sdel);
         hipLaunchKernelGGL((crnn::seq_scan_carry_kernel<CT, NS>), dim3((unsigned)(((int64_t)p.m.n_seq * NS * p.D + 255) / 256)), dim3(256), 0, st, p, S, Gb,
                            (const CT *)sdel);
-        hipLaunchKernelGGL((crnn::seq_scan_bwd_kernel<IO, NS, P8>), grid, block, 0, st, p, (const CT *)maps, (const CT *)S, (const CT *)Gb, part, dA, dD, db);
+        hipLaunchKernelGGL((crnn::seq_scan_bwd_kernel<IO, NS, P8>), grid, block, 0, st, p, (const CT *)S, (const CT *)Gb, part, dA, dD, db);
         if (s.flat > 0)
             hipLaunchKernelGGL((crnn::seq_scan_sum_maps_kernel<CT, NS>), dim3(seq_grid(s.flat * p.G * 2 * NS)), dim3(256), 0, st, p.m, mo, (const CT *)part, p.tpg);
         hipLaunchKernelGGL((crnn::seq_sum_blocks_kernel<CT>), dim3((unsigned)((cA + 31) / 32)), dim3(256), 0, st, (const CT *)dA, p.m.nblk, cA, (CT *)a->dA, (CT *)nullptr, p.D,

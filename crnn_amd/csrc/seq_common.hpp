@@ -270,6 +270,13 @@ __device__ __forceinline__ void seq_put_rows(const SeqMap &m, const SeqV &v, con
         if (i < n) (c + (int64_t)i * v.rs)[d] = b[i];
 }
 
+// what a wavefront wrote to its own part of the LDS is there for all its lanes
+__device__ __forceinline__ void seq_wave_sync() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
 // sum over the wavefront's lanes of V values at once: every exchange halves how many values a lane still carries, about 2 V operations in
 // all where separate sums would take 6 V.  Afterwards the lane holds the sum of value seq_spread_index<V>(lane).
 template <int V>

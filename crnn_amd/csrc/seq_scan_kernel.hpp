@@ -17,12 +17,13 @@
 
 namespace crnn {
 
-constexpr int kScanTB = 8;      // rows whose loads are in flight together
+constexpr int kScanTB = 4;      // rows whose loads are in flight together
 constexpr int kScanWaves = 4;   // wavefronts of a block, each on its own channel tile
 
 struct ScanP {
     SeqMap m;
-    SeqV u, dt, z, y, dy, du, ddt, dz;
+    SeqV u, dt, z, y, dy, du, ddt, dz, B, C;
+    int64_t Bg, Cg, Bn, Cn;                       // elements between groups, between states
     const void *A, *Dskip, *dt_bias;              // in the compute type
     const void *state_in, *dstate_out;            // [n_seq][D][N]
     void *state_out, *dstate_in;
@@ -34,7 +35,7 @@ struct ScanP {
     int32_t softplus, zero_outside;
 };
 
-// ---- B and C of this launch's states in the compute type, [row][group][B: NS | C: NS], 0 behind the last state
+// ---- dB and dC
 struct ScanMapsP {
     SeqV B, C;              // rs: elements between rows, group stride below
     int64_t Bg, Cg;         // elements between groups
@@ -43,24 +44,11 @@ struct ScanMapsP {
     int64_t srows;          // dense: rows of a sequence (0: packed)
     int32_t G, N, n0;
 };
-template <class CT, int NS>
-__global__ __launch_bounds__(256) void seq_scan_maps_kernel(const ScanMapsP p, CT *__restrict__ out) {
-    const int64_t total = p.rows * p.G * 2 * NS;
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
-        const int j = (int)(i % (2 * NS));
-        const int64_t rg = i / (2 * NS), g = rg % p.G, r = rg / p.G;
-        const int n = p.n0 + (j % NS);
-        CT x = CT(0);
-        if (n < p.N) {
-            const SeqV &v = j < NS ? p.B : p.C;
-            const int64_t at = p.srows ? (r / p.srows) * v.bs + (r % p.srows) * v.rs : r * v.rs;
-            x = seq_load1(v, at + g * (j < NS ? p.Bg : p.Cg) + n * (j < NS ? p.Bn : p.Cn), CT(0));
-        }
-        out[i] = x;
-    }
-}
-
 // the place of a wavefront: chunk block, channel tile, channel of the lane
+// the plane of state n of chunk block b in an [block][state][D] array: uniform, the lane adds its channel
+template <int NS, class T>
+__device__ __forceinline__ T *scan_plane(T *x, int64_t b, int n, int D) { return x + (b * NS + n) * D; }
+
 struct ScanAt {
     SeqChunk k;
     int64_t b;
@@ -122,12 +110,59 @@ __device__ __forceinline__ void scan_steps(const ScanP &p, int n, typename SeqIO
     }
 }
 
+// B and C of TB rows on their way to a wavefront's own part of the LDS, [row][B: NS | C: NS] in the compute type, 0 behind the last state: loaded
+// into registers while the rows before are worked on (a lane has TB NS / 32 of them), put down when those are done, read back as
+// broadcasts.  (As scalar operands they are free of the vector registers, but every row then waits for its own scalar load: measured
+// 339 us against the 190 us of this form for 8190 rows of 4096 channels, at five wavefronts a SIMD.)
+template <int IO, int NS, int TB>
+struct ScanMapRows {
+    using CT = typename SeqIO<IO>::C;
+    using E = typename SeqIO<IO>::E;
+    static constexpr int V = TB * 2 * NS / 64, RPV = 64 / (2 * NS);   // values of a lane, rows of 64 values
+    const E *at;            // of the lane's value in the chunk's first row
+    int32_t rs;
+    int32_t row0;
+    bool in;
+    E v[V];
+    __device__ __forceinline__ void init(const ScanP &p, const ScanAt &a) {
+        const int lane = threadIdx.x & 63, j = lane % (2 * NS), n = p.n0 + j % NS;
+        const bool b = j < NS;
+        row0 = lane / (2 * NS);
+        in = n < p.N;
+        const int nn = in ? n : p.N - 1;
+        const E *pb = (const E *)p.B.p + seq_off(p.m, p.B, a.k, a.k.t0) + a.g * p.Bg, *pc = (const E *)p.C.p + seq_off(p.m, p.C, a.k, a.k.t0) + a.g * p.Cg;
+        at = b ? pb + nn * p.Bn : pc + nn * p.Cn;
+        rs = b ? p.B.rs : p.C.rs;
+    }
+    // rows t .. t + TB - 1 of the chunk, those behind its n-th as the n-th
+    __device__ __forceinline__ void load(int t, int n) {
+#pragma unroll
+        for (int k = 0; k < V; ++k) {
+            const int r = t + row0 + k * RPV;
+            v[k] = at[(int64_t)(r < n ? r : n - 1) * rs];
+        }
+    }
+    __device__ __forceinline__ void put(int dt, CT *lds) const {
+        const int lane = threadIdx.x & 63;
+#pragma unroll
+        for (int k = 0; k < V; ++k) {
+            CT x;
+            if (IO == 8) x = (CT)v[k];
+            else if (IO == 4) x = (CT)seq_as_float((uint32_t)v[k]);
+            else x = (CT)(dt == CRNN_DT_BF16 ? seq_as_float((uint32_t)v[k] << 16) : seq_from_f16((uint32_t)v[k]));
+            lds[k * 64 + lane] = in ? x : CT(0);
+        }
+        seq_wave_sync();
+    }
+};
+
 // ---- forward: outputs of a chunk from its first state (start[block][n][d]; null: one chunk a sequence, from state_in)
 template <int IO, int NS, bool P8>
-__global__ __launch_bounds__(64 * kScanWaves) void seq_scan_out_kernel(const ScanP p, const typename SeqIO<IO>::C *__restrict__ maps,
-                                                                       const typename SeqIO<IO>::C *__restrict__ start) {
+__global__ __launch_bounds__(64 * kScanWaves, IO == 8 ? 2 : 4) void seq_scan_out_kernel(const ScanP p, const typename SeqIO<IO>::C *__restrict__ start) {
     using CT = typename SeqIO<IO>::C;
     constexpr int TB = kScanTB;
+    __shared__ CT smaps[kScanWaves][TB * 2 * NS];
+    CT *maps = smaps[threadIdx.x >> 6];
     const ScanAt a = scan_at(p);
     if (!a.on) return;
     if (p.zero_outside && p.fin) seq_zero_outside(p.m, p.y, a.b, a.d, a.valid);
@@ -136,7 +171,7 @@ __global__ __launch_bounds__(64 * kScanWaves) void seq_scan_out_kernel(const Sca
     scan_rates<CT, NS>(p, a.d, A2);
     if (start) {
 #pragma unroll
-        for (int n = 0; n < NS; ++n) h[n] = start[(a.b * NS + n) * p.D + a.d];
+        for (int n = 0; n < NS; ++n) h[n] = scan_plane<NS>(start, a.b, n, p.D)[(uint32_t)a.d];
     } else {
         scan_state<CT, NS>(p, p.state_in, a.k.s, a.d, h);
     }
@@ -144,7 +179,10 @@ __global__ __launch_bounds__(64 * kScanWaves) void seq_scan_out_kernel(const Sca
     const bool gate = p.z.p && p.fin;
     SeqRows<IO, P8, TB> ru, rz;
     SeqRows<IO, false, TB> rd;
+    ScanMapRows<IO, NS, TB> rm;
+    rm.init(p, a);
     if (a.k.n > 0) {
+        rm.load(0, a.k.n);
         const int nv = a.k.n < TB ? a.k.n : TB;
         ru.load(p.m, p.u, a.k, a.k.t0, a.d, nv);
         rd.load(p.m, p.dt, a.k, a.k.t0, a.d, nv);
@@ -157,7 +195,9 @@ __global__ __launch_bounds__(64 * kScanWaves) void seq_scan_out_kernel(const Sca
         ru.get(p.u, u);
         rd.get(p.dt, x);
         if (gate) rz.get(p.z, z);
+        rm.put(p.B.dt, maps);
         if (left > TB) {
+            rm.load(t + TB, a.k.n);
             const int nn = left - TB < TB ? left - TB : TB;
             ru.load(p.m, p.u, a.k, a.k.t0 + t + TB, a.d, nn);
             rd.load(p.m, p.dt, a.k, a.k.t0 + t + TB, a.d, nn);
@@ -165,11 +205,9 @@ __global__ __launch_bounds__(64 * kScanWaves) void seq_scan_out_kernel(const Sca
         }
         scan_steps<IO, TB>(p, nv, bias, x, u, dl);
         const int64_t frow = a.k.flat + a.k.t0 + t;
-        const CT *row = maps + (frow * p.G + a.g) * (2 * NS);
-        const int64_t step = (int64_t)p.G * (2 * NS);
 #pragma unroll
         for (int i = 0; i < TB; ++i) {
-            const CT *bc = row + (i < nv ? i : nv - 1) * step;
+            const CT *bc = maps + i * (2 * NS);
             const CT du = dl[i] * u[i];
             CT s0 = CT(0), s1 = CT(0);
 #pragma unroll
@@ -181,15 +219,13 @@ __global__ __launch_bounds__(64 * kScanWaves) void seq_scan_out_kernel(const Sca
             }
             v[i] = s0 + s1;
         }
+        seq_wave_sync();
         if (p.acc) {
-            for (int i = 0; i < nv; ++i) {
-                CT *acc = (CT *)p.acc + (frow + i) * p.D + a.d;
 #pragma unroll
-                for (int j = 0; j < TB; ++j)
-                    if (j == i) {
-                        if (!p.first) v[j] += *acc;
-                        if (!p.fin && a.valid) *acc = v[j];
-                    }
+            for (int i = 0; i < TB; ++i) {
+                CT *acc = (CT *)p.acc + (frow + (i < nv ? i : nv - 1)) * p.D;
+                if (!p.first) v[i] += acc[(uint32_t)a.d];
+                if (!p.fin && i < nv && a.valid) acc[(uint32_t)a.d] = v[i];
             }
         }
         if (p.fin) {
@@ -208,11 +244,12 @@ __global__ __launch_bounds__(64 * kScanWaves) void seq_scan_out_kernel(const Sca
 // ---- a chunk by itself: S = its last state from zero, sum of delta; BOTH: also G = what its outputs' gradients r pass back to the state
 // before it, sum_t (prod of the decays up to t) r C -- taken in the forward direction, so that one exponential serves both.
 template <int IO, int NS, bool P8, bool BOTH>
-__global__ __launch_bounds__(64 * kScanWaves) void seq_scan_ends_kernel(const ScanP p, const typename SeqIO<IO>::C *__restrict__ maps,
-                                                                        typename SeqIO<IO>::C *__restrict__ S, typename SeqIO<IO>::C *__restrict__ Gb,
+__global__ __launch_bounds__(64 * kScanWaves, IO == 8 ? 2 : BOTH ? 3 : 5) void seq_scan_ends_kernel(const ScanP p, typename SeqIO<IO>::C *__restrict__ S, typename SeqIO<IO>::C *__restrict__ Gb,
                                                                         typename SeqIO<IO>::C *__restrict__ sdel) {
     using CT = typename SeqIO<IO>::C;
-    constexpr int TB = BOTH ? kScanTB / 2 : kScanTB;
+    constexpr int TB = kScanTB;
+    __shared__ CT smaps[kScanWaves][TB * 2 * NS];
+    CT *maps = smaps[threadIdx.x >> 6];
     const ScanAt a = scan_at(p);
     if (!a.on || !a.k.live) return;
     CT A2[NS], h[NS], P[BOTH ? NS : 1], g[BOTH ? NS : 1];
@@ -227,7 +264,10 @@ __global__ __launch_bounds__(64 * kScanWaves) void seq_scan_ends_kernel(const Sc
     CT sd = CT(0);
     SeqRows<IO, P8, TB> ru, rz;
     SeqRows<IO, false, TB> rd, ry;
+    ScanMapRows<IO, NS, TB> rm;
+    rm.init(p, a);
     if (a.k.n > 0) {
+        rm.load(0, a.k.n);
         const int nv = a.k.n < TB ? a.k.n : TB;
         ru.load(p.m, p.u, a.k, a.k.t0, a.d, nv);
         rd.load(p.m, p.dt, a.k, a.k.t0, a.d, nv);
@@ -242,7 +282,9 @@ __global__ __launch_bounds__(64 * kScanWaves) void seq_scan_ends_kernel(const Sc
         rd.get(p.dt, x);
         if (BOTH) ry.get(p.dy, y);
         if (gate) rz.get(p.z, z);
+        rm.put(p.B.dt, maps);
         if (left > TB) {
+            rm.load(t + TB, a.k.n);
             const int nn = left - TB < TB ? left - TB : TB;
             ru.load(p.m, p.u, a.k, a.k.t0 + t + TB, a.d, nn);
             rd.load(p.m, p.dt, a.k, a.k.t0 + t + TB, a.d, nn);
@@ -258,11 +300,9 @@ __global__ __launch_bounds__(64 * kScanWaves) void seq_scan_ends_kernel(const Sc
 #pragma unroll
             for (int i = 0; i < TB; ++i) y[i] = i < nv ? y[i] : CT(0);
         }
-        const CT *row = maps + ((a.k.flat + a.k.t0 + t) * p.G + a.g) * (2 * NS);
-        const int64_t step = (int64_t)p.G * (2 * NS);
 #pragma unroll
         for (int i = 0; i < TB; ++i) {
-            const CT *bc = row + (i < nv ? i : nv - 1) * step;
+            const CT *bc = maps + i * (2 * NS);
             const CT du = dl[i] * u[i];
             sd += dl[i];
 #pragma unroll
@@ -275,12 +315,13 @@ __global__ __launch_bounds__(64 * kScanWaves) void seq_scan_ends_kernel(const Sc
                 }
             }
         }
+        seq_wave_sync();
     }
     if (!a.valid) return;
 #pragma unroll
     for (int n = 0; n < NS; ++n) {
-        S[(a.b * NS + n) * p.D + a.d] = h[n];
-        if (BOTH) Gb[(a.b * NS + n) * p.D + a.d] = g[BOTH ? n : 0];
+        scan_plane<NS>(S, a.b, n, p.D)[(uint32_t)a.d] = h[n];
+        if (BOTH) scan_plane<NS>(Gb, a.b, n, p.D)[(uint32_t)a.d] = g[BOTH ? n : 0];
     }
     sdel[a.b * p.D + a.d] = sd;
 }
@@ -299,20 +340,43 @@ __global__ __launch_bounds__(256) void seq_scan_carry_kernel(const ScanP p, CT *
     const int64_t b0 = seq_first_block(p.m, s), nc = len > 0 ? (len + p.m.Q - 1) / p.m.Q : 1;
     const int64_t at = (s * p.D + d) * p.N + p.n0 + n;
     const CT A2 = ((const CT *)p.A)[(int64_t)d * p.N + p.n0 + n] * CT(kLog2eD);
+    // the loads of eight chunks at once; the sequence of chunks itself is one multiply-add each
+    constexpr int CB = 8;
+    const int64_t stride = (int64_t)NS * p.D;
+    CT *Sp = S + (b0 * NS + n) * p.D + d;
+    const CT *dp = sdel + b0 * p.D + d;
     CT h = p.state_in ? ((const CT *)p.state_in)[at] : CT(0);
-    for (int64_t c = 0; c < nc; ++c) {
-        const int64_t o = ((b0 + c) * NS + n) * p.D + d;
-        const CT own = S[o];
-        S[o] = h;
-        h = seq_fma(seq_exp2(A2 * sdel[(b0 + c) * p.D + d]), h, own);
+    for (int64_t c0 = 0; c0 < nc; c0 += CB) {
+        CT own[CB], e[CB];
+#pragma unroll
+        for (int i = 0; i < CB; ++i) {
+            const int64_t c = c0 + i < nc ? c0 + i : nc - 1;
+            own[i] = Sp[c * stride];
+            e[i] = dp[c * p.D];
+        }
+#pragma unroll
+        for (int i = 0; i < CB; ++i) {
+            if (c0 + i < nc) Sp[(c0 + i) * stride] = h;
+            h = seq_fma(seq_exp2(A2 * e[i]), h, own[i]);
+        }
     }
     if (!Gb) return;
+    CT *Gp = Gb + (b0 * NS + n) * p.D + d;
     CT q = p.dstate_out ? ((const CT *)p.dstate_out)[at] : CT(0);
-    for (int64_t c = nc - 1; c >= 0; --c) {
-        const int64_t o = ((b0 + c) * NS + n) * p.D + d;
-        const CT own = Gb[o];
-        Gb[o] = q;
-        if (len > 0) q = seq_fma(seq_exp2(A2 * sdel[(b0 + c) * p.D + d]), q, own);
+    for (int64_t c0 = nc - 1; len > 0 && c0 >= 0; c0 -= CB) {
+        CT own[CB], e[CB];
+#pragma unroll
+        for (int i = 0; i < CB; ++i) {
+            const int64_t c = c0 - i >= 0 ? c0 - i : 0;
+            own[i] = Gp[c * stride];
+            e[i] = dp[c * p.D];
+        }
+#pragma unroll
+        for (int i = 0; i < CB; ++i)
+            if (c0 - i >= 0) {
+                Gp[(c0 - i) * stride] = q;
+                q = seq_fma(seq_exp2(A2 * e[i]), q, own[i]);
+            }
     }
     if (p.dstate_in) ((CT *)p.dstate_in)[at] = q;
 }
@@ -321,16 +385,17 @@ __global__ __launch_bounds__(256) void seq_scan_carry_kernel(const ScanP p, CT *
 // from the last kScanBwdTB rows to the first: those rows once more, each row's decay a and a h[t - 1] kept in registers (2 NS x kScanBwdTB;
 // h[t] is one multiply-add away, and dA needs the product itself), and the reverse sweep over them.  dB and dC are sums over channels: a
 // wavefront's part goes to part[tile][row][B: NS | C: NS], summed over the tiles in a fixed order by seq_scan_sum_maps_kernel.
-// Four rows and six times four a chunk: two wavefronts a SIMD fill the registers (256 a lane) and the LDS (20 KB each) together.
-constexpr int kScanBwdTB = 4, kScanBwdSub = 6, kScanBwdQ = kScanBwdTB * kScanBwdSub;
+// Four rows and five times four a chunk: two wavefronts a SIMD fill the registers (256 a lane) and the LDS (16.5 KB each) about together.
+constexpr int kScanBwdTB = 4, kScanBwdSub = 5, kScanBwdQ = kScanBwdTB * kScanBwdSub;
 template <int IO, int NS, bool P8>
-__global__ __launch_bounds__(64 * kScanWaves, 2) void seq_scan_bwd_kernel(const ScanP p, const typename SeqIO<IO>::C *__restrict__ maps,
-                                                                          const typename SeqIO<IO>::C *__restrict__ start, const typename SeqIO<IO>::C *__restrict__ back,
+__global__ __launch_bounds__(64 * kScanWaves, 2) void seq_scan_bwd_kernel(const ScanP p, const typename SeqIO<IO>::C *__restrict__ start, const typename SeqIO<IO>::C *__restrict__ back,
                                                                           typename SeqIO<IO>::C *__restrict__ part, typename SeqIO<IO>::C *__restrict__ dApart,
                                                                           typename SeqIO<IO>::C *__restrict__ dDpart, typename SeqIO<IO>::C *__restrict__ dbpart) {
     using CT = typename SeqIO<IO>::C;
     constexpr int TB = kScanBwdTB, H = NS / 2;
     __shared__ CT keep[kScanWaves][kScanBwdSub - 1][NS][64];
+    __shared__ CT smaps[kScanWaves][TB * 2 * NS];
+    CT *maps = smaps[threadIdx.x >> 6];
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
     const ScanAt a = scan_at(p);
     if (!a.on) return;
@@ -347,50 +412,80 @@ __global__ __launch_bounds__(64 * kScanWaves, 2) void seq_scan_bwd_kernel(const 
         scan_rates<CT, NS>(p, a.d, A2);
 #pragma unroll
         for (int n = 0; n < NS; ++n) {
-            h[n] = start[(a.b * NS + n) * p.D + a.d];
-            q[n] = back[(a.b * NS + n) * p.D + a.d];
+            h[n] = scan_plane<NS>(start, a.b, n, p.D)[(uint32_t)a.d];
+            q[n] = scan_plane<NS>(back, a.b, n, p.D)[(uint32_t)a.d];
         }
         const CT bias = p.dt_bias ? ((const CT *)p.dt_bias)[a.d] : CT(0), skip = p.Dskip ? ((const CT *)p.Dskip)[a.d] : CT(0);
-        const int64_t step = (int64_t)p.G * (2 * NS);
         const int nsub = (a.k.n + TB - 1) / TB;
+        SeqRows<IO, P8, TB> ru, rz;
+        SeqRows<IO, false, TB> rd, ry;
+        ScanMapRows<IO, NS, TB> rm;
+        rm.init(p, a);
+        {
+            const int nn = a.k.n < TB ? a.k.n : TB;
+            rm.load(0, a.k.n);
+            ru.load(p.m, p.u, a.k, a.k.t0, a.d, nn);
+            rd.load(p.m, p.dt, a.k, a.k.t0, a.d, nn);
+        }
 #pragma unroll 1
         for (int k = 0; k < nsub - 1; ++k) {
-            SeqRows<IO, P8, TB> ru;
-            SeqRows<IO, false, TB> rd;
             CT u[TB], x[TB], dl[TB];
-            ru.load(p.m, p.u, a.k, a.k.t0 + k * TB, a.d, TB);
-            rd.load(p.m, p.dt, a.k, a.k.t0 + k * TB, a.d, TB);
             ru.get(p.u, u);
             rd.get(p.dt, x);
+            rm.put(p.B.dt, maps);
+            {       // the next rows; the last ones of the chunk stay for the way back
+                const int t = (k + 1) * TB, nn = a.k.n - t < TB ? a.k.n - t : TB;
+                rm.load(t, a.k.n);
+                ru.load(p.m, p.u, a.k, a.k.t0 + t, a.d, nn);
+                rd.load(p.m, p.dt, a.k, a.k.t0 + t, a.d, nn);
+            }
             scan_steps<IO, TB>(p, TB, bias, x, u, dl);
-            const CT *row = maps + ((a.k.flat + a.k.t0 + k * TB) * p.G + a.g) * (2 * NS);
 #pragma unroll
             for (int i = 0; i < TB; ++i) {
-                const CT *bc = row + i * step;
+                const CT *bc = maps + i * (2 * NS);
                 const CT du = dl[i] * u[i];
 #pragma unroll
                 for (int n = 0; n < NS; ++n) h[n] = seq_fma(seq_exp2(dl[i] * A2[n]), h[n], du * bc[n]);
             }
 #pragma unroll
             for (int n = 0; n < NS; ++n) keep[wave][k][n][lane] = h[n];
+            seq_wave_sync();
         }
 #pragma unroll 1
         for (int k = nsub - 1; k >= 0; --k) {
             const int nv = a.k.n - k * TB < TB ? a.k.n - k * TB : TB;
             const int64_t t = a.k.t0 + k * TB, frow = a.k.flat + t;
-            CT u[TB], x[TB], z[TB], y[TB], dl[TB], ah[TB][NS], e[TB][NS];
-            {
-                SeqRows<IO, P8, TB> ru, rz;
-                SeqRows<IO, false, TB> rd, ry;
-                ru.load(p.m, p.u, a.k, t, a.d, nv);
-                rd.load(p.m, p.dt, a.k, t, a.d, nv);
-                ry.load(p.m, p.dy, a.k, t, a.d, nv);
-                if (p.z.p) rz.load(p.m, p.z, a.k, t, a.d, nv);
-                ru.get(p.u, u);
-                rd.get(p.dt, x);
-                ry.get(p.dy, y);
-                if (p.z.p) rz.get(p.z, z);
+            CT u[TB], x[TB], z[TB], y[TB], dl[TB], ah[TB][NS];
+            ry.load(p.m, p.dy, a.k, t, a.d, nv);
+            if (p.z.p) rz.load(p.m, p.z, a.k, t, a.d, nv);
+            ru.get(p.u, u);
+            rd.get(p.dt, x);
+            rm.put(p.B.dt, maps);
+            if (k > 0) {
+                rm.load((k - 1) * TB, a.k.n);
+                ru.load(p.m, p.u, a.k, t - TB, a.d, TB);
+                rd.load(p.m, p.dt, a.k, t - TB, a.d, TB);
             }
+#pragma unroll
+            for (int n = 0; n < NS; ++n) h[n] = keep[wave][k > 0 ? k - 1 : 0][n][lane];
+            if (k == 0) {
+#pragma unroll
+                for (int n = 0; n < NS; ++n) h[n] = scan_plane<NS>(start, a.b, n, p.D)[(uint32_t)a.d];
+            }
+            scan_steps<IO, TB>(p, nv, bias, x, u, dl);
+#pragma unroll
+            for (int i = 0; i < TB; ++i) {
+                __builtin_amdgcn_sched_barrier(0);
+                const CT *bc = maps + i * (2 * NS);
+                const CT du = dl[i] * u[i];
+#pragma unroll
+                for (int n = 0; n < NS; ++n) {
+                    ah[i][n] = seq_exp2(dl[i] * A2[n]) * h[n];
+                    h[n] = seq_fma(du, bc[n], ah[i][n]);
+                }
+            }
+            ry.get(p.dy, y);
+            if (p.z.p) rz.get(p.z, z);
             if (nv < TB) {
 #pragma unroll
                 for (int i = 0; i < TB; ++i) {
@@ -398,33 +493,16 @@ __global__ __launch_bounds__(64 * kScanWaves, 2) void seq_scan_bwd_kernel(const 
                     z[i] = i < nv ? z[i] : CT(0);
                 }
             }
-#pragma unroll
-            for (int n = 0; n < NS; ++n) h[n] = keep[wave][k > 0 ? k - 1 : 0][n][lane];
-            if (k == 0) {
-#pragma unroll
-                for (int n = 0; n < NS; ++n) h[n] = start[(a.b * NS + n) * p.D + a.d];
-            }
-            scan_steps<IO, TB>(p, nv, bias, x, u, dl);
-            const CT *row = maps + (frow * p.G + a.g) * (2 * NS);
-#pragma unroll
-            for (int i = 0; i < TB; ++i) {
-                const CT *bc = row + (i < nv ? i : nv - 1) * step;
-                const CT du = dl[i] * u[i];
-#pragma unroll
-                for (int n = 0; n < NS; ++n) {
-                    e[i][n] = seq_exp2(dl[i] * A2[n]);
-                    ah[i][n] = e[i][n] * h[n];
-                    h[n] = seq_fma(du, bc[n], ah[i][n]);
-                }
-            }
             CT odu[TB], odt[TB], odz[TB];
 #pragma unroll
             for (int i = TB - 1; i >= 0; --i) {
+                __builtin_amdgcn_sched_barrier(0);
                 const CT du = dl[i] * u[i];
                 const CT sg = p.z.p ? seq_sigmoid(z[i]) : CT(1);
                 const CT r = p.z.p ? y[i] * (z[i] * sg) : y[i];
-                const CT *bc = row + (i < nv ? i : nv - 1) * step;
-                CT v = CT(0), qb = CT(0), qa = CT(0), f[H];
+                const CT *bc = maps + i * (2 * NS);
+                CT v = CT(0), qb = CT(0), qa = CT(0), f[H], dle = dl[i];
+                asm volatile("" : "+v"(dle));      // the decays are formed again rather than kept: NS registers a row
                 const CT duv = a.valid ? du : CT(0), rv = a.valid ? r : CT(0);
 #pragma unroll
                 for (int j = 0; j < H; ++j) {       // states j and j + NS / 2 together: their parts of dB, dC fold at once
@@ -440,7 +518,7 @@ __global__ __launch_bounds__(64 * kScanWaves, 2) void seq_scan_bwd_kernel(const 
                         qa = seq_fma(m, A2[n], qa);
                         dA[n] = seq_fma(m, dl[i], dA[n]);
                         w[s] = seq_fold32(q[n] * duv, rv * hn);
-                        q[n] *= e[i][n];
+                        q[n] *= seq_exp2(dle * A2[n]);
                     }
                     f[j] = seq_fold16(w[0], w[1]);
                 }
@@ -467,11 +545,12 @@ __global__ __launch_bounds__(64 * kScanWaves, 2) void seq_scan_bwd_kernel(const 
                 seq_put_rows<IO, TB>(p.m, p.ddt, a.k, t, a.d, nv, a.valid, odt);
                 if (p.dz.p) seq_put_rows<IO, TB>(p.m, p.dz, a.k, t, a.d, nv, a.valid, odz);
             }
+            seq_wave_sync();
         }
     }
     if (!a.valid) return;
 #pragma unroll
-    for (int n = 0; n < NS; ++n) dApart[(a.b * NS + n) * p.D + a.d] = dA[n];
+    for (int n = 0; n < NS; ++n) scan_plane<NS>(dApart, a.b, n, p.D)[(uint32_t)a.d] = dA[n];
     if (p.fin) {
         dDpart[a.b * p.D + a.d] = dD;
         dbpart[a.b * p.D + a.d] = db;
