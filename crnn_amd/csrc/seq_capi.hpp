@@ -109,6 +109,7 @@ constexpr int64_t kSeqMaxGrid = 0x7fffffff;
 // ------------------------------------------------------------------ scan
 struct ScanPlan {
     bool f64, p8, split;
+    int mode;                   // the kernels' MODE
     int NS, nb;                 // states of a launch, launches over the states
     int64_t flat;
     crnn::ScanP p;
@@ -135,8 +136,10 @@ bool scan_plan(SeqCheck &c, const crnn_scan_args *a, bool backward, ScanPlan &s)
     if (a->N < 1 || a->N > CRNN_SEQ_MAX_STATES) return c.bad("N must be in 1 .. 256");
     if (a->G < 1 || a->D % a->G) return c.bad("G must divide D");
     s.f64 = a->dtype == CRNN_DT_F64;
-    s.p8 = a->u.dtype == CRNN_DT_PACKED8 || (a->z.ptr && a->z.dtype == CRNN_DT_PACKED8);
-    s.NS = s.f64 || a->N <= 8 ? 8 : 16;
+    const bool pu = a->u.dtype == CRNN_DT_PACKED8, pz = a->z.ptr ? a->z.dtype == CRNN_DT_PACKED8 : pu;
+    s.p8 = pu || (a->z.ptr && pz);
+    s.mode = s.f64 || a->N > 16 || pu != pz ? crnn::kScanAny : pu ? 1 : 0;
+    s.NS = s.f64 || (s.mode != crnn::kScanAny && a->N <= 8) ? 8 : 16;
     s.nb = (a->N + s.NS - 1) / s.NS;
     s.flat = seq_flat(a->n_seq, a->rows, a->seq_start != nullptr);
     crnn::ScanP &p = s.p;
@@ -167,6 +170,8 @@ bool scan_plan(SeqCheck &c, const crnn_scan_args *a, bool backward, ScanPlan &s)
 void scan_fill(const crnn_scan_args *a, ScanPlan &s) {
     crnn::ScanP &p = s.p;
     p.u = seq_view(a->u, 4); p.dt = seq_view(a->dt, 4); p.z = seq_view(a->z, 4); p.y = seq_view(a->y, 4);
+    p.gate = a->z.ptr != nullptr;
+    if (!p.gate) p.z = p.u;
     p.dy = seq_view(a->dy, 4); p.du = seq_view(a->du, 4); p.ddt = seq_view(a->ddt, 4); p.dz = seq_view(a->dz, 4);
     p.B = seq_view(a->B, 1); p.C = seq_view(a->C, 1);
     p.Bg = a->B_group; p.Bn = a->B_state; p.Cg = a->C_group; p.Cn = a->C_state;
@@ -187,7 +192,7 @@ crnn::ScanMapsP scan_maps(const crnn_scan_args *a, const ScanPlan &s, const crnn
 
 unsigned seq_grid(int64_t n) { return (unsigned)std::min<int64_t>((n + 255) / 256, 65536); }
 
-template <int IO, int NS, bool P8>
+template <int IO, int NS, int MODE>
 void scan_forward_run(const crnn_scan_args *a, ScanPlan &s, hipStream_t st) {
     using CT = typename crnn::SeqIO<IO>::C;
     crnn::ScanP p = s.p;
@@ -199,15 +204,15 @@ void scan_forward_run(const crnn_scan_args *a, ScanPlan &s, hipStream_t st) {
         p.first = b == 0;
         p.fin = b == s.nb - 1;
         if (s.split) {
-            hipLaunchKernelGGL((crnn::seq_scan_ends_kernel<IO, NS, P8, false>), grid, block, 0, st, p, S, (CT *)nullptr, sdel);
+            hipLaunchKernelGGL((crnn::seq_scan_ends_kernel<IO, NS, MODE, false>), grid, block, 0, st, p, S, (CT *)nullptr, sdel);
             hipLaunchKernelGGL((crnn::seq_scan_carry_kernel<CT, NS>), dim3((unsigned)(((int64_t)p.m.n_seq * NS * p.D + 255) / 256)), dim3(256), 0, st, p, S,
                                (CT *)nullptr, (const CT *)sdel);
         }
-        hipLaunchKernelGGL((crnn::seq_scan_out_kernel<IO, NS, P8>), grid, block, 0, st, p, (const CT *)(s.split ? S : nullptr));
+        hipLaunchKernelGGL((crnn::seq_scan_out_kernel<IO, NS, MODE>), grid, block, 0, st, p, (const CT *)(s.split ? S : nullptr));
     }
 }
 
-template <int IO, int NS, bool P8>
+template <int IO, int NS, int MODE>
 void scan_backward_run(const crnn_scan_args *a, ScanPlan &s, hipStream_t st) {
     using CT = typename crnn::SeqIO<IO>::C;
     crnn::ScanP p = s.p;
@@ -221,10 +226,10 @@ void scan_backward_run(const crnn_scan_args *a, ScanPlan &s, hipStream_t st) {
         p.n0 = mo.n0 = b * NS;
         p.first = b == 0;
         p.fin = b == s.nb - 1;
-        hipLaunchKernelGGL((crnn::seq_scan_ends_kernel<IO, NS, P8, true>), grid, block, 0, st, p, S, Gb, sdel);
+        hipLaunchKernelGGL((crnn::seq_scan_ends_kernel<IO, NS, MODE, true>), grid, block, 0, st, p, S, Gb, sdel);
         hipLaunchKernelGGL((crnn::seq_scan_carry_kernel<CT, NS>), dim3((unsigned)(((int64_t)p.m.n_seq * NS * p.D + 255) / 256)), dim3(256), 0, st, p, S, Gb,
                            (const CT *)sdel);
-        hipLaunchKernelGGL((crnn::seq_scan_bwd_kernel<IO, NS, P8>), grid, block, 0, st, p, (const CT *)S, (const CT *)Gb, part, dA, dD, db);
+        hipLaunchKernelGGL((crnn::seq_scan_bwd_kernel<IO, NS, MODE>), grid, block, 0, st, p, (const CT *)S, (const CT *)Gb, part, dA, dD, db);
         if (s.flat > 0)
             hipLaunchKernelGGL((crnn::seq_scan_sum_maps_kernel<CT, NS>), dim3(seq_grid(s.flat * p.G * 2 * NS)), dim3(256), 0, st, p.m, mo, (const CT *)part, p.tpg);
         hipLaunchKernelGGL((crnn::seq_sum_blocks_kernel<CT>), dim3((unsigned)((cA + 31) / 32)), dim3(256), 0, st, (const CT *)dA, p.m.nblk, cA, (CT *)a->dA, (CT *)nullptr, p.D,
@@ -252,17 +257,19 @@ bool scan_views(SeqCheck &c, const crnn_scan_args *a, bool backward) {
            c.view(a->dz, "dz", dt, false, false, true, D) && c.view(a->dB, "dB", dt, true, false, true, GN) && c.view(a->dC, "dC", dt, true, false, true, GN);
 }
 
+// the launches' template: MODE 2 (anything: several launches over the states, one of u and z a checkpoint) has 16 states a launch, 8 in double
 #define SCAN_RUN(run)                                                                                                         \
     do {                                                                                                                      \
         const hipStream_t st_ = (hipStream_t)a->stream;                                                                       \
-        if (s.f64) run<8, 8, false>(a, s, st_);                                                                               \
+        if (s.f64) run<8, 8, 2>(a, s, st_);                                                                                   \
         else if (a->dtype == CRNN_DT_F32) SCAN_RUN_IO(run, 4);                                                                \
         else SCAN_RUN_IO(run, 2);                                                                                             \
     } while (0)
 #define SCAN_RUN_IO(run, IO)                                                                                                  \
     do {                                                                                                                      \
-        if (s.NS == 8) { if (s.p8) run<IO, 8, true>(a, s, st_); else run<IO, 8, false>(a, s, st_); }                           \
-        else { if (s.p8) run<IO, 16, true>(a, s, st_); else run<IO, 16, false>(a, s, st_); }                                   \
+        if (s.mode == 2) run<IO, 16, 2>(a, s, st_);                                                                           \
+        else if (s.NS == 8) { if (s.mode) run<IO, 8, 1>(a, s, st_); else run<IO, 8, 0>(a, s, st_); }                           \
+        else { if (s.mode) run<IO, 16, 1>(a, s, st_); else run<IO, 16, 0>(a, s, st_); }                                        \
     } while (0)
 
 // ------------------------------------------------------------------ convolution

@@ -195,37 +195,39 @@ __device__ __forceinline__ void seq_zero_outside(const SeqMap &m, const SeqV &v,
 }
 
 // TB consecutive rows of one channel on their way into registers: the loads of several arrays are issued before the first one is needed,
-// conversion comes afterwards.  IO: bytes of an element (8: double).  Row addresses are uniform, the lane adds a 32-bit offset; rows
-// behind the n-th are read as the n-th (n >= 1).  P8: the array may be a checkpoint instead.
+// conversion comes afterwards.  IO: bytes of an element (8: double).  PM: 0 plain, 1 a checkpoint, 2 either (looked at per launch).  Row
+// addresses are uniform, the lane adds a 32-bit offset; rows behind the chunk's n-th are read as the n-th (n >= 1): no branch stands between
+// the loads and stores of a loop, so that the wait for a load need not wait for the stores behind it.
 template <int IO> struct SeqIO { using C = float; using E = uint32_t; };
 template <> struct SeqIO<2> { using C = float; using E = uint16_t; };
 template <> struct SeqIO<8> { using C = double; using E = double; };
 
-template <int IO, bool P8, int TB>
+template <int IO, int PM, int TB>
 struct SeqRows {
     using CT = typename SeqIO<IO>::C;
     using E = typename SeqIO<IO>::E;
     E r[TB];                     // checkpoint: the code, its scale byte above it
-    __device__ __forceinline__ void load(const SeqMap &m, const SeqV &v, const SeqChunk &k, int64_t t, uint32_t d, int n) {
-        if (P8 && v.dt == CRNN_DT_PACKED8) {
-            const int8_t *c = (const int8_t *)v.p + seq_off(m, v, k, t);
-            const uint8_t *e = v.sc + seq_soff(m, v, k, t);
+    // rows t .. t + TB - 1 of the chunk
+    __device__ __forceinline__ void load(const SeqMap &m, const SeqV &v, const SeqChunk &k, int t, uint32_t d) {
+        if (PM == 1 || (PM == 2 && v.dt == CRNN_DT_PACKED8)) {
+            const int8_t *c = (const int8_t *)v.p + seq_off(m, v, k, k.t0);
+            const uint8_t *e = v.sc + seq_soff(m, v, k, k.t0);
 #pragma unroll
             for (int i = 0; i < TB; ++i) {
-                const int64_t ii = i < n ? i : n - 1;
+                const int64_t ii = t + i < k.n ? t + i : k.n - 1;
                 r[i] = (E)((uint32_t)(uint8_t)(c + ii * v.rs)[d] | (uint32_t)(e + ii * v.srs)[d >> 5] << 8);
             }
         } else {
-            const E *c = (const E *)v.p + seq_off(m, v, k, t);
+            const E *c = (const E *)v.p + seq_off(m, v, k, k.t0);
 #pragma unroll
             for (int i = 0; i < TB; ++i) {
-                const int64_t ii = i < n ? i : n - 1;
+                const int64_t ii = t + i < k.n ? t + i : k.n - 1;
                 r[i] = (c + ii * v.rs)[d];
             }
         }
     }
     __device__ __forceinline__ void get(const SeqV &v, CT (&o)[TB]) const {
-        if (P8 && v.dt == CRNN_DT_PACKED8) {
+        if (PM == 1 || (PM == 2 && v.dt == CRNN_DT_PACKED8)) {
 #pragma unroll
             for (int i = 0; i < TB; ++i) o[i] = (CT)(int32_t)(int8_t)((uint32_t)r[i] & 0xffu) * (CT)seq_scale((uint32_t)r[i] >> 8);
         } else if (IO == 8) {
@@ -244,12 +246,15 @@ struct SeqRows {
     }
 };
 
-// TB rows of an output from a lane's registers; only the first n are stored
+// Rows t .. t + TB - 1 of the chunk to an output.  Rows behind the n-th store the n-th once more, and a lane without a channel of its own (its
+// inputs are the last channel's) stores the last channel's value once more.
 template <int IO, int TB>
-__device__ __forceinline__ void seq_put_rows(const SeqMap &m, const SeqV &v, const SeqChunk &k, int64_t t, uint32_t d, int n, bool valid, const typename SeqIO<IO>::C (&x)[TB]) {
+__device__ __forceinline__ void seq_put_rows(const SeqMap &m, const SeqV &v, const SeqChunk &k, int t, uint32_t d, typename SeqIO<IO>::C (&x)[TB]) {
     using E = typename SeqIO<IO>::E;
-    E *c = (E *)v.p + seq_off(m, v, k, t);
+    E *c = (E *)v.p + seq_off(m, v, k, k.t0);
     E b[TB];
+#pragma unroll
+    for (int i = 1; i < TB; ++i) x[i] = t + i < k.n ? x[i] : x[i - 1];
 #pragma unroll
     for (int i = 0; i < TB; ++i) {
         if (IO == 8) b[i] = (E)x[i];
@@ -264,10 +269,8 @@ __device__ __forceinline__ void seq_put_rows(const SeqMap &m, const SeqV &v, con
             for (int i = 0; i < TB; ++i) b[i] = (E)seq_to_f16((float)x[i]);
         }
     }
-    if (!valid) return;
 #pragma unroll
-    for (int i = 0; i < TB; ++i)
-        if (i < n) (c + (int64_t)i * v.rs)[d] = b[i];
+    for (int i = 0; i < TB; ++i) (c + (int64_t)(t + i < k.n ? t + i : k.n - 1) * v.rs)[d] = b[i];
 }
 
 // what a wavefront wrote to its own part of the LDS is there for all its lanes

@@ -33,6 +33,7 @@ struct ScanP {
     int32_t n0;                                   // first state of this launch
     int32_t first, fin;                           // first / last launch over the states
     int32_t softplus, zero_outside;
+    int32_t gate;                                 // z is there (else its view is u's, and what it gives is not used)
 };
 
 // ---- dB and dC
@@ -87,6 +88,9 @@ __device__ __forceinline__ void scan_state_put(const ScanP &p, void *st, int64_t
     for (int n = 0; n < NS; ++n)
         if (p.n0 + n < p.N) ((CT *)st)[(s * p.D + d) * p.N + p.n0 + n] = h[n];
 }
+// what a launch may meet: 0 plain arrays, all states at once; 1 the same with u, and z if there is one, as checkpoints; 2 anything
+constexpr int kScanAny = 2;
+
 // step lengths and inputs of TB rows; rows behind the n-th become steps of length 0 with nothing to add, so that the rows need no branches
 template <int IO, int TB>
 __device__ __forceinline__ void scan_steps(const ScanP &p, int n, typename SeqIO<IO>::C bias, typename SeqIO<IO>::C (&x)[TB], typename SeqIO<IO>::C (&u)[TB],
@@ -101,12 +105,10 @@ __device__ __forceinline__ void scan_steps(const ScanP &p, int n, typename SeqIO
 #pragma unroll
         for (int i = 0; i < TB; ++i) dl[i] = x[i];
     }
-    if (n < TB) {
 #pragma unroll
-        for (int i = 0; i < TB; ++i) {
-            dl[i] = i < n ? dl[i] : CT(0);
-            u[i] = i < n ? u[i] : CT(0);
-        }
+    for (int i = 1; i < TB; ++i) {
+        dl[i] = i < n ? dl[i] : CT(0);
+        u[i] = i < n ? u[i] : CT(0);
     }
 }
 
@@ -134,7 +136,7 @@ struct ScanMapRows {
         at = b ? pb + nn * p.Bn : pc + nn * p.Cn;
         rs = b ? p.B.rs : p.C.rs;
     }
-    // rows t .. t + TB - 1 of the chunk, those behind its n-th as the n-th
+    // rows t .. t + TB - 1 of the chunk
     __device__ __forceinline__ void load(int t, int n) {
 #pragma unroll
         for (int k = 0; k < V; ++k) {
@@ -157,7 +159,7 @@ struct ScanMapRows {
 };
 
 // ---- forward: outputs of a chunk from its first state (start[block][n][d]; null: one chunk a sequence, from state_in)
-template <int IO, int NS, bool P8>
+template <int IO, int NS, int MODE>
 __global__ __launch_bounds__(64 * kScanWaves, IO == 8 ? 2 : 4) void seq_scan_out_kernel(const ScanP p, const typename SeqIO<IO>::C *__restrict__ start) {
     using CT = typename SeqIO<IO>::C;
     constexpr int TB = kScanTB;
@@ -165,7 +167,8 @@ __global__ __launch_bounds__(64 * kScanWaves, IO == 8 ? 2 : 4) void seq_scan_out
     CT *maps = smaps[threadIdx.x >> 6];
     const ScanAt a = scan_at(p);
     if (!a.on) return;
-    if (p.zero_outside && p.fin) seq_zero_outside(p.m, p.y, a.b, a.d, a.valid);
+    const bool fin = MODE != kScanAny || p.fin;
+    if (p.zero_outside && fin) seq_zero_outside(p.m, p.y, a.b, a.d, a.valid);
     if (!a.k.live) return;
     CT A2[NS], h[NS];
     scan_rates<CT, NS>(p, a.d, A2);
@@ -175,67 +178,61 @@ __global__ __launch_bounds__(64 * kScanWaves, IO == 8 ? 2 : 4) void seq_scan_out
     } else {
         scan_state<CT, NS>(p, p.state_in, a.k.s, a.d, h);
     }
-    const CT bias = p.dt_bias ? ((const CT *)p.dt_bias)[a.d] : CT(0), skip = p.Dskip ? ((const CT *)p.Dskip)[a.d] : CT(0);
-    const bool gate = p.z.p && p.fin;
-    SeqRows<IO, P8, TB> ru, rz;
-    SeqRows<IO, false, TB> rd;
-    ScanMapRows<IO, NS, TB> rm;
-    rm.init(p, a);
     if (a.k.n > 0) {
+        const CT bias = p.dt_bias ? ((const CT *)p.dt_bias)[a.d] : CT(0), skip = p.Dskip ? ((const CT *)p.Dskip)[a.d] : CT(0);
+        SeqRows<IO, MODE, TB> ru, rz;
+        SeqRows<IO, 0, TB> rd;
+        ScanMapRows<IO, NS, TB> rm;
+        rm.init(p, a);
         rm.load(0, a.k.n);
-        const int nv = a.k.n < TB ? a.k.n : TB;
-        ru.load(p.m, p.u, a.k, a.k.t0, a.d, nv);
-        rd.load(p.m, p.dt, a.k, a.k.t0, a.d, nv);
-        if (gate) rz.load(p.m, p.z, a.k, a.k.t0, a.d, nv);
-    }
+        ru.load(p.m, p.u, a.k, 0, a.d);
+        rd.load(p.m, p.dt, a.k, 0, a.d);
+        rz.load(p.m, p.z, a.k, 0, a.d);
 #pragma unroll 1
-    for (int t = 0; t < a.k.n; t += TB) {
-        const int left = a.k.n - t, nv = left < TB ? left : TB;
-        CT u[TB], x[TB], z[TB], dl[TB], v[TB];
-        ru.get(p.u, u);
-        rd.get(p.dt, x);
-        if (gate) rz.get(p.z, z);
-        rm.put(p.B.dt, maps);
-        if (left > TB) {
+        for (int t = 0; t < a.k.n; t += TB) {
+            CT u[TB], x[TB], z[TB], dl[TB], v[TB];
+            ru.get(p.u, u);
+            rd.get(p.dt, x);
+            rz.get(p.z, z);
+            rm.put(p.B.dt, maps);
             rm.load(t + TB, a.k.n);
-            const int nn = left - TB < TB ? left - TB : TB;
-            ru.load(p.m, p.u, a.k, a.k.t0 + t + TB, a.d, nn);
-            rd.load(p.m, p.dt, a.k, a.k.t0 + t + TB, a.d, nn);
-            if (gate) rz.load(p.m, p.z, a.k, a.k.t0 + t + TB, a.d, nn);
-        }
-        scan_steps<IO, TB>(p, nv, bias, x, u, dl);
-        const int64_t frow = a.k.flat + a.k.t0 + t;
-#pragma unroll
-        for (int i = 0; i < TB; ++i) {
-            const CT *bc = maps + i * (2 * NS);
-            const CT du = dl[i] * u[i];
-            CT s0 = CT(0), s1 = CT(0);
-#pragma unroll
-            for (int n = 0; n < NS; n += 2) {
-                h[n] = seq_fma(seq_exp2(dl[i] * A2[n]), h[n], du * bc[n]);
-                h[n + 1] = seq_fma(seq_exp2(dl[i] * A2[n + 1]), h[n + 1], du * bc[n + 1]);
-                s0 = seq_fma(h[n], bc[NS + n], s0);
-                s1 = seq_fma(h[n + 1], bc[NS + n + 1], s1);
-            }
-            v[i] = s0 + s1;
-        }
-        seq_wave_sync();
-        if (p.acc) {
+            ru.load(p.m, p.u, a.k, t + TB, a.d);
+            rd.load(p.m, p.dt, a.k, t + TB, a.d);
+            rz.load(p.m, p.z, a.k, t + TB, a.d);
+            scan_steps<IO, TB>(p, a.k.n - t, bias, x, u, dl);
 #pragma unroll
             for (int i = 0; i < TB; ++i) {
-                CT *acc = (CT *)p.acc + (frow + (i < nv ? i : nv - 1)) * p.D;
-                if (!p.first) v[i] += acc[(uint32_t)a.d];
-                if (!p.fin && i < nv && a.valid) acc[(uint32_t)a.d] = v[i];
-            }
-        }
-        if (p.fin) {
+                const CT *bc = maps + i * (2 * NS);
+                const CT du = dl[i] * u[i];
+                CT s0 = CT(0), s1 = CT(0);
 #pragma unroll
-            for (int i = 0; i < TB; ++i) v[i] = seq_fma(skip, u[i], v[i]);
-            if (gate) {
-#pragma unroll
-                for (int i = 0; i < TB; ++i) v[i] *= z[i] * seq_sigmoid(z[i]);
+                for (int n = 0; n < NS; n += 2) {
+                    h[n] = seq_fma(seq_exp2(dl[i] * A2[n]), h[n], du * bc[n]);
+                    h[n + 1] = seq_fma(seq_exp2(dl[i] * A2[n + 1]), h[n + 1], du * bc[n + 1]);
+                    s0 = seq_fma(h[n], bc[NS + n], s0);
+                    s1 = seq_fma(h[n + 1], bc[NS + n + 1], s1);
+                }
+                v[i] = s0 + s1;
             }
-            seq_put_rows<IO, TB>(p.m, p.y, a.k, a.k.t0 + t, a.d, nv, a.valid, v);
+            seq_wave_sync();
+            if (MODE == kScanAny && p.acc) {
+#pragma unroll
+                for (int i = 0; i < TB; ++i) {
+                    const int ii = t + i < a.k.n ? t + i : a.k.n - 1;
+                    CT *acc = (CT *)p.acc + (a.k.flat + a.k.t0 + ii) * p.D;
+                    if (!p.first) v[i] += acc[(uint32_t)a.d];
+                    if (!fin && t + i < a.k.n && a.valid) acc[(uint32_t)a.d] = v[i];
+                }
+            }
+            if (fin) {
+#pragma unroll
+                for (int i = 0; i < TB; ++i) {
+                    v[i] = seq_fma(skip, u[i], v[i]);
+                    const CT g = z[i] * seq_sigmoid(z[i]);
+                    v[i] = p.gate ? v[i] * g : v[i];
+                }
+                seq_put_rows<IO, TB>(p.m, p.y, a.k, t, a.d, v);
+            }
         }
     }
     if (a.k.last && p.state_out && a.valid) scan_state_put<CT, NS>(p, p.state_out, a.k.s, a.d, h);
@@ -243,9 +240,10 @@ __global__ __launch_bounds__(64 * kScanWaves, IO == 8 ? 2 : 4) void seq_scan_out
 
 // ---- a chunk by itself: S = its last state from zero, sum of delta; BOTH: also G = what its outputs' gradients r pass back to the state
 // before it, sum_t (prod of the decays up to t) r C -- taken in the forward direction, so that one exponential serves both.
-template <int IO, int NS, bool P8, bool BOTH>
-__global__ __launch_bounds__(64 * kScanWaves, IO == 8 ? 2 : BOTH ? 3 : 5) void seq_scan_ends_kernel(const ScanP p, typename SeqIO<IO>::C *__restrict__ S, typename SeqIO<IO>::C *__restrict__ Gb,
-                                                                        typename SeqIO<IO>::C *__restrict__ sdel) {
+template <int IO, int NS, int MODE, bool BOTH>
+__global__ __launch_bounds__(64 * kScanWaves, IO == 8 ? 2 : BOTH ? 3 : 5) void seq_scan_ends_kernel(const ScanP p, typename SeqIO<IO>::C *__restrict__ S,
+                                                                                                  typename SeqIO<IO>::C *__restrict__ Gb,
+                                                                                                  typename SeqIO<IO>::C *__restrict__ sdel) {
     using CT = typename SeqIO<IO>::C;
     constexpr int TB = kScanTB;
     __shared__ CT smaps[kScanWaves][TB * 2 * NS];
@@ -259,63 +257,63 @@ __global__ __launch_bounds__(64 * kScanWaves, IO == 8 ? 2 : BOTH ? 3 : 5) void s
         h[n] = CT(0);
         if (BOTH) { P[BOTH ? n : 0] = CT(1); g[BOTH ? n : 0] = CT(0); }
     }
-    const CT bias = p.dt_bias ? ((const CT *)p.dt_bias)[a.d] : CT(0);
-    const bool gate = BOTH && p.z.p;
     CT sd = CT(0);
-    SeqRows<IO, P8, TB> ru, rz;
-    SeqRows<IO, false, TB> rd, ry;
-    ScanMapRows<IO, NS, TB> rm;
-    rm.init(p, a);
     if (a.k.n > 0) {
+        const CT bias = p.dt_bias ? ((const CT *)p.dt_bias)[a.d] : CT(0);
+        SeqRows<IO, MODE, TB> ru, rz;
+        SeqRows<IO, 0, TB> rd, ry;
+        ScanMapRows<IO, NS, TB> rm;
+        rm.init(p, a);
         rm.load(0, a.k.n);
-        const int nv = a.k.n < TB ? a.k.n : TB;
-        ru.load(p.m, p.u, a.k, a.k.t0, a.d, nv);
-        rd.load(p.m, p.dt, a.k, a.k.t0, a.d, nv);
-        if (BOTH) ry.load(p.m, p.dy, a.k, a.k.t0, a.d, nv);
-        if (gate) rz.load(p.m, p.z, a.k, a.k.t0, a.d, nv);
-    }
+        ru.load(p.m, p.u, a.k, 0, a.d);
+        rd.load(p.m, p.dt, a.k, 0, a.d);
+        if (BOTH) {
+            ry.load(p.m, p.dy, a.k, 0, a.d);
+            rz.load(p.m, p.z, a.k, 0, a.d);
+        }
 #pragma unroll 1
-    for (int t = 0; t < a.k.n; t += TB) {
-        const int left = a.k.n - t, nv = left < TB ? left : TB;
-        CT u[TB], x[TB], z[TB], y[TB], dl[TB];
-        ru.get(p.u, u);
-        rd.get(p.dt, x);
-        if (BOTH) ry.get(p.dy, y);
-        if (gate) rz.get(p.z, z);
-        rm.put(p.B.dt, maps);
-        if (left > TB) {
+        for (int t = 0; t < a.k.n; t += TB) {
+            CT u[TB], x[TB], z[TB], y[TB], dl[TB];
+            ru.get(p.u, u);
+            rd.get(p.dt, x);
+            if (BOTH) {
+                ry.get(p.dy, y);
+                rz.get(p.z, z);
+            }
+            rm.put(p.B.dt, maps);
             rm.load(t + TB, a.k.n);
-            const int nn = left - TB < TB ? left - TB : TB;
-            ru.load(p.m, p.u, a.k, a.k.t0 + t + TB, a.d, nn);
-            rd.load(p.m, p.dt, a.k, a.k.t0 + t + TB, a.d, nn);
-            if (BOTH) ry.load(p.m, p.dy, a.k, a.k.t0 + t + TB, a.d, nn);
-            if (gate) rz.load(p.m, p.z, a.k, a.k.t0 + t + TB, a.d, nn);
-        }
-        scan_steps<IO, TB>(p, nv, bias, x, u, dl);
-        if (gate) {
+            ru.load(p.m, p.u, a.k, t + TB, a.d);
+            rd.load(p.m, p.dt, a.k, t + TB, a.d);
+            if (BOTH) {
+                ry.load(p.m, p.dy, a.k, t + TB, a.d);
+                rz.load(p.m, p.z, a.k, t + TB, a.d);
+            }
+            scan_steps<IO, TB>(p, a.k.n - t, bias, x, u, dl);
+            if (BOTH) {
 #pragma unroll
-            for (int i = 0; i < TB; ++i) y[i] *= z[i] * seq_sigmoid(z[i]);
-        }
-        if (BOTH && nv < TB) {
-#pragma unroll
-            for (int i = 0; i < TB; ++i) y[i] = i < nv ? y[i] : CT(0);
-        }
-#pragma unroll
-        for (int i = 0; i < TB; ++i) {
-            const CT *bc = maps + i * (2 * NS);
-            const CT du = dl[i] * u[i];
-            sd += dl[i];
-#pragma unroll
-            for (int n = 0; n < NS; ++n) {
-                const CT e = seq_exp2(dl[i] * A2[n]);
-                h[n] = seq_fma(e, h[n], du * bc[n]);
-                if (BOTH) {
-                    P[BOTH ? n : 0] *= e;
-                    g[BOTH ? n : 0] = seq_fma(P[BOTH ? n : 0], y[i] * bc[NS + n], g[BOTH ? n : 0]);
+                for (int i = 0; i < TB; ++i) {
+                    const CT gz = z[i] * seq_sigmoid(z[i]);
+                    y[i] = p.gate ? y[i] * gz : y[i];
+                    y[i] = t + i < a.k.n ? y[i] : CT(0);
                 }
             }
+#pragma unroll
+            for (int i = 0; i < TB; ++i) {
+                const CT *bc = maps + i * (2 * NS);
+                const CT du = dl[i] * u[i];
+                sd += dl[i];
+#pragma unroll
+                for (int n = 0; n < NS; ++n) {
+                    const CT e = seq_exp2(dl[i] * A2[n]);
+                    h[n] = seq_fma(e, h[n], du * bc[n]);
+                    if (BOTH) {
+                        P[BOTH ? n : 0] *= e;
+                        g[BOTH ? n : 0] = seq_fma(P[BOTH ? n : 0], y[i] * bc[NS + n], g[BOTH ? n : 0]);
+                    }
+                }
+            }
+            seq_wave_sync();
         }
-        seq_wave_sync();
     }
     if (!a.valid) return;
 #pragma unroll
@@ -387,19 +385,21 @@ __global__ __launch_bounds__(256) void seq_scan_carry_kernel(const ScanP p, CT *
 // wavefront's part goes to part[tile][row][B: NS | C: NS], summed over the tiles in a fixed order by seq_scan_sum_maps_kernel.
 // Four rows and five times four a chunk: two wavefronts a SIMD fill the registers (256 a lane) and the LDS (16.5 KB each) about together.
 constexpr int kScanBwdTB = 4, kScanBwdSub = 5, kScanBwdQ = kScanBwdTB * kScanBwdSub;
-template <int IO, int NS, bool P8>
-__global__ __launch_bounds__(64 * kScanWaves, 2) void seq_scan_bwd_kernel(const ScanP p, const typename SeqIO<IO>::C *__restrict__ start, const typename SeqIO<IO>::C *__restrict__ back,
-                                                                          typename SeqIO<IO>::C *__restrict__ part, typename SeqIO<IO>::C *__restrict__ dApart,
-                                                                          typename SeqIO<IO>::C *__restrict__ dDpart, typename SeqIO<IO>::C *__restrict__ dbpart) {
+template <int IO, int NS, int MODE>
+__global__ __launch_bounds__(64 * kScanWaves, 2) void seq_scan_bwd_kernel(const ScanP p, const typename SeqIO<IO>::C *__restrict__ start,
+                                                                          const typename SeqIO<IO>::C *__restrict__ back, typename SeqIO<IO>::C *__restrict__ part,
+                                                                          typename SeqIO<IO>::C *__restrict__ dApart, typename SeqIO<IO>::C *__restrict__ dDpart,
+                                                                          typename SeqIO<IO>::C *__restrict__ dbpart) {
     using CT = typename SeqIO<IO>::C;
     constexpr int TB = kScanBwdTB, H = NS / 2;
     __shared__ CT keep[kScanWaves][kScanBwdSub - 1][NS][64];
     __shared__ CT smaps[kScanWaves][TB * 2 * NS];
-    CT *maps = smaps[threadIdx.x >> 6];
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    CT *maps = smaps[wave];
     const ScanAt a = scan_at(p);
     if (!a.on) return;
-    if (p.zero_outside && p.fin) {
+    const bool fin = MODE != kScanAny || p.fin;
+    if (p.zero_outside && fin) {
         seq_zero_outside(p.m, p.du, a.b, a.d, a.valid);
         seq_zero_outside(p.m, p.ddt, a.b, a.d, a.valid);
         seq_zero_outside(p.m, p.dz, a.b, a.d, a.valid);
@@ -417,28 +417,23 @@ __global__ __launch_bounds__(64 * kScanWaves, 2) void seq_scan_bwd_kernel(const 
         }
         const CT bias = p.dt_bias ? ((const CT *)p.dt_bias)[a.d] : CT(0), skip = p.Dskip ? ((const CT *)p.Dskip)[a.d] : CT(0);
         const int nsub = (a.k.n + TB - 1) / TB;
-        SeqRows<IO, P8, TB> ru, rz;
-        SeqRows<IO, false, TB> rd, ry;
+        SeqRows<IO, MODE, TB> ru, rz;
+        SeqRows<IO, 0, TB> rd, ry;
         ScanMapRows<IO, NS, TB> rm;
         rm.init(p, a);
-        {
-            const int nn = a.k.n < TB ? a.k.n : TB;
-            rm.load(0, a.k.n);
-            ru.load(p.m, p.u, a.k, a.k.t0, a.d, nn);
-            rd.load(p.m, p.dt, a.k, a.k.t0, a.d, nn);
-        }
+        rm.load(0, a.k.n);
+        ru.load(p.m, p.u, a.k, 0, a.d);
+        rd.load(p.m, p.dt, a.k, 0, a.d);
 #pragma unroll 1
         for (int k = 0; k < nsub - 1; ++k) {
             CT u[TB], x[TB], dl[TB];
             ru.get(p.u, u);
             rd.get(p.dt, x);
             rm.put(p.B.dt, maps);
-            {       // the next rows; the last ones of the chunk stay for the way back
-                const int t = (k + 1) * TB, nn = a.k.n - t < TB ? a.k.n - t : TB;
-                rm.load(t, a.k.n);
-                ru.load(p.m, p.u, a.k, a.k.t0 + t, a.d, nn);
-                rd.load(p.m, p.dt, a.k, a.k.t0 + t, a.d, nn);
-            }
+            // the next rows; the last ones of the chunk stay for the way back
+            rm.load((k + 1) * TB, a.k.n);
+            ru.load(p.m, p.u, a.k, (k + 1) * TB, a.d);
+            rd.load(p.m, p.dt, a.k, (k + 1) * TB, a.d);
             scan_steps<IO, TB>(p, TB, bias, x, u, dl);
 #pragma unroll
             for (int i = 0; i < TB; ++i) {
@@ -451,24 +446,24 @@ __global__ __launch_bounds__(64 * kScanWaves, 2) void seq_scan_bwd_kernel(const 
             for (int n = 0; n < NS; ++n) keep[wave][k][n][lane] = h[n];
             seq_wave_sync();
         }
+        ry.load(p.m, p.dy, a.k, (nsub - 1) * TB, a.d);
+        rz.load(p.m, p.z, a.k, (nsub - 1) * TB, a.d);
+        CT *prow = part + ((int64_t)a.tile * p.acc_n + a.k.flat + a.k.t0) * (2 * NS);
+        const uint32_t pidx = (uint32_t)seq_spread_index<2 * NS>(lane);
 #pragma unroll 1
         for (int k = nsub - 1; k >= 0; --k) {
-            const int nv = a.k.n - k * TB < TB ? a.k.n - k * TB : TB;
-            const int64_t t = a.k.t0 + k * TB, frow = a.k.flat + t;
+            const int t = k * TB, nv = a.k.n - t, before = k > 0 ? t - TB : 0;
             CT u[TB], x[TB], z[TB], y[TB], dl[TB], ah[TB][NS];
-            ry.load(p.m, p.dy, a.k, t, a.d, nv);
-            if (p.z.p) rz.load(p.m, p.z, a.k, t, a.d, nv);
             ru.get(p.u, u);
             rd.get(p.dt, x);
             rm.put(p.B.dt, maps);
+            rm.load(before, a.k.n);
+            ru.load(p.m, p.u, a.k, before, a.d);
+            rd.load(p.m, p.dt, a.k, before, a.d);
             if (k > 0) {
-                rm.load((k - 1) * TB, a.k.n);
-                ru.load(p.m, p.u, a.k, t - TB, a.d, TB);
-                rd.load(p.m, p.dt, a.k, t - TB, a.d, TB);
-            }
 #pragma unroll
-            for (int n = 0; n < NS; ++n) h[n] = keep[wave][k > 0 ? k - 1 : 0][n][lane];
-            if (k == 0) {
+                for (int n = 0; n < NS; ++n) h[n] = keep[wave][k - 1][n][lane];
+            } else {
 #pragma unroll
                 for (int n = 0; n < NS; ++n) h[n] = scan_plane<NS>(start, a.b, n, p.D)[(uint32_t)a.d];
             }
@@ -485,21 +480,17 @@ __global__ __launch_bounds__(64 * kScanWaves, 2) void seq_scan_bwd_kernel(const 
                 }
             }
             ry.get(p.dy, y);
-            if (p.z.p) rz.get(p.z, z);
-            if (nv < TB) {
-#pragma unroll
-                for (int i = 0; i < TB; ++i) {
-                    y[i] = i < nv ? y[i] : CT(0);
-                    z[i] = i < nv ? z[i] : CT(0);
-                }
-            }
+            rz.get(p.z, z);
+            ry.load(p.m, p.dy, a.k, before, a.d);
+            rz.load(p.m, p.z, a.k, before, a.d);
             CT odu[TB], odt[TB], odz[TB];
 #pragma unroll
             for (int i = TB - 1; i >= 0; --i) {
-                __builtin_amdgcn_sched_barrier(0);
-                const CT du = dl[i] * u[i];
-                const CT sg = p.z.p ? seq_sigmoid(z[i]) : CT(1);
-                const CT r = p.z.p ? y[i] * (z[i] * sg) : y[i];
+                __builtin_amdgcn_sched_barrier(0);      // a row after the other: interleaved they would not fit the registers
+                const bool in = i < nv;
+                const int64_t ii = t + (in ? i : nv - 1);
+                const CT du = dl[i] * u[i], yi = in ? y[i] : CT(0), zi = in ? z[i] : CT(0);
+                const CT sg = seq_sigmoid(zi), gz = zi * sg, r = p.gate ? yi * gz : yi;
                 const CT *bc = maps + i * (2 * NS);
                 CT v = CT(0), qb = CT(0), qa = CT(0), f[H], dle = dl[i];
                 asm volatile("" : "+v"(dle));      // the decays are formed again rather than kept: NS registers a row
@@ -522,36 +513,37 @@ __global__ __launch_bounds__(64 * kScanWaves, 2) void seq_scan_bwd_kernel(const 
                     }
                     f[j] = seq_fold16(w[0], w[1]);
                 }
-                const CT sum = seq_spread_rest(f);
-                if (i < nv && (lane & (64 / (2 * NS) - 1)) == 0)
-                    part[((int64_t)a.tile * p.acc_n + frow + i) * (2 * NS) + seq_spread_index<2 * NS>(lane)] = sum;
-                if (p.acc && i < nv) {
-                    CT *acc = (CT *)p.acc + (frow + i) * p.D + a.d;
+                asm volatile("" : "+v"(v), "+v"(qb), "+v"(qa));      // here, not where they are used: a sum moved there keeps its terms alive
+                // lanes that hold the same sum store it together; rows behind the n-th come first and are overwritten by the n-th
+                (prow + ii * (2 * NS))[pidx] = seq_spread_rest(f);
+                if (MODE == kScanAny && p.acc && in) {
+                    CT *acc = (CT *)p.acc + (a.k.flat + a.k.t0 + ii) * p.D + a.d;
                     const int64_t stride = p.acc_n * p.D;
                     if (!p.first) { v += acc[0]; qb += acc[stride]; qa += acc[2 * stride]; }
-                    if (!p.fin && a.valid) { acc[0] = v; acc[stride] = qb; acc[2 * stride] = qa; }
+                    if (!fin && a.valid) { acc[0] = v; acc[stride] = qb; acc[2 * stride] = qa; }
                 }
                 CT ddt = seq_fma(qa, CT(0.6931471805599453), qb * u[i]);
-                if (p.softplus) ddt *= seq_sigmoid(x[i]);
-                ddt = i < nv ? ddt : CT(0);
+                const CT sx = seq_sigmoid(x[i]);
+                ddt = p.softplus ? ddt * sx : ddt;
+                ddt = in ? ddt : CT(0);
                 dD = seq_fma(r, u[i], dD);
                 db += ddt;
                 odu[i] = seq_fma(dl[i], qb, r * skip);
                 odt[i] = ddt;
-                odz[i] = y[i] * seq_fma(skip, u[i], v) * (sg * seq_fma(z[i], CT(1) - sg, CT(1)));
-            }
-            if (p.fin) {
-                seq_put_rows<IO, TB>(p.m, p.du, a.k, t, a.d, nv, a.valid, odu);
-                seq_put_rows<IO, TB>(p.m, p.ddt, a.k, t, a.d, nv, a.valid, odt);
-                if (p.dz.p) seq_put_rows<IO, TB>(p.m, p.dz, a.k, t, a.d, nv, a.valid, odz);
+                odz[i] = yi * seq_fma(skip, u[i], v) * (sg * seq_fma(zi, CT(1) - sg, CT(1)));
             }
             seq_wave_sync();
+            if (fin) {
+                seq_put_rows<IO, TB>(p.m, p.du, a.k, t, a.d, odu);
+                seq_put_rows<IO, TB>(p.m, p.ddt, a.k, t, a.d, odt);
+                if (p.gate) seq_put_rows<IO, TB>(p.m, p.dz, a.k, t, a.d, odz);
+            }
         }
     }
     if (!a.valid) return;
 #pragma unroll
     for (int n = 0; n < NS; ++n) scan_plane<NS>(dApart, a.b, n, p.D)[(uint32_t)a.d] = dA[n];
-    if (p.fin) {
+    if (fin) {
         dDpart[a.b * p.D + a.d] = dD;
         dbpart[a.b * p.D + a.d] = db;
     }
