@@ -273,22 +273,37 @@ bool scan_views(SeqCheck &c, const crnn_scan_args *a, bool backward) {
     } while (0)
 
 // ------------------------------------------------------------------ convolution
-// Rows of a strip: short enough that strips and channels give each SIMD some wavefronts, long enough that the rows read twice (W - 1 a strip;
-// the gradient 2 (W - 1)) stay few.
-int64_t conv_strip(int64_t flat, int32_t D, bool backward) {
-    const int64_t waves = (D + 64 * crnn::kConvV - 1) / (64 * crnn::kConvV);
-    int64_t q = flat * waves / 8192;
+// channels of a thread: 16 bytes of a row of the call's type (half of that with more than four taps, and in the gradient: registers), one where
+// an array of the call does not allow it
+int conv_wide(int dtype, int W, bool backward) {
+    if (dtype == CRNN_DT_F64) return 2;
+    if (dtype == CRNN_DT_F32) return W > 4 && backward ? 2 : 4;
+    return W > 4 || backward ? 4 : 8;
+}
+// Rows of a strip: strips and channels together give some wavefronts to each SIMD; a strip reads W - 1 rows twice, the gradient 2 (W - 1).
+int64_t conv_strip(int64_t flat, int32_t D, int V, bool backward) {
+    const int64_t waves = (D + 64 * V - 1) / (64 * V);
+    const int64_t q = flat * waves / 4096 / 4 * 4;
     const int64_t lo = backward ? 16 : 8, hi = backward ? 64 : 32;
     return q < lo ? lo : q > hi ? hi : q;
 }
+bool conv_fits(const crnn_view &v, int V) { return !v.ptr || (seq_view(v, V).vec && v.row_stride < 0x7fffffff); }
+// which: 0 forward, 1 backward, 2 step
+int conv_channels(const crnn_conv_args *a, int which) {
+    const int V = conv_wide(a->dtype, a->W, which == 1);
+    const bool fits = a->D % V == 0 && conv_fits(a->x, V) && conv_fits(a->y, V) && conv_fits(a->state_in, V) && conv_fits(a->state_out, V) && conv_fits(a->dy, V) &&
+                      conv_fits(a->dx, V) && conv_fits(a->dstate_out, V) && conv_fits(a->dstate_in, V);
+    return fits ? V : 1;
+}
+// chunks do not depend on V (the workspace is asked for before the arrays are known)
 bool conv_check(SeqCheck &c, const crnn_conv_args *a, bool backward, crnn::ConvP &p) {
     if (!seq_rows_ok(c, a->n_seq, a->rows, a->seq_start, a->seq_len, a->D, a->dtype)) return false;
     if (a->W < 1 || a->W > CRNN_SEQ_MAX_TAPS) return c.bad("W must be in 1 .. 8");
     p = crnn::ConvP{};
     p.D = a->D; p.W = a->W; p.silu = a->silu; p.zero_outside = a->zero_outside;
-    p.m = seq_map(a->n_seq, a->rows, a->seq_start, a->seq_len, conv_strip(seq_flat(a->n_seq, a->rows, a->seq_start != nullptr), a->D, backward));
-    const int64_t gx = (a->D + 64 * crnn::kConvV - 1) / (64 * crnn::kConvV);
-    if ((p.m.nblk + 3) / 4 * gx > kSeqMaxGrid) return c.bad("too many sequences, rows and channels for one launch");
+    p.m = seq_map(a->n_seq, a->rows, a->seq_start, a->seq_len,
+                  conv_strip(seq_flat(a->n_seq, a->rows, a->seq_start != nullptr), a->D, conv_wide(a->dtype, a->W, backward), backward));
+    if ((p.m.nblk + 3) / 4 * ((a->D + 63) / 64) > kSeqMaxGrid) return c.bad("too many sequences, rows and channels for one launch");
     return true;
 }
 bool conv_views(SeqCheck &c, const crnn_conv_args *a, bool backward, crnn::ConvP &p) {
@@ -304,38 +319,52 @@ bool conv_views(SeqCheck &c, const crnn_conv_args *a, bool backward, crnn::ConvP
         if (!c.view(a->y, "y", dt, true, false, true, a->D) || !c.view(a->state_out, "state_out", dt, false, false, true, a->D)) return false;
         if (a->state_out.ptr && a->state_out.ptr == a->state_in.ptr) return c.bad("state_out may not be state_in");
     }
-    const int V = crnn::kConvV;
-    p.x = seq_view(a->x, V); p.y = seq_view(a->y, V); p.dy = seq_view(a->dy, V); p.dx = seq_view(a->dx, V);
-    p.st_in = seq_view(a->state_in, V); p.st_out = seq_view(a->state_out, V); p.dst_out = seq_view(a->dstate_out, V); p.dst_in = seq_view(a->dstate_in, V);
+    p.x = seq_view(a->x, 1); p.y = seq_view(a->y, 1); p.dy = seq_view(a->dy, 1); p.dx = seq_view(a->dx, 1);
+    p.st_in = seq_view(a->state_in, 1); p.st_out = seq_view(a->state_out, 1); p.dst_out = seq_view(a->dstate_out, 1); p.dst_in = seq_view(a->dstate_in, 1);
     p.w = a->weight; p.bias = a->bias;
     return true;
 }
-template <int XT, int YT, int WM>
+template <int XT, int YT, int WM, int V>
 void conv_launch(const crnn::ConvP &p, bool backward, hipStream_t st) {
-    const int64_t gx = (p.D + 64 * crnn::kConvV - 1) / (64 * crnn::kConvV);
+    const int64_t gx = (p.D + 64 * V - 1) / (64 * V);
     const dim3 grid((unsigned)((p.m.nblk + 3) / 4 * gx));
-    if (backward) hipLaunchKernelGGL((crnn::seq_conv_bwd_kernel<XT, YT, WM>), grid, dim3(256), 0, st, p);
-    else hipLaunchKernelGGL((crnn::seq_conv_fwd_kernel<XT, YT, WM>), grid, dim3(256), 0, st, p);
+    if (backward) hipLaunchKernelGGL((crnn::seq_conv_bwd_kernel<XT, YT, WM, V>), grid, dim3(256), 0, st, p);
+    else hipLaunchKernelGGL((crnn::seq_conv_fwd_kernel<XT, YT, WM, V>), grid, dim3(256), 0, st, p);
 }
-template <int XT, int YT>
-void conv_launch_w(const crnn::ConvP &p, bool backward, hipStream_t st) {
-    if (p.W <= 4) conv_launch<XT, YT, 4>(p, backward, st);
-    else conv_launch<XT, YT, 8>(p, backward, st);
+// VF, VB: the wide forms' channels for up to four taps, forward and backward (conv_wide)
+template <int XT, int YT, int VF, int VB>
+void conv_launch_w(const crnn::ConvP &p, int V, bool backward, hipStream_t st) {
+    constexpr int V8 = YT == CRNN_DT_F64 ? 2 : 4, V8B = YT == CRNN_DT_F64 || YT == CRNN_DT_F32 ? 2 : 4;
+    if (p.W <= 4) {
+        if (V == 1) conv_launch<XT, YT, 4, 1>(p, backward, st);
+        else if (backward) { const int64_t gx = (p.D + 64 * VB - 1) / (64 * VB); hipLaunchKernelGGL((crnn::seq_conv_bwd_kernel<XT, YT, 4, VB>), dim3((unsigned)((p.m.nblk + 3) / 4 * gx)), dim3(256), 0, st, p); }
+        else { const int64_t gx = (p.D + 64 * VF - 1) / (64 * VF); hipLaunchKernelGGL((crnn::seq_conv_fwd_kernel<XT, YT, 4, VF>), dim3((unsigned)((p.m.nblk + 3) / 4 * gx)), dim3(256), 0, st, p); }
+    } else {
+        if (V == 1) conv_launch<XT, YT, 8, 1>(p, backward, st);
+        else if (backward) { const int64_t gx = (p.D + 64 * V8B - 1) / (64 * V8B); hipLaunchKernelGGL((crnn::seq_conv_bwd_kernel<XT, YT, 8, V8B>), dim3((unsigned)((p.m.nblk + 3) / 4 * gx)), dim3(256), 0, st, p); }
+        else { const int64_t gx = (p.D + 64 * V8 - 1) / (64 * V8); hipLaunchKernelGGL((crnn::seq_conv_fwd_kernel<XT, YT, 8, V8>), dim3((unsigned)((p.m.nblk + 3) / 4 * gx)), dim3(256), 0, st, p); }
+    }
 }
-void conv_launch_t(const crnn::ConvP &p, int dtype, bool backward, hipStream_t st) {
+void conv_launch_t(const crnn::ConvP &p, int dtype, int V, bool backward, hipStream_t st) {
     const bool q = p.x.dt == CRNN_DT_PACKED8;
-    if (dtype == CRNN_DT_F64) conv_launch_w<CRNN_DT_F64, CRNN_DT_F64>(p, backward, st);
-    else if (dtype == CRNN_DT_F32) { if (q) conv_launch_w<CRNN_DT_PACKED8, CRNN_DT_F32>(p, backward, st); else conv_launch_w<CRNN_DT_F32, CRNN_DT_F32>(p, backward, st); }
-    else if (dtype == CRNN_DT_BF16) { if (q) conv_launch_w<CRNN_DT_PACKED8, CRNN_DT_BF16>(p, backward, st); else conv_launch_w<CRNN_DT_BF16, CRNN_DT_BF16>(p, backward, st); }
-    else { if (q) conv_launch_w<CRNN_DT_PACKED8, CRNN_DT_F16>(p, backward, st); else conv_launch_w<CRNN_DT_F16, CRNN_DT_F16>(p, backward, st); }
+    if (dtype == CRNN_DT_F64) conv_launch_w<CRNN_DT_F64, CRNN_DT_F64, 2, 2>(p, V, backward, st);
+    else if (dtype == CRNN_DT_F32) { if (q) conv_launch_w<CRNN_DT_PACKED8, CRNN_DT_F32, 4, 4>(p, V, backward, st); else conv_launch_w<CRNN_DT_F32, CRNN_DT_F32, 4, 4>(p, V, backward, st); }
+    else if (dtype == CRNN_DT_BF16) { if (q) conv_launch_w<CRNN_DT_PACKED8, CRNN_DT_BF16, 8, 4>(p, V, backward, st); else conv_launch_w<CRNN_DT_BF16, CRNN_DT_BF16, 8, 4>(p, V, backward, st); }
+    else { if (q) conv_launch_w<CRNN_DT_PACKED8, CRNN_DT_F16, 8, 4>(p, V, backward, st); else conv_launch_w<CRNN_DT_F16, CRNN_DT_F16, 8, 4>(p, V, backward, st); }
 }
-template <int YT>
+template <int YT, int WM, int V>
 void conv_step_launch(const crnn::ConvStepP &p, hipStream_t st) {
-    const int64_t gx = (p.D + 256 * crnn::kConvV - 1) / (256 * crnn::kConvV);
-    const dim3 grid((unsigned)(p.rows * gx));
-    if (p.W <= 4) hipLaunchKernelGGL((crnn::seq_conv_step_kernel<YT, 4>), grid, dim3(256), 0, st, p);
-    else hipLaunchKernelGGL((crnn::seq_conv_step_kernel<YT, 8>), grid, dim3(256), 0, st, p);
+    const int64_t gx = (p.D + 256 * V - 1) / (256 * V);
+    hipLaunchKernelGGL((crnn::seq_conv_step_kernel<YT, WM, V>), dim3((unsigned)(p.rows * gx)), dim3(256), 0, st, p);
 }
+// (four channels of a thread at most: the rows are few, the wavefronts should not be)
+template <int YT>
+void conv_step_launch_w(const crnn::ConvStepP &p, int V, hipStream_t st) {
+    constexpr int VW = YT == CRNN_DT_F64 ? 2 : 4;
+    if (p.W <= 4) { if (V == 1) conv_step_launch<YT, 4, 1>(p, st); else conv_step_launch<YT, 4, VW>(p, st); }
+    else { if (V == 1) conv_step_launch<YT, 8, 1>(p, st); else conv_step_launch<YT, 8, VW>(p, st); }
+}
+
 }  // namespace
 
 extern "C" {
@@ -359,7 +388,7 @@ int32_t crnn_conv_forward(const crnn_conv_args *a) {
         if (a->n_seq == 0) return 0;
         if (!conv_views(c, a, false, p)) return sfail(c.err);
         SEQ_DEVICE(a->device, "crnn_conv_forward");
-        conv_launch_t(p, a->dtype, false, (hipStream_t)a->stream);
+        conv_launch_t(p, a->dtype, conv_channels(a, 0), false, (hipStream_t)a->stream);
         SEQ_DONE("crnn_conv_forward");
     } catch (...) { return -1; }
 }
@@ -376,7 +405,7 @@ int32_t crnn_conv_backward(const crnn_conv_args *a) {
         SEQ_DEVICE(a->device, "crnn_conv_backward");
         p.part = a->workspace;
         const hipStream_t st = (hipStream_t)a->stream;
-        if (a->n_seq > 0) conv_launch_t(p, a->dtype, true, st);
+        if (a->n_seq > 0) conv_launch_t(p, a->dtype, conv_channels(a, 1), true, st);
         const int64_t count = (int64_t)(a->W + 1) * a->D;       // [tap][D], then the bias
         const dim3 grid((unsigned)((count + 31) / 32));
         if (f64)
@@ -403,18 +432,19 @@ int32_t crnn_conv_step(const crnn_conv_args *a) {
             return sfail(c.err);
         if (!a->weight) return sfail("crnn_conv_step: weight is missing");
         if (a->W > 1 && a->n_slots > 1 && a->state_in.seq_stride < (a->W - 1) * a->state_in.row_stride) return sfail("crnn_conv_step: the states of two slots overlap");
-        const int64_t gx = (a->D + 256 * crnn::kConvV - 1) / (256 * crnn::kConvV);
-        if (a->n_seq * gx > kSeqMaxGrid) return sfail("crnn_conv_step: too many rows and channels for one launch");
+        if (a->n_seq * (int64_t)((a->D + 255) / 256) > kSeqMaxGrid) return sfail("crnn_conv_step: too many rows and channels for one launch");
         SEQ_DEVICE(a->device, "crnn_conv_step");
         crnn::ConvStepP p{};
-        p.x = seq_view(a->x, crnn::kConvV); p.y = seq_view(a->y, crnn::kConvV); p.st = seq_view(a->state_in, crnn::kConvV);
+        p.x = seq_view(a->x, 1); p.y = seq_view(a->y, 1); p.st = seq_view(a->state_in, 1);
         p.w = a->weight; p.bias = a->bias; p.slot = a->slot; p.rows = a->n_seq; p.n_slots = a->n_slots;
         p.D = a->D; p.W = a->W; p.silu = a->silu;
         const hipStream_t st = (hipStream_t)a->stream;
-        if (a->dtype == CRNN_DT_F64) conv_step_launch<CRNN_DT_F64>(p, st);
-        else if (a->dtype == CRNN_DT_F32) conv_step_launch<CRNN_DT_F32>(p, st);
-        else if (a->dtype == CRNN_DT_BF16) conv_step_launch<CRNN_DT_BF16>(p, st);
-        else conv_step_launch<CRNN_DT_F16>(p, st);
+        const int VW = a->dtype == CRNN_DT_F64 ? 2 : 4;
+        const int V = a->D % VW == 0 && conv_fits(a->x, VW) && conv_fits(a->y, VW) && conv_fits(a->state_in, VW) ? VW : 1;
+        if (a->dtype == CRNN_DT_F64) conv_step_launch_w<CRNN_DT_F64>(p, V, st);
+        else if (a->dtype == CRNN_DT_F32) conv_step_launch_w<CRNN_DT_F32>(p, V, st);
+        else if (a->dtype == CRNN_DT_BF16) conv_step_launch_w<CRNN_DT_BF16>(p, V, st);
+        else conv_step_launch_w<CRNN_DT_F16>(p, V, st);
         SEQ_DONE("crnn_conv_step");
     } catch (...) { return -1; }
 }
@@ -482,13 +512,16 @@ int32_t crnn_scan_step(const crnn_scan_args *a) {
         for (p.lpc = 1; p.lpc * 4 < a->N;) p.lpc *= 2;
         const uintptr_t align = s.f64 ? 32 : 16;
         p.vec = a->N == 4 * p.lpc && (uintptr_t)a->A % align == 0 && (uintptr_t)a->state_out % align == 0;
+        // four channels a thread where that still gives every SIMD a wavefront
         const int cpb = 256 / p.lpc;
-        const int64_t grid = (int64_t)a->n_seq * ((a->D + cpb - 1) / cpb);
+        const int cpt = !s.f64 && (int64_t)a->n_seq * ((a->D + 4 * cpb - 1) / (4 * cpb)) >= 1024 ? 4 : 1;
+        const int64_t grid = (int64_t)a->n_seq * ((a->D + cpt * cpb - 1) / (cpt * cpb));
         if (grid > kSeqMaxGrid) return sfail("crnn_scan_step: too many rows and channels for one launch");
         SEQ_DEVICE(a->device, "crnn_scan_step");
         const hipStream_t st = (hipStream_t)a->stream;
-        if (s.f64) hipLaunchKernelGGL((crnn::seq_scan_step_kernel<double>), dim3((unsigned)grid), dim3(256), 0, st, p);
-        else hipLaunchKernelGGL((crnn::seq_scan_step_kernel<float>), dim3((unsigned)grid), dim3(256), 0, st, p);
+        if (s.f64) hipLaunchKernelGGL((crnn::seq_scan_step_kernel<double, 1>), dim3((unsigned)grid), dim3(256), 0, st, p);
+        else if (cpt == 4) hipLaunchKernelGGL((crnn::seq_scan_step_kernel<float, 4>), dim3((unsigned)grid), dim3(256), 0, st, p);
+        else hipLaunchKernelGGL((crnn::seq_scan_step_kernel<float, 1>), dim3((unsigned)grid), dim3(256), 0, st, p);
         SEQ_DONE("crnn_scan_step");
     } catch (...) { return -1; }
 }

@@ -3,14 +3,16 @@
 //     p[t, d] = bias[d] + sum_j w[d, j] x[t - W + 1 + j, d],   y = p or p sigmoid(p)
 //
 // x before a sequence's first row is its state (the last W - 1 rows before it), or 0.  Depthwise: a few multiply-adds per element read,
-// bound by memory.  A thread owns kConvV neighbouring channels and walks down a strip of rows with the last W rows in registers, so that
-// each row is read once but for the W - 1 rows in front of a strip.
+// bound by memory.  A thread owns V neighbouring channels (16 bytes of them where rows are aligned, else one) and walks down a strip of rows,
+// kConvTB at a time: the next ones are on their way while these are worked on, the last W rows stay in registers, so that each row is read
+// once but for the W - 1 rows in front of a strip.  Rows behind the last one are read as the last, threads behind the last channels do the
+// last channels once more: loads and stores stand without branches between them, and no wait reaches over a store.
 #pragma once
 #include "seq_common.hpp"
 
 namespace crnn {
 
-constexpr int kConvV = 4;        // channels of a thread
+constexpr int kConvTB = 4;       // rows on their way together
 constexpr int kConvMaxW = 8;
 
 struct ConvP {
@@ -25,273 +27,330 @@ struct ConvP {
 template <int DT> struct SeqT { using C = float; };
 template <> struct SeqT<CRNN_DT_F64> { using C = double; };
 
-template <int DT>
-__device__ __forceinline__ void conv_load(const SeqV &v, int64_t off, int64_t soff, int d, int D, typename SeqT<DT>::C (&o)[kConvV]) {
-    using CT = typename SeqT<DT>::C;
-    if (DT == CRNN_DT_PACKED8) {
-        const int8_t *q = (const int8_t *)v.p + off;
-        if (v.vec && d + kConvV <= D) {
-            const uint32_t b = *(const uint32_t *)q;       // four codes; kConvV divides 32: one scale
-            const CT e = (CT)seq_scale(v.sc[soff + (d >> 5)]);
+// V channels of a row as they stand in memory
+template <int DT, int V>
+struct ConvRaw {
+    using C = typename SeqT<DT>::C;
+    static constexpr int ES = DT == CRNN_DT_F64 ? 8 : DT == CRNN_DT_F32 ? 4 : DT == CRNN_DT_PACKED8 ? 1 : 2;
+    static constexpr int NW = V * ES >= 4 ? V * ES / 4 : 1;
+    uint32_t w[NW];
+    uint32_t e;              // checkpoint: the scale byte (V divides 32)
+    // row: the row's first channel (uniform), sc: its first scale
+    __device__ __forceinline__ void load(const void *row, const uint8_t *sc, uint32_t d) {
+        const char *q = (const char *)row + d * ES;
+        if (V * ES == 16) {
+            typedef uint32_t U4 __attribute__((ext_vector_type(4)));
+            const U4 b = *(const U4 *)q;
 #pragma unroll
-            for (int i = 0; i < kConvV; ++i) o[i] = (CT)(int32_t)(int8_t)(b >> (8 * i)) * e;
-        } else {
+            for (int i = 0; i < NW; ++i) w[i] = b[i & 3];
+        } else if (V * ES == 8) {
+            typedef uint32_t U2 __attribute__((ext_vector_type(2)));
+            const U2 b = *(const U2 *)q;
 #pragma unroll
-            for (int i = 0; i < kConvV; ++i) o[i] = d + i < D ? (CT)(int32_t)q[i] * (CT)seq_scale(v.sc[soff + ((d + i) >> 5)]) : CT(0);
-        }
-    } else if (DT == CRNN_DT_F32 || DT == CRNN_DT_F64) {
-        const CT *q = (const CT *)v.p + off;
-        constexpr int L = 16 / (int)sizeof(CT);
-        typedef CT V __attribute__((ext_vector_type(L)));
-        if (v.vec && d + kConvV <= D) {
-#pragma unroll
-            for (int k = 0; k < kConvV / L; ++k) {
-                const V b = *(const V *)(q + k * L);
-#pragma unroll
-                for (int i = 0; i < L; ++i) o[k * L + i] = b[i];
-            }
-        } else {
-#pragma unroll
-            for (int i = 0; i < kConvV; ++i) o[i] = d + i < D ? q[i] : CT(0);
-        }
-    } else {
-        const uint16_t *q = (const uint16_t *)v.p + off;
-        uint32_t b[kConvV];
-        if (v.vec && d + kConvV <= D) {
-            const uint64_t w = *(const uint64_t *)q;
-#pragma unroll
-            for (int i = 0; i < kConvV; ++i) b[i] = (uint32_t)(w >> (16 * i)) & 0xffffu;
-        } else {
-#pragma unroll
-            for (int i = 0; i < kConvV; ++i) b[i] = d + i < D ? q[i] : 0u;
-        }
-#pragma unroll
-        for (int i = 0; i < kConvV; ++i) o[i] = (CT)(DT == CRNN_DT_BF16 ? seq_as_float(b[i] << 16) : seq_from_f16(b[i]));
+            for (int i = 0; i < NW; ++i) w[i] = b[i & 1];
+        } else if (V * ES == 4) w[0] = *(const uint32_t *)q;
+        else if (V * ES == 2) w[0] = *(const uint16_t *)q;
+        else w[0] = *(const uint8_t *)q;
+        if (DT == CRNN_DT_PACKED8) e = sc[d >> 5];
     }
-}
-template <int DT>
-__device__ __forceinline__ void conv_store(const SeqV &v, int64_t off, int d, int D, const typename SeqT<DT>::C (&o)[kConvV]) {
-    using CT = typename SeqT<DT>::C;
-    if (DT == CRNN_DT_F32 || DT == CRNN_DT_F64) {
-        CT *q = (CT *)v.p + off;
-        constexpr int L = 16 / (int)sizeof(CT);
-        typedef CT V __attribute__((ext_vector_type(L)));
-        if (v.vec && d + kConvV <= D) {
-#pragma unroll
-            for (int k = 0; k < kConvV / L; ++k) {
-                V b;
-#pragma unroll
-                for (int i = 0; i < L; ++i) b[i] = o[k * L + i];
-                *(V *)(q + k * L) = b;
-            }
-        } else {
-#pragma unroll
-            for (int i = 0; i < kConvV; ++i)
-                if (d + i < D) q[i] = o[i];
+    __device__ __forceinline__ C get(int i) const {
+        if (DT == CRNN_DT_F64) {
+            const uint64_t b = (uint64_t)w[(2 * i) % NW] | (uint64_t)w[(2 * i + 1) % NW] << 32;
+            return (C)__builtin_bit_cast(double, b);
         }
-    } else {
-        uint16_t *q = (uint16_t *)v.p + off;
-        uint16_t b[kConvV];
-#pragma unroll
-        for (int i = 0; i < kConvV; ++i) b[i] = DT == CRNN_DT_BF16 ? seq_to_bf16((float)o[i]) : seq_to_f16((float)o[i]);
-        if (v.vec && d + kConvV <= D) {
-            *(uint64_t *)q = (uint64_t)b[0] | (uint64_t)b[1] << 16 | (uint64_t)b[2] << 32 | (uint64_t)b[3] << 48;
-        } else {
-#pragma unroll
-            for (int i = 0; i < kConvV; ++i)
-                if (d + i < D) q[i] = b[i];
-        }
+        if (DT == CRNN_DT_F32) return (C)seq_as_float(w[i % NW]);
+        if (DT == CRNN_DT_BF16) return (C)seq_as_float(i & 1 ? w[(i / 2) % NW] & 0xffff0000u : w[(i / 2) % NW] << 16);
+        if (DT == CRNN_DT_F16) return (C)seq_from_f16(w[(i / 2) % NW] >> (16 * (i & 1)) & 0xffffu);
+        return (C)(int32_t)(int8_t)(w[(i / 4) % NW] >> (8 * (i & 3))) * (C)seq_scale(e);
     }
+};
+template <int DT, int V>
+__device__ __forceinline__ void conv_put(void *row, uint32_t d, const typename SeqT<DT>::C (&x)[V]) {
+    using R = ConvRaw<DT, V>;
+    R r;
+#pragma unroll
+    for (int i = 0; i < R::NW; ++i) r.w[i] = 0;
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+        if (DT == CRNN_DT_F64) {
+            const uint64_t b = __builtin_bit_cast(uint64_t, (double)x[i]);
+            r.w[(2 * i) % R::NW] = (uint32_t)b;
+            r.w[(2 * i + 1) % R::NW] = (uint32_t)(b >> 32);
+        } else if (DT == CRNN_DT_F32) r.w[i % R::NW] = seq_as_bits((float)x[i]);
+        else r.w[(i / 2) % R::NW] |= (uint32_t)(DT == CRNN_DT_BF16 ? seq_to_bf16((float)x[i]) : seq_to_f16((float)x[i])) << (16 * (i & 1));
+    }
+    char *q = (char *)row + d * R::ES;
+    if (V * R::ES == 16) {
+        typedef uint32_t U4 __attribute__((ext_vector_type(4)));
+        U4 b;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) b[i] = r.w[i % R::NW];
+        *(U4 *)q = b;
+    } else if (V * R::ES == 8) {
+        typedef uint32_t U2 __attribute__((ext_vector_type(2)));
+        U2 b;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) b[i] = r.w[i % R::NW];
+        *(U2 *)q = b;
+    } else if (V * R::ES == 4) *(uint32_t *)q = r.w[0];
+    else *(uint16_t *)q = (uint16_t)r.w[0];
 }
 
 // weights of a thread's channels, right-aligned in WM taps (tap WM - 1 is the row itself)
-template <class CT, int WM>
-__device__ __forceinline__ void conv_weights(const ConvP &p, int d, CT (&w)[WM][kConvV], CT (&bias)[kConvV]) {
+template <class CT, int WM, int V>
+__device__ __forceinline__ void conv_weights(const void *pw, const void *pb, int W, int d, CT (&w)[WM][V], CT (&bias)[V]) {
 #pragma unroll
-    for (int i = 0; i < kConvV; ++i) {
-        const int di = d + i < p.D ? d + i : p.D - 1;
-        bias[i] = p.bias ? ((const CT *)p.bias)[di] : CT(0);
+    for (int i = 0; i < V; ++i) {
+        bias[i] = pb ? ((const CT *)pb)[d + i] : CT(0);
 #pragma unroll
         for (int j = 0; j < WM; ++j) {
-            const int k = j - (WM - p.W);
-            w[j][i] = k >= 0 ? ((const CT *)p.w)[(int64_t)di * p.W + k] : CT(0);
+            const int k = j - (WM - W);
+            w[j][i] = k >= 0 ? ((const CT *)pw)[(int64_t)(d + i) * W + k] : CT(0);
         }
     }
 }
 
-// x of row t (negative: the state's)
-template <int XT, int YT>
-__device__ __forceinline__ void conv_x(const ConvP &p, const SeqChunk &k, int64_t t, int d, typename SeqT<YT>::C (&o)[kConvV]) {
+template <int DT>
+__device__ __forceinline__ char *conv_row(const SeqMap &m, const SeqV &v, const SeqChunk &k, int64_t t) {
+    return (char *)v.p + seq_off(m, v, k, t) * ConvRaw<DT, 1>::ES;
+}
+template <int DT>
+__device__ __forceinline__ const uint8_t *conv_scales(const SeqMap &m, const SeqV &v, const SeqChunk &k, int64_t t) {
+    return DT == CRNN_DT_PACKED8 ? v.sc + seq_soff(m, v, k, t) : nullptr;
+}
+// x of any row of a sequence (negative: the state's, or 0)
+template <int XT, int YT, int V>
+__device__ __forceinline__ void conv_x(const ConvP &p, const SeqChunk &k, int64_t t, int d, typename SeqT<YT>::C (&o)[V]) {
     using CT = typename SeqT<YT>::C;
     if (t >= 0) {
-        typename SeqT<XT>::C v[kConvV];
-        conv_load<XT>(p.x, seq_off(p.m, p.x, k, t) + d, seq_soff(p.m, p.x, k, t), d, p.D, v);
+        ConvRaw<XT, V> r;
+        r.load(conv_row<XT>(p.m, p.x, k, t), conv_scales<XT>(p.m, p.x, k, t), d);
 #pragma unroll
-        for (int i = 0; i < kConvV; ++i) o[i] = (CT)v[i];
+        for (int i = 0; i < V; ++i) o[i] = (CT)r.get(i);
     } else if (p.st_in.p && t >= -(p.W - 1)) {
-        conv_load<YT>(p.st_in, (int64_t)k.s * p.st_in.bs + (t + p.W - 1) * p.st_in.rs + d, 0, d, p.D, o);
+        ConvRaw<YT, V> r;
+        r.load((const char *)p.st_in.p + ((int64_t)k.s * p.st_in.bs + (t + p.W - 1) * p.st_in.rs) * ConvRaw<YT, 1>::ES, nullptr, d);
+#pragma unroll
+        for (int i = 0; i < V; ++i) o[i] = (CT)r.get(i);
     } else {
 #pragma unroll
-        for (int i = 0; i < kConvV; ++i) o[i] = CT(0);
+        for (int i = 0; i < V; ++i) o[i] = CT(0);
     }
 }
 
-// the place of a thread: blockIdx.x = group of channels + groups x group of blocks; threads (64, 4): 64 threads along the channels, 4 strips
+// the place of a thread: 64 threads along the channels, a strip for each of the block's four wavefronts
 struct ConvAt { SeqChunk k; int64_t b; int d; bool on; };
+template <int V>
 __device__ __forceinline__ ConvAt conv_at(const ConvP &p) {
     ConvAt a;
-    const int64_t gx = (p.D + 64 * kConvV - 1) / (64 * kConvV);
+    const int64_t gx = (p.D + 64 * V - 1) / (64 * V);
     const int64_t by = (int64_t)blockIdx.x / gx;
     const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
     a.b = by * 4 + wave;
-    a.d = (int)((int64_t)blockIdx.x - by * gx) * 64 * kConvV + (int)(threadIdx.x & 63) * kConvV;
+    const int d = (int)((int64_t)blockIdx.x - by * gx) * 64 * V + (int)(threadIdx.x & 63) * V;
+    a.d = d + V <= p.D ? d : p.D - V;
     a.on = a.b < p.m.nblk;
     a.k = seq_locate(p.m, a.on ? a.b : p.m.nblk - 1);
     return a;
 }
 
-// the rows of the state behind a sequence: local rows len - (W - 1) .. len - 1 of (state, x)
-template <int XT, int YT>
-__device__ __forceinline__ void conv_state_out(const ConvP &p, const SeqChunk &k, int d) {
-    for (int j = 0; j < p.W - 1; ++j) {
-        typename SeqT<YT>::C v[kConvV];
-        conv_x<XT, YT>(p, k, k.len - (p.W - 1) + j, d, v);
-        conv_store<YT>(p.st_out, (int64_t)k.s * p.st_out.bs + j * p.st_out.rs + d, d, p.D, v);
-    }
-}
-
-template <int XT, int YT, int WM>
+template <int XT, int YT, int WM, int V>
 __global__ __launch_bounds__(256) void seq_conv_fwd_kernel(const ConvP p) {
     using CT = typename SeqT<YT>::C;
-    const ConvAt a = conv_at(p);
-    if (!a.on || a.d >= p.D) return;
+    constexpr int TB = kConvTB;
+    const ConvAt a = conv_at<V>(p);
+    if (!a.on) return;
     if (p.zero_outside)
-        for (int i = 0; i < kConvV; ++i) seq_zero_outside(p.m, p.y, a.b, a.d + i, a.d + i < p.D);
+        for (int i = 0; i < V; ++i) seq_zero_outside(p.m, p.y, a.b, a.d + i, true);
     if (!a.k.live) return;
-    CT w[WM][kConvV], bias[kConvV], x[WM][kConvV];
-    conv_weights<CT, WM>(p, a.d, w, bias);
+    if (a.k.n > 0) {
+        CT w[WM][V], bias[V], x[WM - 1 + TB][V];
+        conv_weights<CT, WM, V>(p.w, p.bias, p.W, a.d, w, bias);
 #pragma unroll
-    for (int j = 0; j < WM - 1; ++j) conv_x<XT, YT>(p, a.k, a.k.t0 - (WM - 1) + j, a.d, x[j]);
-#pragma unroll 4
-    for (int t = 0; t < a.k.n; ++t) {
-        conv_x<XT, YT>(p, a.k, a.k.t0 + t, a.d, x[WM - 1]);
-        CT y[kConvV];
+        for (int j = 0; j < WM - 1; ++j) conv_x<XT, YT, V>(p, a.k, a.k.t0 - (WM - 1) + j, a.d, x[j]);
+        const char *xrow = conv_row<XT>(p.m, p.x, a.k, a.k.t0);
+        const uint8_t *srow = conv_scales<XT>(p.m, p.x, a.k, a.k.t0);
+        char *yrow = conv_row<YT>(p.m, p.y, a.k, a.k.t0);
+        const int64_t xs = (int64_t)p.x.rs * ConvRaw<XT, V>::ES, ss = p.x.srs, ys = (int64_t)p.y.rs * ConvRaw<YT, V>::ES;
+        ConvRaw<XT, V> raw[TB];
 #pragma unroll
-        for (int i = 0; i < kConvV; ++i) {
-            CT s = bias[i];
-#pragma unroll
-            for (int j = 0; j < WM; ++j) s = seq_fma(w[j][i], x[j][i], s);
-            y[i] = p.silu ? s * seq_sigmoid(s) : s;
-#pragma unroll
-            for (int j = 0; j < WM - 1; ++j) x[j][i] = x[j + 1][i];
+        for (int i = 0; i < TB; ++i) {
+            const int64_t r = i < a.k.n ? i : a.k.n - 1;
+            raw[i].load(xrow + r * xs, srow + r * ss, a.d);
         }
-        conv_store<YT>(p.y, seq_off(p.m, p.y, a.k, a.k.t0 + t) + a.d, a.d, p.D, y);
+#pragma unroll 1
+        for (int t = 0; t < a.k.n; t += TB) {
+#pragma unroll
+            for (int i = 0; i < TB; ++i)
+#pragma unroll
+                for (int c = 0; c < V; ++c) x[WM - 1 + i][c] = (CT)raw[i].get(c);
+#pragma unroll
+            for (int i = 0; i < TB; ++i) {
+                const int64_t r = t + TB + i < a.k.n ? t + TB + i : a.k.n - 1;
+                raw[i].load(xrow + r * xs, srow + r * ss, a.d);
+            }
+            CT y[TB][V];
+#pragma unroll
+            for (int i = 0; i < TB; ++i)
+#pragma unroll
+                for (int c = 0; c < V; ++c) {
+                    CT s = bias[c];
+#pragma unroll
+                    for (int j = 0; j < WM; ++j) s = seq_fma(w[j][c], x[i + j][c], s);
+                    const CT g = s * seq_sigmoid(s);
+                    y[i][c] = p.silu ? g : s;
+                    if (i > 0) y[i][c] = t + i < a.k.n ? y[i][c] : y[i > 0 ? i - 1 : 0][c];
+                }
+#pragma unroll
+            for (int i = 0; i < TB; ++i) conv_put<YT, V>(yrow + (int64_t)(t + i < a.k.n ? t + i : a.k.n - 1) * ys, a.d, y[i]);
+#pragma unroll
+            for (int j = 0; j < WM - 1; ++j)
+#pragma unroll
+                for (int c = 0; c < V; ++c) x[j][c] = x[j + TB][c];
+        }
     }
-    if (a.k.last && p.st_out.p) conv_state_out<XT, YT>(p, a.k, a.d);
+    if (a.k.last && p.st_out.p)        // rows len - (W - 1) .. len - 1 of (state, x)
+        for (int j = 0; j < p.W - 1; ++j) {
+            CT v[V];
+            conv_x<XT, YT, V>(p, a.k, a.k.len - (p.W - 1) + j, a.d, v);
+            conv_put<YT, V>((char *)p.st_out.p + ((int64_t)a.k.s * p.st_out.bs + j * (int64_t)p.st_out.rs) * ConvRaw<YT, V>::ES, a.d, v);
+        }
 }
 
 // Gradient.  dp = dy act'(p) needs p once more; dx[t] = sum_j w[j] dp[t + W - 1 - j] needs the W - 1 rows behind t: the strip is walked W - 1
 // rows past its end.  A sequence's first strip starts W - 1 rows early: those are the state's.  dw, db: a strip's part, summed in order.
-template <int XT, int YT, int WM>
+template <int XT, int YT, int WM, int V>
 __global__ __launch_bounds__(256) void seq_conv_bwd_kernel(const ConvP p) {
     using CT = typename SeqT<YT>::C;
-    const ConvAt a = conv_at(p);
-    if (!a.on || a.d >= p.D) return;
+    constexpr int TB = kConvTB;
+    const ConvAt a = conv_at<V>(p);
+    if (!a.on) return;
     if (p.zero_outside)
-        for (int i = 0; i < kConvV; ++i) seq_zero_outside(p.m, p.dx, a.b, a.d + i, a.d + i < p.D);
-    CT dw[WM][kConvV], db[kConvV];
+        for (int i = 0; i < V; ++i) seq_zero_outside(p.m, p.dx, a.b, a.d + i, true);
+    CT dw[WM][V], db[V];
 #pragma unroll
-    for (int i = 0; i < kConvV; ++i) {
-        db[i] = CT(0);
+    for (int c = 0; c < V; ++c) {
+        db[c] = CT(0);
 #pragma unroll
-        for (int j = 0; j < WM; ++j) dw[j][i] = CT(0);
+        for (int j = 0; j < WM; ++j) dw[j][c] = CT(0);
     }
     if (a.k.live) {
-        CT w[WM][kConvV], bias[kConvV], x[WM][kConvV], dp[WM][kConvV];     // x[WM - 1]: row t; dp[j]: row t - j
-        conv_weights<CT, WM>(p, a.d, w, bias);
+        // x[WM - 1 + i], dp[WM - 1 + i]: the batch's row i
+        CT w[WM][V], bias[V], x[WM - 1 + TB][V], dp[WM - 1 + TB][V];
+        conv_weights<CT, WM, V>(p.w, p.bias, p.W, a.d, w, bias);
 #pragma unroll
-        for (int j = 0; j < WM; ++j)
+        for (int j = 0; j < WM - 1; ++j) {
+            conv_x<XT, YT, V>(p, a.k, a.k.t0 - (WM - 1) + j, a.d, x[j]);
 #pragma unroll
-            for (int i = 0; i < kConvV; ++i) dp[j][i] = CT(0);
-#pragma unroll
-        for (int j = 0; j < WM - 1; ++j) conv_x<XT, YT>(p, a.k, a.k.t0 - (WM - 1) + j, a.d, x[j]);
-        const int64_t end = a.k.t0 + a.k.n;
+            for (int c = 0; c < V; ++c) dp[j][c] = CT(0);
+        }
         const int back = p.W - 1;
-        const int64_t from = a.k.t0 == 0 ? -(int64_t)back : a.k.t0;     // first row whose dx this strip writes
-        for (int64_t t = a.k.t0; t < end + back; ++t) {
-            const bool in = t < a.k.len;
-            if (in) {
-                CT y[kConvV];
-                conv_x<XT, YT>(p, a.k, t, a.d, x[WM - 1]);
-                conv_load<YT>(p.dy, seq_off(p.m, p.dy, a.k, t) + a.d, 0, a.d, p.D, y);
+        const int64_t lo = a.k.t0 == 0 ? -(int64_t)back : a.k.t0, hi = a.k.t0 + a.k.n;     // rows whose dx this strip writes
+        const int64_t lastrow = a.k.len - 1;
+        const char *xrow = conv_row<XT>(p.m, p.x, a.k, 0), *grow = conv_row<YT>(p.m, p.dy, a.k, 0);
+        const uint8_t *srow = conv_scales<XT>(p.m, p.x, a.k, 0);
+        char *orow = conv_row<YT>(p.m, p.dx, a.k, 0);
+        const int64_t xs = (int64_t)p.x.rs * ConvRaw<XT, V>::ES, ss = p.x.srs, gs = (int64_t)p.dy.rs * ConvRaw<YT, V>::ES, os = (int64_t)p.dx.rs * ConvRaw<YT, V>::ES;
+        ConvRaw<XT, V> rx[TB];
+        ConvRaw<YT, V> rg[TB];
+        auto fetch = [&](int64_t t) {
 #pragma unroll
-                for (int i = 0; i < kConvV; ++i) {
-                    CT s = bias[i];
+            for (int i = 0; i < TB; ++i) {
+                const int64_t r = t + i < lastrow ? t + i : lastrow;
+                rx[i].load(xrow + r * xs, srow + r * ss, a.d);
+                rg[i].load(grow + r * gs, nullptr, a.d);
+            }
+        };
+        if (a.k.n > 0) fetch(a.k.t0);
+#pragma unroll 1
+        for (int64_t t = a.k.t0; t < hi + WM - 1; t += TB) {
+            if (a.k.n > 0) {
 #pragma unroll
-                    for (int j = 0; j < WM; ++j) s = seq_fma(w[j][i], x[j][i], s);
-                    CT g = y[i];
-                    if (p.silu) {
+                for (int i = 0; i < TB; ++i)
+#pragma unroll
+                    for (int c = 0; c < V; ++c) {
+                        x[WM - 1 + i][c] = (CT)rx[i].get(c);
+                        dp[WM - 1 + i][c] = (CT)rg[i].get(c);
+                    }
+                fetch(t + TB);
+#pragma unroll
+                for (int i = 0; i < TB; ++i) {
+                    const bool in = t + i <= lastrow, mine = t + i < hi;
+#pragma unroll
+                    for (int c = 0; c < V; ++c) {
+                        CT s = bias[c];
+#pragma unroll
+                        for (int j = 0; j < WM; ++j) s = seq_fma(w[j][c], x[i + j][c], s);
                         const CT sg = seq_sigmoid(s);
-                        g *= sg * seq_fma(s, CT(1) - sg, CT(1));
-                    }
-                    dp[0][i] = g;
-                    if (t < end) {
-                        db[i] += g;
+                        CT g = dp[WM - 1 + i][c];
+                        const CT ga = g * (sg * seq_fma(s, CT(1) - sg, CT(1)));
+                        g = p.silu ? ga : g;
+                        g = in ? g : CT(0);
+                        dp[WM - 1 + i][c] = g;
+                        const CT gm = mine ? g : CT(0);
+                        db[c] += gm;
 #pragma unroll
-                        for (int j = 0; j < WM; ++j) dw[j][i] = seq_fma(g, x[j][i], dw[j][i]);
+                        for (int j = 0; j < WM; ++j) dw[j][c] = seq_fma(gm, x[i + j][c], dw[j][c]);
                     }
-#pragma unroll
-                    for (int j = 0; j < WM - 1; ++j) x[j][i] = x[j + 1][i];
                 }
             } else {
 #pragma unroll
-                for (int i = 0; i < kConvV; ++i) dp[0][i] = CT(0);
+                for (int i = 0; i < TB; ++i)
+#pragma unroll
+                    for (int c = 0; c < V; ++c) dp[WM - 1 + i][c] = CT(0);
             }
-            const int64_t row = t - back;                  // all its uses are in dp[0 .. back]
-            if (row >= from) {
-                CT g[kConvV];
+            // row t - (WM - 1) + i has all its uses now: tap WM - 1 - j met it in output row t - (WM - 1) + i + j
+            CT o[TB][V];
 #pragma unroll
-                for (int i = 0; i < kConvV; ++i) {
-                    g[i] = CT(0);
+            for (int i = 0; i < TB; ++i)
 #pragma unroll
-                    for (int j = 0; j < WM; ++j)           // tap j met row `row` in the output row t - (j - (WM - W)): dp[j - (WM - W)]
-                        if (j >= WM - p.W) {
-                            CT v = CT(0);
+                for (int c = 0; c < V; ++c) {
+                    CT s = CT(0);
 #pragma unroll
-                            for (int k = 0; k < WM; ++k)
-                                if (k == j - (WM - p.W)) v = dp[k][i];
-                            g[i] = seq_fma(w[j][i], v, g[i]);
-                        }
+                    for (int j = 0; j < WM; ++j) s = seq_fma(w[WM - 1 - j][c], dp[i + j][c], s);
+                    o[i][c] = s;
                 }
-                if (p.dst_out.p && row >= a.k.len - back) {
-                    CT s[kConvV];
-                    conv_load<YT>(p.dst_out, (int64_t)a.k.s * p.dst_out.bs + (row - (a.k.len - back)) * p.dst_out.rs + a.d, 0, a.d, p.D, s);
+            const int64_t r0 = t - (WM - 1);
+            if (r0 >= (lo > 0 ? lo : 0) && r0 + TB <= hi && !(p.dst_out.p && r0 + TB > a.k.len - back)) {
 #pragma unroll
-                    for (int i = 0; i < kConvV; ++i) g[i] += s[i];
+                for (int i = 0; i < TB; ++i) conv_put<YT, V>(orow + (r0 + i) * os, a.d, o[i]);
+            } else {
+#pragma unroll
+                for (int i = 0; i < TB; ++i) {
+                    const int64_t r = r0 + i;
+                    if (r < lo || r >= hi) continue;
+                    if (p.dst_out.p && r >= a.k.len - back) {
+                        ConvRaw<YT, V> d;
+                        d.load((const char *)p.dst_out.p + ((int64_t)a.k.s * p.dst_out.bs + (r - (a.k.len - back)) * p.dst_out.rs) * ConvRaw<YT, V>::ES, nullptr, a.d);
+#pragma unroll
+                        for (int c = 0; c < V; ++c) o[i][c] += (CT)d.get(c);
+                    }
+                    if (r >= 0) conv_put<YT, V>(orow + r * os, a.d, o[i]);
+                    else if (p.dst_in.p) conv_put<YT, V>((char *)p.dst_in.p + ((int64_t)a.k.s * p.dst_in.bs + (r + back) * p.dst_in.rs) * ConvRaw<YT, V>::ES, a.d, o[i]);
                 }
-                if (row >= 0) conv_store<YT>(p.dx, seq_off(p.m, p.dx, a.k, row) + a.d, a.d, p.D, g);
-                else if (p.dst_in.p) conv_store<YT>(p.dst_in, (int64_t)a.k.s * p.dst_in.bs + (row + back) * p.dst_in.rs + a.d, a.d, p.D, g);
             }
 #pragma unroll
-            for (int j = WM - 1; j >= 1; --j)
+            for (int j = 0; j < WM - 1; ++j)
 #pragma unroll
-                for (int i = 0; i < kConvV; ++i) dp[j][i] = dp[j - 1][i];
+                for (int c = 0; c < V; ++c) {
+                    x[j][c] = x[j + TB][c];
+                    dp[j][c] = dp[j + TB][c];
+                }
         }
     }
-    CT *part = (CT *)p.part + a.b * (p.W + 1) * p.D;
+    CT *part = (CT *)p.part + a.b * (p.W + 1) * p.D + a.d;
 #pragma unroll
-    for (int i = 0; i < kConvV; ++i) {
-        if (a.d + i >= p.D) continue;
+    for (int c = 0; c < V; ++c) {
 #pragma unroll
         for (int j = 0; j < WM; ++j) {
             const int k = j - (WM - p.W);
-            if (k >= 0) part[(int64_t)k * p.D + a.d + i] = dw[j][i];
+            if (k >= 0) part[(int64_t)k * p.D + c] = dw[j][c];
         }
-        part[(int64_t)p.W * p.D + a.d + i] = db[i];
+        part[(int64_t)p.W * p.D + c] = db[c];
     }
 }
 
-// one row for each of many running sequences; the states (the last W - 1 rows) move up in place.  Rows that name one slot: seq_scan_step_kernel.
+// one row for each of many running sequences; the states (the last W - 1 rows) move up in place.  Rows that name one slot: seq_same_slot.
 struct ConvStepP {
     SeqV x, y, st;                   // st.bs: between slots
     const void *w, *bias;
@@ -299,14 +358,16 @@ struct ConvStepP {
     int64_t rows, n_slots;
     int32_t D, W, silu;
 };
-template <int YT, int WM>
+template <int YT, int WM, int V>
 __global__ __launch_bounds__(256) void seq_conv_step_kernel(const ConvStepP p) {
     using CT = typename SeqT<YT>::C;
+    constexpr int ES = ConvRaw<YT, V>::ES;
     __shared__ int before, next;
-    const int64_t gx = (p.D + 256 * kConvV - 1) / (256 * kConvV);
+    const int64_t gx = (p.D + 256 * V - 1) / (256 * V);
     int64_t r = (int64_t)blockIdx.x / gx;
-    const int d = (int)((int64_t)blockIdx.x - r * gx) * 256 * kConvV + (int)threadIdx.x * kConvV;
-    const bool on = d < p.D;
+    const int d0 = (int)((int64_t)blockIdx.x - r * gx) * 256 * V + (int)threadIdx.x * V;
+    const bool on = d0 < p.D;        // (D is a multiple of V)
+    const int d = on ? d0 : 0;
     const int64_t slot = p.slot ? p.slot[r] : r;
     const bool there = slot >= 0 && slot < p.n_slots;
     int64_t nx = -1;
@@ -318,38 +379,45 @@ __global__ __launch_bounds__(256) void seq_conv_step_kernel(const ConvStepP p) {
         if (before) return;
         nx = next == 0x7fffffff ? -1 : next;
     }
-    CT w[WM][kConvV], bias[kConvV], x[WM][kConvV];
+    CT w[WM][V], bias[V], x[WM][V];
+    char *yp = (char *)p.y.p;
     if (!there) {
 #pragma unroll
-        for (int i = 0; i < kConvV; ++i) bias[i] = CT(0);
-        if (on) conv_store<YT>(p.y, r * (int64_t)p.y.rs + d, d, p.D, bias);
+        for (int c = 0; c < V; ++c) bias[c] = CT(0);
+        if (on) conv_put<YT, V>(yp + r * (int64_t)p.y.rs * ES, d, bias);
         return;
     }
-    ConvP q;
-    q.D = p.D; q.W = p.W; q.w = p.w; q.bias = p.bias;
-    conv_weights<CT, WM>(q, on ? d : 0, w, bias);
-    const int at = on ? d : 0;
+    char *st = (char *)p.st.p + slot * p.st.bs * ES;
 #pragma unroll
     for (int j = 0; j < WM - 1; ++j) {
         const int k = j - (WM - p.W);
-        if (k >= 0) conv_load<YT>(p.st, slot * p.st.bs + k * p.st.rs + at, 0, at, p.D, x[j]);
-        else
+        if (k >= 0) {
+            ConvRaw<YT, V> q;
+            q.load(st + k * (int64_t)p.st.rs * ES, nullptr, d);
 #pragma unroll
-            for (int i = 0; i < kConvV; ++i) x[j][i] = CT(0);
-    }
-    for (;;) {
-        CT y[kConvV];
-        conv_load<YT>(p.x, r * (int64_t)p.x.rs + at, 0, at, p.D, x[WM - 1]);
+            for (int c = 0; c < V; ++c) x[j][c] = q.get(c);
+        } else {
 #pragma unroll
-        for (int i = 0; i < kConvV; ++i) {
-            CT s = bias[i];
-#pragma unroll
-            for (int j = 0; j < WM; ++j) s = seq_fma(w[j][i], x[j][i], s);
-            y[i] = p.silu ? s * seq_sigmoid(s) : s;
-#pragma unroll
-            for (int j = 0; j < WM - 1; ++j) x[j][i] = x[j + 1][i];
+            for (int c = 0; c < V; ++c) x[j][c] = CT(0);
         }
-        if (on) conv_store<YT>(p.y, r * (int64_t)p.y.rs + d, d, p.D, y);
+    }
+    conv_weights<CT, WM, V>(p.w, p.bias, p.W, d, w, bias);
+    for (;;) {
+        CT y[V];
+        ConvRaw<YT, V> q;
+        q.load((const char *)p.x.p + r * (int64_t)p.x.rs * ES, nullptr, d);
+#pragma unroll
+        for (int c = 0; c < V; ++c) {
+            x[WM - 1][c] = q.get(c);
+            CT s = bias[c];
+#pragma unroll
+            for (int j = 0; j < WM; ++j) s = seq_fma(w[j][c], x[j][c], s);
+            const CT g = s * seq_sigmoid(s);
+            y[c] = p.silu ? g : s;
+#pragma unroll
+            for (int j = 0; j < WM - 1; ++j) x[j][c] = x[j + 1][c];
+        }
+        if (on) conv_put<YT, V>(yp + r * (int64_t)p.y.rs * ES, d, y);
         if (nx < 0) break;
         r = nx;
         __syncthreads();
@@ -363,7 +431,7 @@ __global__ __launch_bounds__(256) void seq_conv_step_kernel(const ConvStepP p) {
 #pragma unroll
     for (int j = 0; j < WM - 1; ++j) {
         const int k = j - (WM - p.W);
-        if (k >= 0) conv_store<YT>(p.st, slot * p.st.bs + k * p.st.rs + d, d, p.D, x[j]);
+        if (k >= 0) conv_put<YT, V>(st + k * (int64_t)p.st.rs * ES, d, x[j]);
     }
 }
 
