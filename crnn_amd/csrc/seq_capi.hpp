@@ -85,6 +85,7 @@ crnn::SeqMap seq_map(int32_t n_seq, int64_t rows, const int32_t *start, const in
     m.Q = Q > 0 ? Q : rows + 1;
     m.nch = rows > 0 ? (rows + m.Q - 1) / m.Q : 1;
     m.nblk = start ? rows / m.Q + n_seq : m.nch * n_seq;
+    m.per = m.nblk > 0 ? (rows + m.nblk - 1) / m.nblk : 0;
     return m;
 }
 int64_t seq_flat(int32_t n_seq, int64_t rows, bool packed) { return packed ? rows : rows * n_seq; }
@@ -123,7 +124,6 @@ struct ScanPlan {
 // even out the last round of blocks.  Measured (rows x tiles of 64 channels: us at 16 / 32 / 48 / 64 / 128 rows): 64 x 24: 41 / 44 / 54 / 69 / 69;
 // 512 x 64: 47 / 48 / 57 / 69 / 120; 2048 x 32: 79 / 68 / 79 / 76 / 125; 8190 x 64: 396 / 296 / 279 / 291 / 325.
 int64_t scan_forward_rows(int64_t flat, int32_t n_seq, int64_t ntile) {
-    if (const char *e = getenv("CRNN_DEV_Q")) return atoll(e);
     if ((int64_t)n_seq * ntile >= 2048) return 0;
     const int64_t rows = flat * ntile;
     int64_t q = rows <= 16384 ? 16 : rows <= 131072 ? 32 : 48;
@@ -273,18 +273,20 @@ bool scan_views(SeqCheck &c, const crnn_scan_args *a, bool backward) {
     } while (0)
 
 // ------------------------------------------------------------------ convolution
-// channels of a thread: 16 bytes of a row of the call's type (half of that with more than four taps, and in the gradient: registers), one where
-// an array of the call does not allow it
+// channels of a thread, one where an array of the call does not allow more.  Four of two bytes beat eight (12001 x 4096, W = 4: 46 against 54 us):
+// half the registers are twice the wavefronts.
 int conv_wide(int dtype, int W, bool backward) {
     if (dtype == CRNN_DT_F64) return 2;
     if (dtype == CRNN_DT_F32) return W > 4 && backward ? 2 : 4;
-    return W > 4 || backward ? 4 : 8;
+    return 4;
 }
 // Rows of a strip: strips and channels together give some wavefronts to each SIMD; a strip reads W - 1 rows twice, the gradient 2 (W - 1).
+// Measured (us at 8 / 16 / 24 / 32 / 64 / 128 rows): forward 12001 x 4096 bf16 75 / 50 / 46 / 46 / 47 / 45, 1024 x 2048 14 / 14 / 14 / 15 / 18 / 27;
+// gradient 8192 x 2048 75 / 57 / 45 / 48 / 56 / 63, 12000 x 4096 186 / 120 / 100 / 91 / 79 / 92, 1024 x 2048 25 / 25 / 25 / 25 / 34 / 54.
 int64_t conv_strip(int64_t flat, int32_t D, int V, bool backward) {
     const int64_t waves = (D + 64 * V - 1) / (64 * V);
-    const int64_t q = flat * waves / 4096 / 4 * 4;
-    const int64_t lo = backward ? 16 : 8, hi = backward ? 64 : 32;
+    const int64_t q = flat * waves / (backward ? 3072 : 4096) / 4 * 4;
+    const int64_t lo = backward ? 24 : 8, hi = backward ? 64 : 32;
     return q < lo ? lo : q > hi ? hi : q;
 }
 bool conv_fits(const crnn_view &v, int V) { return !v.ptr || (seq_view(v, V).vec && v.row_stride < 0x7fffffff); }
@@ -331,26 +333,30 @@ void conv_launch(const crnn::ConvP &p, bool backward, hipStream_t st) {
     if (backward) hipLaunchKernelGGL((crnn::seq_conv_bwd_kernel<XT, YT, WM, V>), grid, dim3(256), 0, st, p);
     else hipLaunchKernelGGL((crnn::seq_conv_fwd_kernel<XT, YT, WM, V>), grid, dim3(256), 0, st, p);
 }
-// VF, VB: the wide forms' channels for up to four taps, forward and backward (conv_wide)
-template <int XT, int YT, int VF, int VB>
+// VF, VB, VF8, VB8: the wide forms' channels forward and backward, up to four taps and more (conv_wide)
+template <int XT, int YT, int VF, int VB, int VF8, int VB8>
 void conv_launch_w(const crnn::ConvP &p, int V, bool backward, hipStream_t st) {
-    constexpr int V8 = YT == CRNN_DT_F64 ? 2 : 4, V8B = YT == CRNN_DT_F64 || YT == CRNN_DT_F32 ? 2 : 4;
     if (p.W <= 4) {
         if (V == 1) conv_launch<XT, YT, 4, 1>(p, backward, st);
-        else if (backward) { const int64_t gx = (p.D + 64 * VB - 1) / (64 * VB); hipLaunchKernelGGL((crnn::seq_conv_bwd_kernel<XT, YT, 4, VB>), dim3((unsigned)((p.m.nblk + 3) / 4 * gx)), dim3(256), 0, st, p); }
-        else { const int64_t gx = (p.D + 64 * VF - 1) / (64 * VF); hipLaunchKernelGGL((crnn::seq_conv_fwd_kernel<XT, YT, 4, VF>), dim3((unsigned)((p.m.nblk + 3) / 4 * gx)), dim3(256), 0, st, p); }
+        else if (backward) conv_launch<XT, YT, 4, VB>(p, true, st);
+        else conv_launch<XT, YT, 4, VF>(p, false, st);
     } else {
         if (V == 1) conv_launch<XT, YT, 8, 1>(p, backward, st);
-        else if (backward) { const int64_t gx = (p.D + 64 * V8B - 1) / (64 * V8B); hipLaunchKernelGGL((crnn::seq_conv_bwd_kernel<XT, YT, 8, V8B>), dim3((unsigned)((p.m.nblk + 3) / 4 * gx)), dim3(256), 0, st, p); }
-        else { const int64_t gx = (p.D + 64 * V8 - 1) / (64 * V8); hipLaunchKernelGGL((crnn::seq_conv_fwd_kernel<XT, YT, 8, V8>), dim3((unsigned)((p.m.nblk + 3) / 4 * gx)), dim3(256), 0, st, p); }
+        else if (backward) conv_launch<XT, YT, 8, VB8>(p, true, st);
+        else conv_launch<XT, YT, 8, VF8>(p, false, st);
     }
 }
+template <int YT>
+void conv_launch_x(const crnn::ConvP &p, int V, bool backward, hipStream_t st) {
+    constexpr int VB8 = YT == CRNN_DT_F32 ? 2 : 4;
+    if (p.x.dt == CRNN_DT_PACKED8) conv_launch_w<CRNN_DT_PACKED8, YT, 4, 4, 4, VB8>(p, V, backward, st);
+    else conv_launch_w<YT, YT, 4, 4, 4, VB8>(p, V, backward, st);
+}
 void conv_launch_t(const crnn::ConvP &p, int dtype, int V, bool backward, hipStream_t st) {
-    const bool q = p.x.dt == CRNN_DT_PACKED8;
-    if (dtype == CRNN_DT_F64) conv_launch_w<CRNN_DT_F64, CRNN_DT_F64, 2, 2>(p, V, backward, st);
-    else if (dtype == CRNN_DT_F32) { if (q) conv_launch_w<CRNN_DT_PACKED8, CRNN_DT_F32, 4, 4>(p, V, backward, st); else conv_launch_w<CRNN_DT_F32, CRNN_DT_F32, 4, 4>(p, V, backward, st); }
-    else if (dtype == CRNN_DT_BF16) { if (q) conv_launch_w<CRNN_DT_PACKED8, CRNN_DT_BF16, 8, 4>(p, V, backward, st); else conv_launch_w<CRNN_DT_BF16, CRNN_DT_BF16, 8, 4>(p, V, backward, st); }
-    else { if (q) conv_launch_w<CRNN_DT_PACKED8, CRNN_DT_F16, 8, 4>(p, V, backward, st); else conv_launch_w<CRNN_DT_F16, CRNN_DT_F16, 8, 4>(p, V, backward, st); }
+    if (dtype == CRNN_DT_F64) conv_launch_w<CRNN_DT_F64, CRNN_DT_F64, 2, 2, 2, 2>(p, V, backward, st);
+    else if (dtype == CRNN_DT_F32) conv_launch_x<CRNN_DT_F32>(p, V, backward, st);
+    else if (dtype == CRNN_DT_BF16) conv_launch_x<CRNN_DT_BF16>(p, V, backward, st);
+    else conv_launch_x<CRNN_DT_F16>(p, V, backward, st);
 }
 template <int YT, int WM, int V>
 void conv_step_launch(const crnn::ConvStepP &p, hipStream_t st) {
@@ -509,6 +515,8 @@ int32_t crnn_scan_step(const crnn_scan_args *a) {
         p.A = a->A; p.Dskip = a->skip; p.dt_bias = a->dt_bias; p.state = a->state_out; p.slot = a->slot;
         p.rows = a->n_seq; p.n_slots = a->n_slots;
         p.D = a->D; p.N = a->N; p.G = a->G; p.Dg = a->D / a->G; p.softplus = a->softplus;
+        p.gate = a->z.ptr != nullptr;
+        if (!p.gate) p.z = p.u;
         for (p.lpc = 1; p.lpc * 4 < a->N;) p.lpc *= 2;
         const uintptr_t align = s.f64 ? 32 : 16;
         p.vec = a->N == 4 * p.lpc && (uintptr_t)a->A % align == 0 && (uintptr_t)a->state_out % align == 0;
@@ -519,9 +527,14 @@ int32_t crnn_scan_step(const crnn_scan_args *a) {
         if (grid > kSeqMaxGrid) return sfail("crnn_scan_step: too many rows and channels for one launch");
         SEQ_DEVICE(a->device, "crnn_scan_step");
         const hipStream_t st = (hipStream_t)a->stream;
-        if (s.f64) hipLaunchKernelGGL((crnn::seq_scan_step_kernel<double, 1>), dim3((unsigned)grid), dim3(256), 0, st, p);
-        else if (cpt == 4) hipLaunchKernelGGL((crnn::seq_scan_step_kernel<float, 4>), dim3((unsigned)grid), dim3(256), 0, st, p);
-        else hipLaunchKernelGGL((crnn::seq_scan_step_kernel<float, 1>), dim3((unsigned)grid), dim3(256), 0, st, p);
+        if (s.f64) hipLaunchKernelGGL((crnn::seq_scan_step_kernel<8, 1>), dim3((unsigned)grid), dim3(256), 0, st, p);
+        else if (a->dtype == CRNN_DT_F32) {
+            if (cpt == 4) hipLaunchKernelGGL((crnn::seq_scan_step_kernel<4, 4>), dim3((unsigned)grid), dim3(256), 0, st, p);
+            else hipLaunchKernelGGL((crnn::seq_scan_step_kernel<4, 1>), dim3((unsigned)grid), dim3(256), 0, st, p);
+        } else {
+            if (cpt == 4) hipLaunchKernelGGL((crnn::seq_scan_step_kernel<2, 4>), dim3((unsigned)grid), dim3(256), 0, st, p);
+            else hipLaunchKernelGGL((crnn::seq_scan_step_kernel<2, 1>), dim3((unsigned)grid), dim3(256), 0, st, p);
+        }
         SEQ_DONE("crnn_scan_step");
     } catch (...) { return -1; }
 }

@@ -76,7 +76,8 @@ struct SeqMap {
     int64_t rows;           // packed: rows of the array; dense: rows of a sequence
     int64_t Q;              // rows of a chunk
     int64_t nch;            // dense: chunks of a sequence (at least 1)
-    int64_t nblk;           // chunk blocks in all (an upper bound where packed)
+    int64_t nblk;           // chunk blocks in all (an upper bound where packed), less than 2^31
+    int64_t per;            // rows of the array a block looks after that belong to no sequence (packed)
     int32_t n_seq;
 };
 
@@ -114,7 +115,7 @@ __device__ __forceinline__ SeqChunk seq_locate(const SeqMap &m, int64_t b) {
     SeqChunk k;
     int64_t s, c;
     if (!m.start) {
-        s = (int64_t)((uint64_t)b / (uint64_t)m.nch);
+        s = (int64_t)((uint32_t)b / (uint32_t)m.nch);
         c = b - s * m.nch;
         if (s >= m.n_seq) s = -1;
     } else {
@@ -174,8 +175,7 @@ __device__ __forceinline__ double seq_load1(const SeqV &v, int64_t off, double) 
 __device__ __forceinline__ void seq_zero_outside(const SeqMap &m, const SeqV &v, int64_t b, int64_t d, bool valid) {
     if (!v.p) return;
     if (m.start) {
-        const int64_t per = (m.rows + m.nblk - 1) / m.nblk;
-        const int64_t lo = b * per, hi = lo + per < m.rows ? lo + per : m.rows;
+        const int64_t lo = b * m.per, hi = lo + m.per < m.rows ? lo + m.per : m.rows;
         const int64_t first = m.n_seq > 0 ? seq_clamp(m.start[0], 0, m.rows) : m.rows, end = m.n_seq > 0 ? seq_clamp(m.start[m.n_seq], 0, m.rows) : m.rows;
         if (lo >= first && hi <= end) return;
         for (int64_t r = lo; r < hi; ++r)
@@ -184,7 +184,7 @@ __device__ __forceinline__ void seq_zero_outside(const SeqMap &m, const SeqV &v,
                 else seq_store(v, r * v.rs + d, 0.0f);
             }
     } else if (m.len) {
-        const int64_t s = b / m.nch, c = b - s * m.nch, n = seq_clamp(m.len[s], 0, m.rows);
+        const int64_t s = (uint32_t)b / (uint32_t)m.nch, c = b - s * m.nch, n = seq_clamp(m.len[s], 0, m.rows);
         const int64_t hi = (c + 1) * m.Q < m.rows ? (c + 1) * m.Q : m.rows;
         for (int64_t r = c * m.Q > n ? c * m.Q : n; r < hi; ++r)
             if (valid) {

@@ -143,11 +143,10 @@ struct ConvAt { SeqChunk k; int64_t b; int d; bool on; };
 template <int V>
 __device__ __forceinline__ ConvAt conv_at(const ConvP &p) {
     ConvAt a;
-    const int64_t gx = (p.D + 64 * V - 1) / (64 * V);
-    const int64_t by = (int64_t)blockIdx.x / gx;
+    const uint32_t gx = (uint32_t)(p.D + 64 * V - 1) / (64 * V), by = blockIdx.x / gx;
     const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
-    a.b = by * 4 + wave;
-    const int d = (int)((int64_t)blockIdx.x - by * gx) * 64 * V + (int)(threadIdx.x & 63) * V;
+    a.b = (int64_t)by * 4 + wave;
+    const int d = (int)(blockIdx.x - by * gx) * 64 * V + (int)(threadIdx.x & 63) * V;
     a.d = d + V <= p.D ? d : p.D - V;
     a.on = a.b < p.m.nblk;
     a.k = seq_locate(p.m, a.on ? a.b : p.m.nblk - 1);
@@ -189,6 +188,7 @@ __global__ __launch_bounds__(256) void seq_conv_fwd_kernel(const ConvP p) {
                 const int64_t r = t + TB + i < a.k.n ? t + TB + i : a.k.n - 1;
                 raw[i].load(xrow + r * xs, srow + r * ss, a.d);
             }
+            __builtin_amdgcn_sched_barrier(0);       // (the loads are issued here, not where the compiler would like them)
             CT y[TB][V];
 #pragma unroll
             for (int i = 0; i < TB; ++i)
@@ -197,10 +197,20 @@ __global__ __launch_bounds__(256) void seq_conv_fwd_kernel(const ConvP p) {
                     CT s = bias[c];
 #pragma unroll
                     for (int j = 0; j < WM; ++j) s = seq_fma(w[j][c], x[i + j][c], s);
-                    const CT g = s * seq_sigmoid(s);
-                    y[i][c] = p.silu ? g : s;
-                    if (i > 0) y[i][c] = t + i < a.k.n ? y[i][c] : y[i > 0 ? i - 1 : 0][c];
+                    y[i][c] = s;
                 }
+            if (p.silu) {
+#pragma unroll
+                for (int i = 0; i < TB; ++i)
+#pragma unroll
+                    for (int c = 0; c < V; ++c) y[i][c] *= seq_sigmoid(y[i][c]);
+            }
+            if (t + TB > a.k.n) {
+#pragma unroll
+                for (int i = 1; i < TB; ++i)
+#pragma unroll
+                    for (int c = 0; c < V; ++c) y[i][c] = t + i < a.k.n ? y[i][c] : y[i - 1][c];
+            }
 #pragma unroll
             for (int i = 0; i < TB; ++i) conv_put<YT, V>(yrow + (int64_t)(t + i < a.k.n ? t + i : a.k.n - 1) * ys, a.d, y[i]);
 #pragma unroll
@@ -273,6 +283,7 @@ __global__ __launch_bounds__(256) void seq_conv_bwd_kernel(const ConvP p) {
                         dp[WM - 1 + i][c] = (CT)rg[i].get(c);
                     }
                 fetch(t + TB);
+                __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
                 for (int i = 0; i < TB; ++i) {
                     const bool in = t + i <= lastrow, mine = t + i < hi;
@@ -363,9 +374,9 @@ __global__ __launch_bounds__(256) void seq_conv_step_kernel(const ConvStepP p) {
     using CT = typename SeqT<YT>::C;
     constexpr int ES = ConvRaw<YT, V>::ES;
     __shared__ int before, next;
-    const int64_t gx = (p.D + 256 * V - 1) / (256 * V);
-    int64_t r = (int64_t)blockIdx.x / gx;
-    const int d0 = (int)((int64_t)blockIdx.x - r * gx) * 256 * V + (int)threadIdx.x * V;
+    const uint32_t gx = (uint32_t)(p.D + 256 * V - 1) / (256 * V), r0 = blockIdx.x / gx;
+    int64_t r = r0;
+    const int d0 = (int)(blockIdx.x - r0 * gx) * 256 * V + (int)threadIdx.x * V;
     const bool on = d0 < p.D;        // (D is a multiple of V)
     const int d = on ? d0 : 0;
     const int64_t slot = p.slot ? p.slot[r] : r;

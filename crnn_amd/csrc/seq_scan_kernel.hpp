@@ -59,9 +59,9 @@ struct ScanAt {
 __device__ __forceinline__ ScanAt scan_at(const ScanP &p) {
     ScanAt a;
     const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)), lane = threadIdx.x & 63;
-    const int64_t tb = (p.ntile + kScanWaves - 1) / kScanWaves;
-    a.b = (int64_t)blockIdx.x / tb;
-    a.tile = (int32_t)((int64_t)blockIdx.x - a.b * tb) * kScanWaves + wave;
+    const uint32_t tb = (uint32_t)(p.ntile + kScanWaves - 1) / kScanWaves, b = blockIdx.x / tb;
+    a.b = b;
+    a.tile = (int32_t)(blockIdx.x - b * tb) * kScanWaves + wave;
     a.on = a.tile < p.ntile;
     const int t = a.on ? a.tile : p.ntile - 1;
     a.g = t / p.tpg;
@@ -606,55 +606,54 @@ struct ScanStepP {
     void *state;                        // [n_slots][D][N]
     const int32_t *slot;                // null: row r has slot r
     int64_t rows, n_slots;
-    int32_t D, N, G, Dg, softplus, lpc, vec;
+    int32_t D, N, G, Dg, softplus, gate, lpc, vec;
 };
-// CPT channels a thread, 256 / lpc apart: their states are all on their way before the first is used, and what belongs to the row is looked up
-// once for them (rows of 4096 channels, 16 states, 250 of them: one channel a thread 62 us, four 38 us).
-template <class CT, int CPT>
+// CPT channels a thread, 256 / lpc apart.  All that the row reads is on its way before the first of it is used or another row's slot is looked
+// at, and what belongs to the row is looked up once for the CPT channels.
+template <int IO>
+__device__ __forceinline__ typename SeqIO<IO>::C scan_value(typename SeqIO<IO>::E e, int dt) {
+    using CT = typename SeqIO<IO>::C;
+    if (IO == 8) return (CT)e;
+    if (IO == 4) return (CT)seq_as_float((uint32_t)e);
+    return (CT)(dt == CRNN_DT_BF16 ? seq_as_float((uint32_t)e << 16) : seq_from_f16((uint32_t)e));
+}
+template <int IO, int CPT>
+struct ScanStepRow {
+    using E = typename SeqIO<IO>::E;
+    E u[CPT], x[CPT], z[CPT], b[4], c[4];
+    __device__ __forceinline__ void maps(const ScanStepP &p, int64_t r, int g, int n0) {
+        const E *pb = (const E *)p.B.p + r * p.B.rs + g * p.Bg, *pc = (const E *)p.C.p + r * p.C.rs + g * p.Cg;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int n = n0 + i < p.N ? n0 + i : p.N - 1;
+            b[i] = pb[n * p.Bn];
+            c[i] = pc[n * p.Cn];
+        }
+    }
+    __device__ __forceinline__ void load(const ScanStepP &p, int64_t r, const int (&d)[CPT], int n0) {
+#pragma unroll
+        for (int k = 0; k < CPT; ++k) {
+            u[k] = ((const E *)p.u.p + r * p.u.rs)[(uint32_t)d[k]];
+            x[k] = ((const E *)p.dt.p + r * p.dt.rs)[(uint32_t)d[k]];
+            z[k] = ((const E *)p.z.p + r * p.z.rs)[(uint32_t)d[k]];      // (u's where there is no gate)
+        }
+        maps(p, r, p.G > 1 ? d[0] / p.Dg : 0, n0);
+    }
+};
+template <int IO, int CPT>
 __global__ __launch_bounds__(256) void seq_scan_step_kernel(const ScanStepP p) {
+    using CT = typename SeqIO<IO>::C;
     __shared__ int before, next;
     typedef CT V4 __attribute__((ext_vector_type(4)));
     const int cpb = 256 / p.lpc, sub = threadIdx.x % p.lpc, dl = threadIdx.x / p.lpc;
-    const int64_t cb = (p.D + cpb * CPT - 1) / (cpb * CPT);
-    int64_t r = (int64_t)blockIdx.x / cb;
-    const int d0 = (int)((int64_t)blockIdx.x - r * cb) * cpb * CPT + dl;
+    const uint32_t cb = (uint32_t)(p.D + cpb * CPT - 1) / (uint32_t)(cpb * CPT), r0 = blockIdx.x / cb;
+    int64_t r = r0;
+    const int d0 = (int)(blockIdx.x - r0 * cb) * cpb * CPT + dl;
     int d[CPT];
 #pragma unroll
     for (int c = 0; c < CPT; ++c) d[c] = d0 + c * cpb < p.D ? d0 + c * cpb : p.D - 1;
     const int64_t slot = p.slot ? p.slot[r] : r;
     const bool there = slot >= 0 && slot < p.n_slots;
-    const int n0 = sub * 4;
-    CT A2[CPT][4], h[CPT][4];
-    CT *st = (CT *)p.state + (there ? slot : 0) * (int64_t)p.D * p.N + n0;
-    const CT *pa = (const CT *)p.A + n0;
-    if (there) {
-        if (p.vec) {
-#pragma unroll
-            for (int c = 0; c < CPT; ++c) {
-                const V4 s = *(const V4 *)(st + (int64_t)d[c] * p.N), a = *(const V4 *)(pa + (int64_t)d[c] * p.N);
-#pragma unroll
-                for (int i = 0; i < 4; ++i) { A2[c][i] = a[i]; h[c][i] = s[i]; }
-            }
-        } else {
-#pragma unroll
-            for (int c = 0; c < CPT; ++c)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const bool in = n0 + i < p.N;
-                    A2[c][i] = in ? pa[(int64_t)d[c] * p.N + i] : CT(0);
-                    h[c][i] = in ? st[(int64_t)d[c] * p.N + i] : CT(0);
-                }
-        }
-    }
-    int64_t nx = -1;
-    if (p.slot && there && p.rows > 1) {
-        if (threadIdx.x == 0) { before = 0; next = 0x7fffffff; }
-        __syncthreads();
-        seq_same_slot(p.slot, p.rows, r, &before, &next);
-        __syncthreads();
-        if (before) return;
-        nx = next == 0x7fffffff ? -1 : next;
-    }
     if (!there) {
         if (sub == 0)
 #pragma unroll
@@ -662,48 +661,71 @@ __global__ __launch_bounds__(256) void seq_scan_step_kernel(const ScanStepP p) {
                 if (d0 + c * cpb < p.D) seq_store(p.y, r * (int64_t)p.y.rs + d[c], CT(0));
         return;
     }
-    CT bias[CPT], skip[CPT];
+    const int n0 = sub * 4;
+    CT A2[CPT][4], h[CPT][4], bias[CPT], skip[CPT];
+    CT *st = (CT *)p.state + slot * (int64_t)p.D * p.N + n0;
+    const CT *pa = (const CT *)p.A + n0;
+    if (p.vec) {
+#pragma unroll
+        for (int c = 0; c < CPT; ++c) {
+            const V4 s = *(const V4 *)(st + (int64_t)d[c] * p.N), a = *(const V4 *)(pa + (int64_t)d[c] * p.N);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) { A2[c][i] = a[i]; h[c][i] = s[i]; }
+        }
+    } else {
+#pragma unroll
+        for (int c = 0; c < CPT; ++c)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const bool in = n0 + i < p.N;
+                A2[c][i] = in ? pa[(int64_t)d[c] * p.N + i] : CT(0);
+                h[c][i] = in ? st[(int64_t)d[c] * p.N + i] : CT(0);
+            }
+    }
+    ScanStepRow<IO, CPT> row;
+    row.load(p, r, d, n0);
 #pragma unroll
     for (int c = 0; c < CPT; ++c) {
         bias[c] = p.dt_bias ? ((const CT *)p.dt_bias)[d[c]] : CT(0);
         skip[c] = p.Dskip ? ((const CT *)p.Dskip)[d[c]] : CT(0);
+    }
+    int64_t nx = -1;
+    if (p.slot && p.rows > 1) {
+        if (threadIdx.x == 0) { before = 0; next = 0x7fffffff; }
+        __syncthreads();
+        seq_same_slot(p.slot, p.rows, r, &before, &next);
+        __syncthreads();
+        if (before) return;
+        nx = next == 0x7fffffff ? -1 : next;
+    }
+#pragma unroll
+    for (int c = 0; c < CPT; ++c)
 #pragma unroll
         for (int i = 0; i < 4; ++i) A2[c][i] *= CT(kLog2eD);
-    }
     for (;;) {
-        CT u[CPT], x[CPT], z[CPT], b[4], cc[4];
 #pragma unroll
         for (int c = 0; c < CPT; ++c) {
-            u[c] = seq_load1(p.u, r * (int64_t)p.u.rs + d[c], CT(0));
-            x[c] = seq_load1(p.dt, r * (int64_t)p.dt.rs + d[c], CT(0));
-            z[c] = p.z.p ? seq_load1(p.z, r * (int64_t)p.z.rs + d[c], CT(0)) : CT(0);
-        }
-#pragma unroll
-        for (int c = 0; c < CPT; ++c) {
-            if (c == 0 || p.G > 1) {
-                const int g = p.G > 1 ? d[c] / p.Dg : 0;
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int n = n0 + i < p.N ? n0 + i : p.N - 1;
-                    b[i] = seq_load1(p.B, r * (int64_t)p.B.rs + g * p.Bg + n * p.Bn, CT(0));
-                    cc[i] = seq_load1(p.C, r * (int64_t)p.C.rs + g * p.Cg + n * p.Cn, CT(0));
-                }
-            }
-            const CT pre = x[c] + bias[c], dlt = p.softplus ? seq_softplus(pre) : pre, du = dlt * u[c];
+            if (c > 0 && p.G > 1) row.maps(p, r, d[c] / p.Dg, n0);
+            const CT u = scan_value<IO>(row.u[c], p.u.dt), pre = scan_value<IO>(row.x[c], p.u.dt) + bias[c], z = scan_value<IO>(row.z[c], p.u.dt);
+            const CT dlt = p.softplus ? seq_softplus(pre) : pre, du = dlt * u;
             CT v = CT(0);
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const bool in = n0 + i < p.N;
-                h[c][i] = seq_fma(seq_exp2(dlt * A2[c][i]), h[c][i], in ? du * b[i] : CT(0));
-                v = seq_fma(h[c][i], in ? cc[i] : CT(0), v);
+                h[c][i] = seq_fma(seq_exp2(dlt * A2[c][i]), h[c][i], in ? du * scan_value<IO>(row.b[i], p.u.dt) : CT(0));
+                v = seq_fma(h[c][i], in ? scan_value<IO>(row.c[i], p.u.dt) : CT(0), v);
             }
-            for (int k = 1; k < p.lpc; k <<= 1) v += __shfl_xor(v, k);
-            v = seq_fma(skip[c], u[c], v);
-            if (p.z.p) v = v * (z[c] * seq_sigmoid(z[c]));
+            if (p.lpc > 1) v += seq_dpp<0xb1>(v);
+            if (p.lpc > 2) v += seq_dpp<0x4e>(v);
+            for (int k = 4; k < p.lpc; k <<= 1) v += __shfl_xor(v, k);
+            v = seq_fma(skip[c], u, v);
+            const CT vz = v * (z * seq_sigmoid(z));
+            v = p.gate ? vz : v;
             if (sub == 0 && d0 + c * cpb < p.D) seq_store(p.y, r * (int64_t)p.y.rs + d[c], v);
         }
         if (nx < 0) break;
         r = nx;
+        row.load(p, r, d, n0);
         __syncthreads();
         if (threadIdx.x == 0) next = 0x7fffffff;
         __syncthreads();
