@@ -115,20 +115,22 @@ struct ScanPlan {
     int64_t flat;
     crnn::ScanP p;
     // workspace, in elements of the compute type
-    int64_t S, G, sdel, part, dA, dD, db, acc, total;
+    int64_t S, G, sdel, part, dA, acc, total;
 };
 
-// Rows of a chunk of the forward scan; 0: sequences are not cut.  Cutting costs a second look at every row (the chunk's end without its past), so
-// it is left where the sequences and channel tiles alone give two wavefronts a SIMD (8 sequences of 1024 rows, 4096 channels, 512 wavefronts:
-// 600 us whole, 279 us cut; at 1024 wavefronts a row costs the same either way).  Else chunks are as short as their carry allows: many of them
-// even out the last round of blocks.  Measured (rows x tiles of 64 channels: us at 16 / 32 / 48 / 64 / 128 rows): 64 x 24: 41 / 44 / 54 / 69 / 69;
-// 512 x 64: 47 / 48 / 57 / 69 / 120; 2048 x 32: 79 / 68 / 79 / 76 / 125; 8190 x 64: 396 / 296 / 279 / 291 / 325.
-int64_t scan_forward_rows(int64_t flat, int32_t n_seq, int64_t ntile) {
-    if ((int64_t)n_seq * ntile >= 2048) return 0;
-    const int64_t rows = flat * ntile;
-    int64_t q = rows <= 16384 ? 16 : rows <= 131072 ? 32 : 48;
-    q = std::max(q, rows / 32768);
-    return (q + crnn::kScanTB - 1) / crnn::kScanTB * crnn::kScanTB;
+// Rows of a chunk of the forward scan; 0: sequences are not cut.  Cutting costs a second look at all but a sequence's last chunk and two launches; a
+// block alone takes 0.25 us a row.  So short sequences stay whole, and so do a dense batch's where they give every SIMD a wavefront; packed ones are cut
+// even then, since their lengths are not known here.  Else chunks are as long as they still fill the card.  Measured (bf16, 16 states; sequences x
+// rows x channels: us at 16 / 32 / 64 / 128 / 512 rows a chunk, whole): 1 x 64 x 1536 - / 31 / 31 / 30 / 30, 22; 1 x 256 x 1536 29 / 32 / 42 / 66 / 76, 69;
+// 1 x 512 x 4096 50 / 42 / 46 / 67 / 139, 132; 1 x 2048 x 2048 80 / 65 / 60 / 72 / 220, 509; 9 x 910 x 4096 471 / 318 / 263 / 260 / 300, 657;
+// 8 x 1024 x 4096 458 / 307 / 260 / 245 / 267, 273; 32 x 512 x 4096 878 / 607 / 508 / 458 / 359, 319.
+int64_t scan_forward_rows(int64_t flat, int32_t n_seq, int64_t rows, bool packed, int64_t ntile) {
+    if (rows <= 64) return 0;                      // (packed: no sequence has more)
+    const bool many = (int64_t)n_seq * ntile >= 1024;
+    if (many && !packed) return 0;
+    const int64_t total = flat * ntile;
+    const int64_t q = many ? 512 : total <= 8192 ? 16 : total <= 49152 ? 32 : total <= 262144 ? 64 : 128;
+    return std::max(q, (total / 8192 + 7) / 8 * 8);
 }
 
 bool scan_plan(SeqCheck &c, const crnn_scan_args *a, bool backward, ScanPlan &s) {
@@ -147,11 +149,11 @@ bool scan_plan(SeqCheck &c, const crnn_scan_args *a, bool backward, ScanPlan &s)
     p.D = a->D; p.N = a->N; p.G = a->G; p.Dg = a->D / a->G;
     p.tpg = (p.Dg + 63) / 64;
     p.ntile = p.tpg * a->G;
-    const int64_t Q = backward ? crnn::kScanBwdQ : scan_forward_rows(s.flat, a->n_seq, p.ntile);
+    const int64_t Q = backward ? crnn::kScanBwdQ : scan_forward_rows(s.flat, a->n_seq, a->rows, a->seq_start != nullptr, p.ntile);
     p.m = seq_map(a->n_seq, a->rows, a->seq_start, a->seq_len, Q);
     s.split = backward || Q > 0;
     const int64_t blk = p.m.nblk * a->D;
-    if (p.m.nblk * ((p.ntile + crnn::kScanWaves - 1) / crnn::kScanWaves) > kSeqMaxGrid || (int64_t)a->n_seq * s.NS * a->D / 256 >= kSeqMaxGrid)
+    if (p.m.nblk * p.ntile > kSeqMaxGrid || (int64_t)a->n_seq * s.NS * a->D / 256 >= kSeqMaxGrid)
         return c.bad("too many sequences, rows and channels for one launch");
     int64_t at = 0;
     auto take = [&](int64_t n) { const int64_t o = at; at += (n + 31) / 32 * 32; return o; };
@@ -159,9 +161,7 @@ bool scan_plan(SeqCheck &c, const crnn_scan_args *a, bool backward, ScanPlan &s)
     s.sdel = take(s.split ? blk : 0);
     s.G = take(backward ? blk * s.NS : 0);
     s.part = take(backward ? (int64_t)p.ntile * s.flat * 2 * s.NS : 0);
-    s.dA = take(backward ? blk * s.NS : 0);
-    s.dD = take(backward ? blk : 0);
-    s.db = take(backward ? blk : 0);
+    s.dA = take(backward ? blk * (s.NS + 2) : 0);
     s.acc = take(s.nb > 1 ? s.flat * a->D * (backward ? 3 : 1) : 0);
     s.total = at * (s.f64 ? 8 : 4);
     return true;
@@ -198,17 +198,17 @@ void scan_forward_run(const crnn_scan_args *a, ScanPlan &s, hipStream_t st) {
     crnn::ScanP p = s.p;
     CT *ws = (CT *)a->workspace, *S = ws + s.S, *sdel = ws + s.sdel;
     p.acc = s.nb > 1 ? ws + s.acc : nullptr;
-    const dim3 grid((unsigned)(p.m.nblk * ((p.ntile + crnn::kScanWaves - 1) / crnn::kScanWaves))), block(64 * crnn::kScanWaves);
+    const dim3 grid((unsigned)(p.m.nblk * p.ntile)), block(64 * crnn::kScanWaves);
     for (int b = 0; b < s.nb; ++b) {
         p.n0 = b * NS;
         p.first = b == 0;
         p.fin = b == s.nb - 1;
         if (s.split) {
-            hipLaunchKernelGGL((crnn::seq_scan_ends_kernel<IO, NS, MODE, false>), grid, block, 0, st, p, S, (CT *)nullptr, sdel);
+            hipLaunchKernelGGL((crnn::seq_scan_fwd_kernel<IO, NS, MODE, false>), grid, block, 0, st, p, (const CT *)nullptr, S, sdel);
             hipLaunchKernelGGL((crnn::seq_scan_carry_kernel<CT, NS>), dim3((unsigned)(((int64_t)p.m.n_seq * NS * p.D + 255) / 256)), dim3(256), 0, st, p, S,
                                (CT *)nullptr, (const CT *)sdel);
         }
-        hipLaunchKernelGGL((crnn::seq_scan_out_kernel<IO, NS, MODE>), grid, block, 0, st, p, (const CT *)(s.split ? S : nullptr));
+        hipLaunchKernelGGL((crnn::seq_scan_fwd_kernel<IO, NS, MODE, true>), grid, block, 0, st, p, (const CT *)(s.split ? S : nullptr), (CT *)nullptr, (CT *)nullptr);
     }
 }
 
@@ -216,30 +216,24 @@ template <int IO, int NS, int MODE>
 void scan_backward_run(const crnn_scan_args *a, ScanPlan &s, hipStream_t st) {
     using CT = typename crnn::SeqIO<IO>::C;
     crnn::ScanP p = s.p;
-    CT *ws = (CT *)a->workspace, *S = ws + s.S, *Gb = ws + s.G, *sdel = ws + s.sdel, *part = ws + s.part, *dA = ws + s.dA, *dD = ws + s.dD,
-       *db = ws + s.db;
+    CT *ws = (CT *)a->workspace, *S = ws + s.S, *Gb = ws + s.G, *sdel = ws + s.sdel, *part = ws + s.part, *pp = ws + s.dA;
     p.acc = s.nb > 1 ? ws + s.acc : nullptr;
     const dim3 grid((unsigned)(p.m.nblk * ((p.ntile + crnn::kScanWaves - 1) / crnn::kScanWaves))), block(64 * crnn::kScanWaves);
     crnn::ScanMapsP mo = scan_maps(a, s, a->dB, a->dC, a->N, 1, a->N, 1);
-    const int64_t cA = (int64_t)NS * p.D;
+    const int64_t cA = (int64_t)(NS + 2) * p.D;      // dA's states, then the gradients of the skip and of the step lengths' bias
     for (int b = 0; b < s.nb; ++b) {
         p.n0 = mo.n0 = b * NS;
         p.first = b == 0;
         p.fin = b == s.nb - 1;
-        hipLaunchKernelGGL((crnn::seq_scan_ends_kernel<IO, NS, MODE, true>), grid, block, 0, st, p, S, Gb, sdel);
+        hipLaunchKernelGGL((crnn::seq_scan_ends2_kernel<IO, NS, MODE>), grid, block, 0, st, p, S, Gb, sdel);
         hipLaunchKernelGGL((crnn::seq_scan_carry_kernel<CT, NS>), dim3((unsigned)(((int64_t)p.m.n_seq * NS * p.D + 255) / 256)), dim3(256), 0, st, p, S, Gb,
                            (const CT *)sdel);
-        hipLaunchKernelGGL((crnn::seq_scan_bwd_kernel<IO, NS, MODE>), grid, block, 0, st, p, (const CT *)S, (const CT *)Gb, part, dA, dD, db);
+        hipLaunchKernelGGL((crnn::seq_scan_bwd_kernel<IO, NS, MODE>), grid, block, 0, st, p, (const CT *)S, (const CT *)Gb, part, pp);
         if (s.flat > 0)
             hipLaunchKernelGGL((crnn::seq_scan_sum_maps_kernel<CT, NS>), dim3(seq_grid(s.flat * p.G * 2 * NS)), dim3(256), 0, st, p.m, mo, (const CT *)part, p.tpg);
-        hipLaunchKernelGGL((crnn::seq_sum_blocks_kernel<CT>), dim3((unsigned)((cA + 31) / 32)), dim3(256), 0, st, (const CT *)dA, p.m.nblk, cA, (CT *)a->dA, (CT *)nullptr, p.D,
-                           p.N, p.n0, std::min(NS, p.N - p.n0));
+        hipLaunchKernelGGL((crnn::seq_sum_blocks_kernel<CT>), dim3((unsigned)((cA + 31) / 32)), dim3(256), 0, st, (const CT *)pp, p.m.nblk, cA, (CT *)a->dA,
+                           (CT *)(p.fin ? a->dskip : nullptr), (CT *)(p.fin ? a->ddt_bias : nullptr), p.D, p.N, p.n0, std::min(NS, p.N - p.n0), NS);
     }
-    const dim3 gd((unsigned)((p.D + 31) / 32));
-    if (a->dskip)
-        hipLaunchKernelGGL((crnn::seq_sum_blocks_kernel<CT>), gd, dim3(256), 0, st, (const CT *)dD, p.m.nblk, (int64_t)p.D, (CT *)a->dskip, (CT *)nullptr, p.D, 1, 0, 1);
-    if (a->ddt_bias)
-        hipLaunchKernelGGL((crnn::seq_sum_blocks_kernel<CT>), gd, dim3(256), 0, st, (const CT *)db, p.m.nblk, (int64_t)p.D, (CT *)a->ddt_bias, (CT *)nullptr, p.D, 1, 0, 1);
 }
 
 bool scan_views(SeqCheck &c, const crnn_scan_args *a, bool backward) {
@@ -416,10 +410,10 @@ int32_t crnn_conv_backward(const crnn_conv_args *a) {
         const dim3 grid((unsigned)((count + 31) / 32));
         if (f64)
             hipLaunchKernelGGL((crnn::seq_sum_blocks_kernel<double>), grid, dim3(256), 0, st, (const double *)p.part, p.m.nblk, count, (double *)a->dweight, (double *)a->dbias,
-                               a->D, a->W, 0, a->W);
+                               (double *)nullptr, a->D, a->W, 0, a->W, a->W);
         else
-            hipLaunchKernelGGL((crnn::seq_sum_blocks_kernel<float>), grid, dim3(256), 0, st, (const float *)p.part, p.m.nblk, count, (float *)a->dweight, (float *)a->dbias, a->D,
-                               a->W, 0, a->W);
+            hipLaunchKernelGGL((crnn::seq_sum_blocks_kernel<float>), grid, dim3(256), 0, st, (const float *)p.part, p.m.nblk, count, (float *)a->dweight, (float *)a->dbias,
+                               (float *)nullptr, a->D, a->W, 0, a->W, a->W);
         SEQ_DONE("crnn_conv_backward");
     } catch (...) { return -1; }
 }

@@ -6,19 +6,21 @@
 //
 // the diagonal linear ODE h' = A h + B u stepped exactly over steps of their own length, input held.
 //
-// Split: a lane owns a channel and NS of its states in registers, a wavefront 64 channels of one group, so that B and C of a row are the
-// same for all its lanes and reach the arithmetic as scalar operands (scalar loads from a float copy, seq_scan_maps_kernel).  Per row,
-// channel and state the sweep is one multiplication and one exponential for the decay and three multiply-adds: bound by the vector
-// units, not by memory.  Where sequences and channels do not fill the card, time is cut into chunks: their ends without what came
-// before (mode of seq_scan_ends_kernel), the carry over the chunks of a sequence (seq_scan_carry_kernel: its decay over a chunk is
-// exp(A sum delta)), then the chunks proper.
+// Split.  A block owns 64 channels of one group (a tile), a lane a channel.  Forward, four wavefronts share the states: each row's step length,
+// input and gate are worked out by one of them and handed round in the LDS, so are the row's B and C (the same for all lanes of a tile: read
+// back as broadcasts) and each wavefront's part of sum_n C h.  Per row, channel and state that is one multiplication and one exponential for
+// the decay and three multiply-adds: bound by the vector units, not by memory.  The gradient needs every state's neighbours in registers and
+// gives a wavefront all states of its tile.
+// Where tiles and sequences do not fill the card, time is cut into chunks: their ends without what came before (seq_scan_ends_kernel), the
+// carry over the chunks of a sequence (seq_scan_carry_kernel: the decay over a chunk is exp(A sum delta)), then the chunks proper.
 #pragma once
 #include "seq_common.hpp"
 
 namespace crnn {
 
-constexpr int kScanTB = 4;      // rows whose loads are in flight together
-constexpr int kScanWaves = 4;   // wavefronts of a block, each on its own channel tile
+constexpr int kScanTB = 4;      // gradient: rows whose loads are in flight together
+constexpr int kScanRows = 8;    // forward: rows of a batch, two for each wavefront (16 measured the same)
+constexpr int kScanWaves = 4;   // wavefronts of a block (gradient: each on its own channel tile)
 
 struct ScanP {
     SeqMap m;
@@ -158,90 +160,157 @@ struct ScanMapRows {
     }
 };
 
-// ---- forward: outputs of a chunk from its first state (start[block][n][d]; null: one chunk a sequence, from state_in)
-template <int IO, int NS, int MODE>
-__global__ __launch_bounds__(64 * kScanWaves, IO == 8 ? 2 : 4) void seq_scan_out_kernel(const ScanP p, const typename SeqIO<IO>::C *__restrict__ start) {
+// the place of a block of the forward kernels: chunk block, channel tile
+__device__ __forceinline__ ScanAt scan_tile(const ScanP &p) {
+    ScanAt a;
+    const uint32_t b = blockIdx.x / (uint32_t)p.ntile;
+    a.b = b;
+    a.tile = (int32_t)(blockIdx.x - b * (uint32_t)p.ntile);
+    a.on = true;
+    a.g = a.tile / p.tpg;
+    const int dl = (a.tile - a.g * p.tpg) * 64 + (int)(threadIdx.x & 63);
+    a.valid = dl < p.Dg;
+    a.d = a.g * p.Dg + (dl < p.Dg ? dl : p.Dg - 1);
+    a.k = seq_locate(p.m, a.b);
+    return a;
+}
+
+// What the wavefronts of a forward block hand each other: step length and delta u of a batch's rows, its B and C, the parts of its sums.
+template <class CT, int NS, bool OUT>
+struct ScanShare {
+    CT dl[kScanRows][64], du[kScanRows][64], maps[kScanRows][2 * NS], v[OUT ? kScanWaves : 1][OUT ? kScanRows : 1][64];
+};
+
+// ---- forward, a chunk.  OUT: outputs from its first state (start[block][n][d]; null: one chunk a sequence, from state_in), and the sequence's
+// last state.  Not OUT: S = the chunk's last state from zero and the sum of delta (a sequence's last chunk is not asked).
+template <int IO, int NS, int MODE, bool OUT>
+__global__ __launch_bounds__(64 * kScanWaves, IO == 8 ? 3 : 6) void seq_scan_fwd_kernel(const ScanP p, const typename SeqIO<IO>::C *__restrict__ start,
+                                                                                      typename SeqIO<IO>::C *__restrict__ S, typename SeqIO<IO>::C *__restrict__ sdel) {
     using CT = typename SeqIO<IO>::C;
-    constexpr int TB = kScanTB;
-    __shared__ CT smaps[kScanWaves][TB * 2 * NS];
-    CT *maps = smaps[threadIdx.x >> 6];
-    const ScanAt a = scan_at(p);
-    if (!a.on) return;
+    using E = typename SeqIO<IO>::E;
+    constexpr int R = kScanRows, RW = kScanRows / kScanWaves, NW = NS / kScanWaves;      // rows and states of a wavefront
+    constexpr int MV = R * 2 * NS >= 256 ? R * 2 * NS / 256 : 1;                         // values of B and C a thread brings
+    __shared__ ScanShare<CT, NS, OUT> sh;
+    const ScanAt a = scan_tile(p);
     const bool fin = MODE != kScanAny || p.fin;
-    if (p.zero_outside && fin) seq_zero_outside(p.m, p.y, a.b, a.d, a.valid);
-    if (!a.k.live) return;
-    CT A2[NS], h[NS];
-    scan_rates<CT, NS>(p, a.d, A2);
-    if (start) {
+    const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)), lane = threadIdx.x & 63;
+    if (OUT && p.zero_outside && fin && wave == 0) seq_zero_outside(p.m, p.y, a.b, a.d, a.valid);
+    if (!a.k.live || (!OUT && a.k.last)) return;
+    CT A2[NW], h[NW], sd = CT(0);
 #pragma unroll
-        for (int n = 0; n < NS; ++n) h[n] = scan_plane<NS>(start, a.b, n, p.D)[(uint32_t)a.d];
-    } else {
-        scan_state<CT, NS>(p, p.state_in, a.k.s, a.d, h);
+    for (int j = 0; j < NW; ++j) {
+        const int ns = wave * NW + j, n = p.n0 + ns;
+        A2[j] = n < p.N ? ((const CT *)p.A)[(int64_t)a.d * p.N + n] * CT(kLog2eD) : CT(0);
+        h[j] = CT(0);
+        if (OUT && start && n < p.N) h[j] = scan_plane<NS>(start, a.b, ns, p.D)[(uint32_t)a.d];
+        else if (OUT && !start && p.state_in && n < p.N) h[j] = ((const CT *)p.state_in)[((int64_t)a.k.s * p.D + a.d) * p.N + n];
     }
     if (a.k.n > 0) {
-        const CT bias = p.dt_bias ? ((const CT *)p.dt_bias)[a.d] : CT(0), skip = p.Dskip ? ((const CT *)p.Dskip)[a.d] : CT(0);
-        SeqRows<IO, MODE, TB> ru, rz;
-        SeqRows<IO, 0, TB> rd;
-        ScanMapRows<IO, NS, TB> rm;
-        rm.init(p, a);
-        rm.load(0, a.k.n);
-        ru.load(p.m, p.u, a.k, 0, a.d);
-        rd.load(p.m, p.dt, a.k, 0, a.d);
-        rz.load(p.m, p.z, a.k, 0, a.d);
+        const CT bias = p.dt_bias ? ((const CT *)p.dt_bias)[a.d] : CT(0), skip = OUT && p.Dskip ? ((const CT *)p.Dskip)[a.d] : CT(0);
+        // the thread's values of B and C: column j of rows row0, row0 + 256 / (2 NS), ..
+        const int mj = threadIdx.x % (2 * NS), mrow = threadIdx.x / (2 * NS), mn = p.n0 + mj % NS;
+        const bool min_ = mn < p.N, mb = mj < NS;
+        const int mnn = min_ ? mn : p.N - 1;
+        const E *pb = (const E *)p.B.p + seq_off(p.m, p.B, a.k, a.k.t0) + a.g * p.Bg, *pc = (const E *)p.C.p + seq_off(p.m, p.C, a.k, a.k.t0) + a.g * p.Cg;
+        const E *mat = mb ? pb + mnn * p.Bn : pc + mnn * p.Cn;
+        const int32_t mrs = mb ? p.B.rs : p.C.rs;
+        E mv[MV];
+        SeqRows<IO, MODE, RW> ru, rz;
+        SeqRows<IO, 0, RW> rd;
+        auto fetch = [&](int t) {
+#pragma unroll
+            for (int k = 0; k < MV; ++k) {
+                const int r = t + mrow + k * (256 / (2 * NS));
+                mv[k] = mat[(int64_t)(r < a.k.n ? r : a.k.n - 1) * mrs];
+            }
+            ru.load(p.m, p.u, a.k, t + wave * RW, a.d);
+            rd.load(p.m, p.dt, a.k, t + wave * RW, a.d);
+            if (OUT) rz.load(p.m, p.z, a.k, t + wave * RW, a.d);
+        };
+        fetch(0);
 #pragma unroll 1
-        for (int t = 0; t < a.k.n; t += TB) {
-            CT u[TB], x[TB], z[TB], dl[TB], v[TB];
+        for (int t = 0; t < a.k.n; t += R) {
+            const int mine = t + wave * RW;              // the wavefront's first row of the batch
+            CT u[RW], x[RW], z[RW], dl[RW];
             ru.get(p.u, u);
             rd.get(p.dt, x);
-            rz.get(p.z, z);
-            rm.put(p.B.dt, maps);
-            rm.load(t + TB, a.k.n);
-            ru.load(p.m, p.u, a.k, t + TB, a.d);
-            rd.load(p.m, p.dt, a.k, t + TB, a.d);
-            rz.load(p.m, p.z, a.k, t + TB, a.d);
-            scan_steps<IO, TB>(p, a.k.n - t, bias, x, u, dl);
+            if (OUT) rz.get(p.z, z);
 #pragma unroll
-            for (int i = 0; i < TB; ++i) {
-                const CT *bc = maps + i * (2 * NS);
-                const CT du = dl[i] * u[i];
-                CT s0 = CT(0), s1 = CT(0);
-#pragma unroll
-                for (int n = 0; n < NS; n += 2) {
-                    h[n] = seq_fma(seq_exp2(dl[i] * A2[n]), h[n], du * bc[n]);
-                    h[n + 1] = seq_fma(seq_exp2(dl[i] * A2[n + 1]), h[n + 1], du * bc[n + 1]);
-                    s0 = seq_fma(h[n], bc[NS + n], s0);
-                    s1 = seq_fma(h[n + 1], bc[NS + n + 1], s1);
-                }
-                v[i] = s0 + s1;
+            for (int k = 0; k < MV; ++k) {
+                CT m;
+                if (IO == 8) m = (CT)mv[k];
+                else if (IO == 4) m = (CT)seq_as_float((uint32_t)mv[k]);
+                else m = (CT)(p.B.dt == CRNN_DT_BF16 ? seq_as_float((uint32_t)mv[k] << 16) : seq_from_f16((uint32_t)mv[k]));
+                if (R * 2 * NS >= 256 || mrow < R) sh.maps[(mrow + k * (256 / (2 * NS))) % R][mj] = min_ ? m : CT(0);
             }
-            seq_wave_sync();
-            if (MODE == kScanAny && p.acc) {
+            fetch(t + R);
 #pragma unroll
-                for (int i = 0; i < TB; ++i) {
-                    const int ii = t + i < a.k.n ? t + i : a.k.n - 1;
-                    CT *acc = (CT *)p.acc + (a.k.flat + a.k.t0 + ii) * p.D;
-                    if (!p.first) v[i] += acc[(uint32_t)a.d];
-                    if (!fin && t + i < a.k.n && a.valid) acc[(uint32_t)a.d] = v[i];
-                }
+            for (int i = 0; i < RW; ++i) {
+                x[i] += bias;
+                dl[i] = p.softplus ? seq_softplus(x[i]) : x[i];
+                const bool in = mine + i < a.k.n;
+                dl[i] = in ? dl[i] : CT(0);
+                sh.dl[wave * RW + i][lane] = dl[i];
+                sh.du[wave * RW + i][lane] = in ? dl[i] * u[i] : CT(0);
+                if (!OUT) sd += dl[i];
             }
-            if (fin) {
+            __syncthreads();
 #pragma unroll
-                for (int i = 0; i < TB; ++i) {
-                    v[i] = seq_fma(skip, u[i], v[i]);
+            for (int i = 0; i < R; ++i) {
+                const CT d = sh.dl[i][lane], du = sh.du[i][lane];
+                CT v = CT(0);
+#pragma unroll
+                for (int j = 0; j < NW; ++j) {
+                    h[j] = seq_fma(seq_exp2(d * A2[j]), h[j], du * sh.maps[i][wave * NW + j]);
+                    if (OUT) v = seq_fma(h[j], sh.maps[i][NS + wave * NW + j], v);
+                }
+                if (OUT) sh.v[OUT ? wave : 0][OUT ? i : 0][lane] = v;
+            }
+            __syncthreads();
+            if (OUT) {
+#pragma unroll
+                for (int i = 0; i < RW; ++i) {
+                    CT v = CT(0);
+#pragma unroll
+                    for (int w = 0; w < kScanWaves; ++w) v += sh.v[OUT ? w : 0][OUT ? wave * RW + i : 0][lane];
+                    const int row = mine + i;
+                    if (row >= a.k.n) break;
+                    if (MODE == kScanAny && p.acc) {
+                        CT *acc = (CT *)p.acc + (a.k.flat + a.k.t0 + row) * p.D + a.d;
+                        if (!p.first) v += *acc;
+                        if (!fin && a.valid) *acc = v;
+                    }
+                    if (!fin) continue;
+                    v = seq_fma(skip, u[i], v);
                     const CT g = z[i] * seq_sigmoid(z[i]);
-                    v[i] = p.gate ? v[i] * g : v[i];
+                    v = p.gate ? v * g : v;
+                    seq_store(p.y, seq_off(p.m, p.y, a.k, a.k.t0 + row) + a.d, v);     // (lanes without a channel: the last channel's value again)
                 }
-                seq_put_rows<IO, TB>(p.m, p.y, a.k, t, a.d, v);
             }
         }
     }
-    if (a.k.last && p.state_out && a.valid) scan_state_put<CT, NS>(p, p.state_out, a.k.s, a.d, h);
+    if (OUT) {
+        if (a.k.last && p.state_out && a.valid)
+#pragma unroll
+            for (int j = 0; j < NW; ++j) {
+                const int n = p.n0 + wave * NW + j;
+                if (n < p.N) ((CT *)p.state_out)[((int64_t)a.k.s * p.D + a.d) * p.N + n] = h[j];
+            }
+        return;
+    }
+    // every wavefront summed its own rows' step lengths
+    sh.dl[wave][lane] = sd;
+    __syncthreads();
+    if (!a.valid) return;
+#pragma unroll
+    for (int j = 0; j < NW; ++j) scan_plane<NS>(S, a.b, wave * NW + j, p.D)[(uint32_t)a.d] = h[j];
+    if (wave == 0) sdel[a.b * p.D + a.d] = (sh.dl[0][lane] + sh.dl[1][lane]) + (sh.dl[2][lane] + sh.dl[3][lane]);
 }
 
-// ---- a chunk by itself: S = its last state from zero, sum of delta; BOTH: also G = what its outputs' gradients r pass back to the state
+// ---- gradient, a chunk by itself: S = its last state from zero, the sum of delta, and G = what its outputs' gradients r pass back to the state
 // before it, sum_t (prod of the decays up to t) r C -- taken in the forward direction, so that one exponential serves both.
-template <int IO, int NS, int MODE, bool BOTH>
-__global__ __launch_bounds__(64 * kScanWaves, IO == 8 ? 2 : BOTH ? 3 : 5) void seq_scan_ends_kernel(const ScanP p, typename SeqIO<IO>::C *__restrict__ S,
+template <int IO, int NS, int MODE>
+__global__ __launch_bounds__(64 * kScanWaves, IO == 8 ? 2 : 3) void seq_scan_ends2_kernel(const ScanP p, typename SeqIO<IO>::C *__restrict__ S,
                                                                                                   typename SeqIO<IO>::C *__restrict__ Gb,
                                                                                                   typename SeqIO<IO>::C *__restrict__ sdel) {
     using CT = typename SeqIO<IO>::C;
@@ -250,12 +319,13 @@ __global__ __launch_bounds__(64 * kScanWaves, IO == 8 ? 2 : BOTH ? 3 : 5) void s
     CT *maps = smaps[threadIdx.x >> 6];
     const ScanAt a = scan_at(p);
     if (!a.on || !a.k.live) return;
-    CT A2[NS], h[NS], P[BOTH ? NS : 1], g[BOTH ? NS : 1];
+    CT A2[NS], h[NS], P[NS], g[NS];
     scan_rates<CT, NS>(p, a.d, A2);
 #pragma unroll
     for (int n = 0; n < NS; ++n) {
         h[n] = CT(0);
-        if (BOTH) { P[BOTH ? n : 0] = CT(1); g[BOTH ? n : 0] = CT(0); }
+        P[n] = CT(1);
+        g[n] = CT(0);
     }
     CT sd = CT(0);
     if (a.k.n > 0) {
@@ -267,35 +337,27 @@ __global__ __launch_bounds__(64 * kScanWaves, IO == 8 ? 2 : BOTH ? 3 : 5) void s
         rm.load(0, a.k.n);
         ru.load(p.m, p.u, a.k, 0, a.d);
         rd.load(p.m, p.dt, a.k, 0, a.d);
-        if (BOTH) {
-            ry.load(p.m, p.dy, a.k, 0, a.d);
-            rz.load(p.m, p.z, a.k, 0, a.d);
-        }
+        ry.load(p.m, p.dy, a.k, 0, a.d);
+        rz.load(p.m, p.z, a.k, 0, a.d);
 #pragma unroll 1
         for (int t = 0; t < a.k.n; t += TB) {
             CT u[TB], x[TB], z[TB], y[TB], dl[TB];
             ru.get(p.u, u);
             rd.get(p.dt, x);
-            if (BOTH) {
-                ry.get(p.dy, y);
-                rz.get(p.z, z);
-            }
+            ry.get(p.dy, y);
+            rz.get(p.z, z);
             rm.put(p.B.dt, maps);
             rm.load(t + TB, a.k.n);
             ru.load(p.m, p.u, a.k, t + TB, a.d);
             rd.load(p.m, p.dt, a.k, t + TB, a.d);
-            if (BOTH) {
-                ry.load(p.m, p.dy, a.k, t + TB, a.d);
-                rz.load(p.m, p.z, a.k, t + TB, a.d);
-            }
+            ry.load(p.m, p.dy, a.k, t + TB, a.d);
+            rz.load(p.m, p.z, a.k, t + TB, a.d);
             scan_steps<IO, TB>(p, a.k.n - t, bias, x, u, dl);
-            if (BOTH) {
 #pragma unroll
-                for (int i = 0; i < TB; ++i) {
-                    const CT gz = z[i] * seq_sigmoid(z[i]);
-                    y[i] = p.gate ? y[i] * gz : y[i];
-                    y[i] = t + i < a.k.n ? y[i] : CT(0);
-                }
+            for (int i = 0; i < TB; ++i) {
+                const CT gz = z[i] * seq_sigmoid(z[i]);
+                y[i] = p.gate ? y[i] * gz : y[i];
+                y[i] = t + i < a.k.n ? y[i] : CT(0);
             }
 #pragma unroll
             for (int i = 0; i < TB; ++i) {
@@ -306,10 +368,8 @@ __global__ __launch_bounds__(64 * kScanWaves, IO == 8 ? 2 : BOTH ? 3 : 5) void s
                 for (int n = 0; n < NS; ++n) {
                     const CT e = seq_exp2(dl[i] * A2[n]);
                     h[n] = seq_fma(e, h[n], du * bc[n]);
-                    if (BOTH) {
-                        P[BOTH ? n : 0] *= e;
-                        g[BOTH ? n : 0] = seq_fma(P[BOTH ? n : 0], y[i] * bc[NS + n], g[BOTH ? n : 0]);
-                    }
+                    P[n] *= e;
+                    g[n] = seq_fma(P[n], y[i] * bc[NS + n], g[n]);
                 }
             }
             seq_wave_sync();
@@ -319,7 +379,7 @@ __global__ __launch_bounds__(64 * kScanWaves, IO == 8 ? 2 : BOTH ? 3 : 5) void s
 #pragma unroll
     for (int n = 0; n < NS; ++n) {
         scan_plane<NS>(S, a.b, n, p.D)[(uint32_t)a.d] = h[n];
-        if (BOTH) scan_plane<NS>(Gb, a.b, n, p.D)[(uint32_t)a.d] = g[BOTH ? n : 0];
+        scan_plane<NS>(Gb, a.b, n, p.D)[(uint32_t)a.d] = g[n];
     }
     sdel[a.b * p.D + a.d] = sd;
 }
@@ -388,8 +448,7 @@ constexpr int kScanBwdTB = 4, kScanBwdSub = 5, kScanBwdQ = kScanBwdTB * kScanBwd
 template <int IO, int NS, int MODE>
 __global__ __launch_bounds__(64 * kScanWaves, 2) void seq_scan_bwd_kernel(const ScanP p, const typename SeqIO<IO>::C *__restrict__ start,
                                                                           const typename SeqIO<IO>::C *__restrict__ back, typename SeqIO<IO>::C *__restrict__ part,
-                                                                          typename SeqIO<IO>::C *__restrict__ dApart, typename SeqIO<IO>::C *__restrict__ dDpart,
-                                                                          typename SeqIO<IO>::C *__restrict__ dbpart) {
+                                                                          typename SeqIO<IO>::C *__restrict__ ppart) {
     using CT = typename SeqIO<IO>::C;
     constexpr int TB = kScanBwdTB, H = NS / 2;
     __shared__ CT keep[kScanWaves][kScanBwdSub - 1][NS][64];
@@ -542,11 +601,9 @@ __global__ __launch_bounds__(64 * kScanWaves, 2) void seq_scan_bwd_kernel(const 
     }
     if (!a.valid) return;
 #pragma unroll
-    for (int n = 0; n < NS; ++n) scan_plane<NS>(dApart, a.b, n, p.D)[(uint32_t)a.d] = dA[n];
-    if (fin) {
-        dDpart[a.b * p.D + a.d] = dD;
-        dbpart[a.b * p.D + a.d] = db;
-    }
+    for (int n = 0; n < NS; ++n) scan_plane<NS + 2>(ppart, a.b, n, p.D)[(uint32_t)a.d] = dA[n];
+    scan_plane<NS + 2>(ppart, a.b, NS, p.D)[(uint32_t)a.d] = dD;
+    scan_plane<NS + 2>(ppart, a.b, NS + 1, p.D)[(uint32_t)a.d] = db;
 }
 
 // ---- dB, dC: the tiles of a group in order.  dst: views like B and C.
@@ -560,7 +617,13 @@ __global__ __launch_bounds__(256) void seq_scan_sum_maps_kernel(const SeqMap m, 
         if (n >= p.N) continue;
         CT sum = CT(0);
         if (seq_inside(m, r))
-            for (int k = 0; k < tpg; ++k) sum += part[((g * tpg + k) * p.rows + r) * (2 * NS) + j];
+            for (int k = 0; k < tpg; k += 8) {
+                CT x[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) x[e] = part[((g * tpg + (k + e < tpg ? k + e : tpg - 1)) * p.rows + r) * (2 * NS) + j];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) sum += k + e < tpg ? x[e] : CT(0);
+            }
         const SeqV &v = j < NS ? p.B : p.C;
         const int64_t at = p.srows ? (r / p.srows) * v.bs + (r % p.srows) * v.rs : r * v.rs;
         seq_store(v, at + g * (j < NS ? p.Bg : p.Cg) + n * (j < NS ? p.Bn : p.Cn), sum);
@@ -568,11 +631,11 @@ __global__ __launch_bounds__(256) void seq_scan_sum_maps_kernel(const SeqMap m, 
 }
 
 // ---- sums over the blocks of a launch, in double and in a fixed order: in[block][count] -> out.  A thread block takes 32 neighbouring columns, eight
-// threads each every eighth block of its own, then one of them adds the eight.  Column i goes to out[(i % D) width + off + i / D] while i / D <
-// lim (a [width][D] array transposed: width 1 leaves it as it is), the others to rest[i % D] (may be null).
+// threads each every eighth block of its own, then one of them adds the eight.  in is [block][planes][D]: the first `lim` planes go to
+// out[d width + off + plane], plane p0 to out0[d], plane p0 + 1 to out1[d] (either may be null).
 template <class CT>
-__global__ __launch_bounds__(256) void seq_sum_blocks_kernel(const CT *__restrict__ in, int64_t nblk, int64_t count, CT *__restrict__ out, CT *__restrict__ rest, int32_t D,
-                                                             int32_t width, int32_t off, int32_t lim) {
+__global__ __launch_bounds__(256) void seq_sum_blocks_kernel(const CT *__restrict__ in, int64_t nblk, int64_t count, CT *__restrict__ out, CT *__restrict__ out0, CT *__restrict__ out1,
+                                                             int32_t D, int32_t width, int32_t off, int32_t lim, int32_t p0) {
     __shared__ double sh[8][32];
     const int col = threadIdx.x & 31, k = threadIdx.x >> 5;
     const int64_t i = (int64_t)blockIdx.x * 32 + col;
@@ -594,7 +657,8 @@ __global__ __launch_bounds__(256) void seq_sum_blocks_kernel(const CT *__restric
     for (int j = 1; j < 8; ++j) s += sh[j][col];
     const int64_t j = i / D, d = i % D;
     if (j < lim) out[d * width + off + j] = (CT)s;
-    else if (rest) rest[d] = (CT)s;
+    if (j == p0 && out0) out0[d] = (CT)s;
+    if (j == p0 + 1 && out1) out1[d] = (CT)s;
 }
 
 // ---- one row for each of many running sequences, states updated in place.  LPC lanes share a channel, four states each (16-byte loads of

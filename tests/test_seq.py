@@ -726,7 +726,8 @@ def test_there_is_no_cpu_path():
 
 
 def test_c_entry_points_refuse_before_any_launch():
-    """The C ABI by itself: sizes, missing arrays, types, workspace -- refused with a message, on a host without a device too."""
+    """The C ABI by itself: sizes, missing arrays, types, workspace -- refused with a message, on a host without a device too.  The pointers are
+    made up, so the calls name a device that does not exist: one that got past every check would be refused for that."""
     import ctypes as C
     lib = L.lib
     said = lambda: lib.crnn_last_error(None).decode()  # noqa: E731
@@ -735,7 +736,7 @@ def test_c_entry_points_refuse_before_any_launch():
         return L.View(ptr=ptr, row_stride=rs, seq_stride=48, dtype=dt)
 
     def scan(**over):
-        a = L.ScanArgs(struct_size=C.sizeof(L.ScanArgs), n_seq=2, D=8, N=4, G=1, rows=6, A=4096, u=view(), dt=view(), y=view(), B=view(rs=4), C=view(rs=4))
+        a = L.ScanArgs(struct_size=C.sizeof(L.ScanArgs), device=99, n_seq=2, D=8, N=4, G=1, rows=6, A=4096, u=view(), dt=view(), y=view(), B=view(rs=4), C=view(rs=4))
         for k, v in over.items():
             setattr(a, k, v)
         return a
@@ -743,15 +744,15 @@ def test_c_entry_points_refuse_before_any_launch():
     for over, word in [(dict(struct_size=8), "struct_size"), (dict(N=0), "N must"), (dict(N=257), "N must"), (dict(G=3), "divide"), (dict(rows=-1), "negative"), (dict(rows=1 << 31), "rows"),
                        (dict(D=0), "D must"), (dict(A=None), "A is missing"), (dict(u=view(ptr=None)), "u is missing"), (dict(u=view(L.DT_BF16)), "element type"),
                        (dict(u=view(L.DT_PACKED8)), "scales"), (dict(dt=view(L.DT_PACKED8)), "checkpoint"), (dict(y=view(rs=7)), "overlap"), (dict(dtype=9), "element type"),
-                       (dict(seq_start=64, seq_len=64), "exclude"), ({}, "workspace")]:
+                       (dict(seq_start=64, seq_len=64), "exclude"), (dict(rows=600), "workspace"), ({}, "device")]:
         assert lib.crnn_scan_forward(C.byref(scan(**over))) == -1 and word in said(), (over, said())
     assert lib.crnn_scan_forward(None) == -1 and "null" in said()
-    assert lib.crnn_scan_workspace(C.byref(scan()), 2) == -1 and lib.crnn_scan_workspace(C.byref(scan()), 0) > 0
+    assert lib.crnn_scan_workspace(C.byref(scan()), 2) == -1 and lib.crnn_scan_workspace(C.byref(scan()), 0) == 0 and lib.crnn_scan_workspace(C.byref(scan(rows=600)), 0) > 0
     assert lib.crnn_scan_backward(C.byref(scan())) == -1 and "dA" in said()
     assert lib.crnn_scan_step(C.byref(scan(n_slots=1))) == -1 and "n_slots" in said()
 
     def conv(**over):
-        a = L.ConvArgs(struct_size=C.sizeof(L.ConvArgs), n_seq=2, D=8, W=4, rows=6, weight=4096, x=view(), y=view())
+        a = L.ConvArgs(struct_size=C.sizeof(L.ConvArgs), device=99, n_seq=2, D=8, W=4, rows=6, weight=4096, x=view(), y=view())
         for k, v in over.items():
             setattr(a, k, v)
         return a
@@ -762,6 +763,6 @@ def test_c_entry_points_refuse_before_any_launch():
     assert lib.crnn_conv_backward(C.byref(conv(dx=view(), dy=view(), dweight=64))) == -1 and "workspace" in said()
     assert lib.crnn_conv_step(C.byref(conv(n_slots=1))) == -1 and "n_slots" in said()
     v = view(L.DT_F64)
-    assert lib.crnn_pack8(0, None, C.byref(v), 2, 8, 4096, 4096) == -1 and "half" in said()
+    assert lib.crnn_pack8(99, None, C.byref(v), 2, 8, 4096, 4096) == -1 and "half" in said()
     v = view()
-    assert lib.crnn_unpack8(0, None, 4096, None, 2, 8, C.byref(v)) == -1 and "missing" in said()
+    assert lib.crnn_unpack8(99, None, 4096, None, 2, 8, C.byref(v)) == -1 and "missing" in said()
