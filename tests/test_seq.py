@@ -671,6 +671,165 @@ def test_training_step_through_both_operators(packed):
         assert torch.equal(got[k], want[k]), k
 
 
+# ---------------------------------------------------------------- how the arrays lie
+@gpu
+def test_arrays_of_other_strides():
+    """Maps whose states are not neighbours, an input shared by the batch (stride 0), channels that are not contiguous, parameters in the data's type:
+    the same values as contiguous copies."""
+    g = torch.Generator().manual_seed(8)
+    B, T, D, N, G, dt = 2, 33, 24, 16, 3, torch.bfloat16
+    u, d, z = rnd(g, 1, T, D, dtype=dt).expand(B, T, D), rnd(g, B, D, T, dtype=dt).transpose(1, 2), rnd(g, B, T, 2 * D, dtype=dt)[..., D:]
+    A, skip, bias = (-torch.exp(rnd(g, D, N))).to(dt), rnd(g, D, dtype=dt), rnd(g, D, dtype=dt) - 1
+    Bm, Cm, dy = rnd(g, B, T, N, G, dtype=dt).transpose(2, 3), rnd(g, B, T, G, 2 * N, dtype=dt)[..., ::2], rnd(g, B, T, D, dtype=dt)
+    given = dict(u=u, dt=d, A=A, B=Bm, C_=Cm, D=skip, z=z, dt_bias=bias)
+    plain = {k: v.contiguous() if k not in ("A", "D", "dt_bias") else v.float() for k, v in given.items()}
+    assert not any(given[k].is_contiguous() for k in ("u", "dt", "z", "B", "C_"))
+    assert torch.equal(seq.selective_scan(**given), seq.selective_scan(**plain))
+    for a, b in zip(seq.selective_scan_grad(dy, **given), seq.selective_scan_grad(dy, **plain)):
+        assert (a is None) == (b is None) and (a is None or torch.equal(a, b))
+    w = rnd(g, 4, D, dtype=dt).t()
+    assert torch.equal(seq.causal_conv(z, w, skip), seq.causal_conv(z.contiguous(), w.float().contiguous(), skip.float()))
+    row = lambda k: given[k][:, 5]  # noqa: E731
+    s1, s2 = (torch.zeros(B, D, N, device=DEV) for _ in range(2))
+    y1 = seq.selective_scan_step(row("u"), row("dt"), A, row("B"), row("C_"), s1, D=skip, z=row("z"), dt_bias=bias)
+    y2 = seq.selective_scan_step(*(row(k).contiguous() for k in ("u", "dt")), A.float(), row("B").contiguous(), row("C_").contiguous(), s2, D=skip.float(), z=row("z").contiguous(),
+                                 dt_bias=bias.float())
+    assert torch.equal(y1, y2) and torch.equal(s1, s2)
+    assert torch.equal(seq.unpack8(seq.pack8(d)), seq.unpack8(seq.pack8(d.contiguous())))
+
+
+@gpu
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_nothing_to_do(dtype):
+    """No sequences, no rows, only empty sequences: states pass through, gradients of parameters are 0."""
+    g = torch.Generator().manual_seed(2)
+    D, N, W, dt = 12, 16, 4, DT[dtype]
+    w, A = rnd(g, D, W), -torch.exp(rnd(g, D, N))
+    for shape, n, kw in (((0, 5, D), 0, {}), ((3, 0, D), 3, {}), ((0, D), 2, dict(seq_start=torch.zeros(3, dtype=torch.int32, device=DEV))),
+                         ((4, D), 2, dict(seq_start=torch.tensor([1, 1, 1], dtype=torch.int32, device=DEV)))):
+        x = rnd(g, *shape, dtype=dt)
+        m = rnd(g, *shape[:-1], N, dtype=dt)
+        cst, hst = rnd(g, n, W - 1, D, dtype=dt), rnd(g, n, D, N)
+        y, end = seq.causal_conv(x, w, state=cst, return_state=True, **kw)
+        assert y.shape == x.shape and torch.equal(end, cst) and not bool(y.any())
+        y, end = seq.selective_scan(x, x, A, m, m, state=hst, return_state=True, **kw)
+        assert y.shape == x.shape and torch.equal(end, hst) and not bool(y.any())
+        gc = seq.causal_conv_grad(x, x, w, state=cst, dstate=cst, **kw)
+        assert not bool(gc.x.any()) and not bool(gc.weight.any()) and torch.equal(gc.state, cst)
+        gs = seq.selective_scan_grad(x, x, x, A, m, m, D=A[:, 0], state=hst, dstate=hst, **kw)
+        assert not any(bool(v.any()) for v in (gs.u, gs.dt, gs.A, gs.B, gs.C, gs.D)) and torch.equal(gs.state, hst)
+    y = seq.selective_scan_step(*(torch.zeros(0, D, dtype=dt, device=DEV),) * 2, A, *(torch.zeros(0, N, dtype=dt, device=DEV),) * 2, torch.zeros(2, D, N, device=DEV))
+    assert y.shape == (0, D)
+    assert seq.causal_conv_step(torch.zeros(0, D, dtype=dt, device=DEV), w, None, torch.zeros(2, W - 1, D, dtype=dt, device=DEV)).shape == (0, D)
+
+
+# ---------------------------------------------------------------- streams, graphs, sizes: the device only
+def everything(D=96, N=16, rows=200, dtype=torch.bfloat16, seed=0):
+    """Inputs, and a function that runs every operator on them and returns all results."""
+    g = torch.Generator().manual_seed(seed)
+    at = torch.tensor([0, 70, 70, rows], dtype=torch.int32, device=DEV)
+    x, d, z, dy = (rnd(g, rows, D, dtype=dtype) for _ in range(4))
+    Bm, Cm, w, b = rnd(g, rows, N, dtype=dtype), rnd(g, rows, N, dtype=dtype), rnd(g, D, 4, scale=0.5), rnd(g, D)
+    A, skip, bias, st = -torch.exp(rnd(g, D, N)), rnd(g, D), rnd(g, D) - 2, rnd(g, 3, D, N)
+
+    def run():
+        kw = dict(D=skip, dt_bias=bias, seq_start=at, state=st)
+        px, pz = seq.pack8(x), seq.pack8(z)
+        c = seq.causal_conv(x, w, b, silu=True, seq_start=at)
+        y, end = seq.selective_scan(c, d, A, Bm, Cm, z=z, return_state=True, **kw)
+        s = seq.selective_scan_grad(dy, c, d, A, Bm, Cm, z=pz, **kw)
+        cg = seq.causal_conv_grad(s.u, px, w, b, silu=True, seq_start=at)
+        h, cs = end.clone(), x[:9].view(3, 3, D).clone()
+        c1 = seq.causal_conv_step(x[:3], w, b, cs, silu=True)
+        y1 = seq.selective_scan_step(c1, d[:3], A, Bm[:3], Cm[:3], h, D=skip, z=z[:3], dt_bias=bias)
+        return [seq.unpack8(px), c, y, end, *s, *cg[:3], cs, h, c1, y1]
+
+    return dict(x=x, d=d, z=z, dy=dy, B=Bm, C=Cm), run
+
+
+def same(a, b):
+    return all(p is None and q is None or torch.equal(p, q) for p, q in zip(a, b))
+
+
+@gpu
+def test_on_a_stream_of_its_own_and_two_at_once():
+    if DEV == "cpu":
+        pytest.skip("the emulated device has no streams")
+    calls = [everything(seed=k)[1] for k in range(2)]
+    want = [c() for c in calls]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    for _ in range(3):
+        got = []
+        for s, c in zip(streams, calls):
+            with torch.cuda.stream(s):
+                got.append(c())
+        torch.cuda.synchronize()
+        assert all(same(a, b) for a, b in zip(got, want))
+
+
+@gpu
+def test_captured_into_two_graphs_and_replayed():
+    """Two captured graphs, replayed in turn with other inputs, eager calls and waits between them, give what eager calls give."""
+    if DEV == "cpu":
+        pytest.skip("the emulated device has no graphs")
+    sets = [everything(seed=10 + k) for k in range(2)]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _, run in sets:
+            run()
+    torch.cuda.current_stream().wait_stream(side)
+    graphs = []
+    for _, run in sets:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = run()
+        graphs.append((graph, out))
+    for turn in range(4):
+        for k in (0, 1, 1, 0):
+            inputs, run = sets[k]
+            for v in inputs.values():
+                v.copy_(torch.randn(v.shape, generator=torch.Generator().manual_seed(turn * 7 + k), dtype=torch.float32))
+            graphs[k][0].replay()
+            torch.cuda.synchronize()
+            got = [None if v is None else v.clone() for v in graphs[k][1]]
+            want = run()
+            torch.cuda.synchronize()
+            assert same(got, want), (turn, k)
+
+
+@gpu
+def test_arrays_over_two_to_the_31_elements():
+    """Rows far behind 2^31 elements: the last of them against a call on them alone that starts from the state in front."""
+    if DEV == "cpu":
+        pytest.skip("sizes for the device")
+    D, T, tail, N = 8192, 266_000, 40, 8
+    assert D * T > 2 ** 31 + D * tail
+    g = torch.Generator(device=DEV).manual_seed(0)
+    x = torch.randn(1, T, D, generator=g, device=DEV, dtype=torch.bfloat16)
+    w = torch.randn(D, 4, generator=g, device=DEV)
+    y = seq.causal_conv(x, w, silu=True)
+    assert torch.equal(y[:, -tail:], seq.causal_conv(x[:, -tail:], w, silu=True, state=x[:, -tail - 3:-tail].contiguous()))
+    gx = seq.causal_conv_grad(y, x, w, silu=True).x
+    assert torch.equal(gx[:, -tail:], seq.causal_conv_grad(y[:, -tail:], x[:, -tail:], w, silu=True, state=x[:, -tail - 3:-tail].contiguous()).x)
+    del gx
+    p = seq.pack8(x)
+    q = seq.pack8(x[:, -tail:].contiguous())
+    assert torch.equal(p.codes[:, -tail:], q.codes) and torch.equal(p.scales[:, -tail:], q.scales)
+    assert torch.equal(seq.unpack8(p)[:, -tail:], seq.unpack8(q))
+    del p, q
+    A, m = -torch.rand(D, N, generator=g, device=DEV) - 0.5, torch.randn(1, T, N, generator=g, device=DEV, dtype=torch.bfloat16)
+    _, st = seq.selective_scan(x[:, :-tail], x[:, :-tail], A, m[:, :-tail], m[:, :-tail], return_state=True, out=y[:, :-tail])
+    yy, end = seq.selective_scan(x[:, -tail:], x[:, -tail:], A, m[:, -tail:], m[:, -tail:], state=st, return_state=True)
+    y, e = seq.selective_scan(x, x, A, m, m, return_state=True, out=y)
+    # chunks elsewhere: a unit of bfloat16, and 1e-5 of the sums' size for the order
+    a, b = y[:, -tail:].double(), yy.double()
+    assert bool(((a - b).abs() <= 2.0 ** -7 * b.abs() + 1e-4).all()) and bool(((e - end).abs() <= 1e-4 * (1 + end.abs())).all())
+
+
 # ---------------------------------------------------------------- refusals: before any launch
 def args(**over):
     g = torch.Generator().manual_seed(0)

@@ -16,6 +16,6 @@ pytestmark = [pytest.mark.cpu_only,
 def test_the_device_tests_of_the_sequence_operators_pass_on_the_emulated_device():
     subprocess.run(["bash", os.path.join(SIMT, "build.sh")], check=True, timeout=1500)
     env = dict(os.environ, CRNN_HIP_LIB=os.path.join(SIMT, "libcrnn_simt.so"), SIMT_THREADS=os.environ.get("SIMT_THREADS", "4"))
-    out = subprocess.run([sys.executable, "-m", "pytest", "tests/test_seq.py", "-m", "gpu", "-q", "-p", "no:cacheprovider", "-k", "not captured and not stream"], cwd=ROOT, env=env,
+    out = subprocess.run([sys.executable, "-m", "pytest", "tests/test_seq.py", "-m", "gpu", "-q", "-p", "no:cacheprovider"], cwd=ROOT, env=env,
                          capture_output=True, text=True, timeout=800)
     assert out.returncode == 0 and " passed" in out.stdout, out.stdout[-3000:] + out.stderr[-1000:]
