@@ -275,11 +275,11 @@ int conv_wide(int dtype, int W, bool backward) {
     return 4;
 }
 // Rows of a strip: strips and channels together give some wavefronts to each SIMD; a strip reads W - 1 rows twice, the gradient 2 (W - 1).
-// Measured (us at 8 / 16 / 24 / 32 / 64 / 128 rows): forward 12001 x 4096 bf16 75 / 50 / 46 / 46 / 47 / 45, 1024 x 2048 14 / 14 / 14 / 15 / 18 / 27;
-// gradient 8192 x 2048 75 / 57 / 45 / 48 / 56 / 63, 12000 x 4096 186 / 120 / 100 / 91 / 79 / 92, 1024 x 2048 25 / 25 / 25 / 25 / 34 / 54.
+// Measured, bf16 (us at 8 / 16 / 24 / 32 / 48 / 64 / 128 rows): forward 12001 x 4096 71 / 46 / 45 / 45 / 47 / 46 / 45, 1024 x 2048 14 / 14 / 14 / 15 / 15 / 18 /
+// 28; gradient 8192 x 2048 from 8 bits 69 / 51 / 42 / 44 / 43 / 55 / 58, 12000 x 4096 168 / 111 / 92 / 89 / 77 / 76 / 86, 1024 x 2048 25 / 25 / 25 / 26 / 28 / 33 / 51.
 int64_t conv_strip(int64_t flat, int32_t D, int V, bool backward) {
     const int64_t waves = (D + 64 * V - 1) / (64 * V);
-    const int64_t q = flat * waves / (backward ? 3072 : 4096) / 4 * 4;
+    const int64_t q = (flat * waves / 4096 + 3) / 4 * 4;
     const int64_t lo = backward ? 24 : 8, hi = backward ? 64 : 32;
     return q < lo ? lo : q > hi ? hi : q;
 }
@@ -399,13 +399,14 @@ int32_t crnn_conv_backward(const crnn_conv_args *a) {
         SeqCheck c{"crnn_conv_backward", {}};
         crnn::ConvP p;
         if (!conv_check(c, a, true, p) || !conv_views(c, a, true, p)) return sfail(c.err);
+        if (a->n_seq == 0) return sfail("crnn_conv_backward: no sequences");
         const bool f64 = a->dtype == CRNN_DT_F64;
         const int64_t need = p.m.nblk * (a->W + 1) * a->D * (f64 ? 8 : 4);
         if (need > 0 && (!a->workspace || a->workspace_bytes < need)) return sfail("crnn_conv_backward: workspace is missing or too small");
         SEQ_DEVICE(a->device, "crnn_conv_backward");
         p.part = a->workspace;
         const hipStream_t st = (hipStream_t)a->stream;
-        if (a->n_seq > 0) conv_launch_t(p, a->dtype, conv_channels(a, 1), true, st);
+        conv_launch_t(p, a->dtype, conv_channels(a, 1), true, st);
         const int64_t count = (int64_t)(a->W + 1) * a->D;       // [tap][D], then the bias
         const dim3 grid((unsigned)((count + 31) / 32));
         if (f64)

@@ -230,7 +230,7 @@ __global__ __launch_bounds__(256) void seq_conv_fwd_kernel(const ConvP p) {
 // Gradient.  dp = dy act'(p) needs p once more; dx[t] = sum_j w[j] dp[t + W - 1 - j] needs the W - 1 rows behind t: the strip is walked W - 1
 // rows past its end.  A sequence's first strip starts W - 1 rows early: those are the state's.  dw, db: a strip's part, summed in order.
 template <int XT, int YT, int WM, int V>
-__global__ __launch_bounds__(256) void seq_conv_bwd_kernel(const ConvP p) {
+__global__ __launch_bounds__(256, WM == 4 && (YT == CRNN_DT_BF16 || YT == CRNN_DT_F16) ? 4 : 1) void seq_conv_bwd_kernel(const ConvP p) {
     using CT = typename SeqT<YT>::C;
     constexpr int TB = kConvTB;
     const ConvAt a = conv_at<V>(p);
@@ -255,15 +255,16 @@ __global__ __launch_bounds__(256) void seq_conv_bwd_kernel(const ConvP p) {
             for (int c = 0; c < V; ++c) dp[j][c] = CT(0);
         }
         const int back = p.W - 1;
-        const int64_t lo = a.k.t0 == 0 ? -(int64_t)back : a.k.t0, hi = a.k.t0 + a.k.n;     // rows whose dx this strip writes
-        const int64_t lastrow = a.k.len - 1;
+        // (fewer than 2^31 rows: uniform comparisons of 32 bits stay out of the vector unit)
+        const int t0 = (int)a.k.t0, len = (int)a.k.len, lo = t0 == 0 ? -back : t0, hi = t0 + a.k.n;     // rows whose dx this strip writes
+        const int lastrow = len - 1;
         const char *xrow = conv_row<XT>(p.m, p.x, a.k, 0), *grow = conv_row<YT>(p.m, p.dy, a.k, 0);
         const uint8_t *srow = conv_scales<XT>(p.m, p.x, a.k, 0);
         char *orow = conv_row<YT>(p.m, p.dx, a.k, 0);
         const int64_t xs = (int64_t)p.x.rs * ConvRaw<XT, V>::ES, ss = p.x.srs, gs = (int64_t)p.dy.rs * ConvRaw<YT, V>::ES, os = (int64_t)p.dx.rs * ConvRaw<YT, V>::ES;
         ConvRaw<XT, V> rx[TB];
         ConvRaw<YT, V> rg[TB];
-        auto fetch = [&](int64_t t) {
+        auto fetch = [&](int t) {
 #pragma unroll
             for (int i = 0; i < TB; ++i) {
                 const int64_t r = t + i < lastrow ? t + i : lastrow;
@@ -271,9 +272,9 @@ __global__ __launch_bounds__(256) void seq_conv_bwd_kernel(const ConvP p) {
                 rg[i].load(grow + r * gs, nullptr, a.d);
             }
         };
-        if (a.k.n > 0) fetch(a.k.t0);
+        if (a.k.n > 0) fetch(t0);
 #pragma unroll 1
-        for (int64_t t = a.k.t0; t < hi + WM - 1; t += TB) {
+        for (int t = t0; t < hi + WM - 1; t += TB) {
             if (a.k.n > 0) {
 #pragma unroll
                 for (int i = 0; i < TB; ++i)
@@ -321,23 +322,23 @@ __global__ __launch_bounds__(256) void seq_conv_bwd_kernel(const ConvP p) {
                     for (int j = 0; j < WM; ++j) s = seq_fma(w[WM - 1 - j][c], dp[i + j][c], s);
                     o[i][c] = s;
                 }
-            const int64_t r0 = t - (WM - 1);
-            if (r0 >= (lo > 0 ? lo : 0) && r0 + TB <= hi && !(p.dst_out.p && r0 + TB > a.k.len - back)) {
+            const int r0 = t - (WM - 1);
+            if (r0 >= (lo > 0 ? lo : 0) && r0 + TB <= hi && !(p.dst_out.p && r0 + TB > len - back)) {
 #pragma unroll
-                for (int i = 0; i < TB; ++i) conv_put<YT, V>(orow + (r0 + i) * os, a.d, o[i]);
+                for (int i = 0; i < TB; ++i) conv_put<YT, V>(orow + (int64_t)(r0 + i) * os, a.d, o[i]);
             } else {
 #pragma unroll
                 for (int i = 0; i < TB; ++i) {
-                    const int64_t r = r0 + i;
+                    const int r = r0 + i;
                     if (r < lo || r >= hi) continue;
-                    if (p.dst_out.p && r >= a.k.len - back) {
+                    if (p.dst_out.p && r >= len - back) {
                         ConvRaw<YT, V> d;
-                        d.load((const char *)p.dst_out.p + ((int64_t)a.k.s * p.dst_out.bs + (r - (a.k.len - back)) * p.dst_out.rs) * ConvRaw<YT, V>::ES, nullptr, a.d);
+                        d.load((const char *)p.dst_out.p + ((int64_t)a.k.s * p.dst_out.bs + (int64_t)(r - (len - back)) * p.dst_out.rs) * ConvRaw<YT, V>::ES, nullptr, a.d);
 #pragma unroll
                         for (int c = 0; c < V; ++c) o[i][c] += (CT)d.get(c);
                     }
-                    if (r >= 0) conv_put<YT, V>(orow + r * os, a.d, o[i]);
-                    else if (p.dst_in.p) conv_put<YT, V>((char *)p.dst_in.p + ((int64_t)a.k.s * p.dst_in.bs + (r + back) * p.dst_in.rs) * ConvRaw<YT, V>::ES, a.d, o[i]);
+                    if (r >= 0) conv_put<YT, V>(orow + (int64_t)r * os, a.d, o[i]);
+                    else if (p.dst_in.p) conv_put<YT, V>((char *)p.dst_in.p + ((int64_t)a.k.s * p.dst_in.bs + (int64_t)(r + back) * p.dst_in.rs) * ConvRaw<YT, V>::ES, a.d, o[i]);
                 }
             }
 #pragma unroll

@@ -12,7 +12,7 @@ Arrays are torch tensors on an MI355X; the calls enqueue on that device's curren
 a graph.  Rows are time, channels are contiguous: dense [n_seq, rows, D] (lengths=: how many rows of each are its own, the others are
 padding), or packed [rows, D] with seq_start [n_seq + 1], int32 on the device: sequence s is rows seq_start[s] .. seq_start[s + 1] - 1.
 Lengths and offsets are not read by the host: they are clamped to the arrays.  Rows of a result that belong to no sequence are 0, and stay as
-they were where the caller gave the array (out=).  float32, bfloat16, float16 and float64; weights, rates and scan states are float32
+they were where the caller gave the array (out=).  Results may not share memory with inputs.  float32, bfloat16, float16 and float64; weights, rates and scan states are float32
 (float64 with float64 data).  A checkpoint (Packed8) may stand for x of the convolution, and for u and z of the scan.
 """
 from __future__ import annotations
@@ -202,6 +202,13 @@ class _Rows:
         return given
 
 
+def _none(y, out, end):
+    """The result for no sequences: all rows of y are outside of them."""
+    if out is None:
+        y.zero_()
+    return y if end is None else (y, end)
+
+
 def _slots(rows, slots, n, n_slots):
     if slots is None:
         if n > n_slots:
@@ -251,7 +258,11 @@ def causal_conv(x, weight, bias=None, *, silu=False, seq_start=None, lengths=Non
     D, shape = r.D, (r.n_seq, W - 1, r.D)
     weight, bias, state = r.weight(weight, "weight", (D, W)), r.weight(bias, "bias", (D,)), r.state(state, "state", shape, r.dtype)
     y = r.out(out, r.shape)
+    if out is not None and out.data_ptr() == (x.codes if x.__class__ is Packed8 else x).data_ptr() and out.numel():
+        raise ValueError("out may not be x: a row's result needs the rows before it")
     end = r.new(shape, r.dtype) if return_state else None
+    if r.n_seq == 0:
+        return _none(y, out, end)
     a = _conv_args(r, W, silu, r.rows, r.ragged if out is None else 0, weight, bias, _view(x), _view(y), _view(state) if W > 1 else _ABSENT, _view(end) if W > 1 else _ABSENT)
     if lib.crnn_conv_forward(a):
         check(-1)
@@ -270,6 +281,8 @@ def causal_conv_grad(dy, x, weight, bias=None, *, silu=False, seq_start=None, le
     dx, dw = r.out(None, r.shape), r.new((D, W), r.param)
     db = None if bias is None else r.new((D,), r.param)
     ds = None if state is None else r.new(shape, r.dtype)
+    if r.n_seq == 0:
+        return ConvGrads(dx.zero_(), dw.zero_(), None if db is None else db.zero_(), ds)
 
     def args(ws=0, need=0):
         v = (lambda t: _view(t) if W > 1 else _ABSENT)
@@ -350,6 +363,8 @@ def selective_scan(u, dt, A, B, C_, *, D=None, z=None, dt_bias=None, softplus=Tr
     state = r.state(state, "state", shape, r.param)
     y = r.out(out, r.shape)
     end = r.new(shape, r.param) if return_state else None
+    if r.n_seq == 0:
+        return _none(y, out, end)
 
     def args(ws=0, need=0):
         return _scan_args(r, N, G, r.rows, r.ragged if out is None else 0, softplus, A, D, dt_bias, _view(u), _view(dt), _view(z), _view(y), maps, _ptr(state), _ptr(end), ws=ws,

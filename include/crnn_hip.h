@@ -473,7 +473,8 @@ int32_t crnn_cathode_get_particles(crnn_cathode_ctx *ctx, double *p);
  * many of them each has; the others are padding).  Packed: seq_start[n_seq + 1] on the device, sequence s is rows seq_start[s] ..
  * seq_start[s + 1] - 1 of arrays of `rows` rows.  Sequences may be empty.  Offsets and lengths are clamped to the arrays (offsets that
  * decrease make the sequence empty; what sequences that overlap give is not defined).  Rows of an output that belong to no sequence are
- * left as they were, or set to 0 where zero_outside is set.
+ * left as they were, or set to 0 where zero_outside is set.  With no sequences (n_seq = 0) the forward calls and the steps do nothing and the
+ * backward calls are refused.  Outputs may not share memory with inputs (states of the steps excepted: they are updated in place).
  * Element types: input, output and state activations of one call share one type (CRNN_DT_F32, _BF16, _F16, _F64); x of the convolution
  * and u, z of the scan may be checkpoints (_PACKED8) unless the call's type is _F64.  Weights, A, D, biases, scan states and the gradients of
  * all of these are float (double where the type is _F64); arithmetic is in that type, activations are rounded once, when stored.

@@ -705,7 +705,7 @@ def test_nothing_to_do(dtype):
     g = torch.Generator().manual_seed(2)
     D, N, W, dt = 12, 16, 4, DT[dtype]
     w, A = rnd(g, D, W), -torch.exp(rnd(g, D, N))
-    for shape, n, kw in (((0, 5, D), 0, {}), ((3, 0, D), 3, {}), ((0, D), 2, dict(seq_start=torch.zeros(3, dtype=torch.int32, device=DEV))),
+    for shape, n, kw in (((0, 5, D), 0, {}), ((6, D), 0, dict(seq_start=torch.zeros(1, dtype=torch.int32, device=DEV))), ((3, 0, D), 3, {}), ((0, D), 2, dict(seq_start=torch.zeros(3, dtype=torch.int32, device=DEV))),
                          ((4, D), 2, dict(seq_start=torch.tensor([1, 1, 1], dtype=torch.int32, device=DEV)))):
         x = rnd(g, *shape, dtype=dt)
         m = rnd(g, *shape[:-1], N, dtype=dt)
@@ -864,7 +864,7 @@ def test_other_refusals():
     p = seq.pack8(z(2, 6, 8))
     for err, call in [
             (ValueError, lambda: seq.causal_conv(z(2, 6, 8), z(8, 9))), (ValueError, lambda: seq.causal_conv(z(2, 6, 8), z(7, 4))), (ValueError, lambda: seq.causal_conv(z(6, 8), z(8, 4))),
-            (ValueError, lambda: seq.causal_conv(z(2, 6, 8), z(8, 4), state=z(2, 4, 8))), (ValueError, lambda: seq.causal_conv_grad(z(2, 6, 7), z(2, 6, 8), z(8, 4))),
+            (ValueError, lambda: seq.causal_conv(z(2, 6, 8), z(8, 4), state=z(2, 4, 8))), (ValueError, lambda: (lambda x: seq.causal_conv(x, z(8, 4), out=x))(z(2, 6, 8))), (ValueError, lambda: seq.causal_conv_grad(z(2, 6, 7), z(2, 6, 8), z(8, 4))),
             (TypeError, lambda: seq.causal_conv_grad(p, z(2, 6, 8), z(8, 4))), (TypeError, lambda: seq.selective_scan(**args(dt=p))),
             (ValueError, lambda: seq.causal_conv_step(z(3, 8), z(8, 4), None, z(2, 3, 8))), (ValueError, lambda: seq.causal_conv_step(z(3, 8), z(8, 4), None, z(4, 3, 8), z(2, dtype=torch.int32))),
             (ValueError, lambda: seq.selective_scan_step(z(3, 8), z(3, 8), z(8, 4), z(3, 4), z(3, 4), z(2, 8, 4))),
