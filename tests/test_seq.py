@@ -5,7 +5,7 @@ Tolerances.  A result of type T is rounded once: half a unit, finfo(T).eps / 2 r
 sum of n products is off by at most about (n + 2) eps / 2 of the sum of their magnitudes, the exponentials and reciprocals by a few eps of
 theirs; a recurrence adds each row's share, weighted by decays below one.  So every result is allowed half a unit of its own type of itself
 plus `k` eps of the compute type of the *scale* it was summed at (the same formula with every term's magnitude, computed beside it), with k
-the number of roundings a term meets: see `check`.  The device tests also run on the emulated device (tests/test_seq_emulated.py).
+the number of roundings a term meets: see `check`.  The device tests also run on the emulated device (tests/test_simt_emulation_seq.py).
 """
 import math
 import os
