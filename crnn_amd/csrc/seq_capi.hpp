@@ -67,6 +67,19 @@ struct SeqCheck {
         if (out && v.row_stride < width) return bad(std::string(name) + ": rows of an output overlap");
         return true;
     }
+    // an output's sequences (n of `rows` rows) may lie one behind another or row by row side by side, but not over one another
+    bool apart(const crnn_view &v, const char *name, int64_t n, int64_t rows, int64_t width) {
+        if (!v.ptr || n < 2 || rows < 1 || v.seq_stride >= (rows - 1) * v.row_stride + width) return true;
+        if (v.seq_stride >= width && v.row_stride >= (n - 1) * v.seq_stride + width) return true;
+        return bad(std::string(name) + ": sequences of an output overlap");
+    }
+    // an output is written while other lanes and blocks still read the inputs (arrays that share some rows only are the caller's to avoid)
+    bool other(std::initializer_list<const crnn_view *> outs, std::initializer_list<const crnn_view *> ins, int64_t rows) {
+        for (const crnn_view *y : outs)
+            for (const crnn_view *x : ins)
+                if (rows > 0 && y->ptr && y->ptr == x->ptr) return bad("an output is also an input");
+        return true;
+    }
 };
 
 bool seq_rows_ok(SeqCheck &c, int32_t n_seq, int64_t rows, const int32_t *start, const int32_t *len, int32_t D, int32_t dtype) {
@@ -236,7 +249,8 @@ void scan_backward_run(const crnn_scan_args *a, ScanPlan &s, hipStream_t st) {
     }
 }
 
-bool scan_views(SeqCheck &c, const crnn_scan_args *a, bool backward) {
+// (the arrays of a step have one row a sequence, row_stride apart)
+bool scan_views(SeqCheck &c, const crnn_scan_args *a, bool backward, bool step = false) {
     const int dt = a->dtype;
     const int64_t D = a->D, GN = (int64_t)a->G * a->N;
     if (!a->A) return c.bad("A is missing");
@@ -244,11 +258,15 @@ bool scan_views(SeqCheck &c, const crnn_scan_args *a, bool backward) {
         !c.view(a->B, "B", dt, true, false, false, 0) || !c.view(a->C, "C", dt, true, false, false, 0))
         return false;
     if (a->B_group < 0 || a->B_state < 0 || a->C_group < 0 || a->C_state < 0) return c.bad("negative stride of B or C");
-    if (!backward) return c.view(a->y, "y", dt, true, false, true, D);
+    const int64_t n = a->seq_start || step ? 1 : a->n_seq, rows = a->rows, flat = step ? a->n_seq : seq_flat(a->n_seq, rows, a->seq_start != nullptr);
+    if (!backward)
+        return c.view(a->y, "y", dt, true, false, true, D) && c.apart(a->y, "y", n, rows, D) && c.other({&a->y}, {&a->u, &a->dt, &a->z, &a->B, &a->C}, flat);
     if (!a->dA) return c.bad("dA is missing");
     if ((a->z.ptr != nullptr) != (a->dz.ptr != nullptr)) return c.bad("dz goes with z");
     return c.view(a->dy, "dy", dt, true, false, false, D) && c.view(a->du, "du", dt, true, false, true, D) && c.view(a->ddt, "ddt", dt, true, false, true, D) &&
-           c.view(a->dz, "dz", dt, false, false, true, D) && c.view(a->dB, "dB", dt, true, false, true, GN) && c.view(a->dC, "dC", dt, true, false, true, GN);
+           c.view(a->dz, "dz", dt, false, false, true, D) && c.view(a->dB, "dB", dt, true, false, true, GN) && c.view(a->dC, "dC", dt, true, false, true, GN) &&
+           c.apart(a->du, "du", n, rows, D) && c.apart(a->ddt, "ddt", n, rows, D) && c.apart(a->dz, "dz", n, rows, D) && c.apart(a->dB, "dB", n, rows, GN) &&
+           c.apart(a->dC, "dC", n, rows, GN) && c.other({&a->du, &a->ddt, &a->dz, &a->dB, &a->dC}, {&a->dy, &a->u, &a->dt, &a->z, &a->B, &a->C}, flat);
 }
 
 // the launches' template: MODE 2 (anything: several launches over the states, one of u and z a checkpoint) has 16 states a launch, 8 in double
@@ -283,7 +301,7 @@ int64_t conv_strip(int64_t flat, int32_t D, int V, bool backward) {
     const int64_t lo = backward ? 24 : 8, hi = backward ? 64 : 32;
     return q < lo ? lo : q > hi ? hi : q;
 }
-bool conv_fits(const crnn_view &v, int V) { return !v.ptr || (seq_view(v, V).vec && v.row_stride < 0x7fffffff); }
+bool conv_fits(const crnn_view &v, int V) { return !v.ptr || seq_view(v, V).vec; }
 // which: 0 forward, 1 backward, 2 step
 int conv_channels(const crnn_conv_args *a, int which) {
     const int V = conv_wide(a->dtype, a->W, which == 1);
@@ -305,14 +323,18 @@ bool conv_check(SeqCheck &c, const crnn_conv_args *a, bool backward, crnn::ConvP
 bool conv_views(SeqCheck &c, const crnn_conv_args *a, bool backward, crnn::ConvP &p) {
     const int dt = a->dtype;
     if (!a->weight) return c.bad("weight is missing");
+    const int64_t n = a->seq_start ? 1 : a->n_seq, flat = seq_flat(a->n_seq, a->rows, a->seq_start != nullptr);
     if (!c.view(a->x, "x", dt, true, true, false, a->D) || !c.view(a->state_in, "state_in", dt, false, false, false, a->D)) return false;
     if (backward) {
         if (!a->dweight) return c.bad("dweight is missing");
         if (!c.view(a->dy, "dy", dt, true, false, false, a->D) || !c.view(a->dx, "dx", dt, true, false, true, a->D) ||
-            !c.view(a->dstate_out, "dstate_out", dt, false, false, false, a->D) || !c.view(a->dstate_in, "dstate_in", dt, false, false, true, a->D))
+            !c.view(a->dstate_out, "dstate_out", dt, false, false, false, a->D) || !c.view(a->dstate_in, "dstate_in", dt, false, false, true, a->D) ||
+            !c.apart(a->dx, "dx", n, a->rows, a->D) || !c.apart(a->dstate_in, "dstate_in", a->n_seq, a->W - 1, a->D) || !c.other({&a->dx}, {&a->x, &a->dy}, flat))
             return false;
     } else {
-        if (!c.view(a->y, "y", dt, true, false, true, a->D) || !c.view(a->state_out, "state_out", dt, false, false, true, a->D)) return false;
+        if (!c.view(a->y, "y", dt, true, false, true, a->D) || !c.view(a->state_out, "state_out", dt, false, false, true, a->D) ||
+            !c.apart(a->y, "y", n, a->rows, a->D) || !c.apart(a->state_out, "state_out", a->n_seq, a->W - 1, a->D) || !c.other({&a->y}, {&a->x}, flat))
+            return false;
         if (a->state_out.ptr && a->state_out.ptr == a->state_in.ptr) return c.bad("state_out may not be state_in");
     }
     p.x = seq_view(a->x, 1); p.y = seq_view(a->y, 1); p.dy = seq_view(a->dy, 1); p.dx = seq_view(a->dx, 1);
@@ -429,10 +451,10 @@ int32_t crnn_conv_step(const crnn_conv_args *a) {
         if (a->n_slots < 0 || a->n_slots > 0x7fffffff || (!a->slot && a->n_seq > a->n_slots)) return sfail("crnn_conv_step: n_slots does not fit the rows");
         if (a->n_seq == 0) return 0;
         if (!c.view(a->x, "x", a->dtype, true, false, false, a->D) || !c.view(a->y, "y", a->dtype, true, false, true, a->D) ||
-            !c.view(a->state_in, "state_in", a->dtype, a->W > 1 && a->n_slots > 0, false, true, a->D))
+            !c.view(a->state_in, "state_in", a->dtype, a->W > 1 && a->n_slots > 0, false, true, a->D) || !c.other({&a->y}, {&a->x}, 1) ||
+            !c.apart(a->state_in, "state_in", a->n_slots, a->W - 1, a->D))
             return sfail(c.err);
         if (!a->weight) return sfail("crnn_conv_step: weight is missing");
-        if (a->W > 1 && a->n_slots > 1 && a->state_in.seq_stride < (a->W - 1) * a->state_in.row_stride) return sfail("crnn_conv_step: the states of two slots overlap");
         if (a->n_seq * (int64_t)((a->D + 255) / 256) > kSeqMaxGrid) return sfail("crnn_conv_step: too many rows and channels for one launch");
         SEQ_DEVICE(a->device, "crnn_conv_step");
         crnn::ConvStepP p{};
@@ -501,7 +523,7 @@ int32_t crnn_scan_step(const crnn_scan_args *a) {
         if (a->seq_start || a->seq_len) return sfail("crnn_scan_step: rows are one per sequence (no seq_start, seq_len)");
         if (a->n_slots < 0 || a->n_slots > 0x7fffffff || (!a->slot && a->n_seq > a->n_slots)) return sfail("crnn_scan_step: n_slots does not fit the rows");
         if (a->n_seq == 0) return 0;
-        if (!scan_views(c, a, false)) return sfail(c.err);
+        if (!scan_views(c, a, false, true)) return sfail(c.err);
         if (s.p8) return sfail("crnn_scan_step: u and z cannot be 8-bit checkpoints here");
         if (!a->state_out && a->n_slots > 0) return sfail("crnn_scan_step: the states are missing");
         crnn::ScanStepP p{};

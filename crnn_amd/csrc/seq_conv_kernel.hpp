@@ -3,7 +3,7 @@
 //     p[t, d] = bias[d] + sum_j w[d, j] x[t - W + 1 + j, d],   y = p or p sigmoid(p)
 //
 // x before a sequence's first row is its state (the last W - 1 rows before it), or 0.  Depthwise: a few multiply-adds per element read,
-// bound by memory.  A thread owns V neighbouring channels (16 bytes of them where rows are aligned, else one) and walks down a strip of rows,
+// bound by memory.  A thread owns V neighbouring channels (four, two in double; one where rows are not so aligned) and walks down a strip of rows,
 // kConvTB at a time: the next ones are on their way while these are worked on, the last W rows stay in registers, so that each row is read
 // once but for the W - 1 rows in front of a strip.  Rows behind the last one are read as the last, threads behind the last channels do the
 // last channels once more: loads and stores stand without branches between them, and no wait reaches over a store.

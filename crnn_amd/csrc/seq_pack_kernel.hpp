@@ -2,8 +2,8 @@
 //
 // A row's channels in blocks of 32, one scale 2^e a block (stored e + 127): e = floor(log2 max|x|) - 6, one more where the largest value would
 // round to 128; code = x / 2^e rounded half to even, within +-127.  Scales are powers of two, so that the rounding to a code is the only one:
-// a value comes back within 2^(e - 1), at most max|x| / 128 (the type's largest values, from 127.5 of 128 of its last binade on, within 2^e).  A block that holds an infinity or a NaN, comes back
-// as NaN (scale byte 255).  Reads once, writes 33/32 bytes a value: bound by memory.
+// a value comes back within 2^(e - 1), at most max|x| / 128 (the type's largest values, from 127.5 of 128 of its last binade on, within 2^e).
+// A block that holds an infinity or a NaN comes back as NaN (scale byte 255).  Reads once, writes 33/32 bytes a value: bound by memory.
 #pragma once
 #include "seq_common.hpp"
 

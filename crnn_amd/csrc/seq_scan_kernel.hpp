@@ -11,8 +11,9 @@
 // back as broadcasts) and each wavefront's part of sum_n C h.  Per row, channel and state that is one multiplication and one exponential for
 // the decay and three multiply-adds: bound by the vector units, not by memory.  The gradient needs every state's neighbours in registers and
 // gives a wavefront all states of its tile.
-// Where tiles and sequences do not fill the card, time is cut into chunks: their ends without what came before (seq_scan_ends_kernel), the
-// carry over the chunks of a sequence (seq_scan_carry_kernel: the decay over a chunk is exp(A sum delta)), then the chunks proper.
+// Where tiles and sequences do not fill the card, time is cut into chunks: their ends without what came before (the forward kernel without its
+// outputs, seq_scan_ends2_kernel for the gradient), the carry over the chunks of a sequence (seq_scan_carry_kernel: the decay over a chunk is
+// exp(A sum delta)), then the chunks proper.  Sums over channels and blocks are taken in a fixed order: results do not change from run to run.
 #pragma once
 #include "seq_common.hpp"
 
@@ -47,7 +48,6 @@ struct ScanMapsP {
     int64_t srows;          // dense: rows of a sequence (0: packed)
     int32_t G, N, n0;
 };
-// the place of a wavefront: chunk block, channel tile, channel of the lane
 // the plane of state n of chunk block b in an [block][state][D] array: uniform, the lane adds its channel
 template <int NS, class T>
 __device__ __forceinline__ T *scan_plane(T *x, int64_t b, int n, int D) { return x + (b * NS + n) * D; }
@@ -58,6 +58,7 @@ struct ScanAt {
     int32_t tile, g, d;
     bool on, valid;         // on: the wavefront has a tile; valid: the lane has a channel
 };
+// the place of a wavefront of the gradient's kernels: chunk block, channel tile, channel of the lane
 __device__ __forceinline__ ScanAt scan_at(const ScanP &p) {
     ScanAt a;
     const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)), lane = threadIdx.x & 63;

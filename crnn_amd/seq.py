@@ -194,11 +194,14 @@ class _Rows:
     def new(self, shape, dtype):
         return _t.empty(shape, dtype=dtype, device=self.device)
 
-    def out(self, given, shape):
+    def out(self, given, shape, *inputs):
+        """The result's array.  inputs: arrays of which other rows, or other lanes of the same row, are read after a row of the result is written."""
         if given is None:
             return _t.empty(shape, dtype=self.dtype, device=self.device)
         if given.shape != shape or given.dtype != self.dtype or given.device != self.device or given.stride(-1) != 1 and self.D > 1:
             raise ValueError(f"out must be {tuple(shape)} {self.dtype} on {self.device} with contiguous channels")
+        if given.numel() and any(x is not None and (x.codes if x.__class__ is Packed8 else x).data_ptr() == given.data_ptr() for x in inputs):
+            raise ValueError("out may not be an input")
         return given
 
 
@@ -257,9 +260,7 @@ def causal_conv(x, weight, bias=None, *, silu=False, seq_start=None, lengths=Non
     W = _taps(weight)
     D, shape = r.D, (r.n_seq, W - 1, r.D)
     weight, bias, state = r.weight(weight, "weight", (D, W)), r.weight(bias, "bias", (D,)), r.state(state, "state", shape, r.dtype)
-    y = r.out(out, r.shape)
-    if out is not None and out.data_ptr() == (x.codes if x.__class__ is Packed8 else x).data_ptr() and out.numel():
-        raise ValueError("out may not be x: a row's result needs the rows before it")
+    y = r.out(out, r.shape, x)
     end = r.new(shape, r.dtype) if return_state else None
     if r.n_seq == 0:
         return _none(y, out, end)
@@ -309,7 +310,7 @@ def causal_conv_step(x, weight, bias, state, slots=None, *, silu=False, out=None
     if state.ndim != 3 or state.shape[1:] != (W - 1, D) or state.dtype != r.dtype or state.device != r.device or (D > 1 and W > 1 and state.stride(2) != 1):
         raise ValueError(f"state must be [n_slots, {W - 1}, {D}] {r.dtype} on {r.device} with contiguous channels")
     slot = _slots(r, slots, n, state.shape[0])
-    x, y = _channels(x), r.out(out, x.shape)
+    x, y = _channels(x), r.out(out, x.shape, x, state)
     a = _conv_args(r, W, silu, 1, 0, weight, bias, _view(x), _view(y), _view(state) if W > 1 else _ABSENT, _ABSENT, slot=slot, n_slots=state.shape[0], n_seq=n)
     if lib.crnn_conv_step(a):
         check(-1)
@@ -361,7 +362,7 @@ def selective_scan(u, dt, A, B, C_, *, D=None, z=None, dt_bias=None, softplus=Tr
     N, G, A, D, dt_bias, maps = _scan_params(r, A, B, C_, D, dt_bias, r.shape[:-1])
     shape = (r.n_seq, r.D, N)
     state = r.state(state, "state", shape, r.param)
-    y = r.out(out, r.shape)
+    y = r.out(out, r.shape, u, dt, z, B, C_)
     end = r.new(shape, r.param) if return_state else None
     if r.n_seq == 0:
         return _none(y, out, end)
@@ -427,7 +428,7 @@ def selective_scan_step(u, dt, A, B, C_, state, slots=None, *, D=None, z=None, d
     if state.ndim != 3 or state.shape[1:] != (r.D, N) or state.dtype != r.param or state.device != r.device or not state.is_contiguous():
         raise ValueError(f"state must be a contiguous [n_slots, {r.D}, {N}] {r.param} on {r.device}")
     slot = _slots(r, slots, n, state.shape[0])
-    y = r.out(out, dt.shape)
+    y = r.out(out, dt.shape, u, dt, z, B, C_, state)
     a = _scan_args(r, N, G, 1, 0, softplus, A, D, dt_bias, _view(u), _view(dt), _view(z), _view(y), maps, 0, state.data_ptr(), slot=slot, n_slots=state.shape[0], n_seq=n)
     if lib.crnn_scan_step(a):
         check(-1)

@@ -864,7 +864,10 @@ def test_other_refusals():
     p = seq.pack8(z(2, 6, 8))
     for err, call in [
             (ValueError, lambda: seq.causal_conv(z(2, 6, 8), z(8, 9))), (ValueError, lambda: seq.causal_conv(z(2, 6, 8), z(7, 4))), (ValueError, lambda: seq.causal_conv(z(6, 8), z(8, 4))),
-            (ValueError, lambda: seq.causal_conv(z(2, 6, 8), z(8, 4), state=z(2, 4, 8))), (ValueError, lambda: (lambda x: seq.causal_conv(x, z(8, 4), out=x))(z(2, 6, 8))), (ValueError, lambda: seq.causal_conv_grad(z(2, 6, 7), z(2, 6, 8), z(8, 4))),
+            (ValueError, lambda: seq.causal_conv(z(2, 6, 8), z(8, 4), state=z(2, 4, 8))), (ValueError, lambda: (lambda x: seq.causal_conv(x, z(8, 4), out=x))(z(2, 6, 8))),
+            (ValueError, lambda: (lambda x: seq.causal_conv_step(x, z(8, 4), None, z(2, 3, 8), out=x))(z(2, 8))), (RuntimeError, lambda: seq.causal_conv(z(2, 6, 8), z(8, 4), out=z(1, 6, 8).expand(2, 6, 8))),
+            (ValueError, lambda: (lambda x: seq.selective_scan(z(2, 6, 8), x, z(8, 4), z(2, 6, 4), z(2, 6, 4), out=x))(z(2, 6, 8))),
+            (ValueError, lambda: (lambda x: seq.selective_scan_step(x, z(2, 8), z(8, 4), z(2, 4), z(2, 4), z(2, 8, 4), out=x))(z(2, 8))), (ValueError, lambda: seq.causal_conv_grad(z(2, 6, 7), z(2, 6, 8), z(8, 4))),
             (TypeError, lambda: seq.causal_conv_grad(p, z(2, 6, 8), z(8, 4))), (TypeError, lambda: seq.selective_scan(**args(dt=p))),
             (ValueError, lambda: seq.causal_conv_step(z(3, 8), z(8, 4), None, z(2, 3, 8))), (ValueError, lambda: seq.causal_conv_step(z(3, 8), z(8, 4), None, z(4, 3, 8), z(2, dtype=torch.int32))),
             (ValueError, lambda: seq.selective_scan_step(z(3, 8), z(3, 8), z(8, 4), z(3, 4), z(3, 4), z(2, 8, 4))),
@@ -891,18 +894,19 @@ def test_c_entry_points_refuse_before_any_launch():
     lib = L.lib
     said = lambda: lib.crnn_last_error(None).decode()  # noqa: E731
 
-    def view(dt=L.DT_F32, rs=8, ptr=4096):
-        return L.View(ptr=ptr, row_stride=rs, seq_stride=48, dtype=dt)
+    def view(dt=L.DT_F32, rs=8, ptr=4096, ss=8192):
+        return L.View(ptr=ptr, row_stride=rs, seq_stride=ss, dtype=dt)
 
     def scan(**over):
-        a = L.ScanArgs(struct_size=C.sizeof(L.ScanArgs), device=99, n_seq=2, D=8, N=4, G=1, rows=6, A=4096, u=view(), dt=view(), y=view(), B=view(rs=4), C=view(rs=4))
+        a = L.ScanArgs(struct_size=C.sizeof(L.ScanArgs), device=99, n_seq=2, D=8, N=4, G=1, rows=6, A=4096, u=view(), dt=view(), y=view(ptr=64), B=view(rs=4), C=view(rs=4))
         for k, v in over.items():
             setattr(a, k, v)
         return a
 
     for over, word in [(dict(struct_size=8), "struct_size"), (dict(N=0), "N must"), (dict(N=257), "N must"), (dict(G=3), "divide"), (dict(rows=-1), "negative"), (dict(rows=1 << 31), "rows"),
                        (dict(D=0), "D must"), (dict(A=None), "A is missing"), (dict(u=view(ptr=None)), "u is missing"), (dict(u=view(L.DT_BF16)), "element type"),
-                       (dict(u=view(L.DT_PACKED8)), "scales"), (dict(dt=view(L.DT_PACKED8)), "checkpoint"), (dict(y=view(rs=7)), "overlap"), (dict(dtype=9), "element type"),
+                       (dict(u=view(L.DT_PACKED8)), "scales"), (dict(dt=view(L.DT_PACKED8)), "checkpoint"), (dict(y=view(rs=7)), "overlap"), (dict(y=view(ptr=64, ss=47)), "sequences of an output overlap"),
+                       (dict(y=view(ptr=64, rs=15, ss=8)), "sequences of an output overlap"), (dict(y=view(ptr=64, rs=16, ss=8)), "device"), (dict(y=view()), "also an input"), (dict(dtype=9), "element type"),
                        (dict(seq_start=64, seq_len=64), "exclude"), (dict(rows=600), "workspace"), ({}, "device")]:
         assert lib.crnn_scan_forward(C.byref(scan(**over))) == -1 and word in said(), (over, said())
     assert lib.crnn_scan_forward(None) == -1 and "null" in said()
@@ -911,15 +915,18 @@ def test_c_entry_points_refuse_before_any_launch():
     assert lib.crnn_scan_step(C.byref(scan(n_slots=1))) == -1 and "n_slots" in said()
 
     def conv(**over):
-        a = L.ConvArgs(struct_size=C.sizeof(L.ConvArgs), device=99, n_seq=2, D=8, W=4, rows=6, weight=4096, x=view(), y=view())
+        a = L.ConvArgs(struct_size=C.sizeof(L.ConvArgs), device=99, n_seq=2, D=8, W=4, rows=6, weight=4096, x=view(), y=view(ptr=64))
         for k, v in over.items():
             setattr(a, k, v)
         return a
 
     for over, word in [(dict(struct_size=0), "struct_size"), (dict(W=0), "W must"), (dict(W=9), "W must"), (dict(weight=None), "weight"), (dict(x=view(ptr=None)), "x is missing"),
-                       (dict(y=view(rs=4)), "overlap"), (dict(state_in=view(), state_out=view()), "state_out")]:
+                       (dict(y=view(rs=4)), "overlap"), (dict(state_in=view(), state_out=view()), "state_out"), (dict(y=view()), "also an input"), (dict(y=view(ptr=64, ss=0)), "sequences"),
+                       (dict(state_out=view(ptr=64, ss=23)), "sequences"), ({}, "device")]:
         assert lib.crnn_conv_forward(C.byref(conv(**over))) == -1 and word in said(), (over, said())
-    assert lib.crnn_conv_backward(C.byref(conv(dx=view(), dy=view(), dweight=64))) == -1 and "workspace" in said()
+    assert lib.crnn_conv_backward(C.byref(conv(dx=view(ptr=64), dy=view(), dweight=64))) == -1 and "workspace" in said()
+    assert lib.crnn_conv_backward(C.byref(conv(dx=view(), dy=view(), dweight=64))) == -1 and "also an input" in said()
+    assert lib.crnn_scan_backward(C.byref(scan(dA=64, dy=view(), du=view(ptr=64), ddt=view(), dB=view(rs=4, ptr=64), dC=view(rs=4, ptr=64)))) == -1 and "also an input" in said()
     assert lib.crnn_conv_step(C.byref(conv(n_slots=1))) == -1 and "n_slots" in said()
     v = view(L.DT_F64)
     assert lib.crnn_pack8(99, None, C.byref(v), 2, 8, 4096, 4096) == -1 and "half" in said()
