@@ -18,15 +18,14 @@ struct SeqDevice {
     int prev = -1;
     bool moved = false;
     hipError_t enter(int device) {
+        hipError_t e = hipGetDevice(&prev);
+        if (e != hipSuccess || prev == device) return e;
         int n = 0;
-        hipError_t e = hipGetDeviceCount(&n);
+        e = hipGetDeviceCount(&n);
         if (e != hipSuccess) return e;
         if (device < 0 || device >= n) return hipErrorInvalidValue;
-        e = hipGetDevice(&prev);
-        if (e == hipSuccess && prev != device) {
-            e = hipSetDevice(device);
-            moved = e == hipSuccess;
-        }
+        e = hipSetDevice(device);
+        moved = e == hipSuccess;
         return e;
     }
     ~SeqDevice() {

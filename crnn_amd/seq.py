@@ -33,12 +33,15 @@ _EMULATED = "SIMT-EMULATION" in lib.crnn_build_info().decode()     # the emulate
 _t = None          # torch, imported by the first call
 _DT = {}           # torch's types: ours
 _raw_stream = None
+_like = None       # a contiguous tensor of another's shape (and type): half the host time of torch.empty with a shape, a type and a device
 
 
 def _torch():
-    global _t, _raw_stream
+    global _t, _raw_stream, _like
     if _t is None:
         import torch
+        from functools import partial
+        _like = partial(torch.empty_like, memory_format=torch.contiguous_format)
         _DT.update({torch.float32: L.DT_F32, torch.bfloat16: L.DT_BF16, torch.float16: L.DT_F16, torch.float64: L.DT_F64})
         _t = torch
         _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda i: torch.cuda.current_stream(i).cuda_stream)
@@ -46,7 +49,8 @@ def _torch():
 
 
 def _packer(cls):
-    """The struct as one format string: a call fills its arguments with a single pack (the fields one by one take longer than the launch)."""
+    """The struct as one format string: a call fills its arguments with a single pack (the fields one by one take longer than the launch), and
+    passes the bytes as they are."""
     codes = {C.c_int32: "i", C.c_int64: "q", C.c_void_p: "P"}
 
     def fmt(c):
@@ -59,6 +63,18 @@ def _packer(cls):
 
 
 _pack_conv, _pack_scan, _pack_view = _packer(ConvArgs), _packer(ScanArgs), _packer(View)
+
+
+def _entry(name, at):
+    """An entry point that takes its struct (argument `at`) as bytes."""
+    f, known = lib[name], getattr(lib, name)
+    f.restype, f.argtypes = known.restype, [C.c_char_p if i == at else t for i, t in enumerate(known.argtypes)]
+    return f
+
+
+_conv_workspace, _conv_forward, _conv_backward, _conv_step = (_entry(f"crnn_conv_{k}", 0) for k in ("workspace", "forward", "backward", "step"))
+_scan_workspace, _scan_forward, _scan_backward, _scan_step = (_entry(f"crnn_scan_{k}", 0) for k in ("workspace", "forward", "backward", "step"))
+_pack, _unpack = _entry("crnn_pack8", 2), _entry("crnn_unpack8", 6)
 _CONV_SIZE, _SCAN_SIZE = C.sizeof(ConvArgs), C.sizeof(ScanArgs)
 _ABSENT = (0,) * 8
 # a pointer for arrays without elements: "absent" and "empty" differ
@@ -178,9 +194,10 @@ class _Rows:
         """A parameter in the type parameters have here."""
         if x is None:
             return None
-        if x.shape != shape or x.device != self.device or not x.dtype.is_floating_point:
+        given = x.dtype is self.param
+        if x.shape != shape or x.device != self.device or not (given or x.dtype.is_floating_point):
             raise ValueError(f"{name} must be {shape} on {self.device}, not {tuple(x.shape)} {x.dtype} on {x.device}")
-        if x.dtype != self.param:
+        if not given:
             x = x.to(self.param)
         return x if x.is_contiguous() else x.contiguous()
 
@@ -197,7 +214,8 @@ class _Rows:
     def out(self, given, shape, *inputs):
         """The result's array.  inputs: arrays of which other rows, or other lanes of the same row, are read after a row of the result is written."""
         if given is None:
-            return _t.empty(shape, dtype=self.dtype, device=self.device)
+            x = inputs[0]
+            return _like(x) if x.__class__ is not Packed8 else _t.empty(shape, dtype=self.dtype, device=self.device)
         if given.shape != shape or given.dtype != self.dtype or given.device != self.device or given.stride(-1) != 1 and self.D > 1:
             raise ValueError(f"out must be {tuple(shape)} {self.dtype} on {self.device} with contiguous channels")
         if given.numel() and any(x is not None and (x.codes if x.__class__ is Packed8 else x).data_ptr() == given.data_ptr() for x in inputs):
@@ -247,9 +265,9 @@ def _taps(weight):
 
 def _conv_args(r, W, silu, rows, zero, weight, bias, x, y, state_in, state_out, dy=_ABSENT, dx=_ABSENT, dstate_out=_ABSENT, dstate_in=_ABSENT, dweight=0, dbias=0, slot=0,
                n_slots=0, ws=0, ws_bytes=0, n_seq=None):
-    return ConvArgs.from_buffer_copy(_pack_conv(
+    return _pack_conv(
         _CONV_SIZE, r.ordinal, r.stream, r.n_seq if n_seq is None else n_seq, r.D, W, 1 if silu else 0, rows, r.start, r.len, r.code, zero, _ptr(weight), _ptr(bias), *x, *y,
-        *state_in, *state_out, *dy, *dx, *dstate_out, *dstate_in, dweight, dbias, slot, n_slots, ws, ws_bytes))
+        *state_in, *state_out, *dy, *dx, *dstate_out, *dstate_in, dweight, dbias, slot, n_slots, ws, ws_bytes)
 
 
 def causal_conv(x, weight, bias=None, *, silu=False, seq_start=None, lengths=None, state=None, return_state=False, out=None):
@@ -261,11 +279,11 @@ def causal_conv(x, weight, bias=None, *, silu=False, seq_start=None, lengths=Non
     D, shape = r.D, (r.n_seq, W - 1, r.D)
     weight, bias, state = r.weight(weight, "weight", (D, W)), r.weight(bias, "bias", (D,)), r.state(state, "state", shape, r.dtype)
     y = r.out(out, r.shape, x)
-    end = r.new(shape, r.dtype) if return_state else None
+    end = (r.new(shape, r.dtype) if state is None else _like(state)) if return_state else None
     if r.n_seq == 0:
         return _none(y, out, end)
     a = _conv_args(r, W, silu, r.rows, r.ragged if out is None else 0, weight, bias, _view(x), _view(y), _view(state) if W > 1 else _ABSENT, _view(end) if W > 1 else _ABSENT)
-    if lib.crnn_conv_forward(a):
+    if _conv_forward(a):
         check(-1)
     return (y, end) if return_state else y
 
@@ -279,9 +297,8 @@ def causal_conv_grad(dy, x, weight, bias=None, *, silu=False, seq_start=None, le
     D, shape = r.D, (r.n_seq, W - 1, r.D)
     weight, bias = r.weight(weight, "weight", (D, W)), r.weight(bias, "bias", (D,))
     state, dstate = r.state(state, "state", shape, r.dtype), r.state(dstate, "dstate", shape, r.dtype)
-    dx, dw = r.out(None, r.shape), r.new((D, W), r.param)
-    db = None if bias is None else r.new((D,), r.param)
-    ds = None if state is None else r.new(shape, r.dtype)
+    dx, dw = _like(dy), _like(weight)
+    db, ds = None if bias is None else _like(bias), None if state is None else _like(state)
     if r.n_seq == 0:
         return ConvGrads(dx.zero_(), dw.zero_(), None if db is None else db.zero_(), ds)
 
@@ -290,9 +307,9 @@ def causal_conv_grad(dy, x, weight, bias=None, *, silu=False, seq_start=None, le
         return _conv_args(r, W, silu, r.rows, r.ragged, weight, bias, _view(x), _ABSENT, v(state), _ABSENT, _view(dy), _view(dx), v(dstate), v(ds), dw.data_ptr(), _ptr(db), 0, 0,
                           ws, need)
 
-    need = _workspace(("conv", r.n_seq, r.rows, r.packed, D, W, r.code), lambda: lib.crnn_conv_workspace(args()))
+    need = _workspace(("conv", r.n_seq, r.rows, r.packed, D, W, r.code), lambda: _conv_workspace(args()))
     ws = r.new(max(need, 1), _t.uint8)
-    if lib.crnn_conv_backward(args(ws.data_ptr(), need)):
+    if _conv_backward(args(ws.data_ptr(), need)):
         check(-1)
     return ConvGrads(dx, dw, db, ds)
 
@@ -312,7 +329,7 @@ def causal_conv_step(x, weight, bias, state, slots=None, *, silu=False, out=None
     slot = _slots(r, slots, n, state.shape[0])
     x, y = _channels(x), r.out(out, x.shape, x, state)
     a = _conv_args(r, W, silu, 1, 0, weight, bias, _view(x), _view(y), _view(state) if W > 1 else _ABSENT, _ABSENT, slot=slot, n_slots=state.shape[0], n_seq=n)
-    if lib.crnn_conv_step(a):
+    if _conv_step(a):
         check(-1)
     return y
 
@@ -348,9 +365,9 @@ def _scan_params(r, A, B, C_, D, dt_bias, lead):
 
 def _scan_args(r, N, G, rows, zero, softplus, A, D, dt_bias, u, dt, z, y, maps, state_in, state_out, grads=_ABSENT * 6 + (0,) * 3, dstate_out=0, dstate_in=0, slot=0, n_slots=0,
                ws=0, ws_bytes=0, n_seq=None):
-    return ScanArgs.from_buffer_copy(_pack_scan(
+    return _pack_scan(
         _SCAN_SIZE, r.ordinal, r.stream, r.n_seq if n_seq is None else n_seq, r.D, N, G, rows, r.start, r.len, r.code, zero, 1 if softplus else 0, 0, _ptr(A), _ptr(D), _ptr(dt_bias),
-        *u, *dt, *z, *y, *maps, state_in, state_out, *grads, dstate_out, dstate_in, slot, n_slots, ws, ws_bytes))
+        *u, *dt, *z, *y, *maps, state_in, state_out, *grads, dstate_out, dstate_in, slot, n_slots, ws, ws_bytes)
 
 
 def selective_scan(u, dt, A, B, C_, *, D=None, z=None, dt_bias=None, softplus=True, seq_start=None, lengths=None, state=None, return_state=False, out=None):
@@ -362,8 +379,8 @@ def selective_scan(u, dt, A, B, C_, *, D=None, z=None, dt_bias=None, softplus=Tr
     N, G, A, D, dt_bias, maps = _scan_params(r, A, B, C_, D, dt_bias, r.shape[:-1])
     shape = (r.n_seq, r.D, N)
     state = r.state(state, "state", shape, r.param)
-    y = r.out(out, r.shape, u, dt, z, B, C_)
-    end = r.new(shape, r.param) if return_state else None
+    y = r.out(out, r.shape, dt, u, z, B, C_)
+    end = (r.new(shape, r.param) if state is None else _like(state)) if return_state else None
     if r.n_seq == 0:
         return _none(y, out, end)
 
@@ -372,9 +389,9 @@ def selective_scan(u, dt, A, B, C_, *, D=None, z=None, dt_bias=None, softplus=Tr
                           ws_bytes=need)
 
     need = _workspace((0, r.n_seq, r.rows, r.packed, r.D, N, G, r.code, u.__class__ is Packed8, z is None or z.__class__ is Packed8, z is None),
-                      lambda: lib.crnn_scan_workspace(args(), 0))
+                      lambda: _scan_workspace(args(), 0))
     ws = r.new(need, _t.uint8) if need else None
-    if lib.crnn_scan_forward(args(_ptr(ws), need)):
+    if _scan_forward(args(_ptr(ws), need)):
         check(-1)
     return (y, end) if return_state else y
 
@@ -387,10 +404,8 @@ def selective_scan_grad(dy, u, dt, A, B, C_, *, D=None, z=None, dt_bias=None, so
     N, G, A, D, dt_bias, maps = _scan_params(r, A, B, C_, D, dt_bias, r.shape[:-1])
     shape = (r.n_seq, r.D, N)
     state, dstate = r.state(state, "state", shape, r.param), r.state(dstate, "dstate", shape, r.param)
-    du, ddt, dz = r.out(None, r.shape), r.out(None, r.shape), None if z is None else r.out(None, r.shape)
-    dB, dC, dA = r.new(B.shape, r.dtype), r.new(C_.shape, r.dtype), r.new((r.D, N), r.param)
-    dD, db = None if D is None else r.new((r.D,), r.param), None if dt_bias is None else r.new((r.D,), r.param)
-    ds = None if state is None else r.new(shape, r.param)
+    du, ddt, dz, dB, dC, dA = _like(dt), _like(dt), None if z is None else _like(dt), _like(B), _like(C_), _like(A)
+    dD, db, ds = None if D is None else _like(D), None if dt_bias is None else _like(dt_bias), None if state is None else _like(state)
     if r.n_seq == 0:
         for x in (du, ddt, dz, dB, dC, dA, dD, db):
             if x is not None:
@@ -404,9 +419,9 @@ def selective_scan_grad(dy, u, dt, A, B, C_, *, D=None, z=None, dt_bias=None, so
                           ws_bytes=need)
 
     need = _workspace((1, r.n_seq, r.rows, r.packed, r.D, N, G, r.code, u.__class__ is Packed8, z is None or z.__class__ is Packed8, z is None),
-                      lambda: lib.crnn_scan_workspace(args(), 1))
+                      lambda: _scan_workspace(args(), 1))
     ws = r.new(max(need, 1), _t.uint8)
-    if lib.crnn_scan_backward(args(ws.data_ptr(), need)):
+    if _scan_backward(args(ws.data_ptr(), need)):
         check(-1)
     return ScanGrads(du, ddt, dA, dB, dC, dD, dz, db, ds)
 
@@ -415,22 +430,15 @@ def selective_scan_step(u, dt, A, B, C_, state, slots=None, *, D=None, z=None, d
     """One more row for each of many running sequences: u, dt, z [n, D], B, C [n, G, N] or [n, N], state [n_slots, D, N] updated in place; slots as
     in causal_conv_step.  Returns y [n, D]."""
     r = _Rows(dt, "dt", step=True)
-    for x, name in ((u, "u"), (z, "z")):
-        if x is None:
-            continue
-        if x.__class__ is Packed8:
-            raise TypeError(f"{name} cannot be an 8-bit checkpoint here")
-        if x.shape != dt.shape or x.dtype != dt.dtype or x.device != dt.device:
-            raise ValueError(f"{name} must be {tuple(dt.shape)} {dt.dtype} on {dt.device}, not {tuple(x.shape)} {x.dtype} on {x.device}")
     n = r.n_seq
-    u, dt, z = _channels(u), _channels(dt), None if z is None else _channels(z)
+    u, dt, z = r.like(u, "u"), _channels(dt), None if z is None else r.like(z, "z")
     N, G, A, D, dt_bias, maps = _scan_params(r, A, B, C_, D, dt_bias, (n,))
     if state.ndim != 3 or state.shape[1:] != (r.D, N) or state.dtype != r.param or state.device != r.device or not state.is_contiguous():
         raise ValueError(f"state must be a contiguous [n_slots, {r.D}, {N}] {r.param} on {r.device}")
     slot = _slots(r, slots, n, state.shape[0])
-    y = r.out(out, dt.shape, u, dt, z, B, C_, state)
+    y = r.out(out, dt.shape, dt, u, z, B, C_, state)
     a = _scan_args(r, N, G, 1, 0, softplus, A, D, dt_bias, _view(u), _view(dt), _view(z), _view(y), maps, 0, state.data_ptr(), slot=slot, n_slots=state.shape[0], n_seq=n)
-    if lib.crnn_scan_step(a):
+    if _scan_step(a):
         check(-1)
     return y
 
@@ -447,27 +455,27 @@ def pack8(x):
     dev, ordinal, stream = _on_device(x, "x")
     shape, D = x.shape, x.shape[-1]
     p = Packed8.__new__(Packed8)
-    p.codes, p.dtype = t.empty(shape, dtype=t.int8, device=dev), x.dtype
+    p.codes, p.dtype = _like(x, dtype=t.int8), x.dtype
     p.scales = t.empty((*shape[:-1], -(-D // 32)), dtype=t.uint8, device=dev)
     flat = _channels(x if x.ndim == 2 else x.reshape(p.codes.numel() // D, D))
-    if lib.crnn_pack8(ordinal, stream, View.from_buffer_copy(_pack_view(*_view(flat))), flat.shape[0], D, p.codes.data_ptr(), p.scales.data_ptr()):
+    if _pack(ordinal, stream, _pack_view(*_view(flat)), flat.shape[0], D, p.codes.data_ptr(), p.scales.data_ptr()):
         check(-1)
     return p
 
 
 def unpack8(p, *, dtype=None, out=None):
     """The values a checkpoint holds, in its own type or in `dtype`, rounded once."""
-    t = _torch()
+    _torch()
     dev, ordinal, stream = _on_device(p, "codes")
     if dtype is None:
         dtype = p.dtype if out is None else out.dtype
     if _DT.get(dtype) not in (L.DT_F32, L.DT_BF16, L.DT_F16):
         raise TypeError(f"unpack8: float32, bfloat16 or float16, not {dtype}")
-    y = t.empty(p.shape, dtype=dtype, device=dev) if out is None else out
+    y = _like(p.codes, dtype=dtype) if out is None else out
     if y.shape != p.shape or y.dtype != dtype or y.device != dev or not y.is_contiguous():
         raise ValueError(f"out must be a contiguous {tuple(p.shape)} {dtype} on {dev}")
     D = p.shape[-1]
     v = (y.data_ptr() or _NOTHING, 0, 0, D, 0, 0, _DT[dtype], 0)
-    if lib.crnn_unpack8(ordinal, stream, p.codes.data_ptr(), p.scales.data_ptr(), y.numel() // D, D, View.from_buffer_copy(_pack_view(*v))):
+    if _unpack(ordinal, stream, p.codes.data_ptr(), p.scales.data_ptr(), y.numel() // D, D, _pack_view(*v)):
         check(-1)
     return y
