@@ -191,6 +191,7 @@ void scan_fill(const crnn_scan_args *a, ScanPlan &s) {
     p.state_in = a->state_in; p.state_out = a->state_out; p.dstate_out = a->dstate_out; p.dstate_in = a->dstate_in;
     p.softplus = a->softplus; p.zero_outside = a->zero_outside;
     p.acc_n = s.flat;
+    p.nvec = a->N % 4 == 0 && (uintptr_t)a->A % 16 == 0 && (uintptr_t)a->state_in % 16 == 0;
 }
 crnn::ScanMapsP scan_maps(const crnn_scan_args *a, const ScanPlan &s, const crnn_view &B, const crnn_view &C, int64_t Bg, int64_t Bn, int64_t Cg, int64_t Cn) {
     crnn::ScanMapsP m{};
@@ -301,10 +302,13 @@ int64_t conv_strip(int64_t flat, int32_t D, int V, bool backward) {
     return q < lo ? lo : q > hi ? hi : q;
 }
 bool conv_fits(const crnn_view &v, int V) { return !v.ptr || seq_view(v, V).vec; }
-// which: 0 forward, 1 backward, 2 step
-int conv_channels(const crnn_conv_args *a, int which) {
-    const int V = conv_wide(a->dtype, a->W, which == 1);
-    const bool fits = a->D % V == 0 && conv_fits(a->x, V) && conv_fits(a->y, V) && conv_fits(a->state_in, V) && conv_fits(a->state_out, V) && conv_fits(a->dy, V) &&
+bool conv_weights_fit(const crnn_conv_args *a, int V) {
+    const uintptr_t b = (uintptr_t)V * (a->dtype == CRNN_DT_F64 ? 8 : 4);
+    return (uintptr_t)a->weight % b == 0 && (uintptr_t)a->bias % b == 0;
+}
+int conv_channels(const crnn_conv_args *a, bool backward) {
+    const int V = conv_wide(a->dtype, a->W, backward);
+    const bool fits = a->D % V == 0 && conv_weights_fit(a, V) && conv_fits(a->x, V) && conv_fits(a->y, V) && conv_fits(a->state_in, V) && conv_fits(a->state_out, V) && conv_fits(a->dy, V) &&
                       conv_fits(a->dx, V) && conv_fits(a->dstate_out, V) && conv_fits(a->dstate_in, V);
     return fits ? V : 1;
 }
@@ -409,7 +413,7 @@ int32_t crnn_conv_forward(const crnn_conv_args *a) {
         if (a->n_seq == 0) return 0;
         if (!conv_views(c, a, false, p)) return sfail(c.err);
         SEQ_DEVICE(a->device, "crnn_conv_forward");
-        conv_launch_t(p, a->dtype, conv_channels(a, 0), false, (hipStream_t)a->stream);
+        conv_launch_t(p, a->dtype, conv_channels(a, false), false, (hipStream_t)a->stream);
         SEQ_DONE("crnn_conv_forward");
     } catch (...) { return -1; }
 }
@@ -427,7 +431,7 @@ int32_t crnn_conv_backward(const crnn_conv_args *a) {
         SEQ_DEVICE(a->device, "crnn_conv_backward");
         p.part = a->workspace;
         const hipStream_t st = (hipStream_t)a->stream;
-        conv_launch_t(p, a->dtype, conv_channels(a, 1), true, st);
+        conv_launch_t(p, a->dtype, conv_channels(a, true), true, st);
         const int64_t count = (int64_t)(a->W + 1) * a->D;       // [tap][D], then the bias
         const dim3 grid((unsigned)((count + 31) / 32));
         if (f64)
@@ -462,7 +466,7 @@ int32_t crnn_conv_step(const crnn_conv_args *a) {
         p.D = a->D; p.W = a->W; p.silu = a->silu;
         const hipStream_t st = (hipStream_t)a->stream;
         const int VW = a->dtype == CRNN_DT_F64 ? 2 : 4;
-        const int V = a->D % VW == 0 && conv_fits(a->x, VW) && conv_fits(a->y, VW) && conv_fits(a->state_in, VW) ? VW : 1;
+        const int V = a->D % VW == 0 && conv_weights_fit(a, VW) && conv_fits(a->x, VW) && conv_fits(a->y, VW) && conv_fits(a->state_in, VW) ? VW : 1;
         if (a->dtype == CRNN_DT_F64) conv_step_launch_w<CRNN_DT_F64>(p, V, st);
         else if (a->dtype == CRNN_DT_F32) conv_step_launch_w<CRNN_DT_F32>(p, V, st);
         else if (a->dtype == CRNN_DT_BF16) conv_step_launch_w<CRNN_DT_BF16>(p, V, st);

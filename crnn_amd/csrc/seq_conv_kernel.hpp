@@ -96,18 +96,34 @@ __device__ __forceinline__ void conv_put(void *row, uint32_t d, const typename S
     else *(uint16_t *)q = (uint16_t)r.w[0];
 }
 
-// weights of a thread's channels, right-aligned in WM taps (tap WM - 1 is the row itself)
-template <class CT, int WM, int V>
-__device__ __forceinline__ void conv_weights(const void *pw, const void *pb, int W, int d, CT (&w)[WM][V], CT (&bias)[V]) {
+// Weights of a thread's channels, right-aligned in WM taps (tap WM - 1 is the row itself).  The V W weights of a thread stand together: read V at a
+// time (one at a time, 4 W bytes between the lanes, they took as long as 32 rows).
+template <int W, class CT, int WM, int V>
+__device__ __forceinline__ void conv_weights_of(const CT *pw, CT (&w)[WM][V]) {
+    typedef CT VV __attribute__((ext_vector_type(V)));
+    VV f[W];
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
-        bias[i] = pb ? ((const CT *)pb)[d + i] : CT(0);
+    for (int k = 0; k < W; ++k) f[k] = ((const VV *)pw)[k];
+#pragma unroll
+    for (int i = 0; i < V; ++i)
 #pragma unroll
         for (int j = 0; j < WM; ++j) {
-            const int k = j - (WM - W);
-            w[j][i] = k >= 0 ? ((const CT *)pw)[(int64_t)(d + i) * W + k] : CT(0);
+            const int e = i * W + j - (WM - W);
+            w[j][i] = j >= WM - W ? f[(j >= WM - W ? e : 0) / V][(j >= WM - W ? e : 0) % V] : CT(0);
         }
-    }
+}
+template <class CT, int WM, int V>
+__device__ __forceinline__ void conv_weights(const void *pw, const void *pb, int W, int d, CT (&w)[WM][V], CT (&bias)[V]) {
+    typedef CT VV __attribute__((ext_vector_type(V)));
+    const CT *q = (const CT *)pw + (int64_t)d * W;
+    const VV b = pb ? *(const VV *)((const CT *)pb + d) : VV(CT(0));
+#pragma unroll
+    for (int i = 0; i < V; ++i) bias[i] = b[i];
+    constexpr int L = WM - 4;       // WM is 4 (1 .. 4 taps) or 8 (5 .. 8)
+    if (W == L + 4) conv_weights_of<L + 4>(q, w);
+    else if (W == L + 3) conv_weights_of<L + 3>(q, w);
+    else if (W == L + 2) conv_weights_of<L + 2>(q, w);
+    else conv_weights_of<L + 1>(q, w);
 }
 
 template <int DT>
@@ -382,8 +398,28 @@ __global__ __launch_bounds__(256) void seq_conv_step_kernel(const ConvStepP p) {
     const int d = on ? d0 : 0;
     const int64_t slot = p.slot ? p.slot[r] : r;
     const bool there = slot >= 0 && slot < p.n_slots;
+    char *yp = (char *)p.y.p;
+    if (!there) {
+        CT y[V];
+#pragma unroll
+        for (int c = 0; c < V; ++c) y[c] = CT(0);
+        if (on) conv_put<YT, V>(yp + r * (int64_t)p.y.rs * ES, d, y);
+        return;
+    }
+    // all that the row reads is on its way before other rows' slots are looked at
+    CT w[WM][V], bias[V], x[WM][V];
+    char *st = (char *)p.st.p + slot * p.st.bs * ES;
+    ConvRaw<YT, V> q, qs[WM - 1];
+#pragma unroll
+    for (int j = 0; j < WM - 1; ++j) {
+        const int k = j - (WM - p.W);
+        if (k >= 0) qs[j].load(st + k * (int64_t)p.st.rs * ES, nullptr, d);
+        else qs[j] = ConvRaw<YT, V>{};
+    }
+    q.load((const char *)p.x.p + r * (int64_t)p.x.rs * ES, nullptr, d);
+    conv_weights<CT, WM, V>(p.w, p.bias, p.W, d, w, bias);
     int64_t nx = -1;
-    if (p.slot && there && p.rows > 1) {
+    if (p.slot && p.rows > 1) {
         if (threadIdx.x == 0) { before = 0; next = 0x7fffffff; }
         __syncthreads();
         seq_same_slot(p.slot, p.rows, r, &before, &next);
@@ -391,33 +427,12 @@ __global__ __launch_bounds__(256) void seq_conv_step_kernel(const ConvStepP p) {
         if (before) return;
         nx = next == 0x7fffffff ? -1 : next;
     }
-    CT w[WM][V], bias[V], x[WM][V];
-    char *yp = (char *)p.y.p;
-    if (!there) {
 #pragma unroll
-        for (int c = 0; c < V; ++c) bias[c] = CT(0);
-        if (on) conv_put<YT, V>(yp + r * (int64_t)p.y.rs * ES, d, bias);
-        return;
-    }
-    char *st = (char *)p.st.p + slot * p.st.bs * ES;
+    for (int j = 0; j < WM - 1; ++j)
 #pragma unroll
-    for (int j = 0; j < WM - 1; ++j) {
-        const int k = j - (WM - p.W);
-        if (k >= 0) {
-            ConvRaw<YT, V> q;
-            q.load(st + k * (int64_t)p.st.rs * ES, nullptr, d);
-#pragma unroll
-            for (int c = 0; c < V; ++c) x[j][c] = q.get(c);
-        } else {
-#pragma unroll
-            for (int c = 0; c < V; ++c) x[j][c] = CT(0);
-        }
-    }
-    conv_weights<CT, WM, V>(p.w, p.bias, p.W, d, w, bias);
+        for (int c = 0; c < V; ++c) x[j][c] = qs[j].get(c);
     for (;;) {
         CT y[V];
-        ConvRaw<YT, V> q;
-        q.load((const char *)p.x.p + r * (int64_t)p.x.rs * ES, nullptr, d);
 #pragma unroll
         for (int c = 0; c < V; ++c) {
             x[WM - 1][c] = q.get(c);
@@ -432,6 +447,7 @@ __global__ __launch_bounds__(256) void seq_conv_step_kernel(const ConvStepP p) {
         if (on) conv_put<YT, V>(yp + r * (int64_t)p.y.rs * ES, d, y);
         if (nx < 0) break;
         r = nx;
+        q.load((const char *)p.x.p + r * (int64_t)p.x.rs * ES, nullptr, d);
         __syncthreads();
         if (threadIdx.x == 0) next = 0x7fffffff;
         __syncthreads();

@@ -36,6 +36,7 @@ struct ScanP {
     int32_t n0;                                   // first state of this launch
     int32_t first, fin;                           // first / last launch over the states
     int32_t softplus, zero_outside;
+    int32_t nvec;                                 // N and the arrays that end in it allow four states at a time
     int32_t gate;                                 // z is there (else its view is u's, and what it gives is not used)
 };
 
@@ -75,21 +76,30 @@ __device__ __forceinline__ ScanAt scan_at(const ScanP &p) {
     return a;
 }
 
-template <class CT, int NS>
-__device__ __forceinline__ void scan_rates(const ScanP &p, int d, CT (&A2)[NS]) {
+// K states from the n-th on of row `row` of a [..][N] array (null, or behind the last state: 0), four at a time where the arrays allow it: the lanes
+// are N elements apart, a load of each state by itself touches as many lines as one of four
+template <class CT, int K>
+__device__ __forceinline__ void scan_get(const ScanP &p, const void *x, int64_t row, int n, CT (&o)[K]) {
+    constexpr int V = K < 4 ? K : 4;
+    typedef CT VV __attribute__((ext_vector_type(V)));
+    const CT *q = (const CT *)x + row * p.N + n;
+    if (sizeof(CT) == 4 && x && p.nvec && n + K <= p.N) {
 #pragma unroll
-    for (int n = 0; n < NS; ++n) A2[n] = p.n0 + n < p.N ? ((const CT *)p.A)[(int64_t)d * p.N + p.n0 + n] * CT(kLog2eD) : CT(0);
+        for (int j = 0; j < K; j += V) {
+            const VV v = *(const VV *)(q + j);
+#pragma unroll
+            for (int i = 0; i < V; ++i) o[j + i] = v[i];
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < K; ++j) o[j] = x && n + j < p.N ? q[j] : CT(0);
+    }
 }
-template <class CT, int NS>
-__device__ __forceinline__ void scan_state(const ScanP &p, const void *st, int64_t s, int d, CT (&h)[NS]) {
+template <class CT, int K>
+__device__ __forceinline__ void scan_rates(const ScanP &p, int d, int n, CT (&A2)[K]) {
+    scan_get<CT, K>(p, p.A, d, n, A2);
 #pragma unroll
-    for (int n = 0; n < NS; ++n) h[n] = st && p.n0 + n < p.N ? ((const CT *)st)[(s * p.D + d) * p.N + p.n0 + n] : CT(0);
-}
-template <class CT, int NS>
-__device__ __forceinline__ void scan_state_put(const ScanP &p, void *st, int64_t s, int d, const CT (&h)[NS]) {
-#pragma unroll
-    for (int n = 0; n < NS; ++n)
-        if (p.n0 + n < p.N) ((CT *)st)[(s * p.D + d) * p.N + p.n0 + n] = h[n];
+    for (int j = 0; j < K; ++j) A2[j] *= CT(kLog2eD);
 }
 // what a launch may meet: 0 plain arrays, all states at once; 1 the same with u, and z if there is one, as checkpoints; 2 anything
 constexpr int kScanAny = 2;
@@ -198,14 +208,11 @@ __global__ __launch_bounds__(64 * kScanWaves, IO == 8 ? 3 : 6) void seq_scan_fwd
     if (OUT && p.zero_outside && fin && wave == 0) seq_zero_outside(p.m, p.y, a.b, a.d, a.valid);
     if (!a.k.live || (!OUT && a.k.last)) return;
     CT A2[NW], h[NW], sd = CT(0);
+    scan_rates<CT, NW>(p, a.d, p.n0 + wave * NW, A2);
+    if (OUT && start) {
 #pragma unroll
-    for (int j = 0; j < NW; ++j) {
-        const int ns = wave * NW + j, n = p.n0 + ns;
-        A2[j] = n < p.N ? ((const CT *)p.A)[(int64_t)a.d * p.N + n] * CT(kLog2eD) : CT(0);
-        h[j] = CT(0);
-        if (OUT && start && n < p.N) h[j] = scan_plane<NS>(start, a.b, ns, p.D)[(uint32_t)a.d];
-        else if (OUT && !start && p.state_in && n < p.N) h[j] = ((const CT *)p.state_in)[((int64_t)a.k.s * p.D + a.d) * p.N + n];
-    }
+        for (int j = 0; j < NW; ++j) h[j] = p.n0 + wave * NW + j < p.N ? scan_plane<NS>(start, a.b, wave * NW + j, p.D)[(uint32_t)a.d] : CT(0);
+    } else scan_get<CT, NW>(p, OUT ? p.state_in : nullptr, (int64_t)a.k.s * p.D + a.d, p.n0 + wave * NW, h);
     if (a.k.n > 0) {
         const CT bias = p.dt_bias ? ((const CT *)p.dt_bias)[a.d] : CT(0), skip = OUT && p.Dskip ? ((const CT *)p.Dskip)[a.d] : CT(0);
         // the thread's values of B and C: column j of rows row0, row0 + 256 / (2 NS), ..
@@ -321,7 +328,7 @@ __global__ __launch_bounds__(64 * kScanWaves, IO == 8 ? 2 : 3) void seq_scan_end
     const ScanAt a = scan_at(p);
     if (!a.on || !a.k.live) return;
     CT A2[NS], h[NS], P[NS], g[NS];
-    scan_rates<CT, NS>(p, a.d, A2);
+    scan_rates<CT, NS>(p, a.d, p.n0, A2);
 #pragma unroll
     for (int n = 0; n < NS; ++n) {
         h[n] = CT(0);
@@ -469,7 +476,7 @@ __global__ __launch_bounds__(64 * kScanWaves, 2) void seq_scan_bwd_kernel(const 
     for (int n = 0; n < NS; ++n) dA[n] = CT(0);
     if (a.k.live && a.k.n > 0) {
         CT A2[NS], h[NS], q[NS];
-        scan_rates<CT, NS>(p, a.d, A2);
+        scan_rates<CT, NS>(p, a.d, p.n0, A2);
 #pragma unroll
         for (int n = 0; n < NS; ++n) {
             h[n] = scan_plane<NS>(start, a.b, n, p.D)[(uint32_t)a.d];
