@@ -131,17 +131,17 @@ struct ScanPlan {
 };
 
 // Rows of a chunk of the forward scan; 0: sequences are not cut.  Cutting costs a second look at all but a sequence's last chunk and two launches; a
-// block alone takes 0.25 us a row.  So short sequences stay whole, and so do a dense batch's where they give every SIMD a wavefront; packed ones are cut
+// block alone takes 0.18 us a row.  So short sequences stay whole, and so do a dense batch's where they give every SIMD a wavefront; packed ones are cut
 // even then, since their lengths are not known here.  Else chunks are as long as they still fill the card.  Measured (bf16, 16 states; sequences x
-// rows x channels: us at 16 / 32 / 64 / 128 / 512 rows a chunk, whole): 1 x 64 x 1536 - / 31 / 31 / 30 / 30, 22; 1 x 256 x 1536 29 / 32 / 42 / 66 / 76, 69;
-// 1 x 512 x 4096 50 / 42 / 46 / 67 / 139, 132; 1 x 2048 x 2048 80 / 65 / 60 / 72 / 220, 509; 9 x 910 x 4096 471 / 318 / 263 / 260 / 300, 657;
-// 8 x 1024 x 4096 458 / 307 / 260 / 245 / 267, 273; 32 x 512 x 4096 878 / 607 / 508 / 458 / 359, 319.
+// rows x channels: us a call at 16 / 32 / 64 / 128 / 512 rows a chunk, whole): 1 x 64 x 1536 - / 27 / 26 / 27 / 26, 18; 1 x 256 x 1536 25 / 25 / 32 / 50 / 57, 52;
+// 1 x 512 x 4096 45 / 38 / 39 / 51 / 104, 98; 1 x 2048 x 2048 73 / 59 / 56 / 61 / 161, 375; 1 x 16384 x 1024 285 / 191 / 156 / 143 / 189, 2952; 9 x 910 x 4096 422 /
+// 291 / 253 / 248 / 294, 486; 8 x 1024 x 4096 415 / 286 / 249 / 232 / 242, 224; 32 x 512 x 4096 773 / 558 / 488 / 447 / 319, 289.
 int64_t scan_forward_rows(int64_t flat, int32_t n_seq, int64_t rows, bool packed, int64_t ntile) {
     if (rows <= 64) return 0;                      // (packed: no sequence has more)
     const bool many = (int64_t)n_seq * ntile >= 1024;
     if (many && !packed) return 0;
     const int64_t total = flat * ntile;
-    const int64_t q = many ? 512 : total <= 8192 ? 16 : total <= 49152 ? 32 : total <= 262144 ? 64 : 128;
+    const int64_t q = many ? 512 : total <= 8192 ? 16 : total <= 49152 ? 32 : total <= 131072 ? 64 : 128;
     return std::max(q, (total / 8192 + 7) / 8 * 8);
 }
 
@@ -285,7 +285,7 @@ bool scan_views(SeqCheck &c, const crnn_scan_args *a, bool backward, bool step =
     } while (0)
 
 // ------------------------------------------------------------------ convolution
-// channels of a thread, one where an array of the call does not allow more.  Four of two bytes beat eight (12001 x 4096, W = 4: 46 against 54 us):
+// channels of a thread, one where an array of the call does not allow more.  Four of two bytes beat eight (12001 x 4096, W = 4: 37 against 41 us):
 // half the registers are twice the wavefronts.
 int conv_wide(int dtype, int W, bool backward) {
     if (dtype == CRNN_DT_F64) return 2;
@@ -293,12 +293,12 @@ int conv_wide(int dtype, int W, bool backward) {
     return 4;
 }
 // Rows of a strip: strips and channels together give some wavefronts to each SIMD; a strip reads W - 1 rows twice, the gradient 2 (W - 1).
-// Measured, bf16 (us at 8 / 16 / 24 / 32 / 48 / 64 / 128 rows): forward 12001 x 4096 71 / 46 / 45 / 45 / 47 / 46 / 45, 1024 x 2048 14 / 14 / 14 / 15 / 15 / 18 /
-// 28; gradient 8192 x 2048 from 8 bits 69 / 51 / 42 / 44 / 43 / 55 / 58, 12000 x 4096 168 / 111 / 92 / 89 / 77 / 76 / 86, 1024 x 2048 25 / 25 / 25 / 26 / 28 / 33 / 51.
+// Measured, bf16 (us a call at 8 / 16 / 24 / 32 / 48 / 64 / 128 rows): forward 12001 x 4096 43 / 36 / 38 / 39 / 40 / 40 / 42, 1024 x 2048 12 / 12 / 12 / 12 / 13 /
+// 16 / 26; gradient 8192 x 2048 from 8 bits 60 / 46 / 39 / 42 / 41 / 48 / 56, 12000 x 4096 148 / 99 / 83 / 80 / 72 / 71 / 83, 1024 x 2048 23 / 23 / 23 / 23 / 27 / 31 / 51.
 int64_t conv_strip(int64_t flat, int32_t D, int V, bool backward) {
     const int64_t waves = (D + 64 * V - 1) / (64 * V);
     const int64_t q = (flat * waves / 4096 + 3) / 4 * 4;
-    const int64_t lo = backward ? 24 : 8, hi = backward ? 64 : 32;
+    const int64_t lo = backward ? 24 : 8, hi = backward ? 64 : 16;
     return q < lo ? lo : q > hi ? hi : q;
 }
 bool conv_fits(const crnn_view &v, int V) { return !v.ptr || seq_view(v, V).vec; }
