@@ -273,6 +273,13 @@ __device__ __forceinline__ void seq_put_rows(const SeqMap &m, const SeqV &v, con
     for (int i = 0; i < TB; ++i) (c + (int64_t)(t + i < k.n ? t + i : k.n - 1) * v.rs)[d] = b[i];
 }
 
+// x as an index of the vector unit: an LDS address that the compiler knows to be uniform is kept in a scalar register, and moved for every read
+__device__ __forceinline__ int seq_vector_index(int x) {
+#if defined(__HIP_DEVICE_COMPILE__)
+    asm("" : "+v"(x));
+#endif
+    return x;
+}
 // what a wavefront wrote to its own part of the LDS is there for all its lanes
 __device__ __forceinline__ void seq_wave_sync() {
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");

@@ -201,7 +201,8 @@ __global__ __launch_bounds__(64 * kScanWaves, IO == 8 ? 3 : 6) void seq_scan_fwd
     using E = typename SeqIO<IO>::E;
     constexpr int R = kScanRows, RW = kScanRows / kScanWaves, NW = NS / kScanWaves;      // rows and states of a wavefront
     constexpr int MV = R * 2 * NS >= 256 ? R * 2 * NS / 256 : 1;                         // values of B and C a thread brings
-    __shared__ ScanShare<CT, NS, OUT> sh;
+    typedef CT VN __attribute__((ext_vector_type(NW)));
+    __shared__ __align__(16) ScanShare<CT, NS, OUT> sh;
     const ScanAt a = scan_tile(p);
     const bool fin = MODE != kScanAny || p.fin;
     const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)), lane = threadIdx.x & 63;
@@ -235,6 +236,7 @@ __global__ __launch_bounds__(64 * kScanWaves, IO == 8 ? 3 : 6) void seq_scan_fwd
             rd.load(p.m, p.dt, a.k, t + wave * RW, a.d);
             if (OUT) rz.load(p.m, p.z, a.k, t + wave * RW, a.d);
         };
+        const CT *bc = &sh.maps[0][0] + seq_vector_index(wave * NW);        // the wavefront's states in B, NS further in C
         fetch(0);
 #pragma unroll 1
         for (int t = 0; t < a.k.n; t += R) {
@@ -266,11 +268,12 @@ __global__ __launch_bounds__(64 * kScanWaves, IO == 8 ? 3 : 6) void seq_scan_fwd
 #pragma unroll
             for (int i = 0; i < R; ++i) {
                 const CT d = sh.dl[i][lane], du = sh.du[i][lane];
+                const VN b = *(const VN *)(bc + i * (2 * NS)), c = *(const VN *)(bc + i * (2 * NS) + (OUT ? NS : 0));
                 CT v = CT(0);
 #pragma unroll
                 for (int j = 0; j < NW; ++j) {
-                    h[j] = seq_fma(seq_exp2(d * A2[j]), h[j], du * sh.maps[i][wave * NW + j]);
-                    if (OUT) v = seq_fma(h[j], sh.maps[i][NS + wave * NW + j], v);
+                    h[j] = seq_fma(seq_exp2(d * A2[j]), h[j], du * b[j]);
+                    if (OUT) v = seq_fma(h[j], c[j], v);
                 }
                 if (OUT) sh.v[OUT ? wave : 0][OUT ? i : 0][lane] = v;
             }
