@@ -570,7 +570,7 @@ static bool pack_plan(SeqCheck &c, const crnn_view *x, int64_t rows, int32_t D, 
     if (!c.view(*x, "x", x->dtype, true, false, out, D)) return false;
     p.x = seq_view(*x, 16 / seq_size(x->dtype));
     p.q = (int8_t *)codes; p.sc = (uint8_t *)scales;
-    p.vecq = (uintptr_t)codes % 16 == 0 && D % 16 == 0;
+    p.vecq = (uintptr_t)codes % 16 == 0 && D % 16 == 0 ? 16 : (uintptr_t)codes % 4 == 0 && D % 4 == 0 ? 4 : 1;
     if ((rows * 2 * p.nb + 255) / 256 > kSeqMaxGrid) return c.bad("too many rows and channels for one launch");
     return true;
 }

@@ -4,6 +4,7 @@
 // round to 128; code = x / 2^e rounded half to even, within +-127.  Scales are powers of two, so that the rounding to a code is the only one:
 // a value comes back within 2^(e - 1), at most max|x| / 128 (the type's largest values, from 127.5 of 128 of its last binade on, within 2^e).
 // A block that holds an infinity or a NaN comes back as NaN (scale byte 255).  Reads once, writes 33/32 bytes a value: bound by memory.
+// 16384 rows of 4096 channels, bf16: 204 MB in 38 us (5.4 TB/s), back in 32 us (6.4 TB/s; what was just written is still in a cache).
 #pragma once
 #include "seq_common.hpp"
 
@@ -16,7 +17,7 @@ struct PackP {
     int8_t *q;                  // [rows][D]
     uint8_t *sc;                // [rows][ceil(D / 32)]
     int64_t rows;
-    int32_t D, nb, vecq;        // vecq: the codes can be stored 16 bytes at a time
+    int32_t D, nb, vecq;        // vecq: bytes of the codes that can be accessed at a time: 16, 4 or 1
 };
 
 template <int DT>
@@ -90,12 +91,16 @@ __global__ __launch_bounds__(256) void seq_pack_kernel(const PackP p) {
     }
     if (!in || d >= p.D) return;
     int8_t *q = p.q + r * p.D + d;
-    if (p.vecq && d + kPackV <= p.D) {
+    if (p.vecq == 16 && d + kPackV <= p.D) {
         typedef uint32_t U4 __attribute__((ext_vector_type(4)));
         U4 b;
 #pragma unroll
         for (int k = 0; k < 4; ++k) b[k] = w[k];
         *(U4 *)q = b;
+    } else if (p.vecq >= 4) {          // (D is a multiple of four)
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+            if (d + 4 * k < p.D) ((uint32_t *)q)[k] = w[k];
     } else {
 #pragma unroll
         for (int k = 0; k < kPackV; ++k)
@@ -114,11 +119,24 @@ __global__ __launch_bounds__(256) void seq_unpack_kernel(const PackP p) {
     const int8_t *q = p.q + r * p.D + d;
     const int64_t off = r * (int64_t)p.x.rs + d;
     typedef uint32_t U4 __attribute__((ext_vector_type(4)));
-    if (p.vecq && p.x.vec && d + kPackV <= p.D) {
+    float x[kPackV];
+    uint32_t w[kPackV / 4] = {0, 0, 0, 0};
+    if (p.vecq == 16 && d + kPackV <= p.D) {
         const U4 b = *(const U4 *)q;
-        float x[kPackV];
 #pragma unroll
-        for (int k = 0; k < kPackV; ++k) x[k] = (float)(int32_t)(int8_t)(b[k / 4] >> (8 * (k % 4))) * e;
+        for (int k = 0; k < 4; ++k) w[k] = b[k];
+    } else if (p.vecq >= 4) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+            if (d + 4 * k < p.D) w[k] = ((const uint32_t *)q)[k];
+    } else {
+#pragma unroll
+        for (int k = 0; k < kPackV; ++k)
+            if (d + k < p.D) w[k / 4] |= (uint32_t)(uint8_t)q[k] << (8 * (k % 4));
+    }
+#pragma unroll
+    for (int k = 0; k < kPackV; ++k) x[k] = (float)(int32_t)(int8_t)(w[k / 4] >> (8 * (k % 4))) * e;
+    if (p.x.vec && d + kPackV <= p.D) {
         if (DT == CRNN_DT_F32) {
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
@@ -142,7 +160,7 @@ __global__ __launch_bounds__(256) void seq_unpack_kernel(const PackP p) {
     } else {
 #pragma unroll
         for (int k = 0; k < kPackV; ++k)
-            if (d + k < p.D) seq_store(p.x, off + k, (float)(int32_t)q[k] * e);
+            if (d + k < p.D) seq_store(p.x, off + k, x[k]);
     }
 }
 
