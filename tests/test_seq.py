@@ -698,6 +698,49 @@ def test_arrays_of_other_strides():
     assert torch.equal(seq.unpack8(seq.pack8(d)), seq.unpack8(seq.pack8(d.contiguous())))
 
 
+def shifted(x):
+    """x one element behind a 16-byte boundary, contiguous as before."""
+    if x is None or x.numel() == 0:
+        return x
+    y = torch.empty(x.numel() + 32, dtype=x.dtype, device=x.device)
+    at = next(i for i in range(32) if y[i:].data_ptr() % 16 == x.element_size() % 16)
+    y = y[at:at + x.numel()].view(x.shape)
+    y.copy_(x)
+    assert y.is_contiguous() and y.data_ptr() % 16 != 0
+    return y
+
+
+@gpu
+@pytest.mark.parametrize("dtype,W,N", [("f32", 4, 16), ("f32", 3, 8), ("bf16", 4, 16), ("bf16", 7, 12), ("f16", 1, 4), ("f16", 8, 20), ("f64", 4, 8), ("f64", 6, 5)])
+@pytest.mark.parametrize("which", ["parameters", "all"])
+def test_arrays_off_their_alignment(dtype, W, N, which):
+    """Parameters, or all arrays, one element behind a 16-byte boundary: the narrow loads give the bits of the wide ones."""
+    g = torch.Generator().manual_seed(W)
+    B, T, D, dt = 2, 90, 64, DT[dtype]
+    pt = param_of(dt)
+    x, d, z, dy = (rnd(g, B, T, D, dtype=dt) for _ in range(4))
+    Bm, Cm = (rnd(g, B, T, N, dtype=dt) for _ in range(2))
+    w, b, A, skip, bias = (v.to(pt) for v in (rnd(g, D, W), rnd(g, D), -torch.exp(rnd(g, D, N)), rnd(g, D), rnd(g, D)))
+    cst, hst, dhs = rnd(g, B, W - 1, D, dtype=dt), rnd(g, B, D, N).to(pt), rnd(g, B, D, N).to(pt)
+
+    def run(par, arr):
+        kw = dict(D=par(skip), dt_bias=par(bias), z=arr(z))
+        y, end = seq.causal_conv(arr(x), par(w), par(b), silu=True, state=arr(cst), return_state=True)
+        cg = seq.causal_conv_grad(arr(dy), arr(x), par(w), par(b), silu=True, state=arr(cst), dstate=arr(cst))
+        s, h = seq.selective_scan(arr(x), arr(d), par(A), arr(Bm), arr(Cm), state=par(hst), return_state=True, **kw)
+        sg = seq.selective_scan_grad(arr(dy), arr(x), arr(d), par(A), arr(Bm), arr(Cm), state=par(hst), dstate=par(dhs), **kw)
+        c1, h1 = arr(cst.clone()), par(hst.clone())
+        row = lambda v: arr(v[:, 3].contiguous())  # noqa: E731
+        y1 = seq.causal_conv_step(row(x), par(w), par(b), c1)
+        y2 = seq.selective_scan_step(row(x), row(d), par(A), row(Bm), row(Cm), h1, D=par(skip), z=row(z))
+        back = [] if dtype == "f64" else [seq.unpack8(seq.pack8(arr(x)))]
+        return [y, end, *cg, s, h, *sg, c1, h1, y1, y2, *back]
+
+    keep = lambda v: v  # noqa: E731
+    for k, (p, q) in enumerate(zip(run(keep, keep), run(shifted, shifted if which == "all" else keep))):
+        assert torch.equal(p, q), k
+
+
 @gpu
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
 def test_nothing_to_do(dtype):
