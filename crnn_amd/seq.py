@@ -12,7 +12,8 @@ Arrays are torch tensors on an MI355X; the calls enqueue on that device's curren
 a graph.  Rows are time, channels are contiguous: dense [n_seq, rows, D] (lengths=: how many rows of each are its own, the others are
 padding), or packed [rows, D] with seq_start [n_seq + 1], int32 on the device: sequence s is rows seq_start[s] .. seq_start[s + 1] - 1.
 Lengths and offsets are not read by the host: they are clamped to the arrays.  Rows of a result that belong to no sequence are 0, and stay as
-they were where the caller gave the array (out=).  Results may not share memory with inputs.  float32, bfloat16, float16 and float64; weights, rates and scan states are float32
+they were where the caller gave the array (out=).  Results may not share memory with inputs.  Autograd does not
+record the calls: gradients are the *_grad calls.  float32, bfloat16, float16 and float64; weights, rates and scan states are float32
 (float64 with float64 data).  A checkpoint (Packed8) may stand for x of the convolution, and for u and z of the scan.
 """
 from __future__ import annotations
