@@ -34,6 +34,12 @@ __device__ __forceinline__ float seq_scale(uint32_t byte) {
     return seq_as_float(byte == 255u ? 0x7fc00000u : byte == 0u ? 0x00400000u : byte << 23);
 }
 
+// code * 2^(byte - 127) with the byte at bit 23: 0 is the largest of it and 2^-127's bits, 255 (infinity here) adds 0 * infinity
+__device__ __forceinline__ float seq_unpack(int32_t code, uint32_t byte23) {
+    const float s = seq_as_float(byte23 > 0x00400000u ? byte23 : 0x00400000u);
+    return __builtin_fmaf((float)code, s, s * 0.0f);
+}
+
 // ---- functions in the compute type.  The float forms use the hardware's exp2 and reciprocal (about one unit in the last place).
 __device__ __forceinline__ float seq_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
 __device__ __forceinline__ double seq_exp2(double x) { return exp2(x); }
@@ -229,7 +235,7 @@ struct SeqRows {
     __device__ __forceinline__ void get(const SeqV &v, CT (&o)[TB]) const {
         if (PM == 1 || (PM == 2 && v.dt == CRNN_DT_PACKED8)) {
 #pragma unroll
-            for (int i = 0; i < TB; ++i) o[i] = (CT)(int32_t)(int8_t)((uint32_t)r[i] & 0xffu) * (CT)seq_scale((uint32_t)r[i] >> 8);
+            for (int i = 0; i < TB; ++i) o[i] = (CT)seq_unpack((int8_t)((uint32_t)r[i] & 0xffu), (uint32_t)r[i] >> 8 << 23);
         } else if (IO == 8) {
 #pragma unroll
             for (int i = 0; i < TB; ++i) o[i] = (CT)r[i];

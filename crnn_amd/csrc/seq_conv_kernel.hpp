@@ -61,7 +61,7 @@ struct ConvRaw {
         if (DT == CRNN_DT_F32) return (C)seq_as_float(w[i % NW]);
         if (DT == CRNN_DT_BF16) return (C)seq_as_float(i & 1 ? w[(i / 2) % NW] & 0xffff0000u : w[(i / 2) % NW] << 16);
         if (DT == CRNN_DT_F16) return (C)seq_from_f16(w[(i / 2) % NW] >> (16 * (i & 1)) & 0xffffu);
-        return (C)(int32_t)(int8_t)(w[(i / 4) % NW] >> (8 * (i & 3))) * (C)seq_scale(e);
+        return (C)seq_unpack((int8_t)(w[(i / 4) % NW] >> (8 * (i & 3))), e << 23);
     }
 };
 template <int DT, int V>
