@@ -324,7 +324,7 @@ __global__ __launch_bounds__(64 * kScanWaves, IO == 8 ? 3 : 6) void seq_scan_fwd
 
 // ---- gradient, a chunk by itself: S = its last state from zero, the sum of delta, and G = what its outputs' gradients r pass back to the state
 // before it, sum_t (prod of the decays up to t) r C -- taken in the forward direction, so that one exponential serves both.
-// 6144 rows of 2048 channels, 16 states, u and z in 8 bits: 81 us, vector unit busy 86 %.
+// 6144 rows of 2048 channels, 16 states, u and z in 8 bits: 79 us (72 where they are plain), vector unit busy 86 %.
 template <int IO, int NS, int MODE>
 __global__ __launch_bounds__(64 * kScanWaves, IO == 8 ? 2 : 3) void seq_scan_ends2_kernel(const ScanP p, typename SeqIO<IO>::C *__restrict__ S,
                                                                                                   typename SeqIO<IO>::C *__restrict__ Gb,
@@ -461,7 +461,7 @@ __global__ __launch_bounds__(256) void seq_scan_carry_kernel(const ScanP p, CT *
 // h[t] is one multiply-add away, and dA needs the product itself), and the reverse sweep over them.  dB and dC are sums over channels: a
 // wavefront's part goes to part[tile][row][B: NS | C: NS], summed over the tiles in a fixed order by seq_scan_sum_maps_kernel.
 // Four rows and five times four a chunk: two wavefronts a SIMD fill the registers (256 a lane) and the LDS (16.5 KB each) about together.
-// 6144 rows of 2048 channels, 16 states, u and z in 8 bits: 281 us, vector unit busy 68 %: 33 vector instructions a row, channel and state (21 of
+// 6144 rows of 2048 channels, 16 states, u and z in 8 bits: 275 us (239 where they are plain), vector unit busy 69 %: 33 vector instructions a row, channel and state (21 of
 // them the reverse row, folds of dB and dC included), the rest of the time both wavefronts of a SIMD wait (a row's maps from the LDS, the next rows).
 constexpr int kScanBwdTB = 4, kScanBwdSub = 5, kScanBwdQ = kScanBwdTB * kScanBwdSub;
 template <int IO, int NS, int MODE>
