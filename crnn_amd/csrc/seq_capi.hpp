@@ -345,49 +345,70 @@ bool conv_views(SeqCheck &c, const crnn_conv_args *a, bool backward, crnn::ConvP
     p.w = a->weight; p.bias = a->bias;
     return true;
 }
-template <int XT, int YT, int WM, int V>
+template <int XT, int YT, int W, int V>
 void conv_launch(const crnn::ConvP &p, bool backward, hipStream_t st) {
     const int64_t gx = (p.D + 64 * V - 1) / (64 * V);
     const dim3 grid((unsigned)((p.m.nblk + 3) / 4 * gx));
-    if (backward) hipLaunchKernelGGL((crnn::seq_conv_bwd_kernel<XT, YT, WM, V>), grid, dim3(256), 0, st, p);
-    else hipLaunchKernelGGL((crnn::seq_conv_fwd_kernel<XT, YT, WM, V>), grid, dim3(256), 0, st, p);
+    if (backward) hipLaunchKernelGGL((crnn::seq_conv_bwd_kernel<XT, YT, W, V>), grid, dim3(256), 0, st, p);
+    else hipLaunchKernelGGL((crnn::seq_conv_fwd_kernel<XT, YT, W, V>), grid, dim3(256), 0, st, p);
 }
-// VF, VB, VF8, VB8: the wide forms' channels forward and backward, up to four taps and more (conv_wide)
-template <int XT, int YT, int VF, int VB, int VF8, int VB8>
+// VF, VB: the wide forms' channels forward and backward (conv_wide)
+template <int XT, int YT, int W, int VF, int VB>
+void conv_launch_v(const crnn::ConvP &p, int V, bool backward, hipStream_t st) {
+    if (V == 1) conv_launch<XT, YT, W, 1>(p, backward, st);
+    else if (backward) conv_launch<XT, YT, W, VB>(p, true, st);
+    else conv_launch<XT, YT, W, VF>(p, false, st);
+}
+// VB8: the gradient's channels from five taps on
+template <int XT, int YT, int VF, int VB, int VB8>
 void conv_launch_w(const crnn::ConvP &p, int V, bool backward, hipStream_t st) {
-    if (p.W <= 4) {
-        if (V == 1) conv_launch<XT, YT, 4, 1>(p, backward, st);
-        else if (backward) conv_launch<XT, YT, 4, VB>(p, true, st);
-        else conv_launch<XT, YT, 4, VF>(p, false, st);
-    } else {
-        if (V == 1) conv_launch<XT, YT, 8, 1>(p, backward, st);
-        else if (backward) conv_launch<XT, YT, 8, VB8>(p, true, st);
-        else conv_launch<XT, YT, 8, VF8>(p, false, st);
+    switch (p.W) {
+        case 1: return conv_launch_v<XT, YT, 1, VF, VB>(p, V, backward, st);
+        case 2: return conv_launch_v<XT, YT, 2, VF, VB>(p, V, backward, st);
+        case 3: return conv_launch_v<XT, YT, 3, VF, VB>(p, V, backward, st);
+        case 4: return conv_launch_v<XT, YT, 4, VF, VB>(p, V, backward, st);
+        case 5: return conv_launch_v<XT, YT, 5, VF, VB8>(p, V, backward, st);
+        case 6: return conv_launch_v<XT, YT, 6, VF, VB8>(p, V, backward, st);
+        case 7: return conv_launch_v<XT, YT, 7, VF, VB8>(p, V, backward, st);
+        default: return conv_launch_v<XT, YT, 8, VF, VB8>(p, V, backward, st);
     }
 }
 template <int YT>
 void conv_launch_x(const crnn::ConvP &p, int V, bool backward, hipStream_t st) {
     constexpr int VB8 = YT == CRNN_DT_F32 ? 2 : 4;
-    if (p.x.dt == CRNN_DT_PACKED8) conv_launch_w<CRNN_DT_PACKED8, YT, 4, 4, 4, VB8>(p, V, backward, st);
-    else conv_launch_w<YT, YT, 4, 4, 4, VB8>(p, V, backward, st);
+    if (p.x.dt == CRNN_DT_PACKED8) conv_launch_w<CRNN_DT_PACKED8, YT, 4, 4, VB8>(p, V, backward, st);
+    else conv_launch_w<YT, YT, 4, 4, VB8>(p, V, backward, st);
 }
 void conv_launch_t(const crnn::ConvP &p, int dtype, int V, bool backward, hipStream_t st) {
-    if (dtype == CRNN_DT_F64) conv_launch_w<CRNN_DT_F64, CRNN_DT_F64, 2, 2, 2, 2>(p, V, backward, st);
+    if (dtype == CRNN_DT_F64) conv_launch_w<CRNN_DT_F64, CRNN_DT_F64, 2, 2, 2>(p, V, backward, st);
     else if (dtype == CRNN_DT_F32) conv_launch_x<CRNN_DT_F32>(p, V, backward, st);
     else if (dtype == CRNN_DT_BF16) conv_launch_x<CRNN_DT_BF16>(p, V, backward, st);
     else conv_launch_x<CRNN_DT_F16>(p, V, backward, st);
 }
-template <int YT, int WM, int V>
+template <int YT, int W, int V>
 void conv_step_launch(const crnn::ConvStepP &p, hipStream_t st) {
     const int64_t gx = (p.D + 256 * V - 1) / (256 * V);
-    hipLaunchKernelGGL((crnn::seq_conv_step_kernel<YT, WM, V>), dim3((unsigned)(p.rows * gx)), dim3(256), 0, st, p);
+    hipLaunchKernelGGL((crnn::seq_conv_step_kernel<YT, W, V>), dim3((unsigned)(p.rows * gx)), dim3(256), 0, st, p);
 }
 // (four channels of a thread at most: the rows are few, the wavefronts should not be)
 template <int YT>
 void conv_step_launch_w(const crnn::ConvStepP &p, int V, hipStream_t st) {
     constexpr int VW = YT == CRNN_DT_F64 ? 2 : 4;
-    if (p.W <= 4) { if (V == 1) conv_step_launch<YT, 4, 1>(p, st); else conv_step_launch<YT, 4, VW>(p, st); }
-    else { if (V == 1) conv_step_launch<YT, 8, 1>(p, st); else conv_step_launch<YT, 8, VW>(p, st); }
+    auto run = [&](auto w) {
+        constexpr int W = decltype(w)::value;
+        if (V == 1) conv_step_launch<YT, W, 1>(p, st);
+        else conv_step_launch<YT, W, VW>(p, st);
+    };
+    switch (p.W) {
+        case 1: return run(std::integral_constant<int, 1>{});
+        case 2: return run(std::integral_constant<int, 2>{});
+        case 3: return run(std::integral_constant<int, 3>{});
+        case 4: return run(std::integral_constant<int, 4>{});
+        case 5: return run(std::integral_constant<int, 5>{});
+        case 6: return run(std::integral_constant<int, 6>{});
+        case 7: return run(std::integral_constant<int, 7>{});
+        default: return run(std::integral_constant<int, 8>{});
+    }
 }
 
 }  // namespace

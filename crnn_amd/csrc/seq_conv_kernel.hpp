@@ -13,7 +13,6 @@
 namespace crnn {
 
 constexpr int kConvTB = 4;       // rows on their way together
-constexpr int kConvMaxW = 8;
 
 struct ConvP {
     SeqMap m;
@@ -96,34 +95,23 @@ __device__ __forceinline__ void conv_put(void *row, uint32_t d, const typename S
     else *(uint16_t *)q = (uint16_t)r.w[0];
 }
 
-// Weights of a thread's channels, right-aligned in WM taps (tap WM - 1 is the row itself).  The V W weights of a thread stand together: read V at a
-// time (one at a time, 4 W bytes between the lanes, they took as long as 32 rows).
-template <int W, class CT, int WM, int V>
-__device__ __forceinline__ void conv_weights_of(const CT *pw, CT (&w)[WM][V]) {
-    typedef CT VV __attribute__((ext_vector_type(V)));
-    VV f[W];
-#pragma unroll
-    for (int k = 0; k < W; ++k) f[k] = ((const VV *)pw)[k];
-#pragma unroll
-    for (int i = 0; i < V; ++i)
-#pragma unroll
-        for (int j = 0; j < WM; ++j) {
-            const int e = i * W + j - (WM - W);
-            w[j][i] = j >= WM - W ? f[(j >= WM - W ? e : 0) / V][(j >= WM - W ? e : 0) % V] : CT(0);
-        }
-}
-template <class CT, int WM, int V>
-__device__ __forceinline__ void conv_weights(const void *pw, const void *pb, int W, int d, CT (&w)[WM][V], CT (&bias)[V]) {
+// Weights of a thread's channels (tap W - 1 is the row itself).  The V W weights of a thread stand together: read V at a time (one at a time,
+// 4 W bytes between the lanes, they took as long as 32 rows).  The kernels are built for each W: a tap that a call does not have is not there, for as
+// a weight of 0 it would carry an infinity or a NaN to rows that the call's taps do not reach.
+template <class CT, int W, int V>
+__device__ __forceinline__ void conv_weights(const void *pw, const void *pb, int d, CT (&w)[W][V], CT (&bias)[V]) {
     typedef CT VV __attribute__((ext_vector_type(V)));
     const CT *q = (const CT *)pw + (int64_t)d * W;
     const VV b = pb ? *(const VV *)((const CT *)pb + d) : VV(CT(0));
+    VV f[W];
 #pragma unroll
-    for (int i = 0; i < V; ++i) bias[i] = b[i];
-    constexpr int L = WM - 4;       // WM is 4 (1 .. 4 taps) or 8 (5 .. 8)
-    if (W == L + 4) conv_weights_of<L + 4>(q, w);
-    else if (W == L + 3) conv_weights_of<L + 3>(q, w);
-    else if (W == L + 2) conv_weights_of<L + 2>(q, w);
-    else conv_weights_of<L + 1>(q, w);
+    for (int k = 0; k < W; ++k) f[k] = ((const VV *)q)[k];
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+        bias[i] = b[i];
+#pragma unroll
+        for (int j = 0; j < W; ++j) w[j][i] = f[(i * W + j) / V][(i * W + j) % V];
+    }
 }
 
 template <int DT>
@@ -135,7 +123,7 @@ __device__ __forceinline__ const uint8_t *conv_scales(const SeqMap &m, const Seq
     return DT == CRNN_DT_PACKED8 ? v.sc + seq_soff(m, v, k, t) : nullptr;
 }
 // x of any row of a sequence (negative: the state's, or 0)
-template <int XT, int YT, int V>
+template <int XT, int YT, int W, int V>
 __device__ __forceinline__ void conv_x(const ConvP &p, const SeqChunk &k, int64_t t, int d, typename SeqT<YT>::C (&o)[V]) {
     using CT = typename SeqT<YT>::C;
     if (t >= 0) {
@@ -143,9 +131,9 @@ __device__ __forceinline__ void conv_x(const ConvP &p, const SeqChunk &k, int64_
         r.load(conv_row<XT>(p.m, p.x, k, t), conv_scales<XT>(p.m, p.x, k, t), d);
 #pragma unroll
         for (int i = 0; i < V; ++i) o[i] = (CT)r.get(i);
-    } else if (p.st_in.p && t >= -(p.W - 1)) {
+    } else if (p.st_in.p && t >= -(W - 1)) {
         ConvRaw<YT, V> r;
-        r.load((const char *)p.st_in.p + ((int64_t)k.s * p.st_in.bs + (t + p.W - 1) * p.st_in.rs) * ConvRaw<YT, 1>::ES, nullptr, d);
+        r.load((const char *)p.st_in.p + ((int64_t)k.s * p.st_in.bs + (t + W - 1) * p.st_in.rs) * ConvRaw<YT, 1>::ES, nullptr, d);
 #pragma unroll
         for (int i = 0; i < V; ++i) o[i] = (CT)r.get(i);
     } else {
@@ -171,7 +159,7 @@ __device__ __forceinline__ ConvAt conv_at(const ConvP &p) {
 
 // 12001 rows of 4096 channels, bf16, 4 taps: 197 MB in 47 us where nothing is in a cache (4.2 TB/s; a copy reaches 4.7), 38 us again and again on the
 // same arrays; 60000 rows 193 us (5.1 TB/s).  130 rows of 768: 6.7 us, a thread's chain of dependent loads.
-template <int XT, int YT, int WM, int V>
+template <int XT, int YT, int W, int V>
 __global__ __launch_bounds__(256) void seq_conv_fwd_kernel(const ConvP p) {
     using CT = typename SeqT<YT>::C;
     constexpr int TB = kConvTB;
@@ -181,10 +169,10 @@ __global__ __launch_bounds__(256) void seq_conv_fwd_kernel(const ConvP p) {
         for (int i = 0; i < V; ++i) seq_zero_outside(p.m, p.y, a.b, a.d + i, true);
     if (!a.k.live) return;
     if (a.k.n > 0) {
-        CT w[WM][V], bias[V], x[WM - 1 + TB][V];
-        conv_weights<CT, WM, V>(p.w, p.bias, p.W, a.d, w, bias);
+        CT w[W][V], bias[V], x[W - 1 + TB][V];
+        conv_weights<CT, W, V>(p.w, p.bias, a.d, w, bias);
 #pragma unroll
-        for (int j = 0; j < WM - 1; ++j) conv_x<XT, YT, V>(p, a.k, a.k.t0 - (WM - 1) + j, a.d, x[j]);
+        for (int j = 0; j < W - 1; ++j) conv_x<XT, YT, W, V>(p, a.k, a.k.t0 - (W - 1) + j, a.d, x[j]);
         const char *xrow = conv_row<XT>(p.m, p.x, a.k, a.k.t0);
         const uint8_t *srow = conv_scales<XT>(p.m, p.x, a.k, a.k.t0);
         char *yrow = conv_row<YT>(p.m, p.y, a.k, a.k.t0);
@@ -200,7 +188,7 @@ __global__ __launch_bounds__(256) void seq_conv_fwd_kernel(const ConvP p) {
 #pragma unroll
             for (int i = 0; i < TB; ++i)
 #pragma unroll
-                for (int c = 0; c < V; ++c) x[WM - 1 + i][c] = (CT)raw[i].get(c);
+                for (int c = 0; c < V; ++c) x[W - 1 + i][c] = (CT)raw[i].get(c);
 #pragma unroll
             for (int i = 0; i < TB; ++i) {
                 const int64_t r = t + TB + i < a.k.n ? t + TB + i : a.k.n - 1;
@@ -214,7 +202,7 @@ __global__ __launch_bounds__(256) void seq_conv_fwd_kernel(const ConvP p) {
                 for (int c = 0; c < V; ++c) {
                     CT s = bias[c];
 #pragma unroll
-                    for (int j = 0; j < WM; ++j) s = seq_fma(w[j][c], x[i + j][c], s);
+                    for (int j = 0; j < W; ++j) s = seq_fma(w[j][c], x[i + j][c], s);
                     y[i][c] = s;
                 }
             if (p.silu) {
@@ -232,15 +220,15 @@ __global__ __launch_bounds__(256) void seq_conv_fwd_kernel(const ConvP p) {
 #pragma unroll
             for (int i = 0; i < TB; ++i) conv_put<YT, V>(yrow + (int64_t)(t + i < a.k.n ? t + i : a.k.n - 1) * ys, a.d, y[i]);
 #pragma unroll
-            for (int j = 0; j < WM - 1; ++j)
+            for (int j = 0; j < W - 1; ++j)
 #pragma unroll
                 for (int c = 0; c < V; ++c) x[j][c] = x[j + TB][c];
         }
     }
     if (a.k.last && p.st_out.p)        // rows len - (W - 1) .. len - 1 of (state, x)
-        for (int j = 0; j < p.W - 1; ++j) {
+        for (int j = 0; j < W - 1; ++j) {
             CT v[V];
-            conv_x<XT, YT, V>(p, a.k, a.k.len - (p.W - 1) + j, a.d, v);
+            conv_x<XT, YT, W, V>(p, a.k, a.k.len - (W - 1) + j, a.d, v);
             conv_put<YT, V>((char *)p.st_out.p + ((int64_t)a.k.s * p.st_out.bs + j * (int64_t)p.st_out.rs) * ConvRaw<YT, V>::ES, a.d, v);
         }
 }
@@ -249,32 +237,32 @@ __global__ __launch_bounds__(256) void seq_conv_fwd_kernel(const ConvP p) {
 // rows past its end.  A sequence's first strip starts W - 1 rows early: those are the state's.  dw, db: a strip's part, summed in order.
 // 8192 rows of 2048 channels, x in 8 bits, bf16, 4 taps: 33 us (84 MB, 2.5 TB/s) and 6.6 us for the sums: 30 operations an element at 128
 // registers; more wavefronts do not fit, and longer strips leave SIMDs without one.
-template <int XT, int YT, int WM, int V>
-__global__ __launch_bounds__(256, WM == 4 && (YT == CRNN_DT_BF16 || YT == CRNN_DT_F16) ? 4 : 1) void seq_conv_bwd_kernel(const ConvP p) {
+template <int XT, int YT, int W, int V>
+__global__ __launch_bounds__(256, W <= 4 && (YT == CRNN_DT_BF16 || YT == CRNN_DT_F16) ? 4 : 1) void seq_conv_bwd_kernel(const ConvP p) {
     using CT = typename SeqT<YT>::C;
     constexpr int TB = kConvTB;
     const ConvAt a = conv_at<V>(p);
     if (!a.on) return;
     if (p.zero_outside)
         for (int i = 0; i < V; ++i) seq_zero_outside(p.m, p.dx, a.b, a.d + i, true);
-    CT dw[WM][V], db[V];
+    CT dw[W][V], db[V];
 #pragma unroll
     for (int c = 0; c < V; ++c) {
         db[c] = CT(0);
 #pragma unroll
-        for (int j = 0; j < WM; ++j) dw[j][c] = CT(0);
+        for (int j = 0; j < W; ++j) dw[j][c] = CT(0);
     }
     if (a.k.live) {
-        // x[WM - 1 + i], dp[WM - 1 + i]: the batch's row i
-        CT w[WM][V], bias[V], x[WM - 1 + TB][V], dp[WM - 1 + TB][V];
-        conv_weights<CT, WM, V>(p.w, p.bias, p.W, a.d, w, bias);
+        // x[W - 1 + i], dp[W - 1 + i]: the batch's row i
+        CT w[W][V], bias[V], x[W - 1 + TB][V], dp[W - 1 + TB][V];
+        conv_weights<CT, W, V>(p.w, p.bias, a.d, w, bias);
 #pragma unroll
-        for (int j = 0; j < WM - 1; ++j) {
-            conv_x<XT, YT, V>(p, a.k, a.k.t0 - (WM - 1) + j, a.d, x[j]);
+        for (int j = 0; j < W - 1; ++j) {
+            conv_x<XT, YT, W, V>(p, a.k, a.k.t0 - (W - 1) + j, a.d, x[j]);
 #pragma unroll
             for (int c = 0; c < V; ++c) dp[j][c] = CT(0);
         }
-        const int back = p.W - 1;
+        constexpr int back = W - 1;
         // (fewer than 2^31 rows: uniform comparisons of 32 bits stay out of the vector unit)
         const int t0 = (int)a.k.t0, len = (int)a.k.len, lo = t0 == 0 ? -back : t0, hi = t0 + a.k.n;     // rows whose dx this strip writes
         const int lastrow = len - 1;
@@ -294,14 +282,14 @@ __global__ __launch_bounds__(256, WM == 4 && (YT == CRNN_DT_BF16 || YT == CRNN_D
         };
         if (a.k.n > 0) fetch(t0);
 #pragma unroll 1
-        for (int t = t0; t < hi + WM - 1; t += TB) {
+        for (int t = t0; t < hi + W - 1; t += TB) {
             if (a.k.n > 0) {
 #pragma unroll
                 for (int i = 0; i < TB; ++i)
 #pragma unroll
                     for (int c = 0; c < V; ++c) {
-                        x[WM - 1 + i][c] = (CT)rx[i].get(c);
-                        dp[WM - 1 + i][c] = (CT)rg[i].get(c);
+                        x[W - 1 + i][c] = (CT)rx[i].get(c);
+                        dp[W - 1 + i][c] = (CT)rg[i].get(c);
                     }
                 fetch(t + TB);
                 __builtin_amdgcn_sched_barrier(0);
@@ -312,26 +300,26 @@ __global__ __launch_bounds__(256, WM == 4 && (YT == CRNN_DT_BF16 || YT == CRNN_D
                     for (int c = 0; c < V; ++c) {
                         CT s = bias[c];
 #pragma unroll
-                        for (int j = 0; j < WM; ++j) s = seq_fma(w[j][c], x[i + j][c], s);
+                        for (int j = 0; j < W; ++j) s = seq_fma(w[j][c], x[i + j][c], s);
                         const CT sg = seq_sigmoid(s);
-                        CT g = dp[WM - 1 + i][c];
+                        CT g = dp[W - 1 + i][c];
                         const CT ga = g * (sg * seq_fma(s, CT(1) - sg, CT(1)));
                         g = p.silu ? ga : g;
                         g = in ? g : CT(0);
-                        dp[WM - 1 + i][c] = g;
+                        dp[W - 1 + i][c] = g;
                         const CT gm = mine ? g : CT(0);
                         db[c] += gm;
 #pragma unroll
-                        for (int j = 0; j < WM; ++j) dw[j][c] = seq_fma(gm, x[i + j][c], dw[j][c]);
+                        for (int j = 0; j < W; ++j) dw[j][c] = seq_fma(gm, x[i + j][c], dw[j][c]);
                     }
                 }
             } else {
 #pragma unroll
                 for (int i = 0; i < TB; ++i)
 #pragma unroll
-                    for (int c = 0; c < V; ++c) dp[WM - 1 + i][c] = CT(0);
+                    for (int c = 0; c < V; ++c) dp[W - 1 + i][c] = CT(0);
             }
-            // row t - (WM - 1) + i has all its uses now: tap WM - 1 - j met it in output row t - (WM - 1) + i + j
+            // row t - (W - 1) + i has all its uses now: tap W - 1 - j met it in output row t - (W - 1) + i + j
             CT o[TB][V];
 #pragma unroll
             for (int i = 0; i < TB; ++i)
@@ -339,10 +327,10 @@ __global__ __launch_bounds__(256, WM == 4 && (YT == CRNN_DT_BF16 || YT == CRNN_D
                 for (int c = 0; c < V; ++c) {
                     CT s = CT(0);
 #pragma unroll
-                    for (int j = 0; j < WM; ++j) s = seq_fma(w[WM - 1 - j][c], dp[i + j][c], s);
+                    for (int j = 0; j < W; ++j) s = seq_fma(w[W - 1 - j][c], dp[i + j][c], s);
                     o[i][c] = s;
                 }
-            const int r0 = t - (WM - 1);
+            const int r0 = t - (W - 1);
             if (r0 >= (lo > 0 ? lo : 0) && r0 + TB <= hi && !(p.dst_out.p && r0 + TB > len - back)) {
 #pragma unroll
                 for (int i = 0; i < TB; ++i) conv_put<YT, V>(orow + (int64_t)(r0 + i) * os, a.d, o[i]);
@@ -362,7 +350,7 @@ __global__ __launch_bounds__(256, WM == 4 && (YT == CRNN_DT_BF16 || YT == CRNN_D
                 }
             }
 #pragma unroll
-            for (int j = 0; j < WM - 1; ++j)
+            for (int j = 0; j < W - 1; ++j)
 #pragma unroll
                 for (int c = 0; c < V; ++c) {
                     x[j][c] = x[j + TB][c];
@@ -370,15 +358,12 @@ __global__ __launch_bounds__(256, WM == 4 && (YT == CRNN_DT_BF16 || YT == CRNN_D
                 }
         }
     }
-    CT *part = (CT *)p.part + a.b * (p.W + 1) * p.D + a.d;
+    CT *part = (CT *)p.part + a.b * (W + 1) * p.D + a.d;
 #pragma unroll
     for (int c = 0; c < V; ++c) {
 #pragma unroll
-        for (int j = 0; j < WM; ++j) {
-            const int k = j - (WM - p.W);
-            if (k >= 0) part[(int64_t)k * p.D + c] = dw[j][c];
-        }
-        part[(int64_t)p.W * p.D + c] = db[c];
+        for (int j = 0; j < W; ++j) part[(int64_t)j * p.D + c] = dw[j][c];
+        part[(int64_t)W * p.D + c] = db[c];
     }
 }
 
@@ -391,7 +376,7 @@ struct ConvStepP {
     int64_t rows, n_slots;
     int32_t D, W, silu;
 };
-template <int YT, int WM, int V>
+template <int YT, int W, int V>
 __global__ __launch_bounds__(256) void seq_conv_step_kernel(const ConvStepP p) {
     using CT = typename SeqT<YT>::C;
     constexpr int ES = ConvRaw<YT, V>::ES;
@@ -412,17 +397,13 @@ __global__ __launch_bounds__(256) void seq_conv_step_kernel(const ConvStepP p) {
         return;
     }
     // all that the row reads is on its way before other rows' slots are looked at
-    CT w[WM][V], bias[V], x[WM][V];
+    CT w[W][V], bias[V], x[W][V];
     char *st = (char *)p.st.p + slot * p.st.bs * ES;
-    ConvRaw<YT, V> q, qs[WM - 1];
+    ConvRaw<YT, V> q, qs[W > 1 ? W - 1 : 1];
 #pragma unroll
-    for (int j = 0; j < WM - 1; ++j) {
-        const int k = j - (WM - p.W);
-        if (k >= 0) qs[j].load(st + k * (int64_t)p.st.rs * ES, nullptr, d);
-        else qs[j] = ConvRaw<YT, V>{};
-    }
+    for (int j = 0; j < W - 1; ++j) qs[j].load(st + j * (int64_t)p.st.rs * ES, nullptr, d);
     q.load((const char *)p.x.p + r * (int64_t)p.x.rs * ES, nullptr, d);
-    conv_weights<CT, WM, V>(p.w, p.bias, p.W, d, w, bias);
+    conv_weights<CT, W, V>(p.w, p.bias, d, w, bias);
     int64_t nx = -1;
     if (p.slot && p.rows > 1) {
         if (threadIdx.x == 0) { before = 0; next = 0x7fffffff; }
@@ -433,21 +414,21 @@ __global__ __launch_bounds__(256) void seq_conv_step_kernel(const ConvStepP p) {
         nx = next == 0x7fffffff ? -1 : next;
     }
 #pragma unroll
-    for (int j = 0; j < WM - 1; ++j)
+    for (int j = 0; j < W - 1; ++j)
 #pragma unroll
         for (int c = 0; c < V; ++c) x[j][c] = qs[j].get(c);
     for (;;) {
         CT y[V];
 #pragma unroll
         for (int c = 0; c < V; ++c) {
-            x[WM - 1][c] = q.get(c);
+            x[W - 1][c] = q.get(c);
             CT s = bias[c];
 #pragma unroll
-            for (int j = 0; j < WM; ++j) s = seq_fma(w[j][c], x[j][c], s);
+            for (int j = 0; j < W; ++j) s = seq_fma(w[j][c], x[j][c], s);
             const CT g = s * seq_sigmoid(s);
             y[c] = p.silu ? g : s;
 #pragma unroll
-            for (int j = 0; j < WM - 1; ++j) x[j][c] = x[j + 1][c];
+            for (int j = 0; j < W - 1; ++j) x[j][c] = x[j + 1][c];
         }
         if (on) conv_put<YT, V>(yp + r * (int64_t)p.y.rs * ES, d, y);
         if (nx < 0) break;
@@ -462,10 +443,7 @@ __global__ __launch_bounds__(256) void seq_conv_step_kernel(const ConvStepP p) {
     }
     if (!on) return;
 #pragma unroll
-    for (int j = 0; j < WM - 1; ++j) {
-        const int k = j - (WM - p.W);
-        if (k >= 0) conv_put<YT, V>(st + k * (int64_t)p.st.rs * ES, d, x[j]);
-    }
+    for (int j = 0; j < W - 1; ++j) conv_put<YT, V>(st + j * (int64_t)p.st.rs * ES, d, x[j]);
 }
 
 }  // namespace crnn

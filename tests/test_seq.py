@@ -548,6 +548,43 @@ def test_infinities_and_nan_stay_in_their_channel_and_after_their_row():
     assert int((~torch.isfinite(c)).sum()) == 4 and not bool(torch.isfinite(c[0, 20:24, 3]).any())
 
 
+def not_finite(x):
+    return ~torch.isfinite(x.float()).cpu()
+
+
+@gpu
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f64"])
+@pytest.mark.parametrize("D", [5, 40])
+@pytest.mark.parametrize("W", range(1, 9))
+def test_convolution_takes_nothing_from_rows_its_taps_do_not_reach(W, D, dtype):
+    """An infinity and a NaN reach W rows of their own channel, forward, back and in single rows that share a state; all else keeps its bits."""
+    g = torch.Generator().manual_seed(W)
+    T, dt = 70, DT[dtype]
+    x, dy, w, b = rnd(g, 1, T, D, dtype=dt), rnd(g, 1, T, D, dtype=dt), rnd(g, D, W, dtype=param_of(dt)).abs() + 0.1, rnd(g, D, dtype=param_of(dt))
+    bx, bdy = x.clone(), dy.clone()
+    hit = torch.zeros(1, T, D, dtype=torch.bool)        # rows that see the bad input; back: rows seen by it
+    back = hit.clone()
+    for t, d, v in ((10, 1, math.inf), (33, D - 1, math.nan), (T - 1, 0, -math.inf)):
+        bx[0, t, d] = bdy[0, t, d] = v
+        hit[0, t:t + W, d] = True
+        back[0, max(t - W + 1, 0):t + 1, d] = True
+    y, z = seq.causal_conv(x, w, b), seq.causal_conv(bx, w, b)
+    assert torch.equal(not_finite(z), hit) and torch.equal(z.cpu()[~hit], y.cpu()[~hit])
+    y, z = seq.causal_conv_grad(dy, x, w, b).x, seq.causal_conv_grad(bdy, x, w, b).x
+    assert torch.equal(not_finite(z), back) and torch.equal(z.cpu()[~back], y.cpu()[~back])
+    at = torch.zeros(T, dtype=torch.int32, device=DEV)
+    states = [torch.zeros(1, W - 1, D, dtype=dt, device=DEV) for _ in range(2)]
+    y, z = (seq.causal_conv_step(v[0], w, b, s, at) for v, s in zip((x, bx), states))
+    assert torch.equal(not_finite(z), hit[0]) and torch.equal(z.cpu()[~hit[0]], y.cpu()[~hit[0]])
+    if dtype != "f64":          # a block that a checkpoint gives back as NaN, met by the gate's derivative
+        bx = x.clone()
+        bx[0, 33, 2] = math.inf
+        y, z = (seq.causal_conv_grad(dy, seq.pack8(v), w, b, silu=True).x for v in (x, bx))
+        near = torch.zeros(1, T, D, dtype=torch.bool)
+        near[0, 33 - W + 1:33 + W, :32] = True
+        assert torch.equal(not_finite(z), near) and torch.equal(z.cpu()[~near], y.cpu()[~near])
+
+
 @gpu
 @pytest.mark.parametrize("starts", [[0, 90, 40, 60], [-5, 20, 300], [50, 10], [0]])
 def test_offsets_that_make_no_sense_stay_inside_the_arrays(starts):
