@@ -295,7 +295,7 @@ __global__ __launch_bounds__(256, W <= 4 && (YT == CRNN_DT_BF16 || YT == CRNN_DT
                 __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
                 for (int i = 0; i < TB; ++i) {
-                    const bool in = t + i <= lastrow, mine = t + i < hi;
+                    const bool in = t + i <= lastrow;
 #pragma unroll
                     for (int c = 0; c < V; ++c) {
                         CT s = bias[c];
@@ -305,12 +305,15 @@ __global__ __launch_bounds__(256, W <= 4 && (YT == CRNN_DT_BF16 || YT == CRNN_DT
                         CT g = dp[W - 1 + i][c];
                         const CT ga = g * (sg * seq_fma(s, CT(1) - sg, CT(1)));
                         g = p.silu ? ga : g;
-                        g = in ? g : CT(0);
-                        dp[W - 1 + i][c] = g;
-                        const CT gm = mine ? g : CT(0);
-                        db[c] += gm;
+                        dp[W - 1 + i][c] = in ? g : CT(0);
+                    }
+                    if (t + i < hi) {       // the strip's own rows only: one behind them would add 0 times its x, which an infinity makes NaN
 #pragma unroll
-                        for (int j = 0; j < W; ++j) dw[j][c] = seq_fma(gm, x[i + j][c], dw[j][c]);
+                        for (int c = 0; c < V; ++c) {
+                            db[c] += dp[W - 1 + i][c];
+#pragma unroll
+                            for (int j = 0; j < W; ++j) dw[j][c] = seq_fma(dp[W - 1 + i][c], x[i + j][c], dw[j][c]);
+                        }
                     }
                 }
             } else {

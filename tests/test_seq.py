@@ -586,6 +586,33 @@ def test_convolution_takes_nothing_from_rows_its_taps_do_not_reach(W, D, dtype):
 
 
 @gpu
+@pytest.mark.parametrize("D,dtype", [(5, "f32"), (40, "bf16"), (40, "f64")])
+@pytest.mark.parametrize("W", range(1, 9))
+def test_weight_gradient_takes_each_row_with_its_own_taps_only(W, D, dtype):
+    """dweight[d, j] = sum_t dp[t] x[t - W + 1 + j]: the last row meets the last tap alone, the one before it the last two, and so on."""
+    g = torch.Generator().manual_seed(W)
+    lens, dt = [70, 1, 47], DT[dtype]
+    at = torch.tensor(np.concatenate([[0], np.cumsum(lens)]), dtype=torch.int32, device=DEV)
+    x, dy, w = rnd(g, sum(lens), D, dtype=dt), rnd(g, sum(lens), D, dtype=dt).abs() + 0.1, rnd(g, D, W, dtype=param_of(dt))
+    clean = seq.causal_conv_grad(dy, x, w, torch.zeros(D, device=DEV), seq_start=at)
+    for s, n in enumerate(lens):
+        for back in range(min(n, W + 1)):
+            row, bad = int(at[s + 1]) - 1 - back, x.clone()
+            bad[row, D - 1] = math.inf
+            got = seq.causal_conv_grad(dy, bad, w, torch.zeros(D, device=DEV), seq_start=at)
+            want = torch.zeros(D, W, dtype=torch.bool)
+            want[D - 1, max(W - 1 - back, 0):] = True
+            assert torch.equal(got.weight.cpu() == math.inf, want) and torch.equal(got.weight.cpu()[~want], clean.weight.cpu()[~want]), (row, back)
+            assert torch.equal(got.bias, clean.bias) and torch.equal(got.x, clean.x)
+    # rows at the ends of the strips that a long sequence is cut into
+    for row in (8, 15, 23, 31, 47, 63):
+        bad = x.clone()
+        bad[row, 1] = math.inf
+        got = seq.causal_conv_grad(dy, bad, w, seq_start=at)
+        assert torch.equal(got.weight[1].cpu() == math.inf, torch.arange(W) >= W - 1 - (lens[0] - 1 - row)) and torch.equal(got.weight[2:], clean.weight[2:])
+
+
+@gpu
 @pytest.mark.parametrize("starts", [[0, 90, 40, 60], [-5, 20, 300], [50, 10], [0]])
 def test_offsets_that_make_no_sense_stay_inside_the_arrays(starts):
     g = torch.Generator().manual_seed(1)
