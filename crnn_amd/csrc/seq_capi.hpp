@@ -217,11 +217,13 @@ void scan_forward_run(const crnn_scan_args *a, ScanPlan &s, hipStream_t st) {
         p.first = b == 0;
         p.fin = b == s.nb - 1;
         if (s.split) {
-            hipLaunchKernelGGL((crnn::seq_scan_fwd_kernel<IO, NS, MODE, false>), grid, block, 0, st, p, (const CT *)nullptr, S, sdel);
+            hipLaunchKernelGGL((crnn::seq_scan_fwd_kernel<IO, NS, MODE, false, false>), grid, block, 0, st, p, (const CT *)nullptr, S, sdel);
             hipLaunchKernelGGL((crnn::seq_scan_carry_kernel<CT, NS>), dim3((unsigned)(((int64_t)p.m.n_seq * NS * p.D + 255) / 256)), dim3(256), 0, st, p, S,
                                (CT *)nullptr, (const CT *)sdel);
         }
-        hipLaunchKernelGGL((crnn::seq_scan_fwd_kernel<IO, NS, MODE, true>), grid, block, 0, st, p, (const CT *)(s.split ? S : nullptr), (CT *)nullptr, (CT *)nullptr);
+        const CT *start = s.split ? S : nullptr;
+        if (p.n0 + NS <= p.N) hipLaunchKernelGGL((crnn::seq_scan_fwd_kernel<IO, NS, MODE, true, false>), grid, block, 0, st, p, start, (CT *)nullptr, (CT *)nullptr);
+        else hipLaunchKernelGGL((crnn::seq_scan_fwd_kernel<IO, NS, MODE, true, true>), grid, block, 0, st, p, start, (CT *)nullptr, (CT *)nullptr);
     }
 }
 
@@ -241,7 +243,8 @@ void scan_backward_run(const crnn_scan_args *a, ScanPlan &s, hipStream_t st) {
         hipLaunchKernelGGL((crnn::seq_scan_ends2_kernel<IO, NS, MODE>), grid, block, 0, st, p, S, Gb, sdel);
         hipLaunchKernelGGL((crnn::seq_scan_carry_kernel<CT, NS>), dim3((unsigned)(((int64_t)p.m.n_seq * NS * p.D + 255) / 256)), dim3(256), 0, st, p, S, Gb,
                            (const CT *)sdel);
-        hipLaunchKernelGGL((crnn::seq_scan_bwd_kernel<IO, NS, MODE>), grid, block, 0, st, p, (const CT *)S, (const CT *)Gb, part, pp);
+        if (p.n0 + NS <= p.N) hipLaunchKernelGGL((crnn::seq_scan_bwd_kernel<IO, NS, MODE, false>), grid, block, 0, st, p, (const CT *)S, (const CT *)Gb, part, pp);
+        else hipLaunchKernelGGL((crnn::seq_scan_bwd_kernel<IO, NS, MODE, true>), grid, block, 0, st, p, (const CT *)S, (const CT *)Gb, part, pp);
         if (s.flat > 0)
             hipLaunchKernelGGL((crnn::seq_scan_sum_maps_kernel<CT, NS>), dim3(seq_grid(s.flat * p.G * 2 * NS)), dim3(256), 0, st, p.m, mo, (const CT *)part, p.tpg);
         hipLaunchKernelGGL((crnn::seq_sum_blocks_kernel<CT>), dim3((unsigned)((cA + 31) / 32)), dim3(256), 0, st, (const CT *)pp, p.m.nblk, cA, (CT *)a->dA,

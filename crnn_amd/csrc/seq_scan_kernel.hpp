@@ -101,6 +101,8 @@ __device__ __forceinline__ void scan_rates(const ScanP &p, int d, int n, CT (&A2
 #pragma unroll
     for (int j = 0; j < K; ++j) A2[j] *= CT(kLog2eD);
 }
+// PAD: N does not fill the launch's NS states.  The states behind the last one have rates, maps and first states of 0, but 0 times an infinite step length,
+// input or gradient is NaN: they are put to 0 after every row, or what is summed over the states would take it up.
 // what a launch may meet: 0 plain arrays, all states at once; 1 the same with u, and z if there is one, as checkpoints; 2 anything
 constexpr int kScanAny = 2;
 
@@ -198,7 +200,7 @@ struct ScanShare {
 
 // ---- forward, a chunk.  OUT: outputs from its first state (start[block][n][d]; null: one chunk a sequence, from state_in), and the sequence's
 // last state.  Not OUT: S = the chunk's last state from zero and the sum of delta (a sequence's last chunk is not asked).
-template <int IO, int NS, int MODE, bool OUT>
+template <int IO, int NS, int MODE, bool OUT, bool PAD>
 __global__ __launch_bounds__(64 * kScanWaves, IO == 8 ? 3 : 6) void seq_scan_fwd_kernel(const ScanP p, const typename SeqIO<IO>::C *__restrict__ start,
                                                                                       typename SeqIO<IO>::C *__restrict__ S, typename SeqIO<IO>::C *__restrict__ sdel) {
     using CT = typename SeqIO<IO>::C;
@@ -212,6 +214,7 @@ __global__ __launch_bounds__(64 * kScanWaves, IO == 8 ? 3 : 6) void seq_scan_fwd
     const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)), lane = threadIdx.x & 63;
     if (OUT && p.zero_outside && fin && wave == 0) seq_zero_outside(p.m, p.y, a.b, a.d, a.valid);
     if (!a.k.live || (!OUT && a.k.last)) return;
+    const int lim = p.N - p.n0;
     CT A2[NW], h[NW], sd = CT(0);
     scan_rates<CT, NW>(p, a.d, p.n0 + wave * NW, A2);
     if (OUT && start) {
@@ -277,6 +280,7 @@ __global__ __launch_bounds__(64 * kScanWaves, IO == 8 ? 3 : 6) void seq_scan_fwd
 #pragma unroll
                 for (int j = 0; j < NW; ++j) {
                     h[j] = seq_fma(seq_exp2(d * A2[j]), h[j], du * b[j]);
+                    if (PAD) h[j] = wave * NW + j < lim ? h[j] : CT(0);
                     if (OUT) v = seq_fma(h[j], c[j], v);
                 }
                 if (OUT) sh.v[OUT ? wave : 0][OUT ? i : 0][lane] = v;
@@ -464,7 +468,7 @@ __global__ __launch_bounds__(256) void seq_scan_carry_kernel(const ScanP p, CT *
 // 6144 rows of 2048 channels, 16 states, u and z in 8 bits: 275 us (239 where they are plain), vector unit busy 69 %: 33 vector instructions a row, channel and state (21 of
 // them the reverse row, folds of dB and dC included), the rest of the time both wavefronts of a SIMD wait (a row's maps from the LDS, the next rows).
 constexpr int kScanBwdTB = 4, kScanBwdSub = 5, kScanBwdQ = kScanBwdTB * kScanBwdSub;
-template <int IO, int NS, int MODE>
+template <int IO, int NS, int MODE, bool PAD>
 __global__ __launch_bounds__(64 * kScanWaves, 2) void seq_scan_bwd_kernel(const ScanP p, const typename SeqIO<IO>::C *__restrict__ start,
                                                                           const typename SeqIO<IO>::C *__restrict__ back, typename SeqIO<IO>::C *__restrict__ part,
                                                                           typename SeqIO<IO>::C *__restrict__ ppart) {
@@ -486,6 +490,8 @@ __global__ __launch_bounds__(64 * kScanWaves, 2) void seq_scan_bwd_kernel(const 
 #pragma unroll
     for (int n = 0; n < NS; ++n) dA[n] = CT(0);
     if (a.k.live && a.k.n > 0) {
+        const int lim = p.N - p.n0;
+        auto real = [&](int n, CT x) { return !PAD || n < lim ? x : CT(0); };
         CT A2[NS], h[NS], q[NS];
         scan_rates<CT, NS>(p, a.d, p.n0, A2);
 #pragma unroll
@@ -553,7 +559,7 @@ __global__ __launch_bounds__(64 * kScanWaves, 2) void seq_scan_bwd_kernel(const 
                 const CT du = dl[i] * u[i];
 #pragma unroll
                 for (int n = 0; n < NS; ++n) {
-                    ah[i][n] = seq_exp2(dl[i] * A2[n]) * h[n];
+                    ah[i][n] = real(n, seq_exp2(dl[i] * A2[n]) * h[n]);
                     h[n] = seq_fma(du, bc[n], ah[i][n]);
                 }
             }
@@ -579,8 +585,8 @@ __global__ __launch_bounds__(64 * kScanWaves, 2) void seq_scan_bwd_kernel(const 
 #pragma unroll
                     for (int s = 0; s < 2; ++s) {
                         const int n = j + s * H;
-                        const CT hn = seq_fma(du, bc[n], ah[i][n]);
-                        q[n] = seq_fma(r, bc[NS + n], q[n]);
+                        const CT hn = real(n, seq_fma(du, bc[n], ah[i][n]));
+                        q[n] = real(n, seq_fma(r, bc[NS + n], q[n]));
                         v = seq_fma(hn, bc[NS + n], v);
                         qb = seq_fma(q[n], bc[n], qb);
                         const CT m = q[n] * ah[i][n];
@@ -796,7 +802,7 @@ __global__ __launch_bounds__(256) void seq_scan_step_kernel(const ScanStepP p) {
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const bool in = n0 + i < p.N;
-                h[c][i] = seq_fma(seq_exp2(dlt * A2[c][i]), h[c][i], in ? du * scan_value<IO>(row.b[i], p.u.dt) : CT(0));
+                h[c][i] = in ? seq_fma(seq_exp2(dlt * A2[c][i]), h[c][i], du * scan_value<IO>(row.b[i], p.u.dt)) : CT(0);
                 v = seq_fma(h[c][i], in ? scan_value<IO>(row.c[i], p.u.dt) : CT(0), v);
             }
             if (p.lpc > 1) v += seq_dpp<0xb1>(v);

@@ -612,6 +612,64 @@ def test_weight_gradient_takes_each_row_with_its_own_taps_only(W, D, dtype):
         assert torch.equal(got.weight[1].cpu() == math.inf, torch.arange(W) >= W - 1 - (lens[0] - 1 - row)) and torch.equal(got.weight[2:], clean.weight[2:])
 
 
+def alike(got, want, scale, k, what):
+    """Finite where the 64-bit form is, and there like it."""
+    g, w = got.detach().cpu(), want.cpu()
+    assert torch.equal(torch.isfinite(g), torch.isfinite(w)), (what, torch.isfinite(g) ^ torch.isfinite(w))
+    ok = torch.isfinite(w)
+    check(g[ok], w[ok], torch.nan_to_num(scale.cpu()[ok], nan=math.inf, posinf=math.inf), k, what)
+
+
+def scan_with(T, D, N, bad, dtype=torch.float32, skip=True, seed=0):
+    """Positive inputs (no sum of two infinities is NaN), `bad` = {(array, row, channel): value} put into them."""
+    g = torch.Generator().manual_seed(seed + N)
+    c = {k: rnd(g, T, n, dtype=dtype).abs() + 0.1 for k, n in (("u", D), ("dt", D), ("z", D), ("dy", D), ("B", N), ("C", N))}
+    c.update(A=-(rnd(g, D, N).abs() + 0.1), D=rnd(g, D).abs() + 0.1 if skip else None, bias=None, state=rnd(g, 1, D, N).abs(), dstate=rnd(g, 1, D, N).abs(), spans=[(0, T)],
+             kw=dict(seq_start=torch.tensor([0, T], dtype=torch.int32, device=DEV)))
+    for (name, row, col), v in bad.items():
+        c[name][row, col] = v
+    return c
+
+
+def scan_all(c):
+    """{name: (result, how it is called in the 64-bit form)} of the forward call and the gradient."""
+    kw = dict(D=c["D"], z=c["z"], state=c["state"], softplus=False, **c["kw"])
+    y, end = seq.selective_scan(c["u"], c["dt"], c["A"], c["B"], c["C"], return_state=True, **kw)
+    g = seq.selective_scan_grad(c["dy"], c["u"], c["dt"], c["A"], c["B"], c["C"], dstate=c["dstate"], **kw)
+    return {"y": y, "end": end, **{k: v for k, v in g._asdict().items() if v is not None}}
+
+
+def scan_all_plain(c):
+    N = c["A"].shape[1]
+    m = lambda x: cpu64(x).view(-1, 1, N)  # noqa: E731
+    p = plain_scan(cpu64(c["u"]), cpu64(c["dt"]), cpu64(c["A"]), m(c["B"]), m(c["C"]), cpu64(c["D"]), cpu64(c["z"]), None, False, c["spans"], cpu64(c["state"]), dy=cpu64(c["dy"]),
+                   dstate=cpu64(c["dstate"]))
+    g = {k: tuple(v) for k, v in p["grad"].items()}
+    g["B"], g["C"] = (tuple(v.view(-1, N) for v in g[k]) for k in ("B", "C"))
+    return {"y": p["y"], "end": p["state"], **g}
+
+
+@gpu
+@pytest.mark.parametrize("T", [50, 150])
+@pytest.mark.parametrize("N", [1, 5, 8, 11, 16, 20, 32, 37])
+@pytest.mark.parametrize("name,row", [("u", 5), ("u", 44), ("dt", 23), ("dy", 30), ("dt", 49)])
+def test_states_that_are_not_there_take_no_part(name, row, N, T):
+    """Any number of states, an infinity in the data: infinite where the formula is, finite where it is finite."""
+    c = scan_with(T, 7, N, {(name, row, 3): math.inf})
+    got, want = scan_all(c), scan_all_plain(c)
+    for k, v in got.items():
+        alike(v, *want[k], 60 + N + 8 * 16, k)
+    # the single step: the row with the infinity, its state and the row behind it
+    st = c["state"].clone()
+    at = torch.zeros(2, dtype=torch.int32, device=DEV)
+    s = lambda k: c[k][row - 1:row + 1]  # noqa: E731
+    y = seq.selective_scan_step(s("u"), s("dt"), c["A"], s("B"), s("C"), st, at, D=c["D"], z=s("z"), softplus=False)
+    m = lambda k: cpu64(s(k)).view(2, 1, N)  # noqa: E731
+    p = plain_scan(cpu64(s("u")), cpu64(s("dt")), cpu64(c["A"]), m("B"), m("C"), cpu64(c["D"]), cpu64(s("z")), None, False, [(0, 2)], cpu64(c["state"]))
+    alike(y, *p["y"], 60 + N, "step")
+    alike(st, *p["state"], 60, "state")
+
+
 @gpu
 @pytest.mark.parametrize("starts", [[0, 90, 40, 60], [-5, 20, 300], [50, 10], [0]])
 def test_offsets_that_make_no_sense_stay_inside_the_arrays(starts):
