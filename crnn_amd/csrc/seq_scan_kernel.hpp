@@ -300,7 +300,7 @@ __global__ __launch_bounds__(64 * kScanWaves, IO == 8 ? 3 : 6) void seq_scan_fwd
                         if (!fin && a.valid) *acc = v;
                     }
                     if (!fin) continue;
-                    v = seq_fma(skip, u[i], v);
+                    v = p.Dskip ? seq_fma(skip, u[i], v) : v;        // (absent: not 0 times an infinite input)
                     const CT g = z[i] * seq_sigmoid(z[i]);
                     v = p.gate ? v * g : v;
                     seq_store(p.y, seq_off(p.m, p.y, a.k, a.k.t0 + row) + a.d, v);     // (lanes without a channel: the last channel's value again)
@@ -612,9 +612,10 @@ __global__ __launch_bounds__(64 * kScanWaves, 2) void seq_scan_bwd_kernel(const 
                 ddt = in ? ddt : CT(0);
                 dD = seq_fma(r, u[i], dD);
                 db += ddt;
-                odu[i] = seq_fma(dl[i], qb, r * skip);
+                odu[i] = seq_fma(dl[i], qb, p.Dskip ? r * skip : CT(0));
                 odt[i] = ddt;
-                odz[i] = yi * seq_fma(skip, u[i], v) * (sg * seq_fma(zi, CT(1) - sg, CT(1)));
+                v = p.Dskip ? seq_fma(skip, u[i], v) : v;
+                odz[i] = yi * v * (sg * seq_fma(zi, CT(1) - sg, CT(1)));
             }
             seq_wave_sync();
             if (fin) {
@@ -808,7 +809,7 @@ __global__ __launch_bounds__(256) void seq_scan_step_kernel(const ScanStepP p) {
             if (p.lpc > 1) v += seq_dpp<0xb1>(v);
             if (p.lpc > 2) v += seq_dpp<0x4e>(v);
             for (int k = 4; k < p.lpc; k <<= 1) v += __shfl_xor(v, k);
-            v = seq_fma(skip[c], u, v);
+            v = p.Dskip ? seq_fma(skip[c], u, v) : v;
             const CT vz = v * (z * seq_sigmoid(z));
             v = p.gate ? vz : v;
             if (sub == 0 && d0 + c * cpb < p.D) seq_store(p.y, r * (int64_t)p.y.rs + d[c], v);

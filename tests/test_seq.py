@@ -671,6 +671,28 @@ def test_states_that_are_not_there_take_no_part(name, row, N, T):
 
 
 @gpu
+@pytest.mark.parametrize("T", [50, 150])
+@pytest.mark.parametrize("N", [8, 16, 32])
+@pytest.mark.parametrize("name,row", [("u", 5), ("u", 44), ("dy", 30)])
+def test_absent_skip_is_not_a_skip_of_zero(name, row, N, T):
+    """Without D there is no D u: an infinite u comes through the states as an infinity, not as NaN, and so does an infinite gradient back to u."""
+    c = scan_with(T, 7, N, {(name, row, 3): math.inf}, skip=False)
+    got, want = scan_all(c), scan_all_plain(c)
+    for k in ("y", "u", "z"):
+        v, (w, s) = got[k].cpu(), want[k]
+        reach = {"u": {"y": slice(row, T), "u": None, "z": slice(row, T)}, "dy": {"y": None, "u": slice(0, row + 1), "z": slice(row, row + 1)}}[name][k]
+        bad = torch.zeros(T, 7, dtype=torch.bool)
+        if reach is not None:
+            bad[reach, 3] = True
+        assert torch.equal(v == math.inf, bad) and not bool(torch.isnan(v).any()), k
+        check(v[~bad], w[~bad], torch.nan_to_num(s[~bad], nan=math.inf, posinf=math.inf), 60 + N + 8 * 16, k)
+    st = c["state"].clone()
+    s = lambda k: c[k][row:row + 1]  # noqa: E731
+    y = seq.selective_scan_step(s("u"), s("dt"), c["A"], s("B"), s("C"), st, z=s("z"), softplus=False).cpu()[0]
+    assert bool((y == math.inf)[3]) == (name == "u") and int(torch.isfinite(y).sum()) == (6 if name == "u" else 7)
+
+
+@gpu
 @pytest.mark.parametrize("starts", [[0, 90, 40, 60], [-5, 20, 300], [50, 10], [0]])
 def test_offsets_that_make_no_sense_stay_inside_the_arrays(starts):
     g = torch.Generator().manual_seed(1)
