@@ -66,6 +66,16 @@ __device__ __forceinline__ double seq_softplus(double x) {
     return (x > 0.0 ? x : (x == x ? 0.0 : x)) + log1p(exp(-fabs(x)));
 }
 
+__device__ __forceinline__ float seq_ldexp(float x, int e) { return __builtin_ldexpf(x, e); }
+__device__ __forceinline__ double seq_ldexp(double x, int e) { return __builtin_ldexp(x, e); }
+// h 2^x where 2^x alone may be out of the type's range (growth over a whole chunk: 0 stays 0, and a small h may come out in range)
+template <class CT>
+__device__ __forceinline__ CT seq_grow(CT h, CT x) {
+    x = x > CT(10000) ? CT(10000) : x < CT(-10000) ? CT(-10000) : x;      // (behind either type's range; a NaN stays one)
+    const CT w = __builtin_elementwise_rint(x);
+    return seq_ldexp(h * seq_exp2(x - w), (int)w);
+}
+
 // ---- a caller-owned array [sequence][row][channel], channels contiguous
 struct SeqV {
     void *p;

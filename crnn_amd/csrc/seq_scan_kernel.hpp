@@ -394,6 +394,34 @@ __global__ __launch_bounds__(64 * kScanWaves, IO == 8 ? 2 : 3) void seq_scan_end
             }
             seq_wave_sync();
         }
+        // decays above one (a positive rate, a negative step length) may have taken P out of range, where it makes NaN of an r C of 0: then G row by row
+        // from the last to the first, as the formula has it
+        bool out = false;
+#pragma unroll
+        for (int n = 0; n < NS; ++n) out = out || !(P[n] <= CT(IO == 8 ? 1.7976931348623157e308 : 3.4028234e38));
+        if (__builtin_amdgcn_ballot_w64(out)) {
+#pragma unroll
+            for (int n = 0; n < NS; ++n) g[n] = CT(0);
+#pragma unroll 1
+            for (int t = a.k.n - 1; t >= 0; --t) {
+                SeqRows<IO, MODE, 1> qz;
+                SeqRows<IO, 0, 1> qd, qy;
+                CT z[1], x[1], y[1];
+                qd.load(p.m, p.dt, a.k, t, a.d);
+                qy.load(p.m, p.dy, a.k, t, a.d);
+                qz.load(p.m, p.z, a.k, t, a.d);
+                qd.get(p.dt, x);
+                qy.get(p.dy, y);
+                qz.get(p.z, z);
+                const CT dl = p.softplus ? seq_softplus(x[0] + bias) : x[0] + bias, r = p.gate ? y[0] * (z[0] * seq_sigmoid(z[0])) : y[0];
+                const int64_t c0 = seq_off(p.m, p.C, a.k, a.k.t0 + t) + a.g * p.Cg;
+#pragma unroll
+                for (int n = 0; n < NS; ++n) {
+                    const CT c = p.n0 + n < p.N ? seq_load1(p.C, c0 + (p.n0 + n) * p.Cn, CT(0)) : CT(0);
+                    g[n] = seq_fma(r, c, g[n]) * seq_exp2(dl * A2[n]);
+                }
+            }
+        }
     }
     if (!a.valid) return;
 #pragma unroll
@@ -419,7 +447,7 @@ __global__ __launch_bounds__(256) void seq_scan_carry_kernel(const ScanP p, CT *
     const int64_t b0 = seq_first_block(p.m, s), nc = len > 0 ? (len + p.m.Q - 1) / p.m.Q : 1;
     const int64_t at = (s * p.D + d) * p.N + p.n0 + n;
     const CT A2 = ((const CT *)p.A)[(int64_t)d * p.N + p.n0 + n] * CT(kLog2eD);
-    // the loads of eight chunks at once; the sequence of chunks itself is one multiply-add each
+    // the loads of eight chunks at once; the sequence of chunks itself is a scaled product (seq_grow) and a sum each
     constexpr int CB = 8;
     const int64_t stride = (int64_t)NS * p.D;
     CT *Sp = S + (b0 * NS + n) * p.D + d;
@@ -436,7 +464,7 @@ __global__ __launch_bounds__(256) void seq_scan_carry_kernel(const ScanP p, CT *
 #pragma unroll
         for (int i = 0; i < CB; ++i) {
             if (c0 + i < nc) Sp[(c0 + i) * stride] = h;
-            h = seq_fma(seq_exp2(A2 * e[i]), h, own[i]);
+            h = seq_grow(h, A2 * e[i]) + own[i];
         }
     }
     if (!Gb) return;
@@ -454,7 +482,7 @@ __global__ __launch_bounds__(256) void seq_scan_carry_kernel(const ScanP p, CT *
         for (int i = 0; i < CB; ++i)
             if (c0 - i >= 0) {
                 Gp[(c0 - i) * stride] = q;
-                q = seq_fma(seq_exp2(A2 * e[i]), q, own[i]);
+                q = seq_grow(q, A2 * e[i]) + own[i];
             }
     }
     if (p.dstate_in) ((CT *)p.dstate_in)[at] = q;

@@ -693,6 +693,35 @@ def test_absent_skip_is_not_a_skip_of_zero(name, row, N, T):
 
 
 @gpu
+@pytest.mark.parametrize("T", [40, 70, 200])
+@pytest.mark.parametrize("N", [3, 16, 32])
+@pytest.mark.parametrize("sign", ["rate", "step"])
+@pytest.mark.parametrize("dtype", ["f32", "f64"])
+def test_modes_that_grow_stay_in_range_where_the_formula_does(sign, N, T, dtype):
+    """A positive rate, or a negative step length: exp(A sum delta) over a chunk is out of range (e^120 in 20 rows; double: e^1500), but nothing has come in yet,
+    or nothing is asked of it any more: the states and gradients are 0 there, not 0 times infinity."""
+    c = scan_with(T, 7, N, {}, dtype=DT[dtype])
+    for k in ("A", "D", "state", "dstate"):
+        c[k] = c[k].to(param_of(DT[dtype]))
+    c["A"][:, :] = c["A"] - 2 if sign == "step" else -c["A"] + 2
+    c["dt"] = c["dt"] * 0 + (3.0 if dtype == "f32" else 40.0) * (-1 if sign == "step" else 1)
+    c["u"][:T - 1], c["dy"][1:], c["state"][:], c["dstate"][:] = 0, 0, 0, 0
+    got, want = scan_all(c), scan_all_plain(c)
+    for k, v in got.items():
+        assert bool(torch.isfinite(want[k][0]).all()) and float(want[k][0].abs().max()) < (1e30 if dtype == "f32" else 1e300), k
+        alike(v, *want[k], 60 + N + 8 * 16, k)
+    # a state of 1e-30 that grows by e^96 in 16 rows comes out at 1e11
+    if dtype == "f32" and T > 64:
+        c["A"][:] = 2.0 if sign == "rate" else -2.0
+        c["dt"][:16], c["dt"][16:] = (3.0, 0.0) if sign == "rate" else (-3.0, 0.0)
+        c["u"][:], c["state"][:] = 0, 1e-30
+        y, end = seq.selective_scan(c["u"], c["dt"], c["A"], c["B"], c["C"], state=c["state"], softplus=False, return_state=True, **c["kw"])
+        want = math.exp(96 + math.log(float(c["state"][0, 0, 0])))
+        # 16 rows (or a chunk's one product) with an exponent's relative error of 2^-24 times its size each: 96 + 16 times 3 eps
+        assert bool(((end.double() / want - 1).abs() <= (96 + 48) * 2.0 ** -23).all())
+
+
+@gpu
 @pytest.mark.parametrize("starts", [[0, 90, 40, 60], [-5, 20, 300], [50, 10], [0]])
 def test_offsets_that_make_no_sense_stay_inside_the_arrays(starts):
     g = torch.Generator().manual_seed(1)
