@@ -95,11 +95,16 @@ __device__ __forceinline__ void scan_get(const ScanP &p, const void *x, int64_t 
         for (int j = 0; j < K; ++j) o[j] = x && n + j < p.N ? q[j] : CT(0);
     }
 }
+// Rates for exp2.  An infinite one counts as the type's largest: rows behind a chunk's n-th are steps of length 0, and 0 times infinity is NaN.
 template <class CT, int K>
 __device__ __forceinline__ void scan_rates(const ScanP &p, int d, int n, CT (&A2)[K]) {
+    constexpr CT top = CT(sizeof(CT) == 8 ? 1.7976931348623157e308 : 3.4028234663852886e38);
     scan_get<CT, K>(p, p.A, d, n, A2);
 #pragma unroll
-    for (int j = 0; j < K; ++j) A2[j] *= CT(kLog2eD);
+    for (int j = 0; j < K; ++j) {
+        A2[j] *= CT(kLog2eD);
+        A2[j] = A2[j] < -top ? -top : A2[j] > top ? top : A2[j];
+    }
 }
 // PAD: N does not fill the launch's NS states.  The states behind the last one have rates, maps and first states of 0, but 0 times an infinite step length,
 // input or gradient is NaN: they are put to 0 after every row, or what is summed over the states would take it up.
@@ -159,7 +164,8 @@ struct ScanMapRows {
             v[k] = at[(int64_t)(r < n ? r : n - 1) * rs];
         }
     }
-    __device__ __forceinline__ void put(int dt, CT *lds) const {
+    // nv: rows of the chunk from the first of these on.  Those behind are 0: they stand for the last row once more
+    __device__ __forceinline__ void put(int dt, CT *lds, int nv) const {
         const int lane = threadIdx.x & 63;
 #pragma unroll
         for (int k = 0; k < V; ++k) {
@@ -167,7 +173,7 @@ struct ScanMapRows {
             if (IO == 8) x = (CT)v[k];
             else if (IO == 4) x = (CT)seq_as_float((uint32_t)v[k]);
             else x = (CT)(dt == CRNN_DT_BF16 ? seq_as_float((uint32_t)v[k] << 16) : seq_from_f16((uint32_t)v[k]));
-            lds[k * 64 + lane] = in ? x : CT(0);
+            lds[k * 64 + lane] = in && row0 + k * RPV < nv ? x : CT(0);
         }
         seq_wave_sync();
     }
@@ -258,7 +264,7 @@ __global__ __launch_bounds__(64 * kScanWaves, IO == 8 ? 3 : 6) void seq_scan_fwd
                 if (IO == 8) m = (CT)mv[k];
                 else if (IO == 4) m = (CT)seq_as_float((uint32_t)mv[k]);
                 else m = (CT)(p.B.dt == CRNN_DT_BF16 ? seq_as_float((uint32_t)mv[k] << 16) : seq_from_f16((uint32_t)mv[k]));
-                if (R * 2 * NS >= 256 || mrow < R) sh.maps[(mrow + k * (256 / (2 * NS))) % R][mj] = min_ ? m : CT(0);
+                if (R * 2 * NS >= 256 || mrow < R) sh.maps[(mrow + k * (256 / (2 * NS))) % R][mj] = min_ && t + mrow + k * (256 / (2 * NS)) < a.k.n ? m : CT(0);
             }
             fetch(t + R);
 #pragma unroll
@@ -366,7 +372,7 @@ __global__ __launch_bounds__(64 * kScanWaves, IO == 8 ? 2 : 3) void seq_scan_end
             rd.get(p.dt, x);
             ry.get(p.dy, y);
             rz.get(p.z, z);
-            rm.put(p.B.dt, maps);
+            rm.put(p.B.dt, maps, a.k.n - t);
             rm.load(t + TB, a.k.n);
             ru.load(p.m, p.u, a.k, t + TB, a.d);
             rd.load(p.m, p.dt, a.k, t + TB, a.d);
@@ -398,7 +404,7 @@ __global__ __launch_bounds__(64 * kScanWaves, IO == 8 ? 2 : 3) void seq_scan_end
         // from the last to the first, as the formula has it
         bool out = false;
 #pragma unroll
-        for (int n = 0; n < NS; ++n) out = out || !(P[n] <= CT(IO == 8 ? 1.7976931348623157e308 : 3.4028234e38));
+        for (int n = 0; n < NS; ++n) out = out || !(P[n] <= CT(IO == 8 ? 1.7976931348623157e308 : 3.4028234663852886e38));
         if (__builtin_amdgcn_ballot_w64(out)) {
 #pragma unroll
             for (int n = 0; n < NS; ++n) g[n] = CT(0);
@@ -541,7 +547,7 @@ __global__ __launch_bounds__(64 * kScanWaves, 2) void seq_scan_bwd_kernel(const 
             CT u[TB], x[TB], dl[TB];
             ru.get(p.u, u);
             rd.get(p.dt, x);
-            rm.put(p.B.dt, maps);
+            rm.put(p.B.dt, maps, TB);
             // the next rows; the last ones of the chunk stay for the way back
             rm.load((k + 1) * TB, a.k.n);
             ru.load(p.m, p.u, a.k, (k + 1) * TB, a.d);
@@ -568,7 +574,7 @@ __global__ __launch_bounds__(64 * kScanWaves, 2) void seq_scan_bwd_kernel(const 
             CT u[TB], x[TB], z[TB], y[TB], dl[TB], ah[TB][NS];
             ru.get(p.u, u);
             rd.get(p.dt, x);
-            rm.put(p.B.dt, maps);
+            rm.put(p.B.dt, maps, nv);
             rm.load(before, a.k.n);
             ru.load(p.m, p.u, a.k, before, a.d);
             rd.load(p.m, p.dt, a.k, before, a.d);

@@ -722,6 +722,31 @@ def test_modes_that_grow_stay_in_range_where_the_formula_does(sign, N, T, dtype)
 
 
 @gpu
+@pytest.mark.parametrize("T", [1, 11, 64, 70, 151])
+@pytest.mark.parametrize("N", [5, 16, 32])
+@pytest.mark.parametrize("dtype", ["f32", "f64"])
+def test_rows_behind_the_last_one_change_nothing(N, T, dtype):
+    """Batches of rows that a sequence does not fill: an infinite rate (a decay of 0), an infinity in the last row's maps."""
+    def run(c):
+        y, end = seq.selective_scan(c["u"], c["dt"], c["A"], c["B"], c["C"], D=c["D"], z=c["z"], state=c["state"], softplus=False, return_state=True, **c["kw"])
+        p = scan_all_plain(c)
+        alike(y, *p["y"], 60 + N + 64, "y")
+        alike(end, *p["end"], 60 + N + 64, "end")
+        assert torch.equal(end.cpu() == math.inf, p["end"][0] == math.inf) and torch.equal(torch.isnan(y.cpu()), torch.isnan(p["y"][0]))
+
+    def case():
+        c = scan_with(T, 7, N, {}, dtype=DT[dtype])
+        return {k: v.to(param_of(DT[dtype])) if k in ("A", "D", "state", "dstate") else v for k, v in c.items()}
+
+    c = case()
+    c["A"][2, :], c["A"][4, 1] = -math.inf, -math.inf
+    run(c)
+    c = case()
+    c["B"][T - 1, 0] = math.inf
+    run(c)
+
+
+@gpu
 @pytest.mark.parametrize("starts", [[0, 90, 40, 60], [-5, 20, 300], [50, 10], [0]])
 def test_offsets_that_make_no_sense_stay_inside_the_arrays(starts):
     g = torch.Generator().manual_seed(1)
