@@ -101,7 +101,9 @@ crnn::SeqMap seq_map(int32_t n_seq, int64_t rows, const int32_t *start, const in
     return m;
 }
 int64_t seq_flat(int32_t n_seq, int64_t rows, bool packed) { return packed ? rows : rows * n_seq; }
-constexpr int64_t kSeqMaxGrid = 0x7fffffff;
+// Blocks of 256 threads a launch may have: the hardware counts threads in 32 bits, and a larger grid is cut off without an error (524296 x 32 blocks ran as 256)
+constexpr int64_t kSeqMaxGrid = 0xffffffffLL / 256;
+constexpr int64_t kSeqMaxChunks = 0x7fffffff;      // chunks are counted in 31 bits on the device
 
 #define SEQ_ENTER(a, who)                                                                                                   \
     if (!(a)) return sfail(who ": null arguments");                                                                          \
@@ -145,7 +147,8 @@ int64_t scan_forward_rows(int64_t flat, int32_t n_seq, int64_t rows, bool packed
     return std::max(q, (total / 8192 + 7) / 8 * 8);
 }
 
-bool scan_plan(SeqCheck &c, const crnn_scan_args *a, bool backward, ScanPlan &s) {
+// step: only what a single row has to do with (its launch is checked by itself)
+bool scan_plan(SeqCheck &c, const crnn_scan_args *a, bool backward, ScanPlan &s, bool step = false) {
     if (!seq_rows_ok(c, a->n_seq, a->rows, a->seq_start, a->seq_len, a->D, a->dtype)) return false;
     if (a->N < 1 || a->N > CRNN_SEQ_MAX_STATES) return c.bad("N must be in 1 .. 256");
     if (a->G < 1 || a->D % a->G) return c.bad("G must divide D");
@@ -165,7 +168,8 @@ bool scan_plan(SeqCheck &c, const crnn_scan_args *a, bool backward, ScanPlan &s)
     p.m = seq_map(a->n_seq, a->rows, a->seq_start, a->seq_len, Q);
     s.split = backward || Q > 0;
     const int64_t blk = p.m.nblk * a->D;
-    if (p.m.nblk * p.ntile > kSeqMaxGrid || (int64_t)a->n_seq * s.NS * a->D / 256 >= kSeqMaxGrid)
+    const int64_t tiles = backward ? (p.ntile + crnn::kScanWaves - 1) / crnn::kScanWaves : p.ntile;
+    if (!step && (p.m.nblk > kSeqMaxChunks || p.m.nblk * tiles > kSeqMaxGrid || (s.split && ((int64_t)a->n_seq * s.NS * a->D + 255) / 256 > kSeqMaxGrid)))
         return c.bad("too many sequences, rows and channels for one launch");
     int64_t at = 0;
     auto take = [&](int64_t n) { const int64_t o = at; at += (n + 31) / 32 * 32; return o; };
@@ -323,7 +327,7 @@ bool conv_check(SeqCheck &c, const crnn_conv_args *a, bool backward, crnn::ConvP
     p.D = a->D; p.W = a->W; p.silu = a->silu; p.zero_outside = a->zero_outside;
     p.m = seq_map(a->n_seq, a->rows, a->seq_start, a->seq_len,
                   conv_strip(seq_flat(a->n_seq, a->rows, a->seq_start != nullptr), a->D, conv_wide(a->dtype, a->W, backward), backward));
-    if ((p.m.nblk + 3) / 4 * ((a->D + 63) / 64) > kSeqMaxGrid) return c.bad("too many sequences, rows and channels for one launch");
+    if (p.m.nblk > kSeqMaxChunks) return c.bad("too many sequences, rows and channels for one launch");
     return true;
 }
 bool conv_views(SeqCheck &c, const crnn_conv_args *a, bool backward, crnn::ConvP &p) {
@@ -348,10 +352,10 @@ bool conv_views(SeqCheck &c, const crnn_conv_args *a, bool backward, crnn::ConvP
     p.w = a->weight; p.bias = a->bias;
     return true;
 }
+int64_t conv_grid(const crnn::ConvP &p, int V) { return (p.m.nblk + 3) / 4 * ((p.D + 64 * V - 1) / (64 * V)); }
 template <int XT, int YT, int W, int V>
 void conv_launch(const crnn::ConvP &p, bool backward, hipStream_t st) {
-    const int64_t gx = (p.D + 64 * V - 1) / (64 * V);
-    const dim3 grid((unsigned)((p.m.nblk + 3) / 4 * gx));
+    const dim3 grid((unsigned)conv_grid(p, V));
     if (backward) hipLaunchKernelGGL((crnn::seq_conv_bwd_kernel<XT, YT, W, V>), grid, dim3(256), 0, st, p);
     else hipLaunchKernelGGL((crnn::seq_conv_fwd_kernel<XT, YT, W, V>), grid, dim3(256), 0, st, p);
 }
@@ -436,8 +440,10 @@ int32_t crnn_conv_forward(const crnn_conv_args *a) {
         if (!conv_check(c, a, false, p)) return sfail(c.err);
         if (a->n_seq == 0) return 0;
         if (!conv_views(c, a, false, p)) return sfail(c.err);
+        const int V = conv_channels(a, false);
+        if (conv_grid(p, V) > kSeqMaxGrid) return sfail("crnn_conv_forward: too many sequences, rows and channels for one launch");
         SEQ_DEVICE(a->device, "crnn_conv_forward");
-        conv_launch_t(p, a->dtype, conv_channels(a, false), false, (hipStream_t)a->stream);
+        conv_launch_t(p, a->dtype, V, false, (hipStream_t)a->stream);
         SEQ_DONE("crnn_conv_forward");
     } catch (...) { return -1; }
 }
@@ -452,10 +458,12 @@ int32_t crnn_conv_backward(const crnn_conv_args *a) {
         const bool f64 = a->dtype == CRNN_DT_F64;
         const int64_t need = p.m.nblk * (a->W + 1) * a->D * (f64 ? 8 : 4);
         if (need > 0 && (!a->workspace || a->workspace_bytes < need)) return sfail("crnn_conv_backward: workspace is missing or too small");
+        const int V = conv_channels(a, true);
+        if (conv_grid(p, V) > kSeqMaxGrid) return sfail("crnn_conv_backward: too many sequences, rows and channels for one launch");
         SEQ_DEVICE(a->device, "crnn_conv_backward");
         p.part = a->workspace;
         const hipStream_t st = (hipStream_t)a->stream;
-        conv_launch_t(p, a->dtype, conv_channels(a, true), true, st);
+        conv_launch_t(p, a->dtype, V, true, st);
         const int64_t count = (int64_t)(a->W + 1) * a->D;       // [tap][D], then the bias
         const dim3 grid((unsigned)((count + 31) / 32));
         if (f64)
@@ -482,8 +490,6 @@ int32_t crnn_conv_step(const crnn_conv_args *a) {
             !c.apart(a->state_in, "state_in", a->n_slots, a->W - 1, a->D))
             return sfail(c.err);
         if (!a->weight) return sfail("crnn_conv_step: weight is missing");
-        if (a->n_seq * (int64_t)((a->D + 255) / 256) > kSeqMaxGrid) return sfail("crnn_conv_step: too many rows and channels for one launch");
-        SEQ_DEVICE(a->device, "crnn_conv_step");
         crnn::ConvStepP p{};
         p.x = seq_view(a->x, 1); p.y = seq_view(a->y, 1); p.st = seq_view(a->state_in, 1);
         p.w = a->weight; p.bias = a->bias; p.slot = a->slot; p.rows = a->n_seq; p.n_slots = a->n_slots;
@@ -491,6 +497,8 @@ int32_t crnn_conv_step(const crnn_conv_args *a) {
         const hipStream_t st = (hipStream_t)a->stream;
         const int VW = a->dtype == CRNN_DT_F64 ? 2 : 4;
         const int V = a->D % VW == 0 && conv_weights_fit(a, VW) && conv_fits(a->x, VW) && conv_fits(a->y, VW) && conv_fits(a->state_in, VW) ? VW : 1;
+        if (a->n_seq * (int64_t)((a->D + 256 * V - 1) / (256 * V)) > kSeqMaxGrid) return sfail("crnn_conv_step: too many rows and channels for one launch");
+        SEQ_DEVICE(a->device, "crnn_conv_step");
         if (a->dtype == CRNN_DT_F64) conv_step_launch_w<CRNN_DT_F64>(p, V, st);
         else if (a->dtype == CRNN_DT_F32) conv_step_launch_w<CRNN_DT_F32>(p, V, st);
         else if (a->dtype == CRNN_DT_BF16) conv_step_launch_w<CRNN_DT_BF16>(p, V, st);
@@ -546,7 +554,7 @@ int32_t crnn_scan_step(const crnn_scan_args *a) {
         SEQ_ENTER(a, "crnn_scan_step");
         SeqCheck c{"crnn_scan_step", {}};
         ScanPlan s;
-        if (!scan_plan(c, a, false, s)) return sfail(c.err);
+        if (!scan_plan(c, a, false, s, true)) return sfail(c.err);
         if (a->seq_start || a->seq_len) return sfail("crnn_scan_step: rows are one per sequence (no seq_start, seq_len)");
         if (a->n_slots < 0 || a->n_slots > 0x7fffffff || (!a->slot && a->n_seq > a->n_slots)) return sfail("crnn_scan_step: n_slots does not fit the rows");
         if (a->n_seq == 0) return 0;

@@ -1173,3 +1173,63 @@ def test_c_entry_points_refuse_before_any_launch():
     assert lib.crnn_pack8(99, None, C.byref(v), 2, 8, 4096, 4096) == -1 and "half" in said()
     v = view()
     assert lib.crnn_unpack8(99, None, 4096, None, 2, 8, C.byref(v)) == -1 and "missing" in said()
+
+
+def test_launches_the_card_would_cut_off_are_refused():
+    """A grid counts its threads in 32 bits: 2^24 blocks of 256 and more would be cut off without an error.  Sizes alone decide, on a host without a device too (a call that
+    gets past the checks is refused for a device that does not exist)."""
+    import ctypes as C
+    lib = L.lib
+
+    def view(ptr, D, n):
+        return L.View(ptr=ptr, row_stride=D, seq_stride=D, dtype=L.DT_BF16)
+
+    def scan(n, D, N, **over):
+        v = {k: view((1 + i) << 44, D if k in ("u", "dt", "y", "dy", "du", "ddt") else N, n) for i, k in enumerate(("u", "dt", "y", "B", "C", "dy", "du", "ddt", "dB", "dC"))}
+        a = L.ScanArgs(struct_size=C.sizeof(L.ScanArgs), device=99, n_seq=n, D=D, N=N, G=1, rows=1, dtype=L.DT_BF16, A=1 << 40, dA=1 << 41, workspace=1 << 42, workspace_bytes=1 << 62, **v)
+        for k, w in over.items():
+            setattr(a, k, w)
+        return a
+
+    def conv(n, D, **over):
+        v = {k: view((1 + i) << 44, D, n) for i, k in enumerate(("x", "y", "dy", "dx"))}
+        a = L.ConvArgs(struct_size=C.sizeof(L.ConvArgs), device=99, n_seq=n, D=D, W=1, rows=1, dtype=L.DT_BF16, weight=1 << 40, dweight=1 << 41, workspace=1 << 42, workspace_bytes=1 << 62, **v)
+        for k, w in over.items():
+            setattr(a, k, w)
+        return a
+
+    top = (1 << 24) - 1
+    for call, args, word in [
+            (lib.crnn_scan_forward, scan(top // 32, 2048, 8), "device"), (lib.crnn_scan_forward, scan(top // 32 + 1, 2048, 8), "too many"),
+            (lib.crnn_scan_forward, scan((1 << 19) + 8, 2048, 8), "too many"), (lib.crnn_scan_workspace, scan(1 << 28, 2048, 8), "too many"),
+            # the gradient: four tiles a block, and a thread for each sequence, state and channel of the carry
+            (lib.crnn_scan_backward, scan(top // 64, 2048, 8), "device"), (lib.crnn_scan_backward, scan(top // 64 + 1, 2048, 8), "too many"),
+            # four wavefronts a block, four channels a lane (one where a row does not allow that)
+            (lib.crnn_conv_forward, conv(top // 8 * 4, 2048), "device"), (lib.crnn_conv_forward, conv(top // 8 * 4 + 4, 2048), "too many"),
+            (lib.crnn_conv_forward, conv(top // 33 * 4 + 4, 2049), "too many"), (lib.crnn_conv_backward, conv(top // 8 * 4, 2048), "device"),
+            (lib.crnn_conv_backward, conv(top // 8 * 4 + 4, 2048), "too many"),
+            # single rows: a block has 256 threads of four channels
+            (lib.crnn_conv_step, conv(top // 2, 2048, n_slots=1 << 30), "device"), (lib.crnn_conv_step, conv(top // 2 + 1, 2048, n_slots=1 << 30), "too many"),
+            (lib.crnn_scan_step, scan(top // 2, 2048, 1, n_slots=1 << 30, state_out=1 << 43), "device"), (lib.crnn_scan_step, scan(top // 2 + 1, 2048, 1, n_slots=1 << 30, state_out=1 << 43), "too many")]:
+        got = call(C.byref(args), 0) if call is lib.crnn_scan_workspace else call(C.byref(args))
+        assert got == -1 and word in lib.crnn_last_error(None).decode(), (word, lib.crnn_last_error(None).decode())
+    v = L.View(ptr=1 << 44, row_stride=4096, dtype=L.DT_BF16)
+    for rows, word in ((top, "device"), (top + 1, "too many")):
+        assert lib.crnn_pack8(99, None, C.byref(v), rows, 4096, 1 << 45, 1 << 46) == -1 and word in lib.crnn_last_error(None).decode()
+
+
+@gpu
+def test_the_largest_launch_reaches_its_last_rows():
+    if DEV == "cpu":
+        pytest.skip("sizes for the device")
+    n, D, N = ((1 << 24) - 1) // 32, 2048, 8
+    g = torch.Generator(device=DEV).manual_seed(0)
+    u = torch.randn(n, 1, D, generator=g, device=DEV, dtype=torch.bfloat16)
+    A, m, w = -torch.rand(D, N, generator=g, device=DEV), torch.randn(n, 1, N, generator=g, device=DEV, dtype=torch.bfloat16), torch.randn(D, 2, generator=g, device=DEV)
+    y = seq.selective_scan(u, u, A, m, m, out=torch.full_like(u, 7.0))
+    for rows in (slice(0, 9), slice(n // 2, n // 2 + 9), slice(n - 9, n)):
+        assert torch.equal(y[rows], seq.selective_scan(u[rows], u[rows], A, m[rows], m[rows]))
+    assert not bool((y == 7).all(-1).any())
+    with pytest.raises(L.CrnnError, match="too many"):
+        seq.selective_scan(torch.empty(n + 1, 1, D, dtype=torch.bfloat16, device=DEV), torch.empty(n + 1, 1, D, dtype=torch.bfloat16, device=DEV), A,
+                           *(torch.empty(n + 1, 1, N, dtype=torch.bfloat16, device=DEV),) * 2)
