@@ -72,11 +72,75 @@ struct SeqCheck {
         if (v.seq_stride >= width && v.row_stride >= (n - 1) * v.seq_stride + width) return true;
         return bad(std::string(name) + ": sequences of an output overlap");
     }
-    // an output is written while other lanes and blocks still read the inputs (arrays that share some rows only are the caller's to avoid)
+    // an output is written while other lanes and blocks still read the inputs (the pointers alone; what else they may share: SeqShare)
     bool other(std::initializer_list<const crnn_view *> outs, std::initializer_list<const crnn_view *> ins, int64_t rows) {
         for (const crnn_view *y : outs)
             for (const crnn_view *x : ins)
                 if (rows > 0 && y->ptr && y->ptr == x->ptr) return bad("an output is also an input");
+        return true;
+    }
+};
+
+// Where an array lies: `width` bytes, `n[0]` times `s[0]` bytes apart, all that `n[1]` times `s[1]` bytes apart (s[0] <= s[1]).
+struct SeqSpan {
+    uintptr_t at = 0;
+    int64_t width = 0, n[2] = {0, 0}, s[2] = {0, 0};
+    SeqSpan() = default;
+    SeqSpan(const void *p, int64_t bytes) : SeqSpan(p, bytes, 1, 0, 1, 0) {}
+    SeqSpan(const void *p, int64_t bytes, int64_t rows, int64_t row_bytes, int64_t seqs, int64_t seq_bytes) {
+        if (!p || bytes <= 0 || rows <= 0 || seqs <= 0) return;
+        at = (uintptr_t)p; width = bytes;
+        n[0] = row_bytes ? rows : 1; s[0] = n[0] > 1 ? row_bytes : 0;
+        n[1] = seq_bytes ? seqs : 1; s[1] = n[1] > 1 ? seq_bytes : 0;
+        if (n[0] == 1 || (n[1] > 1 && s[1] < s[0])) { std::swap(n[0], n[1]); std::swap(s[0], s[1]); }
+    }
+    __int128 end() const { return (__int128)at + (__int128)(n[0] - 1) * s[0] + (__int128)(n[1] - 1) * s[1] + width; }
+    bool one(int k) const { return n[k] <= 1; }
+};
+// a and b, each pieces of `wa` and `wb` bytes some multiples of `every` bytes apart, never meet
+inline bool seq_beside(const SeqSpan &a, const SeqSpan &b, __int128 wa, __int128 wb, int64_t every) {
+    if (every <= 0) return false;
+    const int64_t d = (int64_t)((((__int128)b.at - (__int128)a.at) % every + every) % every);
+    return d >= wa && d + wb <= every;
+}
+// Arrays whose ranges of addresses meet are still apart where both are columns of one wider array (row by row side by side), or blocks of rows side by side.
+// What else meets counts as shared.
+inline bool seq_shared(const SeqSpan &a, const SeqSpan &b) {
+    if (!a.at || !b.at || a.end() <= (__int128)b.at || b.end() <= (__int128)a.at) return false;
+    const int64_t in = a.one(0) ? b.s[0] : a.s[0], out = a.one(1) ? b.s[1] : a.s[1];
+    const bool rows = (a.one(0) || a.s[0] == in) && (b.one(0) || b.s[0] == in) && in > 0 && a.s[1] % in == 0 && b.s[1] % in == 0;
+    if (rows && seq_beside(a, b, a.width, b.width, in)) return false;
+    const bool blocks = (a.one(1) || a.s[1] == out) && (b.one(1) || b.s[1] == out);
+    const __int128 wa = (__int128)(a.n[0] - 1) * a.s[0] + a.width, wb = (__int128)(b.n[0] - 1) * b.s[0] + b.width;
+    return !(blocks && seq_beside(a, b, wa, wb, out));
+}
+// The arrays of a call.  Outputs may share memory neither with inputs nor with one another; `same`: an input that an output may be, as a whole
+// (each of its elements is read by the thread that writes it, before).
+struct SeqShare {
+    SeqSpan ins[16], outs[10];
+    int n_in = 0, n_out = 0;
+    void put_in(const SeqSpan &x) { if (x.at) ins[n_in++] = x; }
+    void put_out(const SeqSpan &x) { if (x.at) outs[n_out++] = x; }
+    // rows of `width` elements
+    static SeqSpan span(const crnn_view &v, int64_t width, int64_t rows, int64_t n) {
+        const int64_t e = seq_size(v.dtype);
+        return SeqSpan(v.ptr, width * e, rows, v.row_stride * e, n, v.seq_stride * e);
+    }
+    void in(const crnn_view &v, int64_t width, int64_t rows, int64_t n) {
+        put_in(span(v, width, rows, n));
+        if (v.ptr && v.dtype == CRNN_DT_PACKED8) put_in(SeqSpan(v.scales, (width + 31) / 32, rows, v.scale_row_stride, n, v.scale_seq_stride));
+    }
+    void in(const void *p, int64_t bytes) { put_in(SeqSpan(p, bytes)); }
+    void out(const crnn_view &v, int64_t width, int64_t rows, int64_t n) { put_out(span(v, width, rows, n)); }
+    void out(const void *p, int64_t bytes) { put_out(SeqSpan(p, bytes)); }
+    bool ok(SeqCheck &c, const void *same = nullptr, const void *same2 = nullptr) const {
+        for (int i = 0; i < n_out; ++i) {
+            const SeqSpan &y = outs[i];
+            for (int j = 0; j < n_in; ++j)
+                if (seq_shared(y, ins[j]) && !(y.at == ins[j].at && (y.at == (uintptr_t)same || y.at == (uintptr_t)same2))) return c.bad("an output shares memory with an input");
+            for (int j = 0; j < i; ++j)
+                if (seq_shared(y, outs[j])) return c.bad("two outputs share memory");
+        }
         return true;
     }
 };
@@ -276,6 +340,30 @@ bool scan_views(SeqCheck &c, const crnn_scan_args *a, bool backward, bool step =
            c.apart(a->dC, "dC", n, rows, GN) && c.other({&a->du, &a->ddt, &a->dz, &a->dB, &a->dC}, {&a->dy, &a->u, &a->dt, &a->z, &a->B, &a->C}, flat);
 }
 
+bool scan_apart(SeqCheck &c, const crnn_scan_args *a, bool backward, bool step = false) {
+    SeqShare m;
+    const int64_t pe = a->dtype == CRNN_DT_F64 ? 8 : 4, D = a->D, N = a->N, G = a->G;
+    const int64_t rows = step ? a->n_seq : a->rows, n = step || a->seq_start ? 1 : a->n_seq, states = (step ? a->n_slots : (int64_t)a->n_seq) * D * N * pe;
+    m.in(a->u, D, rows, n); m.in(a->dt, D, rows, n); m.in(a->z, D, rows, n);
+    m.in(a->B, (G - 1) * a->B_group + (N - 1) * a->B_state + 1, rows, n); m.in(a->C, (G - 1) * a->C_group + (N - 1) * a->C_state + 1, rows, n);
+    m.in(a->A, D * N * pe); m.in(a->skip, D * pe); m.in(a->dt_bias, D * pe);
+    m.in(a->seq_start, ((int64_t)a->n_seq + 1) * 4); m.in(a->seq_len, (int64_t)a->n_seq * 4);
+    if (step) {
+        m.in(a->slot, (int64_t)a->n_seq * 4);
+        m.out(a->y, D, rows, n); m.out(a->state_out, states);
+        return m.ok(c);
+    }
+    m.in(a->state_in, states);
+    if (!backward) {
+        m.out(a->y, D, rows, n); m.out(a->state_out, states);
+        return m.ok(c, a->state_in);
+    }
+    m.in(a->dy, D, rows, n); m.in(a->dstate_out, states);
+    m.out(a->du, D, rows, n); m.out(a->ddt, D, rows, n); m.out(a->dz, D, rows, n); m.out(a->dB, G * N, rows, n); m.out(a->dC, G * N, rows, n);
+    m.out(a->dA, D * N * pe); m.out(a->dskip, D * pe); m.out(a->ddt_bias, D * pe); m.out(a->dstate_in, states);
+    return m.ok(c, a->state_in, a->dstate_out);
+}
+
 // the launches' template: MODE 2 (anything: several launches over the states, one of u and z a checkpoint) has 16 states a launch, 8 in double
 #define SCAN_RUN(run)                                                                                                         \
     do {                                                                                                                      \
@@ -351,6 +439,25 @@ bool conv_views(SeqCheck &c, const crnn_conv_args *a, bool backward, crnn::ConvP
     p.st_in = seq_view(a->state_in, 1); p.st_out = seq_view(a->state_out, 1); p.dst_out = seq_view(a->dstate_out, 1); p.dst_in = seq_view(a->dstate_in, 1);
     p.w = a->weight; p.bias = a->bias;
     return true;
+}
+bool conv_apart(SeqCheck &c, const crnn_conv_args *a, bool backward, bool step = false) {
+    SeqShare m;
+    const int64_t pe = a->dtype == CRNN_DT_F64 ? 8 : 4, D = a->D, W = a->W, rows = step ? a->n_seq : a->rows, n = step || a->seq_start ? 1 : a->n_seq;
+    m.in(a->x, D, rows, n); m.in(a->weight, D * W * pe); m.in(a->bias, D * pe);
+    m.in(a->seq_start, ((int64_t)a->n_seq + 1) * 4); m.in(a->seq_len, (int64_t)a->n_seq * 4);
+    if (step) {
+        m.in(a->slot, (int64_t)a->n_seq * 4);
+        m.out(a->y, D, rows, n); m.out(a->state_in, D, W - 1, a->n_slots);
+        return m.ok(c);
+    }
+    m.in(a->state_in, D, W - 1, a->n_seq);
+    if (!backward) {
+        m.out(a->y, D, rows, n); m.out(a->state_out, D, W - 1, a->n_seq);
+        return m.ok(c);
+    }
+    m.in(a->dy, D, rows, n); m.in(a->dstate_out, D, W - 1, a->n_seq);
+    m.out(a->dx, D, rows, n); m.out(a->dstate_in, D, W - 1, a->n_seq); m.out(a->dweight, D * W * pe); m.out(a->dbias, D * pe);
+    return m.ok(c);
 }
 int64_t conv_grid(const crnn::ConvP &p, int V) { return (p.m.nblk + 3) / 4 * ((p.D + 64 * V - 1) / (64 * V)); }
 template <int XT, int YT, int W, int V>
@@ -439,7 +546,7 @@ int32_t crnn_conv_forward(const crnn_conv_args *a) {
         crnn::ConvP p;
         if (!conv_check(c, a, false, p)) return sfail(c.err);
         if (a->n_seq == 0) return 0;
-        if (!conv_views(c, a, false, p)) return sfail(c.err);
+        if (!conv_views(c, a, false, p) || !conv_apart(c, a, false)) return sfail(c.err);
         const int V = conv_channels(a, false);
         if (conv_grid(p, V) > kSeqMaxGrid) return sfail("crnn_conv_forward: too many sequences, rows and channels for one launch");
         SEQ_DEVICE(a->device, "crnn_conv_forward");
@@ -458,6 +565,7 @@ int32_t crnn_conv_backward(const crnn_conv_args *a) {
         const bool f64 = a->dtype == CRNN_DT_F64;
         const int64_t need = p.m.nblk * (a->W + 1) * a->D * (f64 ? 8 : 4);
         if (need > 0 && (!a->workspace || a->workspace_bytes < need)) return sfail("crnn_conv_backward: workspace is missing or too small");
+        if (!conv_apart(c, a, true)) return sfail(c.err);
         const int V = conv_channels(a, true);
         if (conv_grid(p, V) > kSeqMaxGrid) return sfail("crnn_conv_backward: too many sequences, rows and channels for one launch");
         SEQ_DEVICE(a->device, "crnn_conv_backward");
@@ -490,6 +598,7 @@ int32_t crnn_conv_step(const crnn_conv_args *a) {
             !c.apart(a->state_in, "state_in", a->n_slots, a->W - 1, a->D))
             return sfail(c.err);
         if (!a->weight) return sfail("crnn_conv_step: weight is missing");
+        if (!conv_apart(c, a, false, true)) return sfail(c.err);
         crnn::ConvStepP p{};
         p.x = seq_view(a->x, 1); p.y = seq_view(a->y, 1); p.st = seq_view(a->state_in, 1);
         p.w = a->weight; p.bias = a->bias; p.slot = a->slot; p.rows = a->n_seq; p.n_slots = a->n_slots;
@@ -527,6 +636,7 @@ int32_t crnn_scan_forward(const crnn_scan_args *a) {
         if (a->n_seq == 0) return 0;
         if (!scan_views(c, a, false)) return sfail(c.err);
         if (s.total > 0 && (!a->workspace || a->workspace_bytes < s.total)) return sfail("crnn_scan_forward: workspace is missing or too small");
+        if (!scan_apart(c, a, false)) return sfail(c.err);
         SEQ_DEVICE(a->device, "crnn_scan_forward");
         scan_fill(a, s);
         SCAN_RUN(scan_forward_run);
@@ -542,6 +652,7 @@ int32_t crnn_scan_backward(const crnn_scan_args *a) {
         if (!scan_plan(c, a, true, s) || !scan_views(c, a, true)) return sfail(c.err);
         if (s.total > 0 && (!a->workspace || a->workspace_bytes < s.total)) return sfail("crnn_scan_backward: workspace is missing or too small");
         if (a->n_seq == 0) return sfail("crnn_scan_backward: no sequences");
+        if (!scan_apart(c, a, true)) return sfail(c.err);
         SEQ_DEVICE(a->device, "crnn_scan_backward");
         scan_fill(a, s);
         SCAN_RUN(scan_backward_run);
@@ -561,6 +672,7 @@ int32_t crnn_scan_step(const crnn_scan_args *a) {
         if (!scan_views(c, a, false, true)) return sfail(c.err);
         if (s.p8) return sfail("crnn_scan_step: u and z cannot be 8-bit checkpoints here");
         if (!a->state_out && a->n_slots > 0) return sfail("crnn_scan_step: the states are missing");
+        if (!scan_apart(c, a, false, true)) return sfail(c.err);
         crnn::ScanStepP p{};
         p.u = seq_view(a->u, 4); p.dt = seq_view(a->dt, 4); p.z = seq_view(a->z, 4); p.y = seq_view(a->y, 4); p.B = seq_view(a->B, 1); p.C = seq_view(a->C, 1);
         p.Bg = a->B_group; p.Cg = a->C_group; p.Bn = a->B_state; p.Cn = a->C_state;
@@ -600,6 +712,13 @@ static bool pack_plan(SeqCheck &c, const crnn_view *x, int64_t rows, int32_t D, 
     if (rows == 0) return true;
     if (!codes || !scales) return c.bad("codes or scales are missing");
     if (!c.view(*x, "x", x->dtype, true, false, out, D)) return false;
+    SeqShare m;
+    if (out) {
+        m.out(*x, D, rows, 1); m.in(codes, rows * D); m.in(scales, rows * p.nb);
+    } else {
+        m.in(*x, D, rows, 1); m.out(codes, rows * D); m.out(scales, rows * p.nb);
+    }
+    if (!m.ok(c)) return false;
     p.x = seq_view(*x, 16 / seq_size(x->dtype));
     p.q = (int8_t *)codes; p.sc = (uint8_t *)scales;
     p.vecq = (uintptr_t)codes % 16 == 0 && D % 16 == 0 ? 16 : (uintptr_t)codes % 4 == 0 && D % 4 == 0 ? 4 : 1;

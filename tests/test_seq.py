@@ -1233,3 +1233,96 @@ def test_the_largest_launch_reaches_its_last_rows():
     with pytest.raises(L.CrnnError, match="too many"):
         seq.selective_scan(torch.empty(n + 1, 1, D, dtype=torch.bfloat16, device=DEV), torch.empty(n + 1, 1, D, dtype=torch.bfloat16, device=DEV), A,
                            *(torch.empty(n + 1, 1, N, dtype=torch.bfloat16, device=DEV),) * 2)
+
+
+@gpu
+def test_results_over_parts_of_inputs_are_refused():
+    """Memory that an input and a result share is found wherever it lies, not at equal pointers only; columns and blocks of one array beside each other are fine."""
+    g = torch.Generator().manual_seed(3)
+    n, T, D, N, W = 3, 9, 32, 4, 4
+    w, A = rnd(g, D, W), -torch.exp(rnd(g, D, N))
+    buf, m, st = rnd(g, n, T + 1, D), rnd(g, n, T, N), rnd(g, n, W - 1, D)
+    conv = lambda x, out, **kw: seq.causal_conv(x, w, out=out, **kw)  # noqa: E731
+    scan = lambda u, dt, out, B=m, C=m, **kw: seq.selective_scan(u, dt, A, B, C, out=out, **kw)  # noqa: E731
+    x = rnd(g, n, T, D)
+    one = rnd(g, 1, 40, D + 8)
+    h, rows = rnd(g, 8, D, N), rnd(g, 5, D)
+    big = rnd(g, 8 * D * N)
+    wide = rnd(g, n, T, D * D)
+    flat = rnd(g, n * T * D + n * T * N)
+    for call in (lambda: conv(buf[:, :-1], buf[:, 1:]), lambda: conv(buf[:, 1:], buf[:, :-1]), lambda: conv(one[..., 1:D + 1], one[..., :D]), lambda: scan(x, buf[:, :-1], buf[:, 1:]),
+                 lambda: scan(buf[:, :-1], x, buf[:, 1:]), lambda: scan(x, x, buf[:, 1:], z=buf[:, :-1]), lambda: scan(one[:, 1:, :D], one[:, 1:, 8:], one[:, :-1, :D], rnd(g, 1, 39, N), rnd(g, 1, 39, N)),
+                 # a result inside the maps, a state, the weights, and the states of the single steps
+                 lambda: scan(x, x, flat[n * T * N - 4:][:n * T * D].view(n, T, D), flat[:n * T * N].view(n, T, N)),
+                 lambda: conv(x[:, :3], st, state=st), lambda: seq.causal_conv(rnd(g, 1, 4, D), wide[0, 0, :D * W].view(D, W), out=wide[0, 0, :D * W].view(1, W, D)),
+                 lambda: seq.causal_conv_step(rows, w, None, buf.view(-1, 3, D)[:8], out=buf.view(-1, 3, D)[1:6, 0]),
+                 lambda: seq.selective_scan_step(rows, rows, A, m[0, :5], m[0, :5], big.view(8, D, N), out=big[7:7 + 5 * D].view(5, D)),
+                 lambda: seq.unpack8(seq.Packed8(one.view(torch.int8).view(-1)[4:4 + 40 * D].view(40, D), torch.zeros(40, 1, dtype=torch.uint8, device=DEV), torch.float32),
+                                     out=one.view(-1)[:40 * D].view(40, D))):
+        with pytest.raises(L.CrnnError, match="share"):
+            call()
+    with pytest.raises(ValueError):
+        seq.causal_conv(x, w, out=x)
+    was = buf.clone()       # (a state that is not contiguous is copied before the call)
+    assert torch.equal(conv(buf[:, 4:7], buf[:, :3], state=buf[:, 1:4]), seq.causal_conv(was[:, 4:7], w, state=was[:, 1:4]))
+    # beside each other: halves of a row, a sequence's first and last rows, time and batch swapped, another part of the states' array
+    both = rnd(g, n, T, 2 * D)
+    swap = rnd(g, T, n, 2 * D).transpose(0, 1)
+    rest = rnd(g, n, 2 * T, D)
+    for a, b in ((both[..., :D], both[..., D:]), (both[..., D:], both[..., :D]), (swap[..., :D], swap[..., D:]), (rest[:, :T], rest[:, T:]), (rest[:, T:], rest[:, :T]), (rest[:1, :T], rest[2:, :T])):
+        k = a.shape[0]
+        want, src = seq.causal_conv(a.clone(), w), a.clone()
+        assert torch.equal(conv(a, b), want) and torch.equal(a, src)
+        want = seq.selective_scan(a.clone(), a.clone(), A, m[:k], m[:k])
+        assert torch.equal(scan(a, a, b, m[:k], m[:k]), want) and torch.equal(a, src)
+    y = seq.selective_scan_step(rows, rows, A, m[0, :5], m[0, :5], h.clone())
+    room = torch.zeros(8 * D * N + 5 * D, device=DEV)
+    room[:8 * D * N] = h.view(-1)
+    assert torch.equal(seq.selective_scan_step(rows, rows, A, m[0, :5], m[0, :5], room[:8 * D * N].view(8, D, N), out=room[8 * D * N:].view(5, D)), y)
+
+
+def test_c_entry_points_refuse_arrays_that_share_memory():
+    """Pointers of the C ABI that meet: outputs with inputs and with one another; a state that is updated in place is allowed where every element is read by the thread that writes it."""
+    import ctypes as C
+    lib = L.lib
+    KB = 1 << 10
+
+    def view(at, rs=8, ss=48, dt=L.DT_F32, scales=None):
+        return L.View(ptr=at * KB, row_stride=rs, seq_stride=ss, dtype=dt, scales=scales, scale_row_stride=1, scale_seq_stride=6)
+
+    def scan(**over):       # each array in a KB of its own: 2 sequences of 6 rows, 8 channels, 4 states
+        a = L.ScanArgs(struct_size=C.sizeof(L.ScanArgs), device=99, n_seq=2, D=8, N=4, G=1, rows=6, A=KB, u=view(2), dt=view(3), y=view(4), B=view(5, 4, 24), C=view(6, 4, 24), z=view(7), skip=8 * KB,
+                       dt_bias=9 * KB, state_in=10 * KB, state_out=11 * KB, dy=view(12), du=view(13), ddt=view(14), dz=view(15), dB=view(16, 4, 24), dC=view(17, 4, 24), dA=18 * KB,
+                       dskip=19 * KB, ddt_bias=20 * KB, dstate_out=21 * KB, dstate_in=22 * KB, seq_len=23 * KB, workspace=1 << 30, workspace_bytes=1 << 40)
+        for k, v in over.items():
+            setattr(a, k, v)
+        return a
+
+    def conv(**over):
+        a = L.ConvArgs(struct_size=C.sizeof(L.ConvArgs), device=99, n_seq=2, D=8, W=4, rows=6, weight=KB, bias=2 * KB, x=view(3), y=view(4), state_in=view(5, 8, 24), state_out=view(6, 8, 24), dy=view(7),
+                       dx=view(8), dstate_out=view(9, 8, 24), dstate_in=view(10, 8, 24), dweight=11 * KB, dbias=12 * KB, seq_len=13 * KB, workspace=1 << 30, workspace_bytes=1 << 40)
+        for k, v in over.items():
+            setattr(a, k, v)
+        return a
+
+    def at(k, off, **kw):
+        v = view(k, **kw)
+        v.ptr = k * KB + off
+        return v
+
+    IN, OUT = "shares memory with an input", "two outputs"
+    packed = view(2, dt=L.DT_PACKED8, scales=30 * KB)
+    for call, make, over, word in [
+            (lib.crnn_scan_forward, scan, {}, "device"), (lib.crnn_scan_backward, scan, {}, "device"), (lib.crnn_conv_forward, conv, {}, "device"), (lib.crnn_conv_backward, conv, {}, "device"),
+            (lib.crnn_scan_forward, scan, dict(y=at(2, 4)), IN), (lib.crnn_scan_forward, scan, dict(y=at(2, -4)), IN), (lib.crnn_scan_forward, scan, dict(y=at(1, 32)), IN),
+            (lib.crnn_scan_forward, scan, dict(y=at(10, 252)), IN), (lib.crnn_scan_forward, scan, dict(y=at(10, 256)), "device"), (lib.crnn_scan_forward, scan, dict(y=at(23, 4)), IN),
+            (lib.crnn_scan_forward, scan, dict(state_out=10 * KB), "device"), (lib.crnn_scan_forward, scan, dict(state_out=10 * KB + 4), IN), (lib.crnn_scan_forward, scan, dict(state_out=4 * KB + 4), OUT),
+            (lib.crnn_scan_forward, scan, dict(u=packed, y=at(30, -4)), IN), (lib.crnn_scan_forward, scan, dict(u=packed, y=at(30, -384)), "device"),
+            (lib.crnn_scan_backward, scan, dict(du=at(12, 8)), IN), (lib.crnn_scan_backward, scan, dict(ddt=at(13, 8)), OUT), (lib.crnn_scan_backward, scan, dict(dA=KB), IN),
+            (lib.crnn_scan_backward, scan, dict(dstate_in=21 * KB), "device"), (lib.crnn_scan_backward, scan, dict(dstate_in=21 * KB + 8), IN), (lib.crnn_scan_backward, scan, dict(dskip=19 * KB, ddt_bias=19 * KB), OUT),
+            (lib.crnn_conv_forward, conv, dict(y=at(5, 64)), IN), (lib.crnn_conv_forward, conv, dict(y=at(2, 16)), IN), (lib.crnn_conv_forward, conv, dict(state_out=at(5, 32, ss=24)), IN),
+            (lib.crnn_conv_backward, conv, dict(dstate_in=view(9, 8, 24)), IN), (lib.crnn_conv_backward, conv, dict(dweight=KB), IN), (lib.crnn_conv_backward, conv, dict(dx=at(3, 4)), IN)]:
+        assert call(C.byref(make(**over))) == -1 and word in lib.crnn_last_error(None).decode(), (over, lib.crnn_last_error(None).decode())
+    v = view(2)
+    for codes, scales, word in ((2 * KB + 8, 8 * KB, IN), (8 * KB, 2 * KB + 380, IN), (8 * KB, 8 * KB + 95, OUT), (8 * KB, 8 * KB + 96, "device")):
+        assert lib.crnn_pack8(99, None, C.byref(v), 12, 8, codes, scales) == -1 and word in lib.crnn_last_error(None).decode(), (codes, scales)
