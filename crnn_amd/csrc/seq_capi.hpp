@@ -268,6 +268,7 @@ crnn::ScanMapsP scan_maps(const crnn_scan_args *a, const ScanPlan &s, const crnn
     m.rows = s.flat;
     m.srows = a->seq_start ? 0 : a->rows;
     m.G = a->G; m.N = a->N;
+    m.zero_outside = a->zero_outside;
     return m;
 }
 

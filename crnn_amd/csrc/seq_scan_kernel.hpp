@@ -48,6 +48,7 @@ struct ScanMapsP {
     int64_t rows;           // rows of all sequences
     int64_t srows;          // dense: rows of a sequence (0: packed)
     int32_t G, N, n0;
+    int32_t zero_outside;   // rows that belong to no sequence: 0, or left as they are
 };
 // the plane of state n of chunk block b in an [block][state][D] array: uniform, the lane adds its channel
 template <int NS, class T>
@@ -675,8 +676,10 @@ __global__ __launch_bounds__(256) void seq_scan_sum_maps_kernel(const SeqMap m, 
         const int64_t rg = i / (2 * NS), g = rg % p.G, r = rg / p.G;
         const int n = p.n0 + (j % NS);
         if (n >= p.N) continue;
+        const bool inside = seq_inside(m, r);
+        if (!inside && !p.zero_outside) continue;
         CT sum = CT(0);
-        if (seq_inside(m, r))
+        if (inside)
             for (int k = 0; k < tpg; k += 8) {
                 CT x[8];
 #pragma unroll

@@ -1236,6 +1236,39 @@ def test_the_largest_launch_reaches_its_last_rows():
 
 
 @gpu
+@pytest.mark.parametrize("zero", [0, 1])
+@pytest.mark.parametrize("packed", [False, True])
+def test_rows_of_gradients_outside_the_sequences_are_kept_or_cleared(packed, zero):
+    """The C ABI's zero_outside, all five row gradients of the scan and the convolution's."""
+    import ctypes as C
+    g = torch.Generator().manual_seed(5)
+    n, T, D, N, G = (1, 50, 12, 4, 2) if packed else (2, 25, 12, 4, 2)
+    at = torch.tensor([7, 31], dtype=torch.int32, device=DEV) if packed else torch.tensor([25, 9], dtype=torch.int32, device=DEV)
+    outside = torch.ones(50, dtype=torch.bool)
+    for lo, hi in ([(7, 31)] if packed else [(0, 25), (25, 34)]):
+        outside[lo:hi] = False
+    rows = [rnd(g, 50, D) for _ in range(4)]
+    maps = [rnd(g, 50, G * N) for _ in range(2)]
+    A, dA, w, dw = -torch.exp(rnd(g, D, N)), torch.zeros(D, N, device=DEV), rnd(g, D, 3), torch.zeros(D, 3, device=DEV)
+    out = [torch.full((50, D), 7.0, device=DEV) for _ in range(4)] + [torch.full((50, G * N), 7.0, device=DEV) for _ in range(2)]
+    view = lambda x: L.View(ptr=x.data_ptr(), row_stride=x.shape[1], seq_stride=0 if packed else T * x.shape[1], dtype=L.DT_F32)  # noqa: E731
+    stream = 0 if DEV == "cpu" else torch.cuda.current_stream().cuda_stream
+    kw = dict(n_seq=n, D=D, rows=T, dtype=L.DT_F32, zero_outside=zero, stream=stream, **{"seq_start" if packed else "seq_len": at.data_ptr()})
+    a = L.ScanArgs(struct_size=C.sizeof(L.ScanArgs), N=N, G=G, softplus=1, A=A.data_ptr(), dA=dA.data_ptr(), B_group=N, B_state=1, C_group=N, C_state=1,
+                   **{k: view(x) for k, x in zip(("u", "dt", "z", "dy", "B", "C", "du", "ddt", "dz", "dB", "dC"), rows + maps + out[:3] + out[4:])}, **kw)
+    c = L.ConvArgs(struct_size=C.sizeof(L.ConvArgs), W=3, weight=w.data_ptr(), dweight=dw.data_ptr(), x=view(rows[0]), dy=view(rows[1]), dx=view(out[3]), **kw)
+    for args, need, call in ((a, L.lib.crnn_scan_workspace(C.byref(a), 1), L.lib.crnn_scan_backward), (c, L.lib.crnn_conv_workspace(C.byref(c)), L.lib.crnn_conv_backward)):
+        ws = torch.empty(need, dtype=torch.uint8, device=DEV)
+        args.workspace, args.workspace_bytes = ws.data_ptr(), need
+        assert call(C.byref(args)) == 0, L.lib.crnn_last_error(None)
+        if DEV != "cpu":
+            torch.cuda.synchronize()
+    for k, x in enumerate(out):
+        assert bool((x.cpu()[outside] == (0 if zero else 7)).all()), k
+        assert bool((x.cpu()[~outside] != 7).any(-1).all()) and bool((x.cpu()[~outside] != 0).any(-1).all()), k
+
+
+@gpu
 def test_results_over_parts_of_inputs_are_refused():
     """Memory that an input and a result share is found wherever it lies, not at equal pointers only; columns and blocks of one array beside each other are fine."""
     g = torch.Generator().manual_seed(3)
