@@ -12,8 +12,10 @@ Arrays are torch tensors on an MI355X; the calls enqueue on that device's curren
 a graph.  Rows are time, channels are contiguous: dense [n_seq, rows, D] (lengths=: how many rows of each are its own, the others are
 padding), or packed [rows, D] with seq_start [n_seq + 1], int32 on the device: sequence s is rows seq_start[s] .. seq_start[s + 1] - 1.
 Lengths and offsets are not read by the host: they are clamped to the arrays.  Rows of a result that belong to no sequence are 0, and stay as
-they were where the caller gave the array (out=).  Results may not share memory with inputs.  Autograd does not
-record the calls: gradients are the *_grad calls.  float32, bfloat16, float16 and float64; weights, rates and scan states are float32
+they were where the caller gave the array (out=).  Results may not share memory with inputs (refused).  Autograd does not record the calls,
+gradients are the *_grad calls: forward calls and steps on tensors that require gradients are refused while it records (call them under
+torch.no_grad(), or in the forward of a torch.autograd.Function), and so are forward-mode tangents; the *_grad calls give values that
+are not differentiated further.  float32, bfloat16, float16 and float64; weights, rates and scan states are float32
 (float64 with float64 data).  A checkpoint (Packed8) may stand for x of the convolution, and for u and z of the scan.
 """
 from __future__ import annotations
@@ -34,16 +36,22 @@ _EMULATED = "SIMT-EMULATION" in lib.crnn_build_info().decode()     # the emulate
 _t = None          # torch, imported by the first call
 _DT = {}           # torch's types: ours
 _raw_stream = None
+_grad_on = None    # torch.is_grad_enabled
+_asks = None       # whether one of the arguments is a tensor that requires a gradient
+_dual = None       # torch's forward-mode module, if this torch tells whether it is in use
 _like = None       # a contiguous tensor of another's shape (and type): half the host time of torch.empty with a shape, a type and a device
 
 
 def _torch():
-    global _t, _raw_stream, _like
+    global _t, _raw_stream, _like, _dual, _grad_on, _asks
     if _t is None:
         import torch
         from functools import partial
         _like = partial(torch.empty_like, memory_format=torch.contiguous_format)
         _DT.update({torch.float32: L.DT_F32, torch.bfloat16: L.DT_BF16, torch.float16: L.DT_F16, torch.float64: L.DT_F64})
+        _grad_on = torch.is_grad_enabled
+        _asks = getattr(torch._C, "_any_requires_grad", None) or (lambda *xs: any(isinstance(x, torch.Tensor) and x.requires_grad for x in xs))
+        _dual = torch.autograd.forward_ad if hasattr(torch.autograd.forward_ad, "_current_level") else None
         _t = torch
         _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda i: torch.cuda.current_stream(i).cuda_stream)
     return _t
@@ -140,6 +148,17 @@ def _channels(x):
     if x.__class__ is Packed8 or x.stride(-1) == 1 or x.shape[-1] <= 1:
         return x
     return x.contiguous()
+
+
+def _recorded(name, *tensors, values=False):
+    """Refuses what autograd would lose in silence.  values: a gradient's call, whose results are values even where its inputs require gradients."""
+    if not values and _grad_on() and _asks(*tensors):
+        raise RuntimeError(f"{name}: autograd does not record this call, an input's gradient would be lost: call it under torch.no_grad() or on detached tensors, and "
+                           f"{name.removesuffix('_step')}_grad for the gradient")
+    if _dual is not None and _dual._current_level >= 0:
+        for x in tensors:
+            if x is not None and x.__class__ is not Packed8 and _dual.unpack_dual(x).tangent is not None:
+                raise RuntimeError(f"{name}: forward-mode derivatives are not computed, an input's tangent would be lost")
 
 
 class _Rows:
@@ -275,6 +294,7 @@ def causal_conv(x, weight, bias=None, *, silu=False, seq_start=None, lengths=Non
     """The convolution of each sequence with its own past.  weight [D, W]: the last tap meets the row itself.  state [n_seq, W - 1, D]: the rows
     before the first (absent: 0).  Returns y, or (y, the state behind the last rows)."""
     r = _Rows(x, "x", seq_start, lengths)
+    _recorded("causal_conv", x, weight, bias, state, out)
     x = _channels(x)
     W = _taps(weight)
     D, shape = r.D, (r.n_seq, W - 1, r.D)
@@ -293,6 +313,7 @@ def causal_conv_grad(dy, x, weight, bias=None, *, silu=False, seq_start=None, le
     """Gradients of causal_conv from dy (and dstate, the gradient of the state it returned): ConvGrads(x, weight, bias, state); bias and state are
     None where the call had none.  x may be a checkpoint: the gradient is taken at the values it holds."""
     r = _Rows(x, "x", seq_start, lengths)
+    _recorded("causal_conv_grad", dy, x, weight, bias, state, dstate, values=True)
     x, dy = _channels(x), r.like(dy, "dy")
     W = _taps(weight)
     D, shape = r.D, (r.n_seq, W - 1, r.D)
@@ -322,6 +343,7 @@ def causal_conv_step(x, weight, bias, state, slots=None, *, silu=False, out=None
     if x.__class__ is Packed8:
         raise TypeError("x cannot be an 8-bit checkpoint here")
     r = _Rows(x, "x", step=True)
+    _recorded("causal_conv_step", x, weight, bias, state, out)
     n, D = x.shape
     W = _taps(weight)
     weight, bias = r.weight(weight, "weight", (D, W)), r.weight(bias, "bias", (D,))
@@ -376,6 +398,7 @@ def selective_scan(u, dt, A, B, C_, *, D=None, z=None, dt_bias=None, softplus=Tr
     d // (D / G); D, dt_bias [D]; state [n_seq, D, N]: h before the first row (absent: 0).  Returns y, or (y, h behind the last rows).
     What stands beside a sequence in its batch changes its result by rounding only (how time is cut into chunks)."""
     r = _Rows(dt, "dt", seq_start, lengths)
+    _recorded("selective_scan", u, dt, A, B, C_, D, z, dt_bias, state, out)
     u, dt, z = r.like(u, "u", True), _channels(dt), None if z is None else r.like(z, "z", True)
     N, G, A, D, dt_bias, maps = _scan_params(r, A, B, C_, D, dt_bias, r.shape[:-1])
     shape = (r.n_seq, r.D, N)
@@ -401,6 +424,7 @@ def selective_scan_grad(dy, u, dt, A, B, C_, *, D=None, z=None, dt_bias=None, so
     """Gradients of selective_scan from dy (and dstate, the gradient of the state it returned): ScanGrads, None where the call had no such input.
     The states are formed again from the inputs; u and z may be checkpoints: the gradients are taken at the values they hold."""
     r = _Rows(dt, "dt", seq_start, lengths)
+    _recorded("selective_scan_grad", dy, u, dt, A, B, C_, D, z, dt_bias, state, dstate, values=True)
     u, dt, z, dy = r.like(u, "u", True), _channels(dt), None if z is None else r.like(z, "z", True), r.like(dy, "dy")
     N, G, A, D, dt_bias, maps = _scan_params(r, A, B, C_, D, dt_bias, r.shape[:-1])
     shape = (r.n_seq, r.D, N)
@@ -431,6 +455,7 @@ def selective_scan_step(u, dt, A, B, C_, state, slots=None, *, D=None, z=None, d
     """One more row for each of many running sequences: u, dt, z [n, D], B, C [n, G, N] or [n, N], state [n_slots, D, N] updated in place; slots as
     in causal_conv_step.  Returns y [n, D]."""
     r = _Rows(dt, "dt", step=True)
+    _recorded("selective_scan_step", u, dt, A, B, C_, D, z, dt_bias, state, out)
     n = r.n_seq
     u, dt, z = r.like(u, "u"), _channels(dt), None if z is None else r.like(z, "z")
     N, G, A, D, dt_bias, maps = _scan_params(r, A, B, C_, D, dt_bias, (n,))

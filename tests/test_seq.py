@@ -1269,6 +1269,49 @@ def test_rows_of_gradients_outside_the_sequences_are_kept_or_cleared(packed, zer
 
 
 @gpu
+def test_autograd_is_not_cut_in_silence():
+    """A tensor that requires a gradient, or carries a tangent, where the result could not have one: refused; values alone are fine."""
+    import torch.autograd.forward_ad as fwd
+    g = torch.Generator().manual_seed(1)
+    n, T, D, N, W = 2, 5, 8, 4, 4
+    c = dict(x=rnd(g, n, T, D), w=rnd(g, D, W), b=rnd(g, D), cst=rnd(g, n, W - 1, D), u=rnd(g, n, T, D), dt=rnd(g, n, T, D), A=-torch.exp(rnd(g, D, N)), B=rnd(g, n, T, N), C=rnd(g, n, T, N),
+             D=rnd(g, D), z=rnd(g, n, T, D), bias=rnd(g, D), hst=rnd(g, n, D, N), dy=rnd(g, n, T, D), out=rnd(g, n, T, D), out1=rnd(g, n, D))
+    calls = {
+        "conv": (("x", "w", "b", "cst", "out"), lambda k: seq.causal_conv(k["x"], k["w"], k["b"], state=k["cst"], out=k["out"])),
+        "conv_step": (("x", "w", "b", "cst", "out1"), lambda k: seq.causal_conv_step(k["x"][:, 0], k["w"], k["b"], k["cst"], out=k["out1"])),
+        "scan": (("u", "dt", "A", "B", "C", "D", "z", "bias", "hst", "out"),
+                 lambda k: seq.selective_scan(k["u"], k["dt"], k["A"], k["B"], k["C"], D=k["D"], z=k["z"], dt_bias=k["bias"], state=k["hst"], out=k["out"])),
+        "scan_step": (("u", "dt", "A", "B", "C", "D", "z", "bias", "hst", "out1"),
+                      lambda k: seq.selective_scan_step(k["u"][:, 0], k["dt"][:, 0], k["A"], k["B"][:, 0], k["C"][:, 0], k["hst"], D=k["D"], z=k["z"][:, 0], dt_bias=k["bias"], out=k["out1"]))}
+    grads = {"conv_grad": (("dy", "x", "w", "b", "cst"), lambda k: seq.causal_conv_grad(k["dy"], k["x"], k["w"], k["b"], state=k["cst"])),
+             "scan_grad": (("dy", "u", "dt", "A", "B", "C", "D", "z", "bias", "hst"),
+                           lambda k: seq.selective_scan_grad(k["dy"], k["u"], k["dt"], k["A"], k["B"], k["C"], D=k["D"], z=k["z"], dt_bias=k["bias"], state=k["hst"]))}
+    for names, call in calls.values():
+        call(c)
+        for name in names:
+            asks = {**c, name: c[name].clone().requires_grad_()}
+            with pytest.raises(RuntimeError, match="autograd"):
+                call(asks)
+            with torch.no_grad():
+                call(asks)
+            with torch.inference_mode():
+                call({k: v.clone() for k, v in c.items()})
+    for names, call in grads.values():
+        want = call(c)
+        for name in names:
+            assert same(call({**c, name: c[name].clone().requires_grad_()}), want)
+    for names, call in (*calls.values(), *grads.values()):
+        with fwd.dual_level():
+            call(c)
+            for name in names:
+                with pytest.raises(RuntimeError, match="tangent"):
+                    call({**c, name: fwd.make_dual(c[name].clone(), torch.ones_like(c[name]))})
+    assert not any(v.requires_grad for v in c.values())
+    p = seq.pack8(c["x"].clone().requires_grad_())       # codes are whole numbers: nothing to lose
+    assert torch.equal(seq.unpack8(p), seq.unpack8(seq.pack8(c["x"])))
+
+
+@gpu
 def test_results_over_parts_of_inputs_are_refused():
     """Memory that an input and a result share is found wherever it lies, not at equal pointers only; columns and blocks of one array beside each other are fine."""
     g = torch.Generator().manual_seed(3)
