@@ -2,7 +2,9 @@
 //
 // A row's channels in blocks of 32, one scale 2^e a block (stored e + 127): e = floor(log2 max|x|) - 6, one more where the largest value would
 // round to 128; code = x / 2^e rounded half to even, within +-127.  Scales are powers of two, so that the rounding to a code is the only one:
-// a value comes back within 2^(e - 1), at most max|x| / 128 (the type's largest values, from 127.5 of 128 of its last binade on, within 2^e).
+// a value comes back within 2^(e - 1), at most max|x| / 127.5 (64 codes and more up to 127.5 of them; where 128 would be reached the code is twice as large and the
+// largest value has 63.75 to 64 of them), and within 2^-128 where e would be below -127 (max|x| < 2^-121); the type's largest values, from 127.5 of 128 of its
+// last binade on, within 2^e.
 // A block that holds an infinity or a NaN comes back as NaN (scale byte 255).  Reads once, writes 33/32 bytes a value: bound by memory.
 // 16384 rows of 4096 channels, bf16: 204 MB in 38 us (5.4 TB/s), back in 32 us (6.4 TB/s; what was just written is still in a cache).
 #pragma once

@@ -471,8 +471,8 @@ def selective_scan_step(u, dt, A, B, C_, state, slots=None, *, D=None, z=None, d
 
 # ---------------------------------------------------------------- checkpoints
 def pack8(x):
-    """x [..., D] (float32, bfloat16 or float16) in 8 bits: Packed8.  A value comes back within half a code, at most max|x| / 128 of its block of
-    32 channels (within a code where max|x| is within 0.4 % of the type's largest); a block with an infinity or a NaN comes back as NaN."""
+    """x [..., D] (float32, bfloat16 or float16) in 8 bits: Packed8.  A value comes back within half a code, at most max|x| / 127.5 of its block of
+    32 channels, or 2^-128 where that is more (within a code, max|x| / 127.5, where max|x| is within 0.4 % of the type's largest); a block with an infinity or a NaN comes back as NaN."""
     t = _torch()
     if x.__class__ is Packed8 or _DT.get(x.dtype) not in (L.DT_F32, L.DT_BF16, L.DT_F16):
         raise TypeError(f"pack8: float32, bfloat16 or float16, not {x.dtype}")

@@ -549,7 +549,8 @@ int32_t crnn_scan_backward(const crnn_scan_args *a);
 int32_t crnn_scan_step(const crnn_scan_args *a);
 
 /* Checkpoint of x [rows][D] (float, bfloat16 or half; row_stride): codes [rows][D] int8, scales [rows][ceil(D / 32)] bytes e + 127, value = code
- * 2^e.  Within half a code: at most max|x| / 128 of the 32 channels (within one where max|x| is within 0.4 % of the type's largest).  A block with an infinity or a NaN comes back as NaN. */
+ * 2^e.  Within half a code: at most max|x| / 127.5 of the 32 channels, or 2^-128 where that is more (within one code, max|x| / 127.5, where max|x| is within 0.4 % of the
+ * type's largest).  A block with an infinity or a NaN comes back as NaN. */
 int32_t crnn_pack8(int32_t device, void *stream, const crnn_view *x, int64_t rows, int32_t D, void *codes, void *scales);
 int32_t crnn_unpack8(int32_t device, void *stream, const void *codes, const void *scales, int64_t rows, int32_t D, const crnn_view *x);
 

@@ -784,6 +784,29 @@ def test_checkpoint_codes_and_values(dtype, shape, pad):
 
 
 @gpu
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+def test_checkpoint_error_reaches_its_bound(dtype):
+    """max|x| / 127.5 is the bound: reached where the largest value would round to 128 codes and the code is doubled (64 of them, half a code off is max / 127.5); 2^-128
+    where the smallest scale is in use; a code where the type's last binade leaves no room for the doubled one."""
+    dt = DT[dtype]
+    small = -10 if dtype == "f16" else -120
+    x = torch.zeros(4, 32, dtype=torch.float64)
+    for r, e in enumerate((0, 5, small)):
+        x[r, 0] = 255 / 128
+        x[r, 1:] = (2 * torch.arange(31) + 1) / 64           # half a code of 2^-5 each
+        x[r] *= 2.0 ** e
+    x[3, :3] = torch.tensor([2.0 ** -124, 2.0 ** -130, -(2.0 ** -128)], dtype=torch.float64) if dtype != "f16" else 0
+    got = seq.unpack8(seq.pack8(x.to(dt).to(DEV)), dtype=torch.float32).cpu().double()
+    assert torch.equal(x.to(dt).double(), x)
+    big = x.abs().amax(1, keepdim=True)
+    off = (got - x).abs()
+    assert bool((off <= torch.clamp(big / 127.5, min=2.0 ** -128)).all())
+    assert bool((off.amax(1)[:3] == big[:3, 0] / 127.5).all()) and (dtype == "f16" or float(off[3].max()) == 2.0 ** -128)
+    top = torch.full((1, 32), torch.finfo(dt).max, dtype=dt, device=DEV)
+    assert bool(((seq.unpack8(seq.pack8(top)).double() - top.double()).abs() <= top.double() / 127.5).all())
+
+
+@gpu
 def test_checkpoint_of_extreme_values():
     x = torch.zeros(8, 64, device=DEV)
     x[0, 3], x[1, 40], x[2, 0] = float("nan"), float("inf"), float("-inf")
