@@ -4,7 +4,7 @@
 //     h[t, d, n] = exp(delta A[d, n]) h[t - 1, d, n] + delta u B[t, g, n],   v[t, d] = sum_n C[t, g, n] h[t, d, n] + D[d] u
 //     y = v, or v z sigmoid(z);   g = d / (channels of a group)
 //
-// the diagonal linear ODE h' = A h + B u stepped exactly over steps of their own length, input held.
+// the diagonal linear ODE h' = A h + B u over steps of their own length: the decay exact, the input to first order in the step (delta u B).
 //
 // Split.  A block owns 64 channels of one group (a tile), a lane a channel.  Forward, four wavefronts share the states: each row's step length,
 // input and gate are worked out by one of them and handed round in the LDS, so are the row's B and C (the same for all lanes of a tile: read

@@ -1,7 +1,8 @@
 """Sequence operators on the device: a short causal convolution, the selective state space scan and activation checkpoints in 8 bits.
 
 The scan is the linear member of the ODE family this package integrates: a diagonal linear ODE h' = A h + B(t) u(t) with learned rates,
-stepped exactly over steps of their own length (an irregular time grid), thousands of channels and rows, with its discrete adjoint.
+over steps of their own length (an irregular time grid), thousands of channels and rows, with its discrete adjoint.  A step's decay is exact, its
+input enters to first order in the step length (delta B u, as in selective state space models; held over the step it would be (exp(delta A) - 1) / A B u).
 
     causal_conv / causal_conv_grad / causal_conv_step          p[t, d] = bias[d] + sum_j weight[d, j] x[t - W + 1 + j, d];  y = p, or p sigmoid(p)
     selective_scan / selective_scan_grad / selective_scan_step h = exp(delta A) h + delta u B;  y = sum_n C h + D u, or that times z sigmoid(z);

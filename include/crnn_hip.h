@@ -460,8 +460,10 @@ int32_t crnn_cathode_get_particles(crnn_cathode_ctx *ctx, double *p);
 
 /* ======================================================================== *
  * Sequence operators: the linear member of the family of ODE models above, at the sizes of sequence models.  A diagonal linear ODE
- * h' = A h + B(t) u(t) with learned rates, thousands of channels and steps of their own length (an irregular time grid), integrated
- * exactly (input held over a step), with its discrete adjoint: the selective state space scan.  In front of it a short causal
+ * h' = A h + B(t) u(t) with learned rates, thousands of channels and steps of their own length (an irregular time grid), in the form
+ * that selective state space models use, with its discrete adjoint.  The decay of a step is exact, exp(delta A); the input enters to first order in the
+ * step, delta B u (an input held over the step would enter as (exp(delta A) - 1) / A B u: the two agree where |delta A| is small, at delta A = -1.6 they
+ * differ by a factor of two).  In front of it a short causal
  * convolution over time; for training, activation checkpoints in 8 bits, which both gradients read as they are.
  *
  * Unlike the entry points above, these take DEVICE pointers and enqueue on the caller's stream: nothing is copied to the host, nothing

@@ -534,6 +534,22 @@ def test_step_length_keeps_its_relative_accuracy():
 
 
 @gpu
+def test_a_step_has_an_exact_decay_and_an_input_of_first_order():
+    """h = exp(delta A) h + delta B u, not the integral over a held input (exp(delta A) - 1) / A B u; the two agree to first order in delta A."""
+    A = -torch.tensor([[16.0], [1.6], [0.01]], device=DEV)
+    one, state = torch.ones(1, 1, 1, device=DEV), torch.full((1, 3, 1), 0.5, device=DEV)
+    for delta in (0.1, 1e-3):
+        dt = torch.full((1, 1, 3), delta, device=DEV)
+        _, end = seq.selective_scan(torch.ones(1, 1, 3, device=DEV), dt, A, one, one, softplus=False, state=state, return_state=True)
+        d, a = float(dt[0, 0, 0].double()), cpu64(A)
+        want = torch.exp(d * a) * 0.5 + d
+        # decay: the exponent's rounding and the exponential's; product and sum
+        assert bool(((cpu64(end)[0] - want).abs() <= 8 * 2.0 ** -24 * (1 + (d * a).abs()) * want).all())
+        held = torch.exp(d * a) * 0.5 + torch.expm1(d * a) / a
+        assert bool(((want - held).abs() <= d * (d * a).abs()).all())
+
+
+@gpu
 def test_infinities_and_nan_stay_in_their_channel_and_after_their_row():
     g = torch.Generator().manual_seed(0)
     u, dt, z = rnd(g, 2, 50, 80), rnd(g, 2, 50, 80), rnd(g, 2, 50, 80)
