@@ -12,7 +12,8 @@ input enters to first order in the step length (delta B u, as in selective state
 Arrays are torch tensors on an MI355X; the calls enqueue on that device's current stream and do not wait, so that they may be captured into
 a graph.  Rows are time, channels are contiguous: dense [n_seq, rows, D] (lengths=: how many rows of each are its own, the others are
 padding), or packed [rows, D] with seq_start [n_seq + 1], int32 on the device: sequence s is rows seq_start[s] .. seq_start[s + 1] - 1.
-Lengths and offsets are not read by the host: they are clamped to the arrays.  Rows of a result that belong to no sequence are 0, and stay as
+Lengths and offsets are not read by the host: they are clamped to the arrays; offsets may not decrease (entries not in use
+repeat the last one), or the results are not defined.  Rows of a result that belong to no sequence are 0, and stay as
 they were where the caller gave the array (out=).  Results may not share memory with inputs (refused).  Autograd does not record the calls,
 gradients are the *_grad calls: forward calls and steps on tensors that require gradients are refused while it records (call them under
 torch.no_grad(), or in the forward of a torch.autograd.Function), and so are forward-mode tangents; the *_grad calls give values that

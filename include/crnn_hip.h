@@ -473,10 +473,13 @@ int32_t crnn_cathode_get_particles(crnn_cathode_ctx *ctx, double *p);
  *
  * Rows.  Time runs over rows, channels are contiguous in memory.  Dense: n_seq sequences of `rows` rows (seq_len, if given, says how
  * many of them each has; the others are padding).  Packed: seq_start[n_seq + 1] on the device, sequence s is rows seq_start[s] ..
- * seq_start[s + 1] - 1 of arrays of `rows` rows.  Sequences may be empty.  Offsets and lengths are clamped to the arrays (offsets that
- * decrease make the sequence empty; what sequences that overlap give is not defined).  Rows of an output that belong to no sequence are
+ * seq_start[s + 1] - 1 of arrays of `rows` rows.  Sequences may be empty; offsets may not decrease (entries that are not
+ * in use repeat the last one).  Offsets and lengths are clamped to the arrays, so that no content of theirs reaches outside of them; what a call with offsets that
+ * decrease gives is not defined.  Rows of an output that belong to no sequence are
  * left as they were, or set to 0 where zero_outside is set.  With no sequences (n_seq = 0) the forward calls and the steps do nothing and the
- * backward calls are refused.  Outputs may not share memory with inputs (states of the steps excepted: they are updated in place).
+ * backward calls are refused.  Outputs may share memory neither with inputs (states of the steps excepted: they are updated in place; scan states out may be the
+ * scan states in) nor with one another: refused, unless the arrays are columns or blocks beside each other in one array.  A launch has at most 2^24 - 1
+ * blocks of 256 threads: more sequences, rows and channels at once are refused.
  * Element types: input, output and state activations of one call share one type (CRNN_DT_F32, _BF16, _F16, _F64); x of the convolution
  * and u, z of the scan may be checkpoints (_PACKED8) unless the call's type is _F64.  Weights, A, D, biases, scan states and the gradients of
  * all of these are float (double where the type is _F64); arithmetic is in that type, activations are rounded once, when stored.

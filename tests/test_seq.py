@@ -775,6 +775,20 @@ def test_offsets_that_make_no_sense_stay_inside_the_arrays(starts):
     seq.selective_scan_grad(dy, u, dt, A, B, C, seq_start=at)
 
 
+@gpu
+def test_offsets_not_in_use_repeat_the_last_one():
+    g = torch.Generator().manual_seed(6)
+    x, dt, dy, m = (rnd(g, 90, n) for n in (20, 20, 20, 16))
+    A, w = -torch.exp(rnd(g, 20, 16)), rnd(g, 20, 4)
+    few, more = (torch.tensor(v, dtype=torch.int32, device=DEV) for v in ([0, 25, 70], [0, 25, 70] + [70] * 70))
+    assert torch.equal(seq.causal_conv(x, w, seq_start=few), seq.causal_conv(x, w, seq_start=more))
+    ga, gb = (seq.causal_conv_grad(dy, x, w, seq_start=at) for at in (few, more))
+    assert torch.equal(ga.x, gb.x) and torch.allclose(ga.weight, gb.weight, rtol=1e-5, atol=1e-4)
+    (ya, ea), (yb, eb) = (seq.selective_scan(x, dt, A, m, m, seq_start=at, return_state=True) for at in (few, more))
+    # (the number of sequences is part of the rule how time is cut: another order of the same sums)
+    assert bool(((ya - yb).abs() <= 1e-5 * (1 + ya.abs())).all()) and torch.allclose(ea, eb[:2], rtol=1e-5, atol=1e-5) and not bool(eb[2:].any())
+
+
 # ---------------------------------------------------------------- checkpoints
 @gpu
 @pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
