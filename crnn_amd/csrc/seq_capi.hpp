@@ -53,7 +53,7 @@ struct SeqCheck {
         if (err.empty()) err = std::string(who) + ": " + what;
         return false;
     }
-    // a view of the call's type (or, where allowed, a checkpoint); out: rows may not overlap
+    // a view of the call's type (or, where allowed, a checkpoint); out: rows of `width` elements may not overlap (0: there is one row, its stride means nothing)
     bool view(const crnn_view &v, const char *name, int dtype, bool needed, bool packed_ok, bool out, int64_t width) {
         if (!v.ptr) return needed ? bad(std::string(name) + " is missing") : true;
         if (v.dtype == CRNN_DT_PACKED8) {
@@ -331,12 +331,14 @@ bool scan_views(SeqCheck &c, const crnn_scan_args *a, bool backward, bool step =
         return false;
     if (a->B_group < 0 || a->B_state < 0 || a->C_group < 0 || a->C_state < 0) return c.bad("negative stride of B or C");
     const int64_t n = a->seq_start || step ? 1 : a->n_seq, rows = a->rows, flat = step ? a->n_seq : seq_flat(a->n_seq, rows, a->seq_start != nullptr);
+    const bool many = (step ? a->n_seq : rows) > 1;
+    const int64_t Dw = many ? D : 0, GNw = many ? GN : 0;
     if (!backward)
-        return c.view(a->y, "y", dt, true, false, true, D) && c.apart(a->y, "y", n, rows, D) && c.other({&a->y}, {&a->u, &a->dt, &a->z, &a->B, &a->C}, flat);
+        return c.view(a->y, "y", dt, true, false, true, Dw) && c.apart(a->y, "y", n, rows, D) && c.other({&a->y}, {&a->u, &a->dt, &a->z, &a->B, &a->C}, flat);
     if (!a->dA) return c.bad("dA is missing");
     if ((a->z.ptr != nullptr) != (a->dz.ptr != nullptr)) return c.bad("dz goes with z");
-    return c.view(a->dy, "dy", dt, true, false, false, D) && c.view(a->du, "du", dt, true, false, true, D) && c.view(a->ddt, "ddt", dt, true, false, true, D) &&
-           c.view(a->dz, "dz", dt, false, false, true, D) && c.view(a->dB, "dB", dt, true, false, true, GN) && c.view(a->dC, "dC", dt, true, false, true, GN) &&
+    return c.view(a->dy, "dy", dt, true, false, false, D) && c.view(a->du, "du", dt, true, false, true, Dw) && c.view(a->ddt, "ddt", dt, true, false, true, Dw) &&
+           c.view(a->dz, "dz", dt, false, false, true, Dw) && c.view(a->dB, "dB", dt, true, false, true, GNw) && c.view(a->dC, "dC", dt, true, false, true, GNw) &&
            c.apart(a->du, "du", n, rows, D) && c.apart(a->ddt, "ddt", n, rows, D) && c.apart(a->dz, "dz", n, rows, D) && c.apart(a->dB, "dB", n, rows, GN) &&
            c.apart(a->dC, "dC", n, rows, GN) && c.other({&a->du, &a->ddt, &a->dz, &a->dB, &a->dC}, {&a->dy, &a->u, &a->dt, &a->z, &a->B, &a->C}, flat);
 }
@@ -423,15 +425,16 @@ bool conv_views(SeqCheck &c, const crnn_conv_args *a, bool backward, crnn::ConvP
     const int dt = a->dtype;
     if (!a->weight) return c.bad("weight is missing");
     const int64_t n = a->seq_start ? 1 : a->n_seq, flat = seq_flat(a->n_seq, a->rows, a->seq_start != nullptr);
+    const int64_t Dw = a->rows > 1 ? a->D : 0, Sw = a->W > 2 ? a->D : 0;
     if (!c.view(a->x, "x", dt, true, true, false, a->D) || !c.view(a->state_in, "state_in", dt, false, false, false, a->D)) return false;
     if (backward) {
         if (!a->dweight) return c.bad("dweight is missing");
-        if (!c.view(a->dy, "dy", dt, true, false, false, a->D) || !c.view(a->dx, "dx", dt, true, false, true, a->D) ||
-            !c.view(a->dstate_out, "dstate_out", dt, false, false, false, a->D) || !c.view(a->dstate_in, "dstate_in", dt, false, false, true, a->D) ||
+        if (!c.view(a->dy, "dy", dt, true, false, false, a->D) || !c.view(a->dx, "dx", dt, true, false, true, Dw) ||
+            !c.view(a->dstate_out, "dstate_out", dt, false, false, false, a->D) || !c.view(a->dstate_in, "dstate_in", dt, false, false, true, Sw) ||
             !c.apart(a->dx, "dx", n, a->rows, a->D) || !c.apart(a->dstate_in, "dstate_in", a->n_seq, a->W - 1, a->D) || !c.other({&a->dx}, {&a->x, &a->dy}, flat))
             return false;
     } else {
-        if (!c.view(a->y, "y", dt, true, false, true, a->D) || !c.view(a->state_out, "state_out", dt, false, false, true, a->D) ||
+        if (!c.view(a->y, "y", dt, true, false, true, Dw) || !c.view(a->state_out, "state_out", dt, false, false, true, Sw) ||
             !c.apart(a->y, "y", n, a->rows, a->D) || !c.apart(a->state_out, "state_out", a->n_seq, a->W - 1, a->D) || !c.other({&a->y}, {&a->x}, flat))
             return false;
         if (a->state_out.ptr && a->state_out.ptr == a->state_in.ptr) return c.bad("state_out may not be state_in");
@@ -594,8 +597,8 @@ int32_t crnn_conv_step(const crnn_conv_args *a) {
         if (a->seq_start || a->seq_len) return sfail("crnn_conv_step: rows are one per sequence (no seq_start, seq_len)");
         if (a->n_slots < 0 || a->n_slots > 0x7fffffff || (!a->slot && a->n_seq > a->n_slots)) return sfail("crnn_conv_step: n_slots does not fit the rows");
         if (a->n_seq == 0) return 0;
-        if (!c.view(a->x, "x", a->dtype, true, false, false, a->D) || !c.view(a->y, "y", a->dtype, true, false, true, a->D) ||
-            !c.view(a->state_in, "state_in", a->dtype, a->W > 1 && a->n_slots > 0, false, true, a->D) || !c.other({&a->y}, {&a->x}, 1) ||
+        if (!c.view(a->x, "x", a->dtype, true, false, false, a->D) || !c.view(a->y, "y", a->dtype, true, false, true, a->n_seq > 1 ? a->D : 0) ||
+            !c.view(a->state_in, "state_in", a->dtype, a->W > 1 && a->n_slots > 0, false, true, a->W > 2 ? a->D : 0) || !c.other({&a->y}, {&a->x}, 1) ||
             !c.apart(a->state_in, "state_in", a->n_slots, a->W - 1, a->D))
             return sfail(c.err);
         if (!a->weight) return sfail("crnn_conv_step: weight is missing");
@@ -712,7 +715,7 @@ static bool pack_plan(SeqCheck &c, const crnn_view *x, int64_t rows, int32_t D, 
     p.rows = rows; p.D = D; p.nb = (D + 31) / 32;
     if (rows == 0) return true;
     if (!codes || !scales) return c.bad("codes or scales are missing");
-    if (!c.view(*x, "x", x->dtype, true, false, out, D)) return false;
+    if (!c.view(*x, "x", x->dtype, true, false, out, rows > 1 ? D : 0)) return false;
     SeqShare m;
     if (out) {
         m.out(*x, D, rows, 1); m.in(codes, rows * D); m.in(scales, rows * p.nb);

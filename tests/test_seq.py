@@ -949,6 +949,25 @@ def test_arrays_of_other_strides():
     assert torch.equal(seq.unpack8(seq.pack8(d)), seq.unpack8(seq.pack8(d.contiguous())))
 
 
+@gpu
+def test_single_rows_of_any_stride():
+    """One row a sequence, cut out of arrays with time as the fastest index: the stride between rows means nothing, for results and for states of one row either."""
+    g = torch.Generator().manual_seed(9)
+    n, D, N = 3, 12, 4
+    late = lambda k: torch.full((n, D, k), 7.0, device=DEV).transpose(1, 2)  # noqa: E731
+    x, m, w, A = rnd(g, n, D, 1).transpose(1, 2), rnd(g, n, 1, N), rnd(g, D, 2), -torch.exp(rnd(g, D, N))
+    state = rnd(g, n, D, 1).transpose(1, 2)
+    assert x.stride() == (D, 1, 1) and late(1).stride() == (D, 1, 1)
+    y, end = seq.causal_conv(x, w, state=state, return_state=True)
+    assert torch.equal(seq.causal_conv(x, w, state=state, out=late(1)), y)
+    assert torch.equal(seq.selective_scan(x, x, A, m, m, out=late(1)), seq.selective_scan(x.contiguous(), x.contiguous(), A, m, m))
+    st = late(1)
+    st.copy_(state)
+    assert st.stride() == (D, 1, 1) and torch.equal(seq.causal_conv_step(x[:, 0], w, None, st), y[:, 0]) and torch.equal(st, end)
+    one = rnd(g, 1, D).as_strided((1, D), (1, 1))
+    assert torch.equal(seq.causal_conv_step(one, w, None, rnd(g, 1, 1, D) * 0, out=torch.empty(D, device=DEV).as_strided((1, D), (1, 1))), seq.causal_conv(one[None], w)[0])
+
+
 def shifted(x):
     """x one element behind a 16-byte boundary, contiguous as before."""
     if x is None or x.numel() == 0:
