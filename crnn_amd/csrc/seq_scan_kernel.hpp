@@ -402,11 +402,11 @@ __global__ __launch_bounds__(64 * kScanWaves, IO == 8 ? 2 : 3) void seq_scan_end
             seq_wave_sync();
         }
         // decays above one (a positive rate, a negative step length) may have taken P out of range, where it makes NaN of an r C of 0: then G row by row
-        // from the last to the first, as the formula has it
+        // from the last to the first, as the formula has it (only the channels that need it: the others keep their bits)
         bool out = false;
 #pragma unroll
         for (int n = 0; n < NS; ++n) out = out || !(P[n] <= CT(IO == 8 ? 1.7976931348623157e308 : 3.4028234663852886e38));
-        if (__builtin_amdgcn_ballot_w64(out)) {
+        if (out) {
 #pragma unroll
             for (int n = 0; n < NS; ++n) g[n] = CT(0);
 #pragma unroll 1

@@ -738,6 +738,27 @@ def test_modes_that_grow_stay_in_range_where_the_formula_does(sign, N, T, dtype)
 
 
 @gpu
+@pytest.mark.parametrize("T", [50, 200])
+@pytest.mark.parametrize("N", [16, 20])
+@pytest.mark.parametrize("what", ["growth", "nan"])
+def test_a_channel_out_of_range_leaves_the_others_their_bits(what, N, T):
+    c = scan_with(T, 70, N, {})
+    clean = scan_all(c)
+    if what == "growth":
+        c["A"][3, :] = 2.0
+        c["dt"][:, 3] = 3.0
+    else:
+        c["dt"][T // 2, 3] = math.nan
+    got = scan_all(c)
+    others = torch.arange(70, device=DEV) != 3
+    for k, v in got.items():
+        if k in ("B", "C"):
+            continue            # (sums over the channels)
+        at = {"A": 0, "D": 0, "end": 1, "state": 1}.get(k, 1)
+        assert torch.equal(v.movedim(at, 0)[others], clean[k].movedim(at, 0)[others]), k
+
+
+@gpu
 @pytest.mark.parametrize("T", [1, 11, 64, 70, 151])
 @pytest.mark.parametrize("N", [5, 16, 32])
 @pytest.mark.parametrize("dtype", ["f32", "f64"])
