@@ -66,6 +66,10 @@ __device__ __forceinline__ double seq_softplus(double x) {
     return (x > 0.0 ? x : (x == x ? 0.0 : x)) + log1p(exp(-fabs(x)));
 }
 
+__device__ __forceinline__ float seq_abs(float x) { return __builtin_fabsf(x); }
+__device__ __forceinline__ double seq_abs(double x) { return __builtin_fabs(x); }
+__device__ __forceinline__ float seq_max(float a, float b) { return __builtin_fmaxf(a, b); }
+__device__ __forceinline__ double seq_max(double a, double b) { return __builtin_fmax(a, b); }
 __device__ __forceinline__ float seq_ldexp(float x, int e) { return __builtin_ldexpf(x, e); }
 __device__ __forceinline__ double seq_ldexp(double x, int e) { return __builtin_ldexp(x, e); }
 // h 2^x where 2^x alone may be out of the type's range (growth over a whole chunk: 0 stays 0, and a small h may come out in range)

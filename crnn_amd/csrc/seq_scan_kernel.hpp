@@ -102,10 +102,13 @@ __device__ __forceinline__ void scan_rates(const ScanP &p, int d, int n, CT (&A2
     constexpr CT top = CT(sizeof(CT) == 8 ? 1.7976931348623157e308 : 3.4028234663852886e38);
     scan_get<CT, K>(p, p.A, d, n, A2);
 #pragma unroll
-    for (int j = 0; j < K; ++j) {
-        A2[j] *= CT(kLog2eD);
-        A2[j] = A2[j] < -top ? -top : A2[j] > top ? top : A2[j];
-    }
+    for (int j = 0; j < K; ++j) A2[j] *= CT(kLog2eD);
+    CT big = CT(0);
+#pragma unroll
+    for (int j = 0; j < K; ++j) big = seq_max(big, seq_abs(A2[j]));
+    if (big > top)          // (looked at first: a gradient's chunk has 20 rows for what it does once; a NaN stays one)
+#pragma unroll
+        for (int j = 0; j < K; ++j) A2[j] = A2[j] < -top ? -top : A2[j] > top ? top : A2[j];
 }
 // PAD: N does not fill the launch's NS states.  The states behind the last one have rates, maps and first states of 0, but 0 times an infinite step length,
 // input or gradient is NaN: they are put to 0 after every row, or what is summed over the states would take it up.
@@ -333,6 +336,25 @@ __global__ __launch_bounds__(64 * kScanWaves, IO == 8 ? 3 : 6) void seq_scan_fwd
     if (wave == 0) sdel[a.b * p.D + a.d] = (sh.dl[0][lane] + sh.dl[1][lane]) + (sh.dl[2][lane] + sh.dl[3][lane]);
 }
 
+// whether one of these products of decays is infinite or NaN (none is negative: their bits are ordered like the values, infinities and NaN above all)
+template <int NS>
+__device__ __forceinline__ bool scan_left_range(const float (&P)[NS]) {
+    uint32_t m = 0;
+#pragma unroll
+    for (int n = 0; n < NS; ++n) {
+        const uint32_t b = seq_as_bits(P[n]) & 0x7fffffffu;
+        m = b > m ? b : m;
+    }
+    return m >= 0x7f800000u;
+}
+template <int NS>
+__device__ __forceinline__ bool scan_left_range(const double (&P)[NS]) {
+    bool out = false;
+#pragma unroll
+    for (int n = 0; n < NS; ++n) out = out || !(P[n] <= 1.7976931348623157e308);
+    return out;
+}
+
 // ---- gradient, a chunk by itself: S = its last state from zero, the sum of delta, and G = what its outputs' gradients r pass back to the state
 // before it, sum_t (prod of the decays up to t) r C -- taken in the forward direction, so that one exponential serves both.
 // 6144 rows of 2048 channels, 16 states, u and z in 8 bits: 79 us (72 where they are plain), vector unit busy 86 %.
@@ -403,10 +425,7 @@ __global__ __launch_bounds__(64 * kScanWaves, IO == 8 ? 2 : 3) void seq_scan_end
         }
         // decays above one (a positive rate, a negative step length) may have taken P out of range, where it makes NaN of an r C of 0: then G row by row
         // from the last to the first, as the formula has it (only the channels that need it: the others keep their bits)
-        bool out = false;
-#pragma unroll
-        for (int n = 0; n < NS; ++n) out = out || !(P[n] <= CT(IO == 8 ? 1.7976931348623157e308 : 3.4028234663852886e38));
-        if (out) {
+        if (scan_left_range(P)) {
 #pragma unroll
             for (int n = 0; n < NS; ++n) g[n] = CT(0);
 #pragma unroll 1
