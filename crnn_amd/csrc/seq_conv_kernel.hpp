@@ -157,8 +157,8 @@ __device__ __forceinline__ ConvAt conv_at(const ConvP &p) {
     return a;
 }
 
-// 12001 rows of 4096 channels, bf16, 4 taps: 197 MB in 47 us where nothing is in a cache (4.2 TB/s; a copy reaches 4.7), 38 us again and again on the
-// same arrays; 60000 rows 193 us (5.1 TB/s).  130 rows of 768: 6.7 us, a thread's chain of dependent loads.
+// 12001 rows of 4096 channels, bf16, 4 taps: 197 MB in 46 us where nothing is in a cache (4.2 TB/s; a copy reaches 4.7), 38 us again and again on the
+// same arrays; 60000 rows 193 us (5.1 TB/s).  130 rows of 768: 6.5 us, a thread's chain of dependent loads.
 template <int XT, int YT, int W, int V>
 __global__ __launch_bounds__(256) void seq_conv_fwd_kernel(const ConvP p) {
     using CT = typename SeqT<YT>::C;
@@ -235,8 +235,8 @@ __global__ __launch_bounds__(256) void seq_conv_fwd_kernel(const ConvP p) {
 
 // Gradient.  dp = dy act'(p) needs p once more; dx[t] = sum_j w[j] dp[t + W - 1 - j] needs the W - 1 rows behind t: the strip is walked W - 1
 // rows past its end.  A sequence's first strip starts W - 1 rows early: those are the state's.  dw, db: a strip's part, summed in order.
-// 8192 rows of 2048 channels, x in 8 bits, bf16, 4 taps: 33 us (84 MB, 2.5 TB/s) and 6.6 us for the sums: 30 operations an element at 128
-// registers; more wavefronts do not fit, and longer strips leave SIMDs without one.
+// 8192 rows of 2048 channels, x in 8 bits, bf16, 4 taps: 33 us (84 MB, 2.5 TB/s) and 6.3 us for the sums.  Neither memory nor the vector unit (half
+// busy) binds it: at 128 registers four wavefronts a SIMD wait for loads one batch of rows ahead; longer strips leave SIMDs without a wavefront.
 template <int XT, int YT, int W, int V>
 __global__ __launch_bounds__(256, W <= 4 && (YT == CRNN_DT_BF16 || YT == CRNN_DT_F16) ? 4 : 1) void seq_conv_bwd_kernel(const ConvP p) {
     using CT = typename SeqT<YT>::C;
@@ -371,7 +371,7 @@ __global__ __launch_bounds__(256, W <= 4 && (YT == CRNN_DT_BF16 || YT == CRNN_DT
 }
 
 // one row for each of many running sequences; the states (the last W - 1 rows) move up in place.  Rows that name one slot: seq_same_slot.
-// 192 rows of 4096 channels, bf16, 4 taps: 6 us (12.7 MB: 2.7 us of a copy's rate), a chain of slot, state and weights, then the stores.
+// 192 rows of 4096 channels, bf16, 4 taps: 5.6 us (12.7 MB: 2.7 us of a copy's rate), a chain of slot, state and weights, then the stores.
 struct ConvStepP {
     SeqV x, y, st;                   // st.bs: between slots
     const void *w, *bias;

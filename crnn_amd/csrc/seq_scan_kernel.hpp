@@ -20,7 +20,7 @@
 namespace crnn {
 
 constexpr int kScanTB = 4;      // gradient: rows whose loads are in flight together
-constexpr int kScanRows = 8;    // forward: rows of a batch, two for each wavefront (16 measured the same)
+constexpr int kScanRows = 8;    // forward: rows of a batch, two for each wavefront
 constexpr int kScanWaves = 4;   // wavefronts of a block (gradient: each on its own channel tile)
 
 struct ScanP {
@@ -204,8 +204,8 @@ struct ScanShare {
     CT dl[kScanRows][64], du[kScanRows][64], maps[kScanRows][2 * NS], v[OUT ? kScanWaves : 1][OUT ? kScanRows : 1][64];
 };
 
-// 8190 rows of 4096 channels, 16 states, bf16: 155 us with outputs, 105 without, vector unit busy 94 and 95 % of the time.  A row, channel and
-// state cost 8.2 and 5.7 vector instructions, of which 5 and 4 are the recurrence itself, the exponential counting twice: a pass that did
+// 8190 rows of 4096 channels, 16 states, bf16: 157 us with outputs, 107 without, vector unit busy 95 % of the time.  A row, channel and
+// state cost 8.3 and 5.8 vector instructions, of which 5 and 4 are the recurrence itself, the exponential counting twice: a pass that did
 // nothing else would take 83 and 69 us.  The rest is mostly the step lengths and gates of the rows (each worked out once a tile).  1 x 64 x 1536: 17 us.
 
 // ---- forward, a chunk.  OUT: outputs from its first state (start[block][n][d]; null: one chunk a sequence, from state_in), and the sequence's
@@ -357,7 +357,7 @@ __device__ __forceinline__ bool scan_left_range(const double (&P)[NS]) {
 
 // ---- gradient, a chunk by itself: S = its last state from zero, the sum of delta, and G = what its outputs' gradients r pass back to the state
 // before it, sum_t (prod of the decays up to t) r C -- taken in the forward direction, so that one exponential serves both.
-// 6144 rows of 2048 channels, 16 states, u and z in 8 bits: 79 us (72 where they are plain), vector unit busy 86 %.
+// 6144 rows of 2048 channels, 16 states, u and z in 8 bits: 82 us, vector unit busy 84 %.
 template <int IO, int NS, int MODE>
 __global__ __launch_bounds__(64 * kScanWaves, IO == 8 ? 2 : 3) void seq_scan_ends2_kernel(const ScanP p, typename SeqIO<IO>::C *__restrict__ S,
                                                                                                   typename SeqIO<IO>::C *__restrict__ Gb,
@@ -460,7 +460,7 @@ __global__ __launch_bounds__(64 * kScanWaves, IO == 8 ? 2 : 3) void seq_scan_end
 
 // ---- carry over the chunks of a sequence: S becomes each chunk's first state, G (may be null) what reaches each chunk's last state from
 // the rows behind it.  A thread per (sequence, state, channel).  Bound by memory: S and G of 308 chunks x 16 states x 2048 channels once in and once
-// out, 161 MB in 35 us (4.6 TB/s).
+// out, 161 MB in 38 us (4.2 TB/s).
 template <class CT, int NS>
 __global__ __launch_bounds__(256) void seq_scan_carry_kernel(const ScanP p, CT *__restrict__ S, CT *__restrict__ Gb, const CT *__restrict__ sdel) {
     const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, per = (int64_t)NS * p.D;
@@ -519,7 +519,7 @@ __global__ __launch_bounds__(256) void seq_scan_carry_kernel(const ScanP p, CT *
 // h[t] is one multiply-add away, and dA needs the product itself), and the reverse sweep over them.  dB and dC are sums over channels: a
 // wavefront's part goes to part[tile][row][B: NS | C: NS], summed over the tiles in a fixed order by seq_scan_sum_maps_kernel.
 // Four rows and five times four a chunk: two wavefronts a SIMD fill the registers (256 a lane) and the LDS (16.5 KB each) about together.
-// 6144 rows of 2048 channels, 16 states, u and z in 8 bits: 275 us (239 where they are plain), vector unit busy 69 %: 33 vector instructions a row, channel and state (21 of
+// 6144 rows of 2048 channels, 16 states, u and z in 8 bits: 276 to 294 us, vector unit busy 69 %: 33 vector instructions a row, channel and state (21 of
 // them the reverse row, folds of dB and dC included), the rest of the time both wavefronts of a SIMD wait (a row's maps from the LDS, the next rows).
 constexpr int kScanBwdTB = 4, kScanBwdSub = 5, kScanBwdQ = kScanBwdTB * kScanBwdSub;
 template <int IO, int NS, int MODE, bool PAD>
@@ -745,7 +745,7 @@ __global__ __launch_bounds__(256) void seq_sum_blocks_kernel(const CT *__restric
 
 // ---- one row for each of many running sequences, states updated in place.  LPC lanes share a channel, four states each (16-byte loads of
 // the state where its rows are so aligned), so that a wavefront's state accesses are contiguous: the step is bound by them.  250 rows of
-// 4096 channels, 16 states: 140 MB in 34.6 us (4.0 TB/s; a copy of as much reaches 4.7).  One row of 2048 channels: 4.5 us, a chain of three loads.
+// 4096 channels, 16 states: 140 MB in 34.6 us (4.0 TB/s; a copy of as much reaches 4.7).  One row of 2048 channels: 4.2 us, a chain of three loads.
 struct ScanStepP {
     SeqV u, dt, z, y, B, C;             // rs: between rows
     int64_t Bg, Cg, Bn, Cn;
